@@ -42,8 +42,9 @@ extern "C" {
 
 #define LLSA_DTYPE_BF16 0
 #define LLSA_DTYPE_F32 1
+#define LLSA_DTYPE_F16 2
 
-#define LLSA_ABI_VERSION 213     /* changes with every change of a signature or argument structure below */
+#define LLSA_ABI_VERSION 214     /* changes with every change of a signature or argument structure below */
 int llsa_version(void);          /* LLSA_ABI_VERSION of the built library                                    */
 const char* llsa_last_error_string(void);
 
@@ -362,6 +363,80 @@ typedef struct llsa_attn_bwd_args {
 /* topk: `levels` entries, topk[0] = T of the fine blocks, topk[l] = lvl[l-1].T for l < levels */
 int64_t llsa_attn_bwd_workspace_bytes(int B, int H, int N, const int32_t* topk, int levels);
 int llsa_attn_bwd(const llsa_attn_bwd_args* a, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The linear layers around the attention (models/rope_dit_transformer_2d.py:180-260, 581-711: the projections, the gated
+ * residuals and the feed-forward block, torch modules in the reference).  Rows of tokens x (M,K), weights W (N,K):
+ *     z = x W^T + bias,   out = residual + gate * act(z),      gate: one row of N for every per_sample rows of x
+ *     dz = dout * gate * act'(z),  dx = dz W,  dW = dz^T x,  dbias = sum over rows of dz,  dgate = sum over a sample's rows of dout * act(z)
+ * bf16 or fp16 throughout, sums in fp32, one rounding where a tensor is written.  The products read rows that are 16-byte aligned
+ * and hold a multiple of 8 elements, zeros beyond the end; llsa_pad_rows makes such rows out of any.  Activations: */
+#define LLSA_ACT_NONE 0
+#define LLSA_ACT_SILU 1
+#define LLSA_ACT_GELU 2
+#define LLSA_ACT_GELU_TANH 3
+typedef struct llsa_linear_args {
+    const void* x;          /* (M,K) rows ldx apart: fwd, dw                                           */
+    const void* w;          /* (N,K) rows ldw apart: fwd, dx                                           */
+    const void* bias;       /* (N) or NULL: fwd                                                        */
+    const void* gate;       /* (M/per_sample, N) rows s_gate apart, or NULL: fwd, dz                   */
+    const void* residual;   /* (M,N) rows ldr apart, or NULL: fwd                                      */
+    void* out;              /* fwd: out (M,N); dx: dx (M,K); dw: dW (N,K); rows ldo apart              */
+    void* z;                /* (M,N) rows ldz apart, padded like dz.  fwd: written unless NULL; dz: read
+                               (act or dgate);
+                               dx: unless NULL, (M,K), dx is multiplied by act'(z) (the dz of the layer
+                               in front)                                                               */
+    const void* dout;       /* (M,N) rows lddout apart: dz                                             */
+    const void* dz;         /* (M,N) rows lddz apart, padded to a multiple of 8: dx, dw                */
+    void* dz_out;           /* the same, written: dz                                                   */
+    void* dbias;            /* (N) or NULL: dw                                                         */
+    void* dgate;            /* (M/per_sample, N) contiguous, or NULL: dz                               */
+    void* workspace;        /* dw, dz: llsa_linear_{dw,dz}_workspace_bytes                             */
+    int64_t ldx, ldw, s_gate, ldr, ldo, ldz, lddout, lddz;
+    int64_t M, per_sample;
+    int32_t N, K, act, dtype;
+    int32_t padded;         /* fwd, dx: rows of out are padded to a multiple of 8, zeros are written there */
+    int32_t reserved;
+} llsa_linear_args;
+
+int llsa_linear_fwd(const llsa_linear_args* a, void* stream);
+int llsa_linear_dz(const llsa_linear_args* a, void* stream);
+int llsa_linear_dx(const llsa_linear_args* a, void* stream);
+int llsa_linear_dw(const llsa_linear_args* a, void* stream);
+int64_t llsa_linear_dw_workspace_bytes(int64_t M, int N, int K);
+int64_t llsa_linear_dz_workspace_bytes(int64_t M, int64_t per_sample, int N);
+/* (rows, cols) of 16-bit elements, rows ldx apart, to rows ldy apart (a multiple of 8, 16-byte aligned), zeros in columns cols .. ldy - 1 */
+int llsa_pad_rows(const void* x, int64_t ldx, void* y, int64_t ldy, int64_t rows, int cols, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Layer norm with the modulation of an adaLN block (models/rope_dit_transformer_2d.py:295-337, 581-711, torch modules in the
+ * reference).  For every row of C channels, its sample b = row / per_sample:
+ *     h = (x - mean) * rstd,   n = h * weight + bias,   y = n * (1 + scale[b]) + shift[b]
+ * and backward, with g = dy * (1 + scale[b]) * weight and the sums S1 = sum of dy, S2 = sum of dy * h over a sample's rows:
+ *     dx = rstd * (g - mean(g) - h * mean(g * h)),   dshift = S1,   dscale = weight * S2 + bias * S1,
+ *     dweight = sum over b of (1 + scale[b]) * S2[b],   dbias = sum over b of (1 + scale[b]) * S1[b]
+ * x, y, dy, dx: dtype (bf16, fp16, fp32); the small vectors: vtype (dtype or fp32).  Statistics and sums in fp32. */
+#define LLSA_NORM_MAX_CHANNELS 8192
+typedef struct llsa_layer_norm_args {
+    const void* x;          /* (rows,C) ldx apart                                                      */
+    void* y;                /* fwd: (rows,C) ldy apart                                                 */
+    const void *weight, *bias;      /* (C) or NULL                                                     */
+    const void *scale, *shift;      /* (samples,C) rows s_scale / s_shift apart, or NULL               */
+    float* stats;           /* (rows,2) mean and rstd: fwd writes them unless NULL, bwd reads them     */
+    const void* dy;         /* bwd: (rows,C) lddy apart                                                */
+    void* dx;               /* bwd: (rows,C) lddx apart, or NULL                                       */
+    void *dweight, *dbias;  /* bwd: (C) or NULL                                                        */
+    void *dscale, *dshift;  /* bwd: (samples,C) contiguous, or NULL                                    */
+    void* workspace;        /* bwd: llsa_layer_norm_bwd_workspace_bytes where any of these is wanted   */
+    int64_t ldx, ldy, s_scale, s_shift, lddy, lddx;
+    int64_t rows, per_sample;       /* per_sample: rows where there is neither scale nor shift          */
+    int32_t C, dtype, vtype;
+    float eps;
+} llsa_layer_norm_args;
+
+int llsa_layer_norm_fwd(const llsa_layer_norm_args* a, void* stream);
+int llsa_layer_norm_bwd(const llsa_layer_norm_args* a, void* stream);
+int64_t llsa_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t per_sample, int C);
 
 #ifdef __cplusplus
 }

@@ -84,6 +84,18 @@ class TransposeJob(C.Structure):
                 ("Mb", c_int32), ("Kb", c_int32), ("T", c_int32), ("chunk", c_int32), ("nested", c_void_p)]
 
 
+class LinearArgs(C.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "w", "bias", "gate", "residual", "out", "z", "dout", "dz", "dz_out", "dbias", "dgate", "workspace")]
+                + [(n, c_int64) for n in ("ldx", "ldw", "s_gate", "ldr", "ldo", "ldz", "lddout", "lddz", "M", "per_sample")]
+                + [(n, c_int32) for n in ("N", "K", "act", "dtype", "padded", "reserved")])
+
+
+class LayerNormArgs(C.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "y", "weight", "bias", "scale", "shift", "stats", "dy", "dx", "dweight", "dbias", "dscale", "dshift", "workspace")]
+                + [(n, c_int64) for n in ("ldx", "ldy", "s_scale", "s_shift", "lddy", "lddx", "rows", "per_sample")]
+                + [(n, c_int32) for n in ("C", "dtype", "vtype")] + [("eps", c_float)])
+
+
 _SIGNATURES = {
     "llsa_version": (c_int, []),
     "llsa_last_error_string": (C.c_char_p, []),
@@ -120,11 +132,21 @@ _SIGNATURES = {
     "llsa_fine_chunk_for": (c_int, [c_int, c_int, c_int, c_int]),
     "llsa_attn_bwd_workspace_bytes": (c_int64, [c_int, c_int, c_int, C.POINTER(c_int32), c_int]),
     "llsa_attn_bwd": (c_int, [C.POINTER(AttnBwdArgs), c_void_p]),
+    "llsa_layer_norm_fwd": (c_int, [C.POINTER(LayerNormArgs), c_void_p]),
+    "llsa_layer_norm_bwd": (c_int, [C.POINTER(LayerNormArgs), c_void_p]),
+    "llsa_layer_norm_bwd_workspace_bytes": (c_int64, [c_int64, c_int64, c_int]),
+    "llsa_linear_fwd": (c_int, [C.POINTER(LinearArgs), c_void_p]),
+    "llsa_linear_dz": (c_int, [C.POINTER(LinearArgs), c_void_p]),
+    "llsa_linear_dx": (c_int, [C.POINTER(LinearArgs), c_void_p]),
+    "llsa_linear_dw": (c_int, [C.POINTER(LinearArgs), c_void_p]),
+    "llsa_linear_dw_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
+    "llsa_linear_dz_workspace_bytes": (c_int64, [c_int64, c_int64, c_int]),
+    "llsa_pad_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
 }
 
 EXPORTS = tuple(_SIGNATURES)
 CHUNK_FINE_MAX = 256                                        # LLSA_CHUNK_FINE_MAX of include/llsa_hip.h
-ABI_VERSION = 213                                           # LLSA_ABI_VERSION
+ABI_VERSION = 214                                           # LLSA_ABI_VERSION
 STATIC_PARTIALS_MAX = 262144                                # LLSA_STATIC_PARTIALS_MAX
 
 

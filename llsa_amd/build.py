@@ -69,15 +69,22 @@ def build_host() -> str:
     tmp = out + ".tmp"
     inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
            os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), sysconfig.get_paths()["include"]]
-    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f for d in inc for f in ("-isystem", d)), os.path.join(CSRC, "host", "operators.cpp"), "-o", tmp,
-           "-L" + os.path.join(base, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lamdhip64"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("host module:\n" + r.stderr)
-    if r.stderr.strip():
-        print(r.stderr, file=sys.stderr)
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f for d in inc for f in ("-isystem", d))]
+
+    def run(cmd):
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("host module:\n" + r.stderr)
+        if r.stderr.strip():
+            print(r.stderr, file=sys.stderr)
+
+    host = os.path.join(CSRC, "host")
+    srcs = sorted(f for f in os.listdir(host) if f.endswith(".cpp"))
+    objs = [os.path.join(OBJDIR, "host_" + f.replace(".cpp", ".o")) for f in srcs]
+    with cf.ThreadPoolExecutor(max_workers=len(srcs)) as ex:
+        list(ex.map(lambda f, o: run([CXX, *flags, "-c", os.path.join(host, f), "-o", o]), srcs, objs))
+    run([CXX, "-shared", *objs, "-o", tmp, "-L" + os.path.join(base, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lamdhip64"])
     os.replace(tmp, out)
     return out
 

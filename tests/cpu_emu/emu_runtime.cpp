@@ -33,6 +33,7 @@ struct WaveSync {
     uint32_t stage[kWave];
     const void* ptr[kWave];
     bf16x8_t a[kWave], b[kWave];
+    f16x8_t ha[kWave], hb[kWave];
 };
 std::vector<WaveSync> waves;
 
@@ -109,11 +110,11 @@ uint64_t ballot(bool pred) {
 
 // D = A(16x32) * B(32x16) + C.  Lane l holds A[row l%16][k = 8*(l/16) + e], B[k = 8*(l/16) + e][col l%16]
 // and D[row 4*(l/16) + e][col l%16].
-f32x4_t mfma_16x16x32_bf16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
-    WaveSync& ws = waves[cur / kWave];
-    int l = cur % kWave;
-    ws.a[l] = a;
-    ws.b[l] = b;
+template <typename V>
+f32x4_t mfma_16x16x32(V (&wa)[kWave], V (&wb)[kWave], V a, V b, f32x4_t c) {
+    const int l = cur % kWave;
+    wa[l] = a;
+    wb[l] = b;
     wave_barrier();
     int col = l % 16;
     f32x4_t d = c;
@@ -121,14 +122,22 @@ f32x4_t mfma_16x16x32_bf16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
         int row = 4 * (l / 16) + e;
         float s = 0.f;
         for (int k = 0; k < 32; k++) {
-            float av = (float)ws.a[row + 16 * (k / 8)][k % 8];
-            float bv = (float)ws.b[col + 16 * (k / 8)][k % 8];
+            float av = (float)wa[row + 16 * (k / 8)][k % 8];
+            float bv = (float)wb[col + 16 * (k / 8)][k % 8];
             s += av * bv;
         }
         d[e] += s;
     }
     wave_barrier();
     return d;
+}
+f32x4_t mfma_16x16x32_bf16(bf16x8_t a, bf16x8_t b, f32x4_t c) {
+    WaveSync& ws = waves[cur / kWave];
+    return mfma_16x16x32(ws.a, ws.b, a, b, c);
+}
+f32x4_t mfma_16x16x32_f16(f16x8_t a, f16x8_t b, f32x4_t c) {
+    WaveSync& ws = waves[cur / kWave];
+    return mfma_16x16x32(ws.ha, ws.hb, a, b, c);
 }
 
 // ds_read_b64_tr_b16: in each group of 16 lanes, lane i gets element i%4 of the 8-byte chunks
