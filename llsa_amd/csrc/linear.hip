@@ -32,28 +32,38 @@ __device__ __forceinline__ f32x4 product16(f16x8 a, f16x8 b, f32x4 c) { return _
 // ---------------------------------------------------------------------------------------
 constexpr float kGeluC = 0.7978845608028654f, kGeluA = 0.044715f, kRsqrt2 = 0.7071067811865476f, kRsqrt2Pi = 0.3989422804014327f;
 
-__device__ __forceinline__ float logistic(float u) { return __builtin_amdgcn_rcpf(1.f + exp2_fast(-kLog2e * u)); }
+// e^u and 1 / (1 + e^-u) with the hardware's exponential and reciprocal, one step off each
+__device__ __forceinline__ float logistic2(float u) { return __builtin_amdgcn_rcpf(1.f + exp2_fast(-u)); }      // of u ln 2
+// 0.5 erfc(-z / sqrt 2), by the rational approximation 7.1.26 of Abramowitz and Stegun (absolute error 1.5e-7)
+__device__ __forceinline__ float normal_cdf(float z) {
+    const float x = fabsf(z) * kRsqrt2, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * p * exp2_fast(-0.5f * kLog2e * z * z);
+    return z > 0.f ? 1.f - tail : tail;
+}
+constexpr float kTanh1 = 2.f * kGeluC * kLog2e, kTanh3 = kTanh1 * kGeluA;     // 2 u log2 e = z (kTanh1 + kTanh3 z^2)
+
 __device__ __forceinline__ float activate(int act, float z) {
     switch (act) {
-        case LLSA_ACT_SILU: return z * logistic(z);
-        case LLSA_ACT_GELU: return 0.5f * z * erfcf(-z * kRsqrt2);
-        case LLSA_ACT_GELU_TANH: return z * logistic(2.f * kGeluC * (z + kGeluA * z * z * z));
+        case LLSA_ACT_SILU: return z * logistic2(kLog2e * z);
+        case LLSA_ACT_GELU: return z * normal_cdf(z);
+        case LLSA_ACT_GELU_TANH: return z * logistic2(z * fmaf(kTanh3, z * z, kTanh1));
         default: return z;
     }
 }
 __device__ __forceinline__ float activate_slope(int act, float z) {
+    if (act == LLSA_ACT_NONE) return 1.f;
     z = z > 16.f ? 16.f : z < -16.f ? -16.f : z;              // (a NaN stays one)
     switch (act) {
         case LLSA_ACT_SILU: {
-            const float s = logistic(z);
-            return s * (1.f + z * (1.f - s));
+            const float s = logistic2(kLog2e * z);
+            return fmaf(z * s, 1.f - s, s);
         }
-        case LLSA_ACT_GELU: return 0.5f * erfcf(-z * kRsqrt2) + z * kRsqrt2Pi * exp2_fast(-0.5f * kLog2e * z * z);
-        case LLSA_ACT_GELU_TANH: {
-            const float s = logistic(2.f * kGeluC * (z + kGeluA * z * z * z));
-            return s * (1.f + 2.f * kGeluC * z * (1.f - s) * (1.f + 3.f * kGeluA * z * z));
+        case LLSA_ACT_GELU: return fmaf(z * kRsqrt2Pi, exp2_fast(-0.5f * kLog2e * z * z), normal_cdf(z));
+        default: {
+            const float q = z * z, s = logistic2(z * fmaf(kTanh3, q, kTanh1));
+            return fmaf(z * fmaf(6.f * kGeluC * kGeluA, q, 2.f * kGeluC) * s, 1.f - s, s);
         }
-        default: return 1.f;
     }
 }
 
@@ -62,8 +72,7 @@ __device__ __forceinline__ float activate_slope(int act, float z) {
 //
 // A step takes 64 of the contraction.  Copies go straight into LDS, 16 bytes a lane and 1 KB an instruction, so a tile's layout is
 // the order of its source pieces; it is the source address that is permuted, never the place in LDS.
-//   rows     ROWS rows of 64 elements (128 bytes).  Piece p (8 elements) of row r holds the row's piece p ^ ((r >> 1) & 7): the 16 rows a
-//            fragment read touches then lie in 16 different 16-byte columns of the 256 bytes that all banks hold.
+//   rows     ROWS rows of 64 elements.  Piece p (8 elements) of row r holds the row's piece p ^ ((r >> 1) & 7): the 16 rows a fragment read touches then lie in 16 different 16-byte columns of the 256 bytes that all banks hold.
 //   columns  64 rows of ROWS elements.  32-byte granule g of row k holds the row's granule g ^ f(k), f out of bits 0, 1 and 3 of k
 //            (ROWS = 64: 1 and 3): the transposing read takes granules of 4 neighbouring rows in each group of 16 lanes and of
 //            rows 8 further in the next, which then lie in different banks.
@@ -77,41 +86,43 @@ __device__ __forceinline__ void copy_to_lds(const T* g_lane, T* lds_wave_base) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g_lane, (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
 }
 
-template <typename T, bool COLUMNS, int ROWS>
+template <typename T, bool COLUMNS, int ROWS, int WAVES>
 struct Operand {
-    static constexpr int kCopies = ROWS * kStep / 512 / 4;    // instructions of a wave for one step
+    static constexpr int kCopies = ROWS * kStep / 512 / WAVES; // instructions of a wave for one step
     static constexpr int kPerRow = ROWS / 8;                  // columns: 16-byte pieces of a row
-    static constexpr int kMaskG = ROWS == 64 ? 3 : 7;
+    static constexpr int kPieces = kStep / 8;                  // rows: pieces of a row
+    static_assert(kCopies * 512 * WAVES == ROWS * kStep, "a step is whole copies of every wave");
     unsigned off[kCopies];                                    // elements from the step's first, of this lane's pieces
-    int place[kCopies];                                       // along the contraction
 
+    static __device__ __forceinline__ int swap(int r) { return (r >> 1) & 7; }
     static __device__ __forceinline__ int turn(int k) { return ROWS == 64 ? ((k >> 1) & 1) | ((k >> 3) & 1) << 1 : (k & 3) | ((k >> 3) & 1) << 2; }
+    // of the lane's j-th piece: its row and its first element along the row, in the tile
+    static __device__ __forceinline__ int row_of(int i, int lane) { return COLUMNS ? i * (512 / ROWS) + lane / kPerRow : i * (64 / kPieces) + lane / kPieces; }
+    static __device__ __forceinline__ int place_of(int row, int lane) {
+        if (!COLUMNS) return ((lane % kPieces) ^ swap(row)) * 8;
+        const int unit = lane % kPerRow;
+        return (((unit >> 1) ^ turn(row)) * 2 + (unit & 1)) * 8;
+    }
 
     // left: rows (columns: elements of a row, a multiple of 8) from the tile's first to the matrix's last
     __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int left) {
 #pragma unroll
         for (int j = 0; j < kCopies; j++) {
-            const int i = wave * kCopies + j;
-            if constexpr (COLUMNS) {
-                const int k = i * (64 / kPerRow) + lane / kPerRow, unit = lane % kPerRow;
-                const int col = (((unit >> 1) ^ turn(k)) * 2 + (unit & 1)) * 8;
-                place[j] = k;
-                off[j] = (unsigned)(k * ld) + (unsigned)min(col, left - 8);
-            } else {
-                const int r = i * 8 + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
-                place[j] = piece * 8;
-                off[j] = (unsigned)(min(r, left - 1) * ld) + (unsigned)(piece * 8);
-            }
+            const int r = row_of(wave * kCopies + j, lane), e = place_of(r, lane);
+            off[j] = COLUMNS ? (unsigned)(r * ld) + (unsigned)min(e, left - 8) : (unsigned)(min(r, left - 1) * ld) + (unsigned)e;
         }
     }
     // k_left: what is left of the contraction from this step on
-    __device__ __forceinline__ void request(const T* base, T* tile, int wave, int k_left) const {
+    __device__ __forceinline__ void request(const T* base, T* tile, int wave, int lane, int k_left) const {
         if (k_left >= kStep) {
 #pragma unroll
             for (int j = 0; j < kCopies; j++) copy_to_lds(base + off[j], tile + (wave * kCopies + j) * 512);
         } else {
 #pragma unroll
-            for (int j = 0; j < kCopies; j++) copy_to_lds(place[j] < k_left ? base + off[j] : reinterpret_cast<const T*>(kZeros), tile + (wave * kCopies + j) * 512);
+            for (int j = 0; j < kCopies; j++) {
+                const int r = row_of(wave * kCopies + j, lane), k = COLUMNS ? r : place_of(r, lane);
+                copy_to_lds(k < k_left ? base + off[j] : reinterpret_cast<const T*>(kZeros), tile + (wave * kCopies + j) * 512);
+            }
         }
     }
     // the fragment of the 16 rows from `row` on (a multiple of 16), half `ks` of the step: lane l gets row l%16, contraction 32 ks + 8 (l/16) .. +7
@@ -123,7 +134,7 @@ struct Operand {
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * ROWS));
             return __builtin_shufflevector(__builtin_bit_cast(vec4<T>, lo), __builtin_bit_cast(vec4<T>, hi), 0, 1, 2, 3, 4, 5, 6, 7);
         } else {
-            const int r = row + (lane & 15), piece = (4 * ks + (lane >> 4)) ^ ((lane >> 1) & 7);
+            const int r = row + (lane & 15), piece = (4 * ks + (lane >> 4)) ^ swap(lane & 15);
             return *reinterpret_cast<const vec8<T>*>(tile + r * kStep + piece * 8);
         }
     }
@@ -153,10 +164,19 @@ struct Product {
     int64_t ld_part;
 };
 
-// Workgroups go round the eight XCDs: each gets a run of consecutive tiles, which share rows of x and y in its L2.
+// Workgroups go round the eight XCDs: each XCD gets a run of consecutive tiles, which share rows of x and y in its L2.
 __device__ __forceinline__ int xcd_order(int id, int total) {
     const int xcd = id & 7, q = total >> 3, r = total & 7;
     return xcd * q + min(xcd, r) + (id >> 3);
+}
+struct Place { int m0, n0, split, tn; };
+template <int BM, int BN, typename P>
+__device__ __forceinline__ Place place_of_tile(const P& a, int at) {
+    const int per_split = a.tiles_m * a.tiles_n, split = at / per_split, tile = at - split * per_split;
+    const int in_group = a.group * a.tiles_n, g = tile / in_group, rest = tile - g * in_group;
+    const int rows_here = min(a.group, a.tiles_m - g * a.group);
+    const int tn = rest / rows_here, tm = g * a.group + rest - tn * rows_here;
+    return {tm * BM, tn * BN, split, tn};
 }
 
 template <typename T>
@@ -169,6 +189,15 @@ __device__ __forceinline__ void load8(float (&v)[8], const T* p, bool wide, int 
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = e < n ? (float)p[e] : 0.f;
     }
+}
+// the same as they are; zeros of no memory
+template <typename T>
+__device__ __forceinline__ vec8<T> take8(const T* p, bool wide, int n) {
+    vec8<T> v;
+    if (p != nullptr && wide) return *reinterpret_cast<const vec8<T>*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = p != nullptr && e < n ? p[e] : (T)0.f;
+    return v;
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8], bool wide, int n) {
@@ -184,72 +213,122 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], bool wide, int
     }
 }
 
-// Eight values of one row of C on their way out: columns n .. n + 7 (left of them inside the matrix) of row m
-template <typename T>
-__device__ __forceinline__ void way_out(const Product<T>& a, float (&v)[8], const float (&bias)[8], int64_t m, int sample, int n, int left) {
-    const bool wide = a.wide;
-    if (a.bias != nullptr) {
+// What happens on the way out, as far as the kernel is compiled for it: an activation (its LLSA_ACT_ number), the slope of one, or anything, with
+// rows and vectors of any alignment.  All forms but the last read and write pieces of 16 bytes.
+enum Way { kSlope = 4, kAnything = 8 };
+
+// Where a lane's eight values of one row of C lie in the tensors of the way out.  Uniform parts are kept apart from the lane's (32 bits, the same for
+// all rows of its tile), so that one register a tensor addresses them all.
+struct Lane { unsigned out, z, residual; };
+
+// Eight values on their way out: columns n .. n + 7 of row m, `left` of them inside the matrix; row and col are the uniform parts of m and n.  Returns
+// what out gets, and in z what the backward wants of it.
+template <int WAY, typename T>
+__device__ __forceinline__ vec8<T> way_out(const Product<T>& a, float (&v)[8], const vec8<T>& bias, const vec8<T>& gate, const vec8<T>& early, int64_t row, int col,
+                                           const Lane& at, int left, vec8<T>& z) {
+    constexpr bool any = WAY == kAnything;
+    const bool wide = any ? a.wide : true, slope = any ? a.slope_at != nullptr : WAY >= kSlope;
+    const int act = any ? a.act : WAY & 3;
+    if (!slope) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += bias[e];
-    }
-    if (a.z != nullptr) store8(a.z + m * a.ldz + n, v, true, 8);
-    if (a.act != LLSA_ACT_NONE) {
-        if (a.slope_at != nullptr) {
-            float z[8];
-            load8(z, a.slope_at + m * a.ldz + n, true, 8);
+        for (int e = 0; e < 8; e++) v[e] += (float)bias[e];
+        if (a.z != nullptr) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] *= activate_slope(a.act, z[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = activate(a.act, v[e]);
+            for (int e = 0; e < 8; e++) z[e] = (T)v[e];
         }
     }
-    if (a.gate != nullptr) {
-        float g[8];
-        load8(g, a.gate + sample * a.s_gate + n, wide, left);
+    if (any ? act != LLSA_ACT_NONE : (WAY & 3) != 0) {
+        if (slope) {
+            float at_z[8];
+            if (any) load8(at_z, a.slope_at + (row * a.ldz + col) + at.z, true, 8);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] *= g[e];
+            for (int e = 0; e < 8; e++) v[e] *= activate_slope(act, any ? at_z[e] : (float)early[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = activate(act, v[e]);
+        }
     }
-    if (a.residual != nullptr) {
+    if (!slope && a.gate != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] *= (float)gate[e];
+    }
+    if (!slope && a.residual != nullptr) {
         float r[8];
-        load8(r, a.residual + m * a.ldr + n, wide, left);
+        if (any) load8(r, a.residual + (row * a.ldr + col) + at.residual, wide, left);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += r[e];
+        for (int e = 0; e < 8; e++) v[e] += any ? r[e] : (float)early[e];
     }
-    if (a.wide_out && left < 8) {
+    vec8<T> o;
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = e < left ? v[e] : 0.f;
-    }
-    store8(a.out + m * a.ldo + n, v, a.wide_out, left);
+    for (int e = 0; e < 8; e++) o[e] = (T)(any && e >= left ? 0.f : v[e]);
+    return o;
 }
 
-template <typename T, bool XC, bool YC, int BM, int BN>
-__global__ __launch_bounds__(256, 2) void product_kernel(const Product<T> a) {
-    constexpr int WM = BM / 2, WN = BN / 2, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
+// The value of lane l ^ 8
+__device__ __forceinline__ u32x4 from_other_half(u32x4 v) {
+    u32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; e++) r[e] = __float_as_uint(across<8>(__uint_as_float(v[e])));
+    return r;
+}
+// Two pieces of sixteen rows, 64 bytes of each row in either, stored as eight whole lines of 128 bytes twice: lanes l and l ^ 8 exchange a piece, so that
+// the first store takes rows 0 .. 7 and the second rows 8 .. 15.  lane_at: elements from `base` to the lane's first piece; the other one is 32 elements further.
+template <typename T>
+__device__ __forceinline__ void store_lines(T* base, unsigned lane_at, unsigned ld8, const vec8<T>& first, const vec8<T>& second, int lane) {
+    const bool upper = lane & 8;
+    const u32x4 f = __builtin_bit_cast(u32x4, first), s = __builtin_bit_cast(u32x4, second), theirs = from_other_half(upper ? f : s);
+    const u32x4 low = upper ? theirs : f, high = upper ? s : theirs;
+    T* const to = base + (upper ? lane_at - ld8 + 32 : lane_at);
+    __builtin_nontemporal_store(low, reinterpret_cast<u32x4*>(to));
+    __builtin_nontemporal_store(high, reinterpret_cast<u32x4*>(to + ld8));
+}
+// The same pieces read: requested as lines, and once they are there put back where the lanes want them
+template <typename T>
+__device__ __forceinline__ void request_lines(vec8<T>& low, vec8<T>& high, const T* base, unsigned lane_at, unsigned ld8, int lane) {
+    const T* const from = base + ((lane & 8) ? lane_at - ld8 + 32 : lane_at);
+    low = __builtin_nontemporal_load(reinterpret_cast<const vec8<T>*>(from));
+    high = __builtin_nontemporal_load(reinterpret_cast<const vec8<T>*>(from + ld8));
+}
+template <typename T>
+__device__ __forceinline__ void arrange_lines(vec8<T>& first, vec8<T>& second, int lane) {
+    const bool upper = lane & 8;
+    const u32x4 low = __builtin_bit_cast(u32x4, first), high = __builtin_bit_cast(u32x4, second), theirs = from_other_half(upper ? low : high);
+    first = __builtin_bit_cast(vec8<T>, upper ? theirs : low);
+    second = __builtin_bit_cast(vec8<T>, upper ? high : theirs);
+}
+
+template <typename T, bool XC, bool YC, int BM, int BN, int WAVES_M, int WAVES_N, int WAY>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(const Product<T> a) {
+    constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
+    typedef Operand<T, XC, BM, kWaves> OperandX;
+    typedef Operand<T, YC, BN, kWaves> OperandY;
     HIP_DYNAMIC_SHARED(char, shared)
     T* const lds = reinterpret_cast<T*>(shared);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int quad = lane >> 4;
+    const int quad = lane >> 4, wm = (wave % WAVES_M) * WM, wn = (wave / WAVES_M) * WN;
 
-    const int per_split = a.tiles_m * a.tiles_n;
-    const int at = xcd_order((int)blockIdx.x, (int)gridDim.x);
-    const int split = at / per_split, tile = at - split * per_split;
-    const int in_group = a.group * a.tiles_n, g = tile / in_group, rest = tile - g * in_group;
-    const int rows_here = min(a.group, a.tiles_m - g * a.group);
-    const int tn = rest / rows_here, tm = g * a.group + rest - tn * rows_here;
-    const int m0 = tm * BM, n0 = tn * BN;
-    const int64_t k0 = (int64_t)split * a.k_per_split, k1 = min(a.K, k0 + a.k_per_split);
-
-    Operand<T, XC, BM> ox;
-    Operand<T, YC, BN> oy;
-    ox.init(wave, lane, a.ldx, min(BM, (XC ? a.nx : a.M) - m0));
-    oy.init(wave, lane, a.ldy, min(BN, (YC ? a.ny : a.N) - n0));
-    const T* px = a.x + (XC ? k0 * a.ldx + m0 : (int64_t)m0 * a.ldx + k0);
-    const T* py = a.y + (YC ? k0 * a.ldy + n0 : (int64_t)n0 * a.ldy + k0);
+    const Place here = place_of_tile<BM, BN>(a, xcd_order((int)blockIdx.x, (int)gridDim.x));
+    const int64_t k0 = (int64_t)here.split * a.k_per_split;
+    int64_t k_left = min(a.K, k0 + a.k_per_split) - k0;
+    const int steps = (int)((k_left + kStep - 1) / kStep);
+    OperandX ox;
+    OperandY oy;
+    ox.init(wave, lane, a.ldx, min(BM, (XC ? a.nx : a.M) - here.m0));
+    oy.init(wave, lane, a.ldy, min(BN, (YC ? a.ny : a.N) - here.n0));
+    const T* px = a.x + (XC ? k0 * a.ldx + here.m0 : (int64_t)here.m0 * a.ldx + k0);
+    const T* py = a.y + (YC ? k0 * a.ldy + here.n0 : (int64_t)here.n0 * a.ldy + k0);
     const int64_t stepx = XC ? kStep * a.ldx : kStep, stepy = YC ? kStep * a.ldy : kStep;
+    auto request = [&](int buffer) {
+        T* const t = lds + buffer * (kTileX + kTileY);
+        const int left = (int)min(k_left, (int64_t)kStep);
+        ox.request(px, t, wave, lane, left);
+        oy.request(py, t + kTileX, wave, lane, left);
+        px += stepx;
+        py += stepy;
+        k_left -= kStep;
+    };
 
-    const int wm = (wave & 1) * WM, wn = (wave >> 1) * WN;
-    const bool sums = XC && a.part_sum != nullptr && tn == 0 && wn == 0;
+    const bool sums = XC && a.part_sum != nullptr && here.tn == 0 && wn == 0;
     f32x4 acc[NT][MT], sum[XC ? MT : 1];
 #pragma unroll
     for (int i = 0; i < NT; i++)
@@ -260,32 +339,16 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const Product<T> a) {
     vec8<T> ones;
 #pragma unroll
     for (int e = 0; e < 8; e++) ones[e] = (T)1.f;
-
-    const int steps = (int)((k1 - k0 + kStep - 1) / kStep);
-    int64_t k_left = k1 - k0;
-    auto request = [&](int buffer) {
-        T* const t = lds + buffer * (kTileX + kTileY);
-        const int left = (int)min(k_left, (int64_t)kStep);
-        ox.request(px, t, wave, left);
-        oy.request(py, t + kTileX, wave, left);
-        px += stepx;
-        py += stepy;
-        k_left -= kStep;
-    };
-    request(0);
-    for (int s = 0; s < steps; s++) {
-        wait_vm0();
-        __syncthreads();                                      // everyone's copies of this step are there, and everyone is done with the other buffer
-        if (s + 1 < steps) request((s + 1) & 1);
-        const T* const tx = lds + (s & 1) * (kTileX + kTileY);
+    auto multiply = [&](int buffer) {
+        const T* const tx = lds + buffer * (kTileX + kTileY);
         const T* const ty = tx + kTileX;
 #pragma unroll
-        for (int ks = 0; ks < 2; ks++) {
+        for (int ks = 0; ks < kStep / 32; ks++) {
             vec8<T> fx[MT], fy[NT];
 #pragma unroll
-            for (int j = 0; j < MT; j++) fx[j] = Operand<T, XC, BM>::fragment(tx, wm + 16 * j, ks, lane);
+            for (int j = 0; j < MT; j++) fx[j] = OperandX::fragment(tx, wm + 16 * j, ks, lane);
 #pragma unroll
-            for (int i = 0; i < NT; i++) fy[i] = Operand<T, YC, BN>::fragment(ty, wn + 16 * i, ks, lane);
+            for (int i = 0; i < NT; i++) fy[i] = OperandY::fragment(ty, wn + 16 * i, ks, lane);
 #pragma unroll
             for (int i = 0; i < NT; i++)
 #pragma unroll
@@ -297,44 +360,119 @@ __global__ __launch_bounds__(256, 2) void product_kernel(const Product<T> a) {
                 }
             }
         }
-    }
+    };
 
-    int sample[MT];
-#pragma unroll
-    for (int j = 0; j < MT; j++) sample[j] = !XC && a.gate != nullptr ? (m0 + wm + 16 * j + (lane & 15)) / a.per_sample : 0;
     // Lane l holds rows n of four: columns 4 (l/16) .. +3 of every 16, of row l%16 of C.  Swapped between sixteens of lanes, a pair of tiles gives it
     // eight neighbouring ones, so that everything on the way out is read and written in pieces of 16 bytes.
+    const int lane_row = lane & 15, lane_col = 16 * (quad & 1) + 8 * (quad >> 1);
+    const int row0 = here.m0 + wm, col0 = here.n0 + wn, rows_left = a.M - row0 - lane_row, cols_left = a.N - col0 - lane_col;
+    const Lane at = {(unsigned)(lane_row * a.ldo) + lane_col, (unsigned)(lane_row * a.ldz) + lane_col, (unsigned)(lane_row * a.ldr) + lane_col};
+    const T* const side = WAY == kAnything || XC || (YC && WAY < kSlope) ? nullptr : WAY >= kSlope ? a.slope_at : a.residual;
+    constexpr int kPair = NT % 4 == 0 && !XC ? 2 : 1;     // pieces of 32 columns that leave together
+    const bool whole = kPair == 2 && here.m0 + BM <= a.M && here.n0 + BN <= a.N && (WAY != kAnything || a.wide_out);
+    vec8<T> early[kPair][MT];                             // what is read on the way out
+    auto read_side = [&](int p0) {
+        if (side == nullptr) return;
+        const int64_t ld = WAY >= kSlope ? a.ldz : a.ldr;
+        const unsigned lane_at = WAY >= kSlope ? at.z : at.residual;
+        if constexpr (kPair == 2) {
+            if (whole) {
 #pragma unroll
-    for (int p = 0; p < NT / 2; p++) {
-        const int n = n0 + wn + 32 * p + 16 * (quad & 1) + 8 * (quad >> 1), left = a.N - n;
-        float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (!XC && a.bias != nullptr && left > 0) load8(bias, a.bias + n, a.wide, left);
-#pragma unroll
-        for (int j = 0; j < MT; j++) {
-            const int m = m0 + wm + 16 * j + (lane & 15);
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const u32x2 w = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[2 * p][j][e]), __float_as_uint(acc[2 * p + 1][j][e]), false, false);
-                v[e] = __uint_as_float(w[0]);
-                v[4 + e] = __uint_as_float(w[1]);
-            }
-            if (m >= a.M || left <= 0) continue;
-            if constexpr (XC) {
-                float* const o = a.part + ((int64_t)split * a.M + m) * a.ld_part + n;
-                *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
-                *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
-            } else {
-                way_out(a, v, bias, m, sample[j], n, left);
+                for (int j = 0; j < MT; j++)
+                    request_lines(early[0][j], early[1][j], side + ((row0 + 16 * j) * ld + (col0 + 32 * p0)), lane_at, (unsigned)(8 * ld), lane);
+                return;
             }
         }
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int h = 0; h < kPair; h++) {
+                const int p = p0 + h;
+                if (16 * j < rows_left && 32 * p < cols_left) early[h][j] = *reinterpret_cast<const vec8<T>*>(side + ((row0 + 16 * j) * ld + (col0 + 32 * p)) + lane_at);
+            }
+    };
+
+    request(0);
+    for (int s = 0; s + 1 < steps; s++) {
+        wait_vm0();
+        __syncthreads();                                      // everyone's copies of this step are there, and everyone is done with the other buffer
+        request((s + 1) & 1);
+        multiply(s & 1);
+    }
+    wait_vm0();
+    __syncthreads();
+    read_side(0);                                             // (on its way during the last step's products)
+    multiply((steps - 1) & 1);
+
+    const bool gated = !XC && !YC && a.gate != nullptr;
+    const int sample = gated ? here.m0 / a.per_sample : 0;
+    const bool one_sample = gated && min(here.m0 + BM, a.M) <= (int64_t)(sample + 1) * a.per_sample;
+#pragma unroll
+    for (int p0 = 0; p0 < NT / 2; p0 += kPair) {
+        constexpr int kPairs = kPair;
+        vec8<T> bias[kPair], gate[kPair];
+#pragma unroll
+        for (int h = 0; h < kPairs; h++) {
+            const int n = col0 + lane_col + 32 * (p0 + h), left = cols_left - 32 * (p0 + h);
+            bias[h] = take8(!XC && a.bias != nullptr && left > 0 ? a.bias + n : nullptr, WAY != kAnything || a.wide, left);
+            gate[h] = take8(one_sample && left > 0 ? a.gate + sample * a.s_gate + n : nullptr, WAY != kAnything || a.wide, left);
+        }
+#pragma unroll
+        for (int j = 0; j < MT; j++) {
+            const int64_t row = row0 + 16 * j;
+            vec8<T> o[kPair], z[kPair];
+            if constexpr (kPair == 2) {
+                if (side != nullptr && whole) arrange_lines<T>(early[0][j], early[1][j], lane);
+            }
+#pragma unroll
+            for (int h = 0; h < kPairs; h++) {
+                const int p = p0 + h, col = col0 + 32 * p, left = cols_left - 32 * p;
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const u32x2 w = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[2 * p][j][e]), __float_as_uint(acc[2 * p + 1][j][e]), false, false);
+                    v[e] = __uint_as_float(w[0]);
+                    v[4 + e] = __uint_as_float(w[1]);
+                }
+                const bool inside = 16 * j < rows_left && left > 0;
+                if constexpr (XC) {
+                    if (!inside) continue;
+                    float* const o = a.part + (((int64_t)here.split * a.M + row) * a.ld_part + col) + at.out;
+                    *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+                    *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+                } else {
+                    if (inside) {
+                        if (gated && !one_sample) gate[h] = take8(a.gate + (int)(row + lane_row) / a.per_sample * a.s_gate + col + lane_col, WAY != kAnything || a.wide, left);
+                        o[h] = way_out<WAY>(a, v, bias[h], gate[h], early[h][j], row, col, at, left, z[h]);
+                    }
+                    if (whole || !inside) continue;
+                    if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (row * a.ldz + col) + at.z) = z[h];
+                    T* const to = a.out + (row * a.ldo + col) + at.out;
+                    if (WAY != kAnything || a.wide_out) {
+                        *reinterpret_cast<vec8<T>*>(to) = o[h];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (e < left) to[e] = o[h][e];
+                    }
+                }
+            }
+            if constexpr (!XC && kPair == 2) {
+                if (whole) {
+                    if (!YC && a.z != nullptr) store_lines(a.z + (row * a.ldz + (col0 + 32 * p0)), at.z, (unsigned)(8 * a.ldz), z[0], z[1], lane);
+                    store_lines(a.out + (row * a.ldo + (col0 + 32 * p0)), at.out, (unsigned)(8 * a.ldo), o[0], o[1], lane);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);            // (rows one after another: all at once do not fit the registers)
+        }
+        if (p0 + kPair < NT / 2) read_side(p0 + kPair);
     }
     if constexpr (XC) {
         if (sums && quad == 0) {
 #pragma unroll
             for (int j = 0; j < MT; j++) {
-                const int m = m0 + wm + 16 * j + lane;
-                if (m < a.M) a.part_sum[(int64_t)split * a.M + m] = sum[j][0];
+                const int m = here.m0 + wm + 16 * j + lane;
+                if (m < a.M) a.part_sum[(int64_t)here.split * a.M + m] = sum[j][0];
             }
         }
     }
@@ -442,21 +580,73 @@ __global__ __launch_bounds__(256) void pad_kernel(const uint16_t* x, int64_t ldx
 constexpr int64_t kMaxGrid = (int64_t(1) << 31) - 1;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-template <typename T, bool XC, bool YC, int BM, int BN>
+constexpr int kCus = 256;
+template <typename T, bool XC, bool YC, int BM, int BN, int WAVES_M, int WAVES_N, int WAY>
 int launch_tiles(Product<T>& a, int splits, hipStream_t stream) {
     const int64_t tm = ceil_div(a.M, BM), tn = ceil_div(a.N, BN);
     if (tm * tn * splits > kMaxGrid) return fail(-1, "linear: too many rows");
     a.tiles_m = (int)tm;
     a.tiles_n = (int)tn;
-    constexpr size_t lds = 2 * (BM + BN) * kStep * sizeof(T);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(product_kernel<T, XC, YC, BM, BN>), dim3((unsigned)(tm * tn * splits)), dim3(256), lds, stream, a);
+    constexpr int lds = 2 * (BM + BN) * kStep * (int)sizeof(T);
+    auto kernel = product_kernel<T, XC, YC, BM, BN, WAVES_M, WAVES_N, WAY>;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return fail(-101, "linear: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn * splits)), dim3(64 * WAVES_M * WAVES_N), lds, stream, a);
     return 0;
+}
+// Which tiles.  Measured (us, forward of M rows, K channels in, N out), 64 x 64 / 128 x 128 / 192 x 128 / 256 x 256:
+//     2048, 1024 > 1024    9.6 / 14.6 / 18.7 / 31        32768, 384 > 1536    68 / 56 / 61 / 61
+//     4096, 1024 > 1024     15 / 15.2 / 19.1 / 32       131072, 384 > 1536     - / 214 / 203 / 220
+//     8192, 1024 > 1024     27 / 20.9 / 25.6 / 33       131072, 1536 > 384     - / 203 / 190 / 235
+//     8192, 2048 > 2048     98 / 70 / 78 / 64             8192, 4096 > 4096    - / 260 / 260 / 226
+// Small tiles keep a grid of few tiles busy, up to four for each CU.  Beyond that it is rounds times the length of one: two workgroups of 128 x 128 or
+// 192 x 128 fit a CU, one of 256 x 256, and a round of these takes 1, 1.42 and (the longer the contraction, the less its ends weigh) 1.75 + 160 / K.
+enum Tiles { k64, k128, k192, k256 };
+Tiles tiles_for(int64_t M, int64_t N, int64_t K) {
+    if (ceil_div(M, 64) * ceil_div(N, 64) <= 4 * kCus) return k64;
+    const auto rounds = [&](int bm, int bn, int slots) { return (double)ceil_div(ceil_div(M, bm) * ceil_div(N, bn), slots); };
+    const double t128 = rounds(128, 128, 2 * kCus), t192 = 1.42 * rounds(192, 128, 2 * kCus), t256 = (1.75 + 160. / (double)K) * rounds(256, 256, kCus);
+    return t256 < std::min(t128, t192) ? k256 : t192 < t128 ? k192 : k128;
+}
+template <typename T, bool XC, bool YC, int WAY>
+int launch_way(Product<T>& a, int splits, hipStream_t stream) {
+    a.group = (int64_t)a.N * a.K <= (1 << 20) || XC ? 1 : 8;  // (rows of tiles that share y while it does not fit the L2 beside them)
+    if constexpr (XC) {
+        if (ceil_div(a.M, 128) * ceil_div(a.N, 128) * splits >= kCus) return launch_tiles<T, XC, YC, 128, 128, 2, 2, WAY>(a, splits, stream);
+        return launch_tiles<T, XC, YC, 64, 64, 2, 2, WAY>(a, splits, stream);
+    } else {
+        switch (tiles_for(a.M, a.N, a.K)) {
+            case k64: return launch_tiles<T, XC, YC, 64, 64, 2, 2, WAY>(a, splits, stream);
+            case k128: return launch_tiles<T, XC, YC, 128, 128, 2, 2, WAY>(a, splits, stream);
+            case k192: return launch_tiles<T, XC, YC, 192, 128, 2, 2, WAY>(a, splits, stream);
+            default: return launch_tiles<T, XC, YC, 256, 256, 2, 4, WAY>(a, splits, stream);
+        }
+    }
 }
 template <typename T, bool XC, bool YC>
 int launch_product(Product<T>& a, int splits, hipStream_t stream) {
-    a.group = (int64_t)a.N * a.K <= (1 << 20) || XC ? 1 : 8;  // (rows of tiles that share y while it does not fit the L2 beside them)
-    if (ceil_div(a.M, 128) * ceil_div(a.N, 128) * splits >= 256) return launch_tiles<T, XC, YC, 128, 128>(a, splits, stream);
-    return launch_tiles<T, XC, YC, 64, 64>(a, splits, stream);
+    if constexpr (XC) {
+        return launch_way<T, XC, YC, 0>(a, splits, stream);
+    } else {
+        if (!a.wide || !a.wide_out) return launch_way<T, XC, YC, kAnything>(a, splits, stream);
+        if constexpr (YC) {
+            switch (a.act) {
+                case LLSA_ACT_SILU: return launch_way<T, XC, YC, kSlope + LLSA_ACT_SILU>(a, splits, stream);
+                case LLSA_ACT_GELU: return launch_way<T, XC, YC, kSlope + LLSA_ACT_GELU>(a, splits, stream);
+                case LLSA_ACT_GELU_TANH: return launch_way<T, XC, YC, kSlope + LLSA_ACT_GELU_TANH>(a, splits, stream);
+                default: return launch_way<T, XC, YC, LLSA_ACT_NONE>(a, splits, stream);
+            }
+        } else {
+            switch (a.act) {
+                case LLSA_ACT_SILU: return launch_way<T, XC, YC, LLSA_ACT_SILU>(a, splits, stream);
+                case LLSA_ACT_GELU: return launch_way<T, XC, YC, LLSA_ACT_GELU>(a, splits, stream);
+                case LLSA_ACT_GELU_TANH: return launch_way<T, XC, YC, LLSA_ACT_GELU_TANH>(a, splits, stream);
+                default: return launch_way<T, XC, YC, LLSA_ACT_NONE>(a, splits, stream);
+            }
+        }
+    }
 }
 
 bool wide8(const void* p, int64_t ld) { return p == nullptr || (aligned16(p) && ld % 8 == 0); }
@@ -505,6 +695,7 @@ int linear_dx(const llsa_linear_args& q, hipStream_t stream) {
     a.M = (int)q.M; a.N = q.K; a.ny = (int)pad8(q.K); a.K = q.N; a.k_per_split = ceil_div(q.N, kStep) * kStep;
     a.out = (T*)q.out; a.ldo = q.ldo;
     a.slope_at = (const T*)q.z; a.ldz = q.ldz; a.act = q.z != nullptr ? q.act : LLSA_ACT_NONE;
+    a.wide = q.K % 8 == 0;
     a.wide_out = (q.K % 8 == 0 && wide8(q.out, q.ldo)) || q.padded;
     if (int rc = launch_product<T, false, true>(a, 1, stream)) return rc;
     return launch_status("linear_dx");
@@ -518,6 +709,7 @@ int linear_dw(const llsa_linear_args& q, hipStream_t stream) {
     a.M = q.N; a.N = q.K; a.K = q.M; a.k_per_split = p.length;
     a.ld_part = pad8(q.K);
     a.part = (float*)q.workspace;
+    a.ldo = a.ld_part;
     a.part_sum = q.dbias != nullptr ? a.part + (int64_t)p.count * a.M * a.ld_part : nullptr;
     if (int rc = launch_product<T, true, true>(a, p.count, stream)) return rc;
     const int64_t threads = (int64_t)a.M * (a.ld_part / 4) + (q.dbias != nullptr ? a.M : 0);
