@@ -377,9 +377,9 @@ int llsa_attn_bwd(const llsa_attn_bwd_args* a, void* stream);
 #define LLSA_ACT_GELU_TANH 3
 typedef struct llsa_linear_args {
     const void* x;          /* (M,K) rows ldx apart: fwd, dw                                           */
-    const void* w;          /* (N,K) rows ldw apart: fwd, dx                                           */
-    const void* bias;       /* (N) or NULL: fwd                                                        */
-    const void* gate;       /* (M/per_sample, N) rows s_gate apart, or NULL: fwd, dz                   */
+    const void* w;          /* (N,K) rows ldw apart: fwd, dx, dw (for dgate), gate_rows                */
+    const void* bias;       /* (N) or NULL: fwd, dw (for dgate)                                        */
+    const void* gate;       /* (M/per_sample, N) rows s_gate apart, or NULL: fwd, dz, dw, gate_rows    */
     const void* residual;   /* (M,N) rows ldr apart, or NULL: fwd                                      */
     void* out;              /* fwd: out (M,N); dx: dx (M,K); dw: dW (N,K); rows ldo apart              */
     void* z;                /* (M,N) rows ldz apart, padded like dz.  fwd: written unless NULL; dz: read
@@ -390,9 +390,10 @@ typedef struct llsa_linear_args {
     const void* dz;         /* (M,N) rows lddz apart, padded to a multiple of 8: dx, dw                */
     void* dz_out;           /* the same, written: dz                                                   */
     void* dbias;            /* (N) or NULL: dw                                                         */
-    void* dgate;            /* (M/per_sample, N) contiguous, or NULL: dz                               */
+    void* dgate;            /* (M/per_sample, N) contiguous, or NULL: dz, dw                           */
     void* workspace;        /* dw, dz: llsa_linear_{dw,dz}_workspace_bytes                             */
     int64_t ldx, ldw, s_gate, ldr, ldo, ldz, lddout, lddz;
+    int64_t s_w;            /* dx: unless 0, every sample has weights of its own, this far apart       */
     int64_t M, per_sample;
     int32_t N, K, act, dtype;
     int32_t padded;         /* fwd, dx: rows of out are padded to a multiple of 8, zeros are written there */
@@ -403,7 +404,12 @@ int llsa_linear_fwd(const llsa_linear_args* a, void* stream);
 int llsa_linear_dz(const llsa_linear_args* a, void* stream);
 int llsa_linear_dx(const llsa_linear_args* a, void* stream);
 int llsa_linear_dw(const llsa_linear_args* a, void* stream);
-int64_t llsa_linear_dw_workspace_bytes(int64_t M, int N, int K);
+/* A gate without an activation can stay out of the rows.  With `gate` set, llsa_linear_dw takes dout itself as dz (its `samples` is then
+ * M / per_sample, else 1) and returns dW and dbias of the gated layer, and dgate unless NULL; llsa_linear_dx takes dout with the gated
+ * weights of every sample, which llsa_linear_gate_rows writes: out (M/per_sample, N, K) = gate * w, rows ldo = K padded to a multiple of 8. */
+#define LLSA_LINEAR_MAX_GATED_SAMPLES 1024
+int llsa_linear_gate_rows(const llsa_linear_args* a, void* stream);
+int64_t llsa_linear_dw_workspace_bytes(int64_t M, int64_t samples, int N, int K);
 int64_t llsa_linear_dz_workspace_bytes(int64_t M, int64_t per_sample, int N);
 /* (rows, cols) of 16-bit elements, rows ldx apart, to rows ldy apart (a multiple of 8, 16-byte aligned), zeros in columns cols .. ldy - 1 */
 int llsa_pad_rows(const void* x, int64_t ldx, void* y, int64_t ldy, int64_t rows, int cols, void* stream);

@@ -86,7 +86,7 @@ class TransposeJob(C.Structure):
 
 class LinearArgs(C.Structure):
     _fields_ = ([(n, c_void_p) for n in ("x", "w", "bias", "gate", "residual", "out", "z", "dout", "dz", "dz_out", "dbias", "dgate", "workspace")]
-                + [(n, c_int64) for n in ("ldx", "ldw", "s_gate", "ldr", "ldo", "ldz", "lddout", "lddz", "M", "per_sample")]
+                + [(n, c_int64) for n in ("ldx", "ldw", "s_gate", "ldr", "ldo", "ldz", "lddout", "lddz", "s_w", "M", "per_sample")]
                 + [(n, c_int32) for n in ("N", "K", "act", "dtype", "padded", "reserved")])
 
 
@@ -139,7 +139,8 @@ _SIGNATURES = {
     "llsa_linear_dz": (c_int, [C.POINTER(LinearArgs), c_void_p]),
     "llsa_linear_dx": (c_int, [C.POINTER(LinearArgs), c_void_p]),
     "llsa_linear_dw": (c_int, [C.POINTER(LinearArgs), c_void_p]),
-    "llsa_linear_dw_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
+    "llsa_linear_gate_rows": (c_int, [C.POINTER(LinearArgs), c_void_p]),
+    "llsa_linear_dw_workspace_bytes": (c_int64, [c_int64, c_int64, c_int, c_int]),
     "llsa_linear_dz_workspace_bytes": (c_int64, [c_int64, c_int64, c_int]),
     "llsa_pad_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
 }

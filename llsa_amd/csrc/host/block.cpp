@@ -320,22 +320,53 @@ Rows layer_dz(const Call& call, const Rows& dout_any, const Tensor& dout, const 
     call.lib().check(call.lib().linear_dz(&a, call.stream()), "linear_dz");
     return dz;
 }
-// dx (rows `out`), multiplied by act'(z) if there is a z
-void layer_dx(const Call& call, const Rows& dz, const Rows& w, const Tensor& out, int64_t ldo, const Tensor& z, int act, int dtype) {
+// Whether the gate of a layer without an activation stays out of the rows in the backward.  It then costs sums and weights of every sample, 12 N K bytes
+// each, in place of passes over its rows: dout and the kept x W^T + b in, dz out, that kept in the forward, 10 T N bytes.
+bool gate_in_weights(int64_t per_sample, int64_t samples, int64_t K) { return per_sample >= 2 * K && samples <= LLSA_LINEAR_MAX_GATED_SAMPLES; }
+// every sample's weights with its gate
+Rows gated_weights(const Call& call, const Rows& w, const Tensor& gate, int64_t samples, int dtype) {
+    Rows r;
+    r.t = call.rows(samples * w.count, w.cols);
+    r.ld = r.t.size(1); r.count = w.count; r.cols = w.cols;
+    llsa_linear_args a{};
+    a.w = w.p(); a.ldw = w.ld; a.gate = gate.data_ptr(); a.s_gate = gate.size(0) > 1 ? gate.stride(0) : 0;
+    a.out = r.p(); a.ldo = r.ld;
+    a.M = samples; a.per_sample = 1; a.N = static_cast<int32_t>(w.count); a.K = static_cast<int32_t>(w.cols); a.dtype = dtype;
+    call.lib().check(call.lib().linear_gate_rows(&a, call.stream()), "linear_gate_rows");
+    return r;
+}
+// dx (rows `out`), multiplied by act'(z) if there is a z.  per_sample: of gated weights, else 0
+void layer_dx(const Call& call, const Rows& dz, const Rows& w, const Tensor& out, int64_t ldo, const Tensor& z, int act, int dtype, int64_t per_sample = 0) {
     llsa_linear_args a{};
     a.dz = dz.p(); a.lddz = dz.ld; a.w = w.p(); a.ldw = w.ld;
     a.out = out.data_ptr(); a.ldo = ldo;
     if (z.defined()) { a.z = z.data_ptr(); a.ldz = z.size(1); a.act = act; a.padded = 1; }
-    a.M = dz.count; a.per_sample = 1; a.N = static_cast<int32_t>(dz.cols); a.K = static_cast<int32_t>(w.cols); a.dtype = dtype;
+    if (per_sample > 0) a.s_w = w.count * w.ld;
+    a.M = dz.count; a.per_sample = std::max<int64_t>(1, per_sample); a.N = static_cast<int32_t>(dz.cols); a.K = static_cast<int32_t>(w.cols); a.dtype = dtype;
     call.lib().check(call.lib().linear_dx(&a, call.stream()), "linear_dx");
 }
-void layer_dw(const Call& call, const Rows& dz, const Rows& x, const Tensor& dw, const Tensor& db, int dtype) {
+// dw and db; with a gate (that stays out of the rows: dz is dout) also dgate, if `dgate` is defined, for which w and bias are needed
+struct Gated {
+    Tensor gate, bias, dgate;
+    Rows w;
+    int64_t per_sample = 1;
+};
+void layer_dw(const Call& call, const Rows& dz, const Rows& x, const Tensor& dw, const Tensor& db, int dtype, const Gated* gated = nullptr) {
     llsa_linear_args a{};
     a.dz = dz.p(); a.lddz = dz.ld; a.x = x.p(); a.ldx = x.ld;
     a.out = dw.data_ptr(); a.ldo = x.cols;
     if (db.defined()) a.dbias = db.data_ptr();
     a.M = dz.count; a.per_sample = 1; a.N = static_cast<int32_t>(dz.cols); a.K = static_cast<int32_t>(x.cols); a.dtype = dtype;
-    const Tensor workspace = call.bytes(call.lib().linear_dw_workspace_bytes(a.M, a.N, a.K));
+    if (gated != nullptr) {
+        a.gate = gated->gate.data_ptr(); a.s_gate = gated->gate.size(0) > 1 ? gated->gate.stride(0) : 0;
+        a.per_sample = gated->per_sample;
+        if (gated->dgate.defined()) {
+            a.dgate = gated->dgate.data_ptr();
+            a.w = gated->w.p(); a.ldw = gated->w.ld;
+            if (gated->bias.defined()) a.bias = gated->bias.data_ptr();
+        }
+    }
+    const Tensor workspace = call.bytes(call.lib().linear_dw_workspace_bytes(a.M, gated != nullptr ? a.M / a.per_sample : 1, a.N, a.K));
     a.workspace = workspace.data_ptr();
     call.lib().check(call.lib().linear_dw(&a, call.stream()), "linear_dw");
 }
@@ -394,7 +425,7 @@ Tensor zeros_like_weight(int64_t n, int64_t k, const Tensor& like) { return at::
 struct LinearBackward : public BlockNode {
     std::vector<int64_t> sizes;
     int64_t rows, per_sample, samples, K, N;
-    bool has_bias, has_gate, has_residual, has_z;
+    bool has_bias, has_gate, has_residual, has_z, gate_out;      // gate_out: the gate stays out of the rows
     int act, dtype;
     std::string name() const override { return "LinearBackward"; }
     variable_list run(const Tensor& grad, const std::vector<Tensor>& saved) override {
@@ -410,15 +441,19 @@ struct LinearBackward : public BlockNode {
             const Tensor z = has_z ? as_kept(saved[3], {rows, pad8(N)}, grad.scalar_type()) : Tensor();
             const Tensor gate = has_gate ? dense_vector(&saved[2]) : Tensor();
             if (want_x || want_w || want_b || want_g) {
-                const Rows dz = layer_dz(call, rows_of(grad), grad, gate, z, per_sample, act, dtype, want_g ? &dg : nullptr);
-                if (want_x) {
-                    const Rows w = call.operand(saved[1]);
-                    layer_dx(call, dz, w, dx, K, Tensor(), act, dtype);
-                }
-                if (want_w || want_b) {
+                const Rows dz = gate_out ? call.operand(grad) : layer_dz(call, rows_of(grad), grad, gate, z, per_sample, act, dtype, want_g ? &dg : nullptr);
+                const Rows w = want_x || (gate_out && want_g) ? call.operand(saved[1]) : Rows();
+                if (want_x) layer_dx(call, dz, gate_out ? gated_weights(call, w, gate, samples, dtype) : w, dx, K, Tensor(), act, dtype, gate_out ? per_sample : 0);
+                if (want_w || want_b || (gate_out && want_g)) {
                     dw = at::empty({N, K}, grad.options());
                     if (want_b) db = at::empty({N}, grad.options());
-                    layer_dw(call, dz, call.operand(saved[0]), dw, db, dtype);
+                    Gated g;
+                    if (gate_out) {
+                        if (want_g) g.dgate = dg = at::empty({samples, N}, grad.options());
+                        g.gate = gate; g.w = w; g.per_sample = per_sample;
+                        g.bias = saved[4].defined() ? dense_vector(&saved[4]) : Tensor();
+                    }
+                    layer_dw(call, dz, call.operand(saved[0]), dw, db, dtype, gate_out ? &g : nullptr);
                 }
             }
         } else {
@@ -428,7 +463,7 @@ struct LinearBackward : public BlockNode {
         }
         variable_list r{dx, want_w ? dw : Tensor()};
         if (has_bias) r.push_back(db);
-        if (has_gate) r.push_back(dg);
+        if (has_gate) r.push_back(want_g ? dg : Tensor());
         if (has_residual) r.push_back(want_r ? grad : Tensor());
         return r;
     }
@@ -447,6 +482,7 @@ Tensor linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, const Ten
     const LayerInputs in = layer_inputs("linear", x_in, gate_p, residual_p, N);
     const bool grad = wants({&x_in, &w_in, bias_p, gate_p, residual_p});
     const bool inner = grad && wants({&x_in, &w_in, bias_p}), gates = grad && wants({gate_p});
+    const bool gate_out = gate_p != nullptr && act == LLSA_ACT_NONE && gate_in_weights(in.per_sample(), in.samples, K);
     std::vector<int64_t> out_sizes = x_in.sizes().vec();
     out_sizes.back() = N;
     Tensor out, z, gate;
@@ -461,7 +497,7 @@ Tensor linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, const Ten
         if (in.rows > 0) {
             x = call.operand(x_in);
             w = call.operand(w_in);
-            if ((act != LLSA_ACT_NONE && inner) || gates) z = call.rows(in.rows, N);
+            if ((act != LLSA_ACT_NONE && inner) || (gates && !gate_out)) z = call.rows(in.rows, N);
             layer_fwd(call, x, w, dense_vector(bias_p), gate, residual_p != nullptr ? rows_of(*residual_p) : Rows(), z, out, N, false, in.per_sample(), act, dtype);
         } else {
             x.t = x_in;
@@ -471,7 +507,7 @@ Tensor linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, const Ten
             node = make_node<LinearBackward>(lib);
             node->sizes = x_in.sizes().vec();
             node->rows = in.rows; node->per_sample = in.per_sample(); node->samples = in.samples; node->K = K; node->N = N;
-            node->has_bias = bias_p != nullptr; node->has_gate = gate_p != nullptr; node->has_residual = residual_p != nullptr; node->has_z = z.defined();
+            node->has_bias = bias_p != nullptr; node->has_gate = gate_p != nullptr; node->has_residual = residual_p != nullptr; node->has_z = z.defined(); node->gate_out = gate_out;
             node->act = act; node->dtype = dtype;
         }
     }
@@ -479,10 +515,11 @@ Tensor linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, const Ten
         node->set_next_edges(torch::autograd::collect_next_edges(present({&x_in, &w_in, bias_p, gate_p, residual_p})));
         torch::autograd::set_history(out, node);
         // (x is needed for the gradient of the weight, the weight for that of x)
-        node->keep(w_in.requires_grad() || wants({bias_p}) ? x_in : Tensor(), x_in);
-        node->keep(x_in.requires_grad() ? w_in : Tensor(), w_in);
+        node->keep(wants({&w_in, bias_p}) || (gates && gate_out) ? x_in : Tensor(), x_in);
+        node->keep(x_in.requires_grad() || (gates && gate_out) ? w_in : Tensor(), w_in);
         node->keep(gate, gate_p != nullptr ? *gate_p : gate);
         node->keep(z, z);
+        node->keep(gates && gate_out && bias_p != nullptr ? *bias_p : Tensor(), bias_p != nullptr ? *bias_p : Tensor());
     }
     return out;
 }
@@ -493,7 +530,7 @@ Tensor linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, const Ten
 struct FeedForwardBackward : public BlockNode {
     std::vector<int64_t> sizes;
     int64_t rows, per_sample, samples, C, F, N;
-    bool has_b1, has_b2, has_gate, has_residual, has_y;
+    bool has_b1, has_b2, has_gate, has_residual, has_y, gate_out;
     int act, dtype;
     std::string name() const override { return "FeedForwardBackward"; }
     variable_list run(const Tensor& grad, const std::vector<Tensor>& saved) override {
@@ -511,20 +548,28 @@ struct FeedForwardBackward : public BlockNode {
             const auto type = grad.scalar_type();
             const Tensor gate = has_gate ? dense_vector(&saved[3]) : Tensor();
             const Tensor y = has_y ? as_kept(saved[6], {rows, pad8(N)}, type) : Tensor();
-            const Rows dz2 = layer_dz(call, rows_of(grad), grad, gate, y, per_sample, LLSA_ACT_NONE, dtype, want_g ? &dg : nullptr);
-            if (outer) {
+            const Rows dz2 = gate_out ? call.operand(grad) : layer_dz(call, rows_of(grad), grad, gate, y, per_sample, LLSA_ACT_NONE, dtype, want_g ? &dg : nullptr);
+            const Rows w2 = inner || (gate_out && want_g) ? call.operand(saved[2]) : Rows();
+            if (outer || (gate_out && want_g)) {
                 Rows h;
                 h.t = as_kept(saved[5], {rows, pad8(F)}, type);
                 h.ld = h.t.size(1); h.count = rows; h.cols = F;
                 dw2 = at::empty({N, F}, o);
                 if (want_b2) db2 = at::empty({N}, o);
-                layer_dw(call, dz2, h, dw2, db2, dtype);
+                Gated g;
+                if (gate_out) {
+                    if (want_g) g.dgate = dg = at::empty({samples, N}, o);
+                    g.gate = gate; g.w = w2; g.per_sample = per_sample;
+                    g.bias = saved[7].defined() ? dense_vector(&saved[7]) : Tensor();
+                }
+                layer_dw(call, dz2, h, dw2, db2, dtype, gate_out ? &g : nullptr);
             }
             if (inner) {
                 Rows dz1;
                 dz1.t = call.rows(rows, F);
                 dz1.ld = dz1.t.size(1); dz1.count = rows; dz1.cols = F;
-                layer_dx(call, dz2, call.operand(saved[2]), dz1.t, dz1.ld, as_kept(saved[4], {rows, pad8(F)}, type), act, dtype);
+                layer_dx(call, dz2, gate_out ? gated_weights(call, w2, gate, samples, dtype) : w2, dz1.t, dz1.ld, as_kept(saved[4], {rows, pad8(F)}, type), act, dtype,
+                         gate_out ? per_sample : 0);
                 if (want_x) layer_dx(call, dz1, call.operand(saved[1]), dx, C, Tensor(), act, dtype);
                 if (want_w1 || want_b1) {
                     dw1 = at::empty({F, C}, o);
@@ -543,7 +588,7 @@ struct FeedForwardBackward : public BlockNode {
         if (has_b1) r.push_back(db1);
         r.push_back(want_w2 ? dw2 : Tensor());
         if (has_b2) r.push_back(db2);
-        if (has_gate) r.push_back(dg);
+        if (has_gate) r.push_back(want_g ? dg : Tensor());
         if (has_residual) r.push_back(want_r ? grad : Tensor());
         return r;
     }
@@ -566,6 +611,7 @@ Tensor feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_in, con
     const LayerInputs in = layer_inputs(what, x_in, gate_p, residual_p, N);
     const bool grad = wants({&x_in, &w1_in, b1, &w2_in, b2, gate_p, residual_p});
     const bool inner = grad && wants({&x_in, &w1_in, b1}), outer = grad && wants({&w2_in, b2}), gates = grad && wants({gate_p});
+    const bool gate_out = gate_p != nullptr && gate_in_weights(in.per_sample(), in.samples, F);
     std::vector<int64_t> out_sizes = x_in.sizes().vec();
     out_sizes.back() = N;
     Tensor out, z, h, y, gate;
@@ -581,7 +627,7 @@ Tensor feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_in, con
             h = call.rows(in.rows, F);
             hidden.t = h; hidden.ld = h.size(1); hidden.count = in.rows; hidden.cols = F;
             if (inner) z = call.rows(in.rows, F);
-            if (gates) y = call.rows(in.rows, N);
+            if (gates && !gate_out) y = call.rows(in.rows, N);
             layer_fwd(call, call.operand(x_in), call.operand(w1_in), dense_vector(b1), Tensor(), Rows(), z, h, hidden.ld, true, 1, act, dtype);
             layer_fwd(call, hidden, call.operand(w2_in), dense_vector(b2), gate, residual_p != nullptr ? rows_of(*residual_p) : Rows(), y, out, N, false, in.per_sample(),
                       LLSA_ACT_NONE, dtype);
@@ -591,7 +637,7 @@ Tensor feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_in, con
             node->sizes = x_in.sizes().vec();
             node->rows = in.rows; node->per_sample = in.per_sample(); node->samples = in.samples; node->C = C; node->F = F; node->N = N;
             node->has_b1 = b1 != nullptr; node->has_b2 = b2 != nullptr; node->has_gate = gate_p != nullptr; node->has_residual = residual_p != nullptr;
-            node->has_y = y.defined();
+            node->has_y = y.defined(); node->gate_out = gate_out;
             node->act = act; node->dtype = dtype;
         }
     }
@@ -600,11 +646,12 @@ Tensor feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_in, con
         torch::autograd::set_history(out, node);
         node->keep(wants({&w1_in, b1}) ? x_in : Tensor(), x_in);
         node->keep(wants({&x_in}) ? w1_in : Tensor(), w1_in);
-        node->keep(inner ? w2_in : Tensor(), w2_in);
+        node->keep(inner || (gates && gate_out) ? w2_in : Tensor(), w2_in);
         node->keep(gate, gate_p != nullptr ? *gate_p : gate);
         node->keep(z, z);
-        node->keep(outer ? h : Tensor(), h);
+        node->keep(outer || (gates && gate_out) ? h : Tensor(), h);
         node->keep(y, y);
+        node->keep(gates && gate_out && b2 != nullptr ? *b2 : Tensor(), b2 != nullptr ? *b2 : Tensor());
     }
     return out;
 }

@@ -106,6 +106,7 @@ struct Library {
     decltype(&llsa_linear_dz) linear_dz;
     decltype(&llsa_linear_dx) linear_dx;
     decltype(&llsa_linear_dw) linear_dw;
+    decltype(&llsa_linear_gate_rows) linear_gate_rows;
     decltype(&llsa_linear_dw_workspace_bytes) linear_dw_workspace_bytes;
     decltype(&llsa_linear_dz_workspace_bytes) linear_dz_workspace_bytes;
     decltype(&llsa_pad_rows) pad_rows;
@@ -137,6 +138,7 @@ struct Library {
         get("llsa_linear_dz", linear_dz);
         get("llsa_linear_dx", linear_dx);
         get("llsa_linear_dw", linear_dw);
+        get("llsa_linear_gate_rows", linear_gate_rows);
         get("llsa_linear_dw_workspace_bytes", linear_dw_workspace_bytes);
         get("llsa_linear_dz_workspace_bytes", linear_dz_workspace_bytes);
         get("llsa_pad_rows", pad_rows);

@@ -7,6 +7,7 @@
 // All three products are one kernel, C[m][n] = sum over k of X[m,k] Y[n,k], whose operands lie in memory either with the contraction
 // along a row ("rows": x and W of the forward, dz of dx) or across the rows ("columns": W of dx, both operands of dW).
 #include <algorithm>
+#include <cmath>
 
 #include "llsa_device.h"
 #include "llsa_host.h"
@@ -150,8 +151,13 @@ struct Product {
     int M, N;                             // rows (token rows, or channels out of dW) and columns of C
     int nx, ny;                           // elements of a row of x / y where it has its columns in C (a multiple of 8)
     int64_t K;                            // contraction
-    int64_t k_per_split;                  // of one piece of it (a multiple of 64)
     int tiles_m, tiles_n, group;          // tiles are taken `group` rows of tiles at a time
+    // dx with weights of its own for each sample: rows and rows of tiles of a sample, elements from one sample's weights to the next's.  Else: one sample.
+    int rows, tiles_rows;
+    int64_t y_sample;
+    // dW: the contraction in pieces, `pieces` of k_piece rows (a multiple of 64) for every k_sample of them.  Else: one piece.
+    int64_t k_piece, k_sample;
+    int pieces;
     // way out
     const T *bias, *gate, *residual, *slope_at;
     int64_t s_gate, ldr, ldz, ldo;
@@ -160,7 +166,7 @@ struct Product {
     int wide;                             // N and the pointers and strides of bias, gate and residual allow 16-byte accesses
     int wide_out;                         // and those of out; or its rows are padded with zeros to a multiple of 8 elements (those of z always are)
     // dW: pieces of the sum
-    float *part, *part_sum;               // [split][M][ld_part], [split][M] or NULL
+    float *part, *part_sum;               // [sample][piece][M][ld_part], [sample][piece][M] or NULL
     int64_t ld_part;
 };
 
@@ -169,14 +175,15 @@ __device__ __forceinline__ int xcd_order(int id, int total) {
     const int xcd = id & 7, q = total >> 3, r = total & 7;
     return xcd * q + min(xcd, r) + (id >> 3);
 }
-struct Place { int m0, n0, split, tn; };
+struct Place { int m0, m_end, n0, split, tn, sample; };
 template <int BM, int BN, typename P>
 __device__ __forceinline__ Place place_of_tile(const P& a, int at) {
     const int per_split = a.tiles_m * a.tiles_n, split = at / per_split, tile = at - split * per_split;
     const int in_group = a.group * a.tiles_n, g = tile / in_group, rest = tile - g * in_group;
     const int rows_here = min(a.group, a.tiles_m - g * a.group);
     const int tn = rest / rows_here, tm = g * a.group + rest - tn * rows_here;
-    return {tm * BM, tn * BN, split, tn};
+    const int sample = tm / a.tiles_rows;
+    return {sample * a.rows + (tm - sample * a.tiles_rows) * BM, (sample + 1) * a.rows, tn * BN, split, tn, sample};
 }
 
 template <typename T>
@@ -308,15 +315,16 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(cons
     const int quad = lane >> 4, wm = (wave % WAVES_M) * WM, wn = (wave / WAVES_M) * WN;
 
     const Place here = place_of_tile<BM, BN>(a, xcd_order((int)blockIdx.x, (int)gridDim.x));
-    const int64_t k0 = (int64_t)here.split * a.k_per_split;
-    int64_t k_left = min(a.K, k0 + a.k_per_split) - k0;
+    const int k_of = here.split / a.pieces;
+    const int64_t k_first = (int64_t)(here.split - k_of * a.pieces) * a.k_piece, k0 = k_of * a.k_sample + k_first;
+    int64_t k_left = min(a.k_sample - k_first, a.k_piece);
     const int steps = (int)((k_left + kStep - 1) / kStep);
     OperandX ox;
     OperandY oy;
-    ox.init(wave, lane, a.ldx, min(BM, (XC ? a.nx : a.M) - here.m0));
+    ox.init(wave, lane, a.ldx, min(BM, (XC ? a.nx : here.m_end) - here.m0));
     oy.init(wave, lane, a.ldy, min(BN, (YC ? a.ny : a.N) - here.n0));
     const T* px = a.x + (XC ? k0 * a.ldx + here.m0 : (int64_t)here.m0 * a.ldx + k0);
-    const T* py = a.y + (YC ? k0 * a.ldy + here.n0 : (int64_t)here.n0 * a.ldy + k0);
+    const T* py = a.y + here.sample * a.y_sample + (YC ? k0 * a.ldy + here.n0 : (int64_t)here.n0 * a.ldy + k0);
     const int64_t stepx = XC ? kStep * a.ldx : kStep, stepy = YC ? kStep * a.ldy : kStep;
     auto request = [&](int buffer) {
         T* const t = lds + buffer * (kTileX + kTileY);
@@ -365,11 +373,11 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(cons
     // Lane l holds rows n of four: columns 4 (l/16) .. +3 of every 16, of row l%16 of C.  Swapped between sixteens of lanes, a pair of tiles gives it
     // eight neighbouring ones, so that everything on the way out is read and written in pieces of 16 bytes.
     const int lane_row = lane & 15, lane_col = 16 * (quad & 1) + 8 * (quad >> 1);
-    const int row0 = here.m0 + wm, col0 = here.n0 + wn, rows_left = a.M - row0 - lane_row, cols_left = a.N - col0 - lane_col;
+    const int row0 = here.m0 + wm, col0 = here.n0 + wn, rows_left = here.m_end - row0 - lane_row, cols_left = a.N - col0 - lane_col;
     const Lane at = {(unsigned)(lane_row * a.ldo) + lane_col, (unsigned)(lane_row * a.ldz) + lane_col, (unsigned)(lane_row * a.ldr) + lane_col};
     const T* const side = WAY == kAnything || XC || (YC && WAY < kSlope) ? nullptr : WAY >= kSlope ? a.slope_at : a.residual;
     constexpr int kPair = NT % 4 == 0 && !XC ? 2 : 1;     // pieces of 32 columns that leave together
-    const bool whole = kPair == 2 && here.m0 + BM <= a.M && here.n0 + BN <= a.N && (WAY != kAnything || a.wide_out);
+    const bool whole = kPair == 2 && here.m0 + BM <= here.m_end && here.n0 + BN <= a.N && (WAY != kAnything || a.wide_out);
     vec8<T> early[kPair][MT];                             // what is read on the way out
     auto read_side = [&](int p0) {
         if (side == nullptr) return;
@@ -406,7 +414,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(cons
 
     const bool gated = !XC && !YC && a.gate != nullptr;
     const int sample = gated ? here.m0 / a.per_sample : 0;
-    const bool one_sample = gated && min(here.m0 + BM, a.M) <= (int64_t)(sample + 1) * a.per_sample;
+    const bool one_sample = gated && min(here.m0 + BM, here.m_end) <= (int64_t)(sample + 1) * a.per_sample;
 #pragma unroll
     for (int p0 = 0; p0 < NT / 2; p0 += kPair) {
         constexpr int kPairs = kPair;
@@ -472,7 +480,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(cons
 #pragma unroll
             for (int j = 0; j < MT; j++) {
                 const int m = here.m0 + wm + 16 * j + lane;
-                if (m < a.M) a.part_sum[(int64_t)here.split * a.M + m] = sum[j][0];
+                if (m < here.m_end) a.part_sum[(int64_t)here.split * a.M + m] = sum[j][0];
             }
         }
     }
@@ -497,6 +505,86 @@ __global__ __launch_bounds__(256) void product_join_kernel(const float* part, co
         for (int s = 0; s < splits; s++) v += part_sum[(int64_t)s * M + m];
         sums[m] = (T)v;
     }
+}
+
+// The same for a layer whose gate was left out of the products: G_b = dout^T x of sample b, S_b = sum of its rows of dout, in pieces.
+//     dW = sum over b of gate_b G_b,   db = sum of gate_b S_b,   dgate_b = sum over k of W G_b + bias S_b
+// (the last is sum over the rows of dout (x W^T + bias), without those rows).  A workgroup takes a row of G.
+struct GatedJoin {
+    const float *part, *part_sum;
+    const void *gate, *w, *bias;
+    void *out, *sums, *dgate;
+    int64_t ld_part, s_gate, ldw, ldo;
+    int M, N, samples, pieces;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void gated_join_kernel(const GatedJoin a) {
+    HIP_DYNAMIC_SHARED(float, dots)                           // [wave][sample]
+    const int m = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const T* const gate = static_cast<const T*>(a.gate) + m;
+    const T* const w = static_cast<const T*>(a.w);
+    float* const dot = dots + wave * a.samples;
+    if (a.dgate != nullptr)
+        for (int b = lane; b < a.samples; b += 64) dot[b] = 0.f;
+    for (int first = 0; first < a.N; first += 1024) {         // (the same count for all lanes)
+        const int n = first + threadIdx.x * 4;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f}, wn = {0.f, 0.f, 0.f, 0.f};
+        if (a.dgate != nullptr)
+#pragma unroll
+            for (int e = 0; e < 4; e++) wn[e] = n + e < a.N ? (float)w[m * a.ldw + n + e] : 0.f;
+        for (int b = 0; b < a.samples; b++) {
+            f32x4 g = {0.f, 0.f, 0.f, 0.f};
+            if (n < a.N)
+                for (int p = 0; p < a.pieces; p++) g += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)(b * a.pieces + p) * a.M + m) * a.ld_part + n);
+            v += (float)gate[b * a.s_gate] * g;
+            if (a.dgate != nullptr) {
+                float d = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) d += n + e < a.N ? g[e] * wn[e] : 0.f;
+                d = quad_sum(octet_sum(d));
+                d += across<8>(d);
+                if (lane == 0) dot[b] += d;
+            }
+        }
+        if (a.out != nullptr)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (n + e < a.N) static_cast<T*>(a.out)[m * a.ldo + n + e] = (T)v[e];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    float sum = 0.f;
+    const float bias = a.bias != nullptr ? (float)static_cast<const T*>(a.bias)[m] : 0.f;
+    for (int b = lane; b < a.samples; b += 64) {
+        float s = 0.f;
+        if (a.part_sum != nullptr)
+            for (int p = 0; p < a.pieces; p++) s += a.part_sum[(int64_t)(b * a.pieces + p) * a.M + m];
+        sum += (float)gate[b * a.s_gate] * s;
+        if (a.dgate != nullptr) {
+            float d = bias * s;
+            for (int i = 0; i < 4; i++) d += dots[i * a.samples + b];
+            static_cast<T*>(a.dgate)[(int64_t)b * a.M + m] = (T)d;
+        }
+    }
+    if (a.sums != nullptr) {
+        sum = quad_sum(octet_sum(sum));
+        sum += across<8>(sum);
+        if (lane == 0) static_cast<T*>(a.sums)[m] = (T)sum;
+    }
+}
+
+// The weights of every sample with its gate: gate_b[n] W[n][k].  Rounded to 16 bits, as dout * gate would be: the products take operands of that size.
+template <typename T>
+__global__ __launch_bounds__(256) void gate_rows_kernel(const T* w, int64_t ldw, const T* gate, int64_t s_gate, T* out, int64_t ldo, int N, int64_t pieces) {
+    const int64_t per = ldo / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= pieces) return;
+    const int64_t r = i / per, b = r / N;
+    const int n = (int)(r - b * N), c = (int)(i - r * per) * 8;
+    const float g = (float)gate[b * s_gate + n];
+    vec8<T> v = *reinterpret_cast<const vec8<T>*>(w + n * ldw + c);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = (T)((float)v[e] * g);
+    *reinterpret_cast<vec8<T>*>(out + r * ldo + c) = v;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -583,7 +671,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int kCus = 256;
 template <typename T, bool XC, bool YC, int BM, int BN, int WAVES_M, int WAVES_N, int WAY>
 int launch_tiles(Product<T>& a, int splits, hipStream_t stream) {
-    const int64_t tm = ceil_div(a.M, BM), tn = ceil_div(a.N, BN);
+    a.tiles_rows = (int)ceil_div(a.rows, BM);
+    const int64_t tm = (int64_t)(a.M / a.rows) * a.tiles_rows, tn = ceil_div(a.N, BN);
     if (tm * tn * splits > kMaxGrid) return fail(-1, "linear: too many rows");
     a.tiles_m = (int)tm;
     a.tiles_n = (int)tn;
@@ -606,7 +695,10 @@ int launch_tiles(Product<T>& a, int splits, hipStream_t stream) {
 enum Tiles { k64, k128, k192, k256 };
 Tiles tiles_for(int64_t M, int64_t N, int64_t K) {
     if (ceil_div(M, 64) * ceil_div(N, 64) <= 4 * kCus) return k64;
-    const auto rounds = [&](int bm, int bn, int slots) { return (double)ceil_div(ceil_div(M, bm) * ceil_div(N, bn), slots); };
+    const auto rounds = [&](int bm, int bn, int slots) {      // (many rounds run into one another: only the last one is not full)
+        const double n = (double)(ceil_div(M, bm) * ceil_div(N, bn)) / slots;
+        return n > 8 ? n + 0.5 : std::ceil(n);
+    };
     const double t128 = rounds(128, 128, 2 * kCus), t192 = 1.42 * rounds(192, 128, 2 * kCus), t256 = (1.75 + 160. / (double)K) * rounds(256, 256, kCus);
     return t256 < std::min(t128, t192) ? k256 : t192 < t128 ? k192 : k128;
 }
@@ -651,13 +743,21 @@ int launch_product(Product<T>& a, int splits, hipStream_t stream) {
 
 bool wide8(const void* p, int64_t ld) { return p == nullptr || (aligned16(p) && ld % 8 == 0); }
 
-// The pieces of dW's contraction over the token rows
-struct Pieces { int count; int64_t length; };
-Pieces weight_pieces(int64_t M, int N, int K) {
-    const int64_t tiles = ceil_div(N, 128) * ceil_div(K, 128);
-    int64_t count = std::max<int64_t>(1, std::min(512 / tiles, ceil_div(M, 512)));
-    const int64_t length = ceil_div(ceil_div(M, count), kStep) * kStep;
-    return {(int)ceil_div(M, length), length};
+// The pieces of dW's contraction over the token rows, of which `samples` runs have to be kept apart.  More pieces fill the chip's workgroups more evenly
+// but are more sums to write and read: the products run at about 0.72 PFLOP/s where all workgroups are busy, the sums at 4 TB/s.  131072 rows of 1536 and
+// 384 channels: 14 pieces (504 workgroups of 512) 216 + 7 us; of 8 samples, 1 piece each (288 workgroups) 324 + 15.
+struct Pieces { int samples, pieces; int64_t sample, piece; int count() const { return samples * pieces; } };
+Pieces weight_pieces(int64_t M, int64_t samples, int N, int K) {
+    const int64_t tiles = ceil_div(N, 128) * ceil_div(K, 128), rows = M / samples;
+    const double all = 2. * (double)M * N * K / 0.72e9, sums = 8. * (double)samples * N * K / 4e6;      // us
+    int64_t best = 1;
+    double least = 0;
+    for (int64_t p = 1; p <= std::max<int64_t>(1, rows / 256) && (p - 1) * tiles * samples < 8 * kCus; p++) {
+        const double n = (double)(tiles * samples * p) / (2 * kCus), t = all * std::ceil(n) / n + sums * p;
+        if (p == 1 || t < least) best = p, least = t;
+    }
+    const int64_t length = ceil_div(ceil_div(rows, best), kStep) * kStep;
+    return {(int)samples, (int)ceil_div(rows, length), rows, length};
 }
 int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
@@ -673,11 +773,18 @@ int check_sizes(const char* what, int64_t M, int N, int K, int dtype, int act) {
 }
 
 template <typename T>
+void one_piece(Product<T>& a) {
+    a.rows = a.M;
+    a.k_sample = a.k_piece = a.K;
+    a.pieces = 1;
+}
+template <typename T>
 int linear_fwd(const llsa_linear_args& q, hipStream_t stream) {
     Product<T> a{};
     a.x = (const T*)q.x; a.ldx = q.ldx;
     a.y = (const T*)q.w; a.ldy = q.ldw;
-    a.M = (int)q.M; a.N = q.N; a.K = q.K; a.k_per_split = ceil_div(q.K, kStep) * kStep;
+    a.M = (int)q.M; a.N = q.N; a.K = q.K;
+    one_piece(a);
     a.bias = (const T*)q.bias; a.gate = (const T*)q.gate; a.s_gate = q.s_gate; a.per_sample = (int)q.per_sample;
     a.residual = (const T*)q.residual; a.ldr = q.ldr;
     a.out = (T*)q.out; a.ldo = q.ldo; a.z = (T*)q.z; a.ldz = q.ldz;
@@ -691,8 +798,10 @@ template <typename T>
 int linear_dx(const llsa_linear_args& q, hipStream_t stream) {
     Product<T> a{};
     a.x = (const T*)q.dz; a.ldx = q.lddz;
-    a.y = (const T*)q.w; a.ldy = q.ldw;
-    a.M = (int)q.M; a.N = q.K; a.ny = (int)pad8(q.K); a.K = q.N; a.k_per_split = ceil_div(q.N, kStep) * kStep;
+    a.y = (const T*)q.w; a.ldy = q.ldw; a.y_sample = q.s_w;
+    a.M = (int)q.M; a.N = q.K; a.ny = (int)pad8(q.K); a.K = q.N;
+    one_piece(a);
+    if (q.s_w != 0) a.rows = (int)q.per_sample;
     a.out = (T*)q.out; a.ldo = q.ldo;
     a.slope_at = (const T*)q.z; a.ldz = q.ldz; a.act = q.z != nullptr ? q.act : LLSA_ACT_NONE;
     a.wide = q.K % 8 == 0;
@@ -702,20 +811,38 @@ int linear_dx(const llsa_linear_args& q, hipStream_t stream) {
 }
 template <typename T>
 int linear_dw(const llsa_linear_args& q, hipStream_t stream) {
-    const Pieces p = weight_pieces(q.M, q.N, q.K);
+    const Pieces p = weight_pieces(q.M, q.gate != nullptr ? q.M / q.per_sample : 1, q.N, q.K);
     Product<T> a{};
     a.x = (const T*)q.dz; a.ldx = q.lddz; a.nx = (int)pad8(q.N);
     a.y = (const T*)q.x; a.ldy = q.ldx; a.ny = (int)pad8(q.K);
-    a.M = q.N; a.N = q.K; a.K = q.M; a.k_per_split = p.length;
+    a.M = q.N; a.N = q.K; a.K = q.M;
+    one_piece(a);
+    a.k_sample = p.sample; a.k_piece = p.piece; a.pieces = p.pieces;
     a.ld_part = pad8(q.K);
     a.part = (float*)q.workspace;
     a.ldo = a.ld_part;
-    a.part_sum = q.dbias != nullptr ? a.part + (int64_t)p.count * a.M * a.ld_part : nullptr;
-    if (int rc = launch_product<T, true, true>(a, p.count, stream)) return rc;
-    const int64_t threads = (int64_t)a.M * (a.ld_part / 4) + (q.dbias != nullptr ? a.M : 0);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(product_join_kernel<T>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, stream, a.part, a.part_sum, (T*)q.out, q.ldo,
-                       (T*)q.dbias, a.M, a.N, a.ld_part, p.count);
+    const bool sums = q.dbias != nullptr || (q.dgate != nullptr && q.bias != nullptr);
+    a.part_sum = sums ? a.part + (int64_t)p.count() * a.M * a.ld_part : nullptr;
+    if (int rc = launch_product<T, true, true>(a, p.count(), stream)) return rc;
+    if (q.gate != nullptr) {
+        GatedJoin j{};
+        j.part = a.part; j.part_sum = a.part_sum; j.gate = q.gate; j.s_gate = q.s_gate; j.w = q.w; j.ldw = q.ldw; j.bias = q.bias;
+        j.out = q.out; j.ldo = q.ldo; j.sums = q.dbias; j.dgate = q.dgate;
+        j.ld_part = a.ld_part; j.M = a.M; j.N = a.N; j.samples = p.samples; j.pieces = p.pieces;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_join_kernel<T>), dim3((unsigned)a.M), dim3(256), 4 * 4 * p.samples, stream, j);
+    } else {
+        const int64_t threads = (int64_t)a.M * (a.ld_part / 4) + (q.dbias != nullptr ? a.M : 0);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_join_kernel<T>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, stream, a.part, a.part_sum, (T*)q.out, q.ldo,
+                           (T*)q.dbias, a.M, a.N, a.ld_part, p.count());
+    }
     return launch_status("linear_dw");
+}
+template <typename T>
+int gate_rows(const llsa_linear_args& q, hipStream_t stream) {
+    const int64_t pieces = q.M / q.per_sample * q.N * (q.ldo / 8);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(gate_rows_kernel<T>), dim3((unsigned)ceil_div(pieces, 256)), dim3(256), 0, stream, (const T*)q.w, q.ldw, (const T*)q.gate, q.s_gate, (T*)q.out,
+                       q.ldo, q.N, pieces);
+    return launch_status("linear_gate_rows");
 }
 struct DzPieces { int count, rows; };
 DzPieces dz_pieces(int64_t M, int64_t per_sample, int N) {
@@ -749,9 +876,9 @@ using namespace llsa;
 
 #define BY_TYPE(fn) (a->dtype == LLSA_DTYPE_BF16 ? fn<bf16>(*a, (hipStream_t)stream) : fn<_Float16>(*a, (hipStream_t)stream))
 
-extern "C" int64_t llsa_linear_dw_workspace_bytes(int64_t M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
-    return 4 * (int64_t)weight_pieces(M, N, K).count * N * (pad8(K) + 1);
+extern "C" int64_t llsa_linear_dw_workspace_bytes(int64_t M, int64_t samples, int N, int K) {
+    if (M <= 0 || samples <= 0 || N <= 0 || K <= 0) return 0;
+    return 4 * (int64_t)weight_pieces(M, samples, N, K).count() * N * (pad8(K) + 1);
 }
 extern "C" int64_t llsa_linear_dz_workspace_bytes(int64_t M, int64_t per_sample, int N) {
     if (M <= 0 || N <= 0 || per_sample <= 0) return 0;
@@ -774,6 +901,7 @@ extern "C" int llsa_linear_dx(const llsa_linear_args* a, void* stream) {
     if (a->M == 0) return 0;
     LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->w, a->ldw) && a->lddz >= pad8(a->N) && a->ldw >= pad8(a->K),
                  "linear_dx: rows of dz and w must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->s_w == 0 || (a->s_w % 8 == 0 && a->per_sample > 0 && a->M % a->per_sample == 0), "linear_dx: weights of each sample: whole samples, 16-byte aligned");
     LLSA_REQUIRE(a->out != nullptr && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->K))), "linear_dx: output, padded rows 16-byte aligned and a multiple of 8 long");
     LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->K)), "linear_dx: rows of z must be 16-byte aligned and padded to a multiple of 8");
     return BY_TYPE(linear_dx);
@@ -785,7 +913,19 @@ extern "C" int llsa_linear_dw(const llsa_linear_args* a, void* stream) {
     LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->x, a->ldx) && a->lddz >= pad8(a->N) && a->ldx >= pad8(a->K),
                  "linear_dw: rows of dz and x must be 16-byte aligned and padded to a multiple of 8");
     LLSA_REQUIRE(a->out != nullptr && a->workspace != nullptr && aligned16(a->workspace), "linear_dw: output and workspace (16-byte aligned)");
+    LLSA_REQUIRE(a->gate == nullptr || (a->per_sample > 0 && a->M % a->per_sample == 0 && a->M / a->per_sample <= LLSA_LINEAR_MAX_GATED_SAMPLES),
+                 "linear_dw: a gate needs whole samples, at most %d", LLSA_LINEAR_MAX_GATED_SAMPLES);
+    LLSA_REQUIRE(a->dgate == nullptr || (a->gate != nullptr && a->w != nullptr), "linear_dw: dgate needs the gate and the weight");
     return BY_TYPE(linear_dw);
+}
+extern "C" int llsa_linear_gate_rows(const llsa_linear_args* a, void* stream) {
+    LLSA_REQUIRE(a != nullptr, "linear_gate_rows: no arguments");
+    if (int rc = check_sizes("linear_gate_rows", a->M, a->N, a->K, a->dtype, a->act)) return rc;
+    if (a->M == 0) return 0;
+    LLSA_REQUIRE(a->gate != nullptr && a->per_sample > 0 && a->M % a->per_sample == 0, "linear_gate_rows: gate, whole samples");
+    LLSA_REQUIRE(rows16(a->w, a->ldw) && rows16(a->out, a->ldo) && a->ldo == pad8(a->K) && a->ldw >= a->ldo, "linear_gate_rows: rows 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(ceil_div(a->M / a->per_sample * a->N * (a->ldo / 8), 256) <= kMaxGrid, "linear_gate_rows: too many samples");
+    return BY_TYPE(gate_rows);
 }
 extern "C" int llsa_linear_dz(const llsa_linear_args* a, void* stream) {
     LLSA_REQUIRE(a != nullptr, "linear_dz: no arguments");

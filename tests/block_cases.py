@@ -1,5 +1,6 @@
 """The operators around the attention (layer_norm, linear, feed_forward) against their formulas in 64 bits, with bounds on every element that
-follow from the roundings: u = finfo(dtype).eps / 2 for each value written in 16 bits, and n * 2^-24 times the sum of magnitudes for n additions in fp32."""
+follow from the roundings: u = finfo(dtype).eps / 2 for each value written in 16 bits, and n * 2^-24 times the sum of magnitudes for n additions in fp32.
+Below the smallest normal number a step does not shrink any more: a rounding there is off by up to `least` = finfo(dtype).tiny * u (fp16: 2^-14 * 2^-11 = 2^-25)."""
 import torch
 
 import llsa_amd
@@ -11,6 +12,10 @@ SLOPE, CURVE = 1.2, 1.0                                       # |act'| <= 1.13, 
 
 def half_step(dtype):
     return torch.finfo(dtype).eps / 2
+
+
+def least(dtype):
+    return torch.finfo(dtype).tiny * half_step(dtype)
 
 
 def act64(name, z):
@@ -55,7 +60,7 @@ def check_norm(x, weight, bias, scale, shift, dout, eps=1e-5):
     got = dict(zip([n for n, _ in named], torch.autograd.grad(y, [t for _, t in named], dout)))
     leaf = {n: t.detach().double().cpu().requires_grad_() for n, t in named}
     v = lambda n: leaf.get(n)
-    x64, C, u = leaf["x"], x.shape[-1], half_step(x.dtype)
+    x64, C, u, lo = leaf["x"], x.shape[-1], half_step(x.dtype), least(x.dtype)
     h, n, ref = norm64(x64, v("weight"), v("bias"), v("scale"), v("shift"), eps)
     d64 = dout.double().cpu()
     grads = dict(zip(leaf, torch.autograd.grad(ref, list(leaf.values()), d64)))
@@ -67,11 +72,11 @@ def check_norm(x, weight, bias, scale, shift, dout, eps=1e-5):
         dh = rstd * (c * x64.abs().mean(-1, keepdim=True) + 2 * E * x64.abs()) + 3 * c * h.abs()
         up = (v("weight").abs() if "weight" in leaf else one) * (1 + per_sample(v("scale").abs(), x64) if "scale" in leaf else one)
         add = (v("bias").abs() if "bias" in leaf else 0 * one) * (1 + per_sample(v("scale").abs(), x64) if "scale" in leaf else one)
-        within(y.detach().cpu(), ref, up * dh + 6 * E * (up * h.abs() + add + ref.abs()) + u * ref.abs(), "y")
+        within(y.detach().cpu(), ref, up * dh + 6 * E * (up * h.abs() + add + ref.abs()) + u * ref.abs() + lo, "y")
         g, gh = d64.abs() * up, (d64 * h).abs() * up
         dgh = g * dh
         bound = rstd * (6 * E * g + c * g.mean(-1, keepdim=True) + h.abs() * (c * gh.mean(-1, keepdim=True) + dgh.mean(-1, keepdim=True)) + dh * gh.mean(-1, keepdim=True))
-        within(got["x"].cpu(), grads["x"], bound + (4 * c + u) * grads["x"].abs() + 4 * E * rstd * (g + gh.mean(-1, keepdim=True) * h.abs()), "dx")
+        within(got["x"].cpu(), grads["x"], bound + (4 * c + u) * grads["x"].abs() + 4 * E * rstd * (g + gh.mean(-1, keepdim=True) * h.abs()) + lo, "dx")
         rows = x64.numel() // C
         flat = lambda t: t.reshape(-1, C)
         S1, S2, dS2 = d64.abs(), (d64 * h).abs(), d64.abs() * dh
@@ -79,15 +84,15 @@ def check_norm(x, weight, bias, scale, shift, dout, eps=1e-5):
         scale_up = (1 + per_sample(v("scale").abs(), x64)) if "scale" in leaf else one
         if "weight" in leaf:
             uw = half_step(weight.dtype)
-            within(got["weight"].cpu(), grads["weight"], flat(scale_up * (dS2 + many * S2)).sum(0) + uw * grads["weight"].abs(), "dweight")
+            within(got["weight"].cpu(), grads["weight"], flat(scale_up * (dS2 + many * S2)).sum(0) + uw * grads["weight"].abs() + least(weight.dtype), "dweight")
         if "bias" in leaf:
-            within(got["bias"].cpu(), grads["bias"], flat(scale_up * many * S1).sum(0) + half_step(bias.dtype) * grads["bias"].abs(), "dbias")
+            within(got["bias"].cpu(), grads["bias"], flat(scale_up * many * S1).sum(0) + half_step(bias.dtype) * grads["bias"].abs() + least(bias.dtype), "dbias")
         each = lambda t: t.reshape(t.shape[0], -1, C).sum(1)
         if "scale" in leaf:
             w, b = (v("weight").abs() if "weight" in leaf else one), (v("bias").abs() if "bias" in leaf else 0 * one)
-            within(got["scale"].cpu(), grads["scale"], each(w * (dS2 + many * S2) + b * many * S1) + half_step(scale.dtype) * grads["scale"].abs(), "dscale")
+            within(got["scale"].cpu(), grads["scale"], each(w * (dS2 + many * S2) + b * many * S1) + half_step(scale.dtype) * grads["scale"].abs() + least(scale.dtype), "dscale")
         if "shift" in leaf:
-            within(got["shift"].cpu(), grads["shift"], each(many * S1) + half_step(shift.dtype) * grads["shift"].abs(), "dshift")
+            within(got["shift"].cpu(), grads["shift"], each(many * S1) + half_step(shift.dtype) * grads["shift"].abs() + least(shift.dtype), "dshift")
     return y, got
 
 
@@ -107,11 +112,12 @@ def check_layers(x, layers, gate, residual, dout, call):
     named += [(n, t) for n, t in (("gate", gate), ("residual", residual)) if t is not None]
     named = [(n, t) for n, t in named if t.requires_grad]
     out = call()
-    u = half_step(x.dtype)
+    u, lo = half_step(x.dtype), least(x.dtype)
     got = dict(zip([n for n, _ in named], torch.autograd.grad(out, [t for _, t in named], dout)))
-    c = lambda t: None if t is None else t.detach().double().cpu()
+    where = x.device if x.numel() * layers[0][0].shape[0] > 1 << 26 else torch.device("cpu")
+    c = lambda t: None if t is None else t.detach().double().to(where)
     # forward
-    h, dh, steps = c(x).reshape(-1, x.shape[-1]), torch.zeros(1, dtype=torch.float64), []
+    h, steps = c(x).reshape(-1, x.shape[-1]), []
     dh = torch.zeros_like(h)
     for i, (w, b, act) in enumerate(layers):
         z, dz, a, da = _layer_bounds(h, c(w), c(b), act, dh)
@@ -120,10 +126,10 @@ def check_layers(x, layers, gate, residual, dout, call):
         h, dh = a, da if last else da + u * (a.abs() + da)    # (the hidden rows are rounded, the output is not yet)
     N = layers[-1][0].shape[0]
     T = h.shape[0] // x.shape[0] if gate is not None else 1
-    rep = c(gate).repeat_interleave(T, 0) if gate is not None else torch.ones(1, dtype=torch.float64)
-    res = c(residual).reshape(-1, N) if residual is not None else torch.zeros(1, dtype=torch.float64)
+    rep = c(gate).repeat_interleave(T, 0) if gate is not None else torch.ones(1, dtype=torch.float64, device=where)
+    res = c(residual).reshape(-1, N) if residual is not None else torch.zeros(1, dtype=torch.float64, device=where)
     ref = res + rep * h
-    within(out.detach().cpu().reshape(-1, N), ref, rep.abs() * dh + 4 * E * (res.abs() + (rep * h).abs()) + u * (ref.abs() + rep.abs() * dh), "out")
+    within(out.detach().to(where).reshape(-1, N), ref, rep.abs() * dh + 4 * E * (res.abs() + (rep * h).abs()) + u * (ref.abs() + rep.abs() * dh) + lo, "out")
     # backward
     d = c(dout).reshape(-1, N)
     if residual is not None and residual.requires_grad:
@@ -133,10 +139,10 @@ def check_layers(x, layers, gate, residual, dout, call):
         y, dy = h, dh
         zs = steps[-1]
         # (act(z) is taken of the z that was kept in 16 bits)
-        dy = dy + SLOPE * u * (zs[2].abs() + zs[3]) + FAST * zs[2].abs()
+        dy = dy + SLOPE * (u * (zs[2].abs() + zs[3]) + lo) + FAST * zs[2].abs()
         each = lambda t: t.reshape(x.shape[0], -1, N).sum(1)
         r = each(d * y)
-        within(got["gate"].cpu(), r, each(d.abs() * dy + (T + 32) * E * (d * y).abs()) * (1 + u) + u * r.abs(), "dgate")
+        within(got["gate"].to(where), r, each(d.abs() * dy + (T + 32) * E * (d * y).abs()) * (1 + u) + u * r.abs() + lo, "dgate")
     g, dg = d * rep, E * (d * rep).abs()
     rounded = gate is not None
     for i in range(len(layers) - 1, -1, -1):
@@ -144,23 +150,25 @@ def check_layers(x, layers, gate, residual, dout, call):
         hh, dhh, z, dz, a, da = steps[i]
         if act:
             slope_ref = torch.autograd.functional.jvp(lambda t: act64(act, t), z, torch.ones_like(z))[1]
-            off = CURVE * (dz + u * (z.abs() + dz)) + FAST
+            off = CURVE * (dz + u * (z.abs() + dz) + lo) + FAST
             dg = dg * SLOPE + g.abs() * off
             g = g * slope_ref
             rounded = True
         if rounded:
-            dg = dg + u * (g.abs() + dg)
+            dg = dg + u * (g.abs() + dg) + lo
         more = lambda n: (n + 32) * E
         if f"weight{i}" in got:
             r = g.t() @ hh
             bound = dg.t() @ (hh.abs() + dhh) + g.abs().t() @ dhh + more(M) * (g.abs().t() @ hh.abs())
-            within(got[f"weight{i}"].cpu(), r, bound * (1 + u) + u * r.abs(), f"dweight{i}")
+            within(got[f"weight{i}"].to(where), r, bound * (1 + u) + u * r.abs() + lo, f"dweight{i}")
         if f"bias{i}" in got:
             r = g.sum(0)
-            within(got[f"bias{i}"].cpu(), r, (dg.sum(0) + more(M) * g.abs().sum(0)) * (1 + u) + u * r.abs(), f"dbias{i}")
+            within(got[f"bias{i}"].to(where), r, (dg.sum(0) + more(M) * g.abs().sum(0)) * (1 + u) + u * r.abs() + lo, f"dbias{i}")
         wc = c(w)
-        dg, g = dg @ wc.abs() + more(wc.shape[0]) * (g.abs() @ wc.abs()), g @ wc
+        # (a gate in the weights is rounded there: gate * w instead of dout * gate, u of each product either way, but at least `lo` for each weight)
+        small = lo * (d.abs() if gate is not None and i == len(layers) - 1 else g.abs()).sum(1, keepdim=True)
+        dg, g = dg @ wc.abs() + more(wc.shape[0]) * (g.abs() @ wc.abs()) + small, g @ wc
         rounded = False
     if "x" in got:
-        within(got["x"].cpu().reshape(g.shape), g, dg * (1 + u) + u * g.abs(), "dx")
+        within(got["x"].to(where).reshape(g.shape), g, dg * (1 + u) + u * g.abs() + lo, "dx")
     return out, got

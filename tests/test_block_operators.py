@@ -81,6 +81,14 @@ def test_linear_sizes(dev, dtype, B, T, K, N):
     check_linear(dev, dtype, B, T, K, N, None, bias=False, seed=N)
 
 
+@pytest.mark.parametrize("B,T,K,N", [(2, 40, 16, 24), (3, 130, 40, 33), (1, 70, 8, 5), (70, 9, 4, 3)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_linear_gate_in_the_weights(dev, dtype, B, T, K, N):
+    """Samples long enough that the backward gates the weights instead of the rows."""
+    check_linear(dev, dtype, B, T, K, N, None, gate=True, residual=True, seed=K)
+    check_linear(dev, dtype, B, T, K, N, None, bias=False, gate=True, seed=N)
+
+
 def check_ffn(dev, dtype, B, T, C, F, act="gelu_tanh", bias=True, gate=True, residual=True, N=None, seed=0):
     r = Draw(dev, dtype, seed)
     N = N or C
@@ -100,3 +108,27 @@ def test_feed_forward(dev, dtype, act):
 def test_feed_forward_sizes(dev, B, T, C, F, N):
     check_ffn(dev, BF16, B, T, C, F, N=N, seed=F)
     check_ffn(dev, FP16, B, T, C, F, "silu", bias=False, gate=False, residual=False, N=N, seed=C)
+
+
+@pytest.mark.parametrize("B,T,C,F,N", [(2, 80, 24, 40, 24), (3, 66, 9, 33, 7)])
+def test_feed_forward_gate_in_the_weights(dev, B, T, C, F, N):
+    check_ffn(dev, BF16, B, T, C, F, N=N, seed=F)
+    check_ffn(dev, FP16, B, T, C, F, "gelu", bias=False, N=N, seed=C)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("B,T,K,N", [(3, 5459, 136, 264), (3, 32765, 40, 120), (1, 4090, 1032, 4090), (2, 2046, 1032, 4088), (5, 1639, 320, 1025)])
+def test_large_tiles(dtype, B, T, K, N):
+    """Sizes at which the larger tiles are taken, with edges inside them in every direction: each activation once."""
+    dev = torch.device("cuda")
+    for act, gate, residual in ((None, True, True), ("gelu_tanh", False, True), ("silu", True, False), ("gelu", False, False)):
+        check_linear(dev, dtype, B, T, K, N, act, gate=gate, residual=residual, seed=N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("B,T,C,F", [(3, 32765, 40, 120), (2, 8190, 264, 520), (4, 1021, 1032, 4088)])
+def test_large_feed_forward(dtype, B, T, C, F):
+    for act in ("gelu_tanh", "gelu", "silu"):
+        check_ffn(torch.device("cuda"), dtype, B, T, C, F, act, seed=F)
