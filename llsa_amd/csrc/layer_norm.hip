@@ -18,43 +18,78 @@ namespace {
 
 template <typename T> struct Eight { typedef __attribute__((ext_vector_type(8))) T type; };
 
-// Channels c .. c + 7 of a row, `left` of them inside (none if it is not positive): zeros beyond.  WIDE: rows are 16-byte aligned and whole pieces.
-template <bool WIDE, typename T>
-__device__ __forceinline__ void load8(float (&v)[8], const T* row, int c, int left) {
-    if (WIDE) {
-        if (left > 0) {
-            const typename Eight<T>::type a = *reinterpret_cast<const typename Eight<T>::type*>(row + c);
+// Where a row's channels are held.  WIDE (rows are 16-byte aligned and whole pieces of eight): piece j of a lane is channels (j LANES + lane) 8 .. + 7, read
+// and written in pieces.  Otherwise value e of piece j is channel (j 8 + e) LANES + lane, so that what the lanes read one by one lies side by side too.
+template <bool WIDE, int LANES>
+__device__ __forceinline__ int channel(int j, int e, int lane) { return WIDE ? (j * LANES + lane) * 8 + e : (j * 8 + e) * LANES + lane; }
+
+template <bool WIDE, int LANES, int CHUNKS, typename T>
+struct Row {
+    typename Eight<T>::type piece[CHUNKS];                    // as they are in memory; zeros beyond the row
+    __device__ __forceinline__ void load(const T* row, int C, int lane) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = (float)a[e];
-        } else {
+        for (int j = 0; j < CHUNKS; j++) {
+            if (WIDE) {
+                const int c = channel<WIDE, LANES>(j, 0, lane);
+                if (c < C) {
+                    piece[j] = __builtin_nontemporal_load(reinterpret_cast<const typename Eight<T>::type*>(row + c));
+                } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = 0.f;
+                    for (int e = 0; e < 8; e++) piece[j][e] = (T)0.f;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int c = channel<WIDE, LANES>(j, e, lane);
+                    piece[j][e] = c < C ? row[c] : (T)0.f;
+                }
+            }
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = e < left ? (float)row[c + e] : 0.f;
     }
-}
-template <bool WIDE, typename T>
-__device__ __forceinline__ void store8(T* row, int c, int left, const float (&v)[8]) {
+};
+template <bool WIDE, int LANES, typename T>
+__device__ __forceinline__ void store8(T* row, int j, int lane, int C, const float (&v)[8]) {
     if (WIDE) {
-        if (left > 0) {
+        const int c = channel<WIDE, LANES>(j, 0, lane);
+        if (c < C) {
             typename Eight<T>::type a;
 #pragma unroll
             for (int e = 0; e < 8; e++) a[e] = (T)v[e];
-            *reinterpret_cast<typename Eight<T>::type*>(row + c) = a;
+            __builtin_nontemporal_store(a, reinterpret_cast<typename Eight<T>::type*>(row + c));
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (e < left) row[c + e] = (T)v[e];
+        for (int e = 0; e < 8; e++) {
+            const int c = channel<WIDE, LANES>(j, e, lane);
+            if (c < C) row[c] = (T)v[e];
+        }
     }
 }
-// a small vector, of the rows' type or fp32
-template <typename T>
-__device__ __forceinline__ void load_vector(float (&v)[8], const void* p, bool f32, int c, int left) {
+// A small vector, of the rows' type or fp32, in pieces if it allows them: `otherwise` where there is none or beyond the row
+template <bool WIDE, int LANES, typename T>
+__device__ __forceinline__ void load_vector(float (&v)[8], const void* p, bool f32, int j, int lane, int C, float otherwise = 0.f) {
+    const int first = channel<WIDE, LANES>(j, 0, lane);
+    const bool aligned = WIDE && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+    if (p != nullptr && aligned && first < C) {
+        if (f32) {
+            const Eight<float>::type a = *reinterpret_cast<const Eight<float>::type*>(static_cast<const float*>(p) + first);
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = e >= left ? 0.f : f32 ? static_cast<const float*>(p)[c + e] : (float)static_cast<const T*>(p)[c + e];
+            for (int e = 0; e < 8; e++) v[e] = a[e];
+        } else {
+            const typename Eight<T>::type a = *reinterpret_cast<const typename Eight<T>::type*>(static_cast<const T*>(p) + first);
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = (float)a[e];
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const int c = channel<WIDE, LANES>(j, e, lane);
+        v[e] = p == nullptr || c >= C ? otherwise : f32 ? static_cast<const float*>(p)[c] : (float)static_cast<const T*>(p)[c];
+    }
+}
+__device__ __forceinline__ const void* row_of(const void* p, int64_t elements, int size) {
+    return p == nullptr ? nullptr : static_cast<const char*>(p) + elements * size;
 }
 
 // Sum over the LANES lanes of a row, the same bits in all of them.  Up to 64 lanes inside a wave; more go through LDS, one slot a wave.
@@ -94,7 +129,7 @@ struct Norm {
     float eps;
 };
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kCus = 256;
 
 // rows first .. last - 1 of the workgroup's sample
 struct Share { int64_t first, last; int64_t sample; };
@@ -110,55 +145,49 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const Norm a) {
     __shared__ float slots[LANES > 64 ? LANES / 64 : 1];
     const int lane = threadIdx.x % LANES, row = threadIdx.x / LANES;
     const Share share = share_of(a);
+    Row<WIDE, LANES, CHUNKS, T> next;                         // a row on its way while the one before is worked on
+    auto request = [&](int64_t first) { next.load(static_cast<const T*>(a.x) + min(first + row, share.last - 1) * a.ldx, a.C, lane); };
+    request(share.first);
     float up[CHUNKS][8], add[CHUNKS][8];                      // y = h * up + add
+    const int es = a.f32 ? 4 : (int)sizeof(T);
+    const void *scale = row_of(a.scale, share.sample * a.s_scale, es), *shift = row_of(a.shift, share.sample * a.s_shift, es);
 #pragma unroll
     for (int j = 0; j < CHUNKS; j++) {
-        const int c = (j * LANES + lane) * 8, left = a.C - c;
-        float t[8];
+        float t[8], u[8];
+        load_vector<WIDE, LANES, T>(up[j], a.weight, a.f32, j, lane, a.C, 1.f);
+        load_vector<WIDE, LANES, T>(add[j], a.bias, a.f32, j, lane, a.C);
+        load_vector<WIDE, LANES, T>(t, scale, a.f32, j, lane, a.C);
+        load_vector<WIDE, LANES, T>(u, shift, a.f32, j, lane, a.C);
 #pragma unroll
-        for (int e = 0; e < 8; e++) up[j][e] = 1.f, add[j][e] = 0.f;
-        if (a.weight != nullptr) load_vector<T>(up[j], a.weight, a.f32, c, left);
-        if (a.bias != nullptr) load_vector<T>(add[j], a.bias, a.f32, c, left);
-        const int es = a.f32 ? 4 : (int)sizeof(T);
-        if (a.scale != nullptr) {
-            load_vector<T>(t, static_cast<const char*>(a.scale) + share.sample * a.s_scale * es, a.f32, c, left);
-#pragma unroll
-            for (int e = 0; e < 8; e++) up[j][e] *= 1.f + t[e], add[j][e] *= 1.f + t[e];
-        }
-        if (a.shift != nullptr) {
-            load_vector<T>(t, static_cast<const char*>(a.shift) + share.sample * a.s_shift * es, a.f32, c, left);
-#pragma unroll
-            for (int e = 0; e < 8; e++) add[j][e] += t[e];
+        for (int e = 0; e < 8; e++) {
+            up[j][e] *= 1.f + t[e];
+            add[j][e] = fmaf(add[j][e], 1.f + t[e], u[e]);
         }
     }
     const float per = 1.f / (float)a.C;
     for (int64_t first = share.first; first < share.last; first += kRows) {       // (the same count for all lanes: row sums may meet at barriers)
         const int64_t r = first + row;
-        const bool there = r < share.last;
-        const T* const x = static_cast<const T*>(a.x) + (there ? r : share.first) * a.ldx;
         float v[CHUNKS][8], s = 0.f;
-#pragma unroll
-        for (int j = 0; j < CHUNKS; j++) {
-            const int c = (j * LANES + lane) * 8;
-            load8<WIDE>(v[j], x, c, a.C - c);
-        }
 #pragma unroll
         for (int j = 0; j < CHUNKS; j++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) s += v[j][e];
+            for (int e = 0; e < 8; e++) {
+                v[j][e] = (float)next.piece[j][e];
+                s += v[j][e];
+            }
+        if (first + kRows < share.last) request(first + kRows);
         const float mean = row_sum<LANES>(s, slots) * per;
         s = 0.f;
 #pragma unroll
         for (int j = 0; j < CHUNKS; j++) {
-            const int left = a.C - (j * LANES + lane) * 8;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                v[j][e] = e < left ? v[j][e] - mean : 0.f;
-                s += v[j][e] * v[j][e];
+                v[j][e] = channel<WIDE, LANES>(j, e, lane) < a.C ? v[j][e] - mean : 0.f;
+                s = fmaf(v[j][e], v[j][e], s);
             }
         }
         const float rstd = rsqrtf(row_sum<LANES>(s, slots) * per + a.eps);
-        if (!there) continue;
+        if (r >= share.last) continue;
         if (a.stats != nullptr && lane == 0) {
             a.stats[2 * r] = mean;
             a.stats[2 * r + 1] = rstd;
@@ -166,10 +195,9 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const Norm a) {
         T* const y = static_cast<T*>(a.y) + r * a.ldy;
 #pragma unroll
         for (int j = 0; j < CHUNKS; j++) {
-            const int c = (j * LANES + lane) * 8;
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[j][e] = v[j][e] * rstd * up[j][e] + add[j][e];
-            store8<WIDE>(y, c, a.C - c, v[j]);
+            for (int e = 0; e < 8; e++) v[j][e] = fmaf(v[j][e] * rstd, up[j][e], add[j][e]);
+            store8<WIDE, LANES>(y, j, lane, a.C, v[j]);
         }
     }
 }
@@ -182,49 +210,50 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const Norm a) {
     __shared__ float sums[kRows > 1 ? kThreads * 8 : 1];
     const int lane = threadIdx.x % LANES, row = threadIdx.x / LANES;
     const Share share = share_of(a);
+    Row<WIDE, LANES, CHUNKS, T> next_x, next_dy;
+    float next_mean, next_rstd;
+    auto request = [&](int64_t first) {
+        const int64_t r = min(first + row, share.last - 1);
+        next_x.load(static_cast<const T*>(a.x) + r * a.ldx, a.C, lane);
+        next_dy.load(static_cast<const T*>(a.dy) + r * a.lddy, a.C, lane);
+        next_mean = a.stats[2 * r];
+        next_rstd = a.stats[2 * r + 1];
+    };
+    request(share.first);
     float up[CHUNKS][8], s1[CHUNKS][8], s2[CHUNKS][8];
+    const void* scale = row_of(a.scale, share.sample * a.s_scale, a.f32 ? 4 : (int)sizeof(T));
 #pragma unroll
     for (int j = 0; j < CHUNKS; j++) {
-        const int c = (j * LANES + lane) * 8, left = a.C - c;
+        float t[8];
+        load_vector<WIDE, LANES, T>(up[j], a.weight, a.f32, j, lane, a.C, 1.f);
+        load_vector<WIDE, LANES, T>(t, scale, a.f32, j, lane, a.C);
 #pragma unroll
-        for (int e = 0; e < 8; e++) up[j][e] = 1.f, s1[j][e] = 0.f, s2[j][e] = 0.f;
-        if (a.weight != nullptr) load_vector<T>(up[j], a.weight, a.f32, c, left);
-        if (a.scale != nullptr) {
-            float t[8];
-            load_vector<T>(t, static_cast<const char*>(a.scale) + share.sample * a.s_scale * (a.f32 ? 4 : (int)sizeof(T)), a.f32, c, left);
-#pragma unroll
-            for (int e = 0; e < 8; e++) up[j][e] *= 1.f + t[e];
-        }
+        for (int e = 0; e < 8; e++) up[j][e] *= 1.f + t[e], s1[j][e] = 0.f, s2[j][e] = 0.f;
     }
     const float per = 1.f / (float)a.C;
     for (int64_t first = share.first; first < share.last; first += kRows) {
         const int64_t r = first + row;
         const bool there = r < share.last;
-        const int64_t at = there ? r : share.first;
-        const T* const x = static_cast<const T*>(a.x) + at * a.ldx;
-        const T* const dy = static_cast<const T*>(a.dy) + at * a.lddy;
-        const float mean = a.stats[2 * at], rstd = a.stats[2 * at + 1];
+        const float mean = next_mean, rstd = next_rstd;
         float h[CHUNKS][8], d[CHUNKS][8], sg = 0.f, sgh = 0.f;
 #pragma unroll
-        for (int j = 0; j < CHUNKS; j++) {
-            const int c = (j * LANES + lane) * 8;
-            load8<WIDE>(h[j], x, c, a.C - c);
-            load8<WIDE>(d[j], dy, c, a.C - c);
-        }
-#pragma unroll
-        for (int j = 0; j < CHUNKS; j++) {
+        for (int j = 0; j < CHUNKS; j++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                h[j][e] = (h[j][e] - mean) * rstd;            // (beyond the row d is zero, and so is all that h enters)
-                if (there) {
-                    s1[j][e] += d[j][e];
-                    s2[j][e] += d[j][e] * h[j][e];
-                }
+                h[j][e] = ((float)next_x.piece[j][e] - mean) * rstd;        // (beyond the row d is zero, and so is all that h enters)
+                d[j][e] = there ? (float)next_dy.piece[j][e] : 0.f;
+            }
+        if (first + kRows < share.last) request(first + kRows);
+#pragma unroll
+        for (int j = 0; j < CHUNKS; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                s1[j][e] += d[j][e];
+                s2[j][e] = fmaf(d[j][e], h[j][e], s2[j][e]);
                 d[j][e] *= up[j][e];
                 sg += d[j][e];
-                sgh += d[j][e] * h[j][e];
+                sgh = fmaf(d[j][e], h[j][e], sgh);
             }
-        }
         if (a.dx == nullptr) continue;
         sg = row_sum<LANES>(sg, slots) * per;
         sgh = row_sum<LANES>(sgh, slots) * per;
@@ -232,10 +261,9 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const Norm a) {
         T* const dx = static_cast<T*>(a.dx) + r * a.lddx;
 #pragma unroll
         for (int j = 0; j < CHUNKS; j++) {
-            const int c = (j * LANES + lane) * 8;
 #pragma unroll
             for (int e = 0; e < 8; e++) d[j][e] = rstd * (d[j][e] - sg - h[j][e] * sgh);
-            store8<WIDE>(dx, c, a.C - c, d[j]);
+            store8<WIDE, LANES>(dx, j, lane, a.C, d[j]);
         }
     }
     if (a.part == nullptr) return;
@@ -244,7 +272,6 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const Norm a) {
     for (int which = 0; which < 2; which++)
 #pragma unroll
         for (int j = 0; j < CHUNKS; j++) {
-            const int c = (j * LANES + lane) * 8;
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = which == 0 ? s1[j][e] : s2[j][e];
@@ -260,8 +287,10 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const Norm a) {
                     for (int e = 0; e < 8; e++) v[e] += sums[e * kThreads + i * LANES + lane];
             }
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (c + e < a.C) part[(int64_t)which * a.C + c + e] = v[e];
+            for (int e = 0; e < 8; e++) {
+                const int c = channel<WIDE, LANES>(j, e, lane);
+                if (c < a.C) part[(int64_t)which * a.C + c] = v[e];
+            }
         }
 }
 
@@ -281,24 +310,27 @@ __device__ __forceinline__ void put(void* p, bool f32, int64_t i, float v) {
     if (f32) static_cast<float*>(p)[i] = v;
     else static_cast<T*>(p)[i] = (T)v;
 }
-// S1 and S2 of a sample out of its pieces: 32 channels a workgroup, eight threads for each, which take every eighth piece
+// S1 and S2 of a sample out of its pieces: 16 channels a workgroup, sixteen threads for each, which take every sixteenth piece
+constexpr int kJoinChannels = 16, kJoinLanes = 16;
 template <typename T>
 __global__ __launch_bounds__(256) void norm_join_kernel(const Join a) {
-    __shared__ float sums[2][8][32];
-    const int k = threadIdx.x & 31, lane = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + k, sample = blockIdx.y;
+    __shared__ float sums[2][kJoinLanes][kJoinChannels];
+    const int k = threadIdx.x % kJoinChannels, lane = threadIdx.x / kJoinChannels, c = (int)blockIdx.x * kJoinChannels + k, sample = blockIdx.y;
     float s1 = 0.f, s2 = 0.f;
-    if (c < a.C)
-        for (int p = lane; p < a.pieces; p += 8) {
-            const float* const part = a.part + ((int64_t)sample * a.pieces + p) * 2 * a.C;
-            s1 += part[c];
-            s2 += part[a.C + c];
+    if (c < a.C) {
+        const float* const part = a.part + (int64_t)sample * a.pieces * 2 * a.C + c;
+#pragma unroll 8
+        for (int p = lane; p < a.pieces; p += kJoinLanes) {
+            s1 += part[(int64_t)p * 2 * a.C];
+            s2 += part[(int64_t)p * 2 * a.C + a.C];
         }
+    }
     sums[0][lane][k] = s1;
     sums[1][lane][k] = s2;
     __syncthreads();
     if (lane > 0 || c >= a.C) return;
 #pragma unroll
-    for (int i = 1; i < 8; i++) s1 += sums[0][i][k], s2 += sums[1][i][k];
+    for (int i = 1; i < kJoinLanes; i++) s1 += sums[0][i][k], s2 += sums[1][i][k];
     const int64_t at = (int64_t)sample * a.C + c;
     if (a.dshift != nullptr) put<T>(a.dshift, a.f32, at, s1);
     if (a.dscale != nullptr) {
@@ -330,44 +362,59 @@ __global__ __launch_bounds__(256) void norm_join_samples_kernel(const Join a) {
 constexpr int64_t kMaxGrid = (int64_t(1) << 31) - 1;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Lanes and pieces of eight channels a lane: as few idle lanes as there can be, then as few lanes (several rows of a wave are in flight together)
+// Lanes and pieces of eight channels a lane: as few idle lanes as there can be with at most three pieces (backward: two, whose sums take registers from the
+// waves that hide the loads), then as few lanes.  us, forward + backward of 131072 x 384: 16 lanes of 3 pieces 39.5 + 80.8, 64 of 1 42.0 + 65.1; 8192 x 2048:
+// 64 of 4 18.9 + 44.0, 256 of 1 15.5 + 37.0.
 struct Shape { int lanes, chunks; };
-Shape shape_for(int C) {
+Shape shape_for(int C, bool backward) {
     const int pieces = (int)ceil_div(C, 8);
     Shape best{256, 4};
     for (int lanes : {16, 64, 256})
-        for (int chunks = 1; chunks <= 4; chunks++)
+        for (int chunks = 1; chunks <= (backward ? 2 : 3); chunks++)
             if (lanes * chunks >= pieces && (lanes * chunks < best.lanes * best.chunks)) best = {lanes, chunks};
-    return best;
+    return best.chunks == 4 && 3 * 256 >= pieces ? Shape{256, 3} : best;
 }
-// The split of the rows over workgroups.  Where the rows have no samples (neither scale nor shift) the whole is one.
+// The split of the rows over workgroups, each of one sample's rows.  A workgroup first reads the vectors, so it gets several rows for every one that it holds
+// at a time.  The backward's leave sums that are added up in a launch of their own: 64 rows each, but 512 to 768 workgroups (us, 512 / 768 / 1536: 131072 x
+// 384 72 / 65 / 72, 32768 x 1024 49.6 / 51.5 / 54.9, 8192 x 2048 34.0 / 37.0 / 47.1).
 struct Split { int pieces, rows; };
 Split split_rows(int64_t rows, int64_t per_sample, int C, bool backward) {
-    const Shape s = shape_for(C);
-    const int64_t at_once = std::max(1, 256 / s.lanes), samples = rows / per_sample;
-    const int64_t wanted = std::max<int64_t>(1, (backward ? 1024 : 4096) / samples);
-    const int64_t each = ceil_div(ceil_div(per_sample, wanted), at_once) * at_once;
+    const Shape s = shape_for(C, backward);
+    const int64_t at_once = std::max(1, kThreads / s.lanes), samples = rows / per_sample;
+    const int64_t most = backward ? std::min<int64_t>(768, std::max<int64_t>(512, rows / 64)) : 2048;
+    const int64_t wanted = std::max<int64_t>(1, most / samples);
+    int64_t each = ceil_div(ceil_div(per_sample, wanted), at_once) * at_once;
+    each = std::max(each, std::min<int64_t>(2, ceil_div(rows, at_once * kCus)) * at_once);      // (twice as many rows as at a time, if that leaves a workgroup for each CU)
     return {(int)ceil_div(per_sample, each), (int)each};
 }
 
 template <typename T, int LANES, int CHUNKS>
+void launch_fwd(const Norm& a, int64_t grid, bool wide, hipStream_t stream) {
+    const dim3 g((unsigned)grid), b(kThreads);
+    if (wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_fwd_kernel<T, LANES, CHUNKS, true>), g, b, 0, stream, a);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_fwd_kernel<T, LANES, CHUNKS, false>), g, b, 0, stream, a);
+}
+template <typename T, int LANES, int CHUNKS>
 void launch(const Norm& a, int64_t grid, bool backward, bool wide, hipStream_t stream) {
     const dim3 g((unsigned)grid), b(kThreads);
-    if (backward && wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_bwd_kernel<T, LANES, CHUNKS, true>), g, b, 0, stream, a);
-    else if (backward) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_bwd_kernel<T, LANES, CHUNKS, false>), g, b, 0, stream, a);
-    else if (wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_fwd_kernel<T, LANES, CHUNKS, true>), g, b, 0, stream, a);
-    else hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_fwd_kernel<T, LANES, CHUNKS, false>), g, b, 0, stream, a);
+    if (!backward) return launch_fwd<T, LANES, CHUNKS>(a, grid, wide, stream);
+    if (wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_bwd_kernel<T, LANES, CHUNKS, true>), g, b, 0, stream, a);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_bwd_kernel<T, LANES, CHUNKS, false>), g, b, 0, stream, a);
 }
 template <typename T, int LANES>
 void launch_chunks(const Norm& a, int chunks, int64_t grid, bool backward, bool wide, hipStream_t stream) {
-    if (chunks == 1) launch<T, LANES, 1>(a, grid, backward, wide, stream);
-    else if (chunks == 2) launch<T, LANES, 2>(a, grid, backward, wide, stream);
-    else if (chunks == 3) launch<T, LANES, 3>(a, grid, backward, wide, stream);
-    else launch<T, LANES, 4>(a, grid, backward, wide, stream);
+    if (chunks == 1) return launch<T, LANES, 1>(a, grid, backward, wide, stream);
+    if (chunks == 2) return launch<T, LANES, 2>(a, grid, backward, wide, stream);
+    if constexpr (LANES == 256) {
+        if (chunks == 3) return launch<T, LANES, 3>(a, grid, backward, wide, stream);
+        return launch<T, LANES, 4>(a, grid, backward, wide, stream);
+    } else {
+        return launch_fwd<T, LANES, 3>(a, grid, wide, stream);
+    }
 }
 template <typename T>
 int launch_norm(const Norm& a, bool backward, bool wide, hipStream_t stream) {
-    const Shape s = shape_for(a.C);
+    const Shape s = shape_for(a.C, backward);
     const int64_t grid = a.rows / a.per_sample * a.pieces;
     if (grid > kMaxGrid) return fail(-1, "layer_norm: too many samples");
     switch (s.lanes) {
@@ -416,7 +463,7 @@ int backward(const llsa_layer_norm_args* a, hipStream_t stream) {
         j.weight = a->weight; j.bias = a->bias; j.scale = a->scale; j.s_scale = a->s_scale;
         j.dscale = a->dscale; j.dshift = a->dshift; j.dweight = a->dweight; j.dbias = a->dbias;
         if (a->dweight != nullptr || a->dbias != nullptr) j.per_sample = n.part + samples * n.pieces * 2 * a->C;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_join_kernel<T>), dim3((unsigned)ceil_div(a->C, 32), (unsigned)samples), dim3(256), 0, stream, j);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_join_kernel<T>), dim3((unsigned)ceil_div(a->C, kJoinChannels), (unsigned)samples), dim3(256), 0, stream, j);
         if (j.per_sample != nullptr) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_join_samples_kernel<T>), dim3((unsigned)ceil_div(a->C, 256)), dim3(256), 0, stream, j);
     }
     return launch_status("layer_norm_bwd");
