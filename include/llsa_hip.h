@@ -411,8 +411,16 @@ int llsa_linear_dw(const llsa_linear_args* a, void* stream);
 int llsa_linear_gate_rows(const llsa_linear_args* a, void* stream);
 int64_t llsa_linear_dw_workspace_bytes(int64_t M, int64_t samples, int N, int K);
 int64_t llsa_linear_dz_workspace_bytes(int64_t M, int64_t per_sample, int N);
-/* (rows, cols) of 16-bit elements, rows ldx apart, to rows ldy apart (a multiple of 8, 16-byte aligned), zeros in columns cols .. ldy - 1 */
-int llsa_pad_rows(const void* x, int64_t ldx, void* y, int64_t ldy, int64_t rows, int cols, void* stream);
+/* (rows, cols) of 16-bit elements, rows ldx apart, to rows ldy apart (a multiple of 8, 16-byte aligned), zeros in columns cols .. ldy - 1;
+ * n such copies in one launch */
+#define LLSA_PAD_JOBS 4
+typedef struct llsa_pad_job {
+    const void* x;
+    void* y;
+    int64_t ldx, ldy, rows;
+    int32_t cols, reserved;
+} llsa_pad_job;
+int llsa_pad_rows(const llsa_pad_job* jobs, int n, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Layer norm with the modulation of an adaLN block (models/rope_dit_transformer_2d.py:295-337, 581-711, torch modules in the

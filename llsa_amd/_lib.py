@@ -90,6 +90,10 @@ class LinearArgs(C.Structure):
                 + [(n, c_int32) for n in ("N", "K", "act", "dtype", "padded", "reserved")])
 
 
+class PadJob(C.Structure):
+    _fields_ = [("x", c_void_p), ("y", c_void_p), ("ldx", c_int64), ("ldy", c_int64), ("rows", c_int64), ("cols", c_int32), ("reserved", c_int32)]
+
+
 class LayerNormArgs(C.Structure):
     _fields_ = ([(n, c_void_p) for n in ("x", "y", "weight", "bias", "scale", "shift", "stats", "dy", "dx", "dweight", "dbias", "dscale", "dshift", "workspace")]
                 + [(n, c_int64) for n in ("ldx", "ldy", "s_scale", "s_shift", "lddy", "lddx", "rows", "per_sample")]
@@ -142,7 +146,7 @@ _SIGNATURES = {
     "llsa_linear_gate_rows": (c_int, [C.POINTER(LinearArgs), c_void_p]),
     "llsa_linear_dw_workspace_bytes": (c_int64, [c_int64, c_int64, c_int, c_int]),
     "llsa_linear_dz_workspace_bytes": (c_int64, [c_int64, c_int64, c_int]),
-    "llsa_pad_rows": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
+    "llsa_pad_rows": (c_int, [C.POINTER(PadJob), c_int, c_void_p]),
 }
 
 EXPORTS = tuple(_SIGNATURES)

@@ -59,14 +59,25 @@ public:
     void* stream() const { return stream_; }
     Tensor rows(int64_t count, int64_t cols) const { return at::empty({count, pad8(cols)}, options_); }
     Tensor bytes(int64_t n) const { return n > 0 ? at::empty({n}, options_.dtype(at::kByte)) : Tensor(); }
-    // rows that the products read: 16-byte aligned, whole pieces of eight elements
+    // Rows that the products read: 16-byte aligned, whole pieces of eight elements.  Matrices that are not are copied, in one launch.
+    void operands(std::initializer_list<std::pair<const Tensor*, Rows*>> all) const {
+        llsa_pad_job jobs[LLSA_PAD_JOBS];
+        int n = 0;
+        for (const auto& [t, r] : all) {
+            *r = rows_of(*t);
+            if (aligned(r->t) && r->ld % 8 == 0 && r->cols % 8 == 0 && r->ld <= (int64_t(1) << 23)) continue;
+            const Tensor y = rows(r->count, r->cols);
+            jobs[n++] = llsa_pad_job{r->p(), y.data_ptr(), r->ld, y.size(1), r->count, static_cast<int32_t>(r->cols), 0};
+            copied_.push_back(r->t);                          // (until the copies are issued)
+            r->t = y;
+            r->ld = y.size(1);
+        }
+        if (n > 0) lib_.check(lib_.pad_rows(jobs, n, stream_), "pad_rows");
+        copied_.clear();
+    }
     Rows operand(const Tensor& t) const {
-        Rows r = rows_of(t);
-        if (aligned(r.t) && r.ld % 8 == 0 && r.cols % 8 == 0 && r.ld <= (int64_t(1) << 23)) return r;
-        const Tensor y = rows(r.count, r.cols);
-        lib_.check(lib_.pad_rows(r.p(), r.ld, y.data_ptr(), y.size(1), r.count, static_cast<int>(r.cols), stream_), "pad_rows");
-        r.t = y;
-        r.ld = y.size(1);
+        Rows r;
+        operands({{&t, &r}});
         return r;
     }
 
@@ -74,6 +85,7 @@ private:
     const Library& lib_;
     void* stream_;
     at::TensorOptions options_;
+    mutable std::vector<Tensor> copied_;
 };
 
 // The node of an operator with one output: what is common to the three of them.  `kept` are the saved tensors in the order run() unpacks them.
@@ -422,6 +434,13 @@ int activation(const char* what, int64_t act) {
 }
 Tensor zeros_like_weight(int64_t n, int64_t k, const Tensor& like) { return at::zeros({n, k}, like.options()); }
 
+// An operand of the forward, which may be a copy with padded rows, of which `cols` elements count
+Rows kept_operand(const Call& call, const Tensor& t, int64_t cols) {
+    Rows r = call.operand(t);
+    r.cols = cols;
+    return r;
+}
+
 struct LinearBackward : public BlockNode {
     std::vector<int64_t> sizes;
     int64_t rows, per_sample, samples, K, N;
@@ -442,7 +461,7 @@ struct LinearBackward : public BlockNode {
             const Tensor gate = has_gate ? dense_vector(&saved[2]) : Tensor();
             if (want_x || want_w || want_b || want_g) {
                 const Rows dz = gate_out ? call.operand(grad) : layer_dz(call, rows_of(grad), grad, gate, z, per_sample, act, dtype, want_g ? &dg : nullptr);
-                const Rows w = want_x || (gate_out && want_g) ? call.operand(saved[1]) : Rows();
+                const Rows w = want_x || (gate_out && want_g) ? kept_operand(call, saved[1], K) : Rows();
                 if (want_x) layer_dx(call, dz, gate_out ? gated_weights(call, w, gate, samples, dtype) : w, dx, K, Tensor(), act, dtype, gate_out ? per_sample : 0);
                 if (want_w || want_b || (gate_out && want_g)) {
                     dw = at::empty({N, K}, grad.options());
@@ -453,7 +472,7 @@ struct LinearBackward : public BlockNode {
                         g.gate = gate; g.w = w; g.per_sample = per_sample;
                         g.bias = saved[4].defined() ? dense_vector(&saved[4]) : Tensor();
                     }
-                    layer_dw(call, dz, call.operand(saved[0]), dw, db, dtype, gate_out ? &g : nullptr);
+                    layer_dw(call, dz, kept_operand(call, saved[0], K), dw, db, dtype, gate_out ? &g : nullptr);
                 }
             }
         } else {
@@ -495,8 +514,7 @@ Tensor linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, const Ten
         out = at::empty(out_sizes, x_in.options());
         gate = dense_vector(gate_p);
         if (in.rows > 0) {
-            x = call.operand(x_in);
-            w = call.operand(w_in);
+            call.operands({{&x_in, &x}, {&w_in, &w}});
             if ((act != LLSA_ACT_NONE && inner) || (gates && !gate_out)) z = call.rows(in.rows, N);
             layer_fwd(call, x, w, dense_vector(bias_p), gate, residual_p != nullptr ? rows_of(*residual_p) : Rows(), z, out, N, false, in.per_sample(), act, dtype);
         } else {
@@ -514,9 +532,9 @@ Tensor linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, const Ten
     if (node) {
         node->set_next_edges(torch::autograd::collect_next_edges(present({&x_in, &w_in, bias_p, gate_p, residual_p})));
         torch::autograd::set_history(out, node);
-        // (x is needed for the gradient of the weight, the weight for that of x)
-        node->keep(wants({&w_in, bias_p}) || (gates && gate_out) ? x_in : Tensor(), x_in);
-        node->keep(x_in.requires_grad() || (gates && gate_out) ? w_in : Tensor(), w_in);
+        // (x is needed for the gradient of the weight, the weight for that of x; each as the products read it)
+        node->keep(wants({&w_in, bias_p}) || (gates && gate_out) ? x.t : Tensor(), x_in);
+        node->keep(x_in.requires_grad() || (gates && gate_out) ? w.t : Tensor(), w_in);
         node->keep(gate, gate_p != nullptr ? *gate_p : gate);
         node->keep(z, z);
         node->keep(gates && gate_out && bias_p != nullptr ? *bias_p : Tensor(), bias_p != nullptr ? *bias_p : Tensor());
@@ -549,7 +567,7 @@ struct FeedForwardBackward : public BlockNode {
             const Tensor gate = has_gate ? dense_vector(&saved[3]) : Tensor();
             const Tensor y = has_y ? as_kept(saved[6], {rows, pad8(N)}, type) : Tensor();
             const Rows dz2 = gate_out ? call.operand(grad) : layer_dz(call, rows_of(grad), grad, gate, y, per_sample, LLSA_ACT_NONE, dtype, want_g ? &dg : nullptr);
-            const Rows w2 = inner || (gate_out && want_g) ? call.operand(saved[2]) : Rows();
+            const Rows w2 = inner || (gate_out && want_g) ? kept_operand(call, saved[2], F) : Rows();
             if (outer || (gate_out && want_g)) {
                 Rows h;
                 h.t = as_kept(saved[5], {rows, pad8(F)}, type);
@@ -570,11 +588,11 @@ struct FeedForwardBackward : public BlockNode {
                 dz1.ld = dz1.t.size(1); dz1.count = rows; dz1.cols = F;
                 layer_dx(call, dz2, gate_out ? gated_weights(call, w2, gate, samples, dtype) : w2, dz1.t, dz1.ld, as_kept(saved[4], {rows, pad8(F)}, type), act, dtype,
                          gate_out ? per_sample : 0);
-                if (want_x) layer_dx(call, dz1, call.operand(saved[1]), dx, C, Tensor(), act, dtype);
+                if (want_x) layer_dx(call, dz1, kept_operand(call, saved[1], C), dx, C, Tensor(), act, dtype);
                 if (want_w1 || want_b1) {
                     dw1 = at::empty({F, C}, o);
                     if (want_b1) db1 = at::empty({F}, o);
-                    layer_dw(call, dz1, call.operand(saved[0]), dw1, db1, dtype);
+                    layer_dw(call, dz1, kept_operand(call, saved[0], C), dw1, db1, dtype);
                 }
             }
         } else if (rows == 0) {
@@ -615,6 +633,7 @@ Tensor feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_in, con
     std::vector<int64_t> out_sizes = x_in.sizes().vec();
     out_sizes.back() = N;
     Tensor out, z, h, y, gate;
+    Rows x, w1, w2;
     std::shared_ptr<FeedForwardBackward> node;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -624,12 +643,13 @@ Tensor feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_in, con
         gate = dense_vector(gate_p);
         if (in.rows > 0) {
             Rows hidden;
+            call.operands({{&x_in, &x}, {&w1_in, &w1}, {&w2_in, &w2}});
             h = call.rows(in.rows, F);
             hidden.t = h; hidden.ld = h.size(1); hidden.count = in.rows; hidden.cols = F;
             if (inner) z = call.rows(in.rows, F);
             if (gates && !gate_out) y = call.rows(in.rows, N);
-            layer_fwd(call, call.operand(x_in), call.operand(w1_in), dense_vector(b1), Tensor(), Rows(), z, h, hidden.ld, true, 1, act, dtype);
-            layer_fwd(call, hidden, call.operand(w2_in), dense_vector(b2), gate, residual_p != nullptr ? rows_of(*residual_p) : Rows(), y, out, N, false, in.per_sample(),
+            layer_fwd(call, x, w1, dense_vector(b1), Tensor(), Rows(), z, h, hidden.ld, true, 1, act, dtype);
+            layer_fwd(call, hidden, w2, dense_vector(b2), gate, residual_p != nullptr ? rows_of(*residual_p) : Rows(), y, out, N, false, in.per_sample(),
                       LLSA_ACT_NONE, dtype);
         }
         if (grad) {
@@ -644,9 +664,9 @@ Tensor feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_in, con
     if (node) {
         node->set_next_edges(torch::autograd::collect_next_edges(present({&x_in, &w1_in, b1, &w2_in, b2, gate_p, residual_p})));
         torch::autograd::set_history(out, node);
-        node->keep(wants({&w1_in, b1}) ? x_in : Tensor(), x_in);
-        node->keep(wants({&x_in}) ? w1_in : Tensor(), w1_in);
-        node->keep(inner || (gates && gate_out) ? w2_in : Tensor(), w2_in);
+        node->keep(wants({&w1_in, b1}) ? x.t : Tensor(), x_in);
+        node->keep(wants({&x_in}) ? w1.t : Tensor(), w1_in);
+        node->keep(inner || (gates && gate_out) ? w2.t : Tensor(), w2_in);
         node->keep(gate, gate_p != nullptr ? *gate_p : gate);
         node->keep(z, z);
         node->keep(outer || (gates && gate_out) ? h : Tensor(), h);

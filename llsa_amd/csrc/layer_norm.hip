@@ -337,7 +337,11 @@ __global__ __launch_bounds__(256) void norm_join_kernel(const Join a) {
         const float w = a.weight != nullptr ? entry<T>(a.weight, a.f32, c) : 1.f, b = a.bias != nullptr ? entry<T>(a.bias, a.f32, c) : 0.f;
         put<T>(a.dscale, a.f32, at, w * s2 + b * s1);
     }
-    if (a.per_sample != nullptr) {
+    if (a.samples == 1) {                                     // (their sum over the samples already)
+        const float up = a.scale != nullptr ? 1.f + entry<T>(a.scale, a.f32, c) : 1.f;
+        if (a.dbias != nullptr) put<T>(a.dbias, a.f32, c, up * s1);
+        if (a.dweight != nullptr) put<T>(a.dweight, a.f32, c, up * s2);
+    } else if (a.per_sample != nullptr) {
         const float up = a.scale != nullptr ? 1.f + entry<T>(a.scale, a.f32, sample * a.s_scale + c) : 1.f;
         a.per_sample[(int64_t)sample * 2 * a.C + c] = up * s1;
         a.per_sample[(int64_t)sample * 2 * a.C + a.C + c] = up * s2;
@@ -462,7 +466,7 @@ int backward(const llsa_layer_norm_args* a, hipStream_t stream) {
         j.part = n.part; j.pieces = n.pieces; j.samples = (int)samples; j.C = a->C; j.f32 = n.f32;
         j.weight = a->weight; j.bias = a->bias; j.scale = a->scale; j.s_scale = a->s_scale;
         j.dscale = a->dscale; j.dshift = a->dshift; j.dweight = a->dweight; j.dbias = a->dbias;
-        if (a->dweight != nullptr || a->dbias != nullptr) j.per_sample = n.part + samples * n.pieces * 2 * a->C;
+        if (samples > 1 && (a->dweight != nullptr || a->dbias != nullptr)) j.per_sample = n.part + samples * n.pieces * 2 * a->C;
         hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_join_kernel<T>), dim3((unsigned)ceil_div(a->C, kJoinChannels), (unsigned)samples), dim3(256), 0, stream, j);
         if (j.per_sample != nullptr) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_join_samples_kernel<T>), dim3((unsigned)ceil_div(a->C, 256)), dim3(256), 0, stream, j);
     }

@@ -26,6 +26,19 @@ template <typename T> using vec4 = typename Vec8<T>::half;
 __device__ __forceinline__ f32x4 product16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 product16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
+// Waits of a single wave that nothing is moved across: for its copies into LDS (vmcnt(0)), for its reads of LDS (lgkmcnt(0))
+__device__ __forceinline__ void wave_waits_for_copies() {
+    asm volatile("" ::: "memory");
+    wait_vm0();
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wave_waits_for_reads() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
+}
+
 // ---------------------------------------------------------------------------------------
 // activations, in fp32.  Written with the logistic function: 0.5 (1 + tanh u) = s(2u), which saturates to 0 and 1 without an
 // overflow.  The derivatives are taken at z held to +-16, where they are 0 and 1 to the last bit of fp32, so that a large z does not
@@ -75,7 +88,7 @@ __device__ __forceinline__ float activate_slope(int act, float z) {
 // the order of its source pieces; it is the source address that is permuted, never the place in LDS.
 //   rows     ROWS rows of 64 elements.  Piece p (8 elements) of row r holds the row's piece p ^ ((r >> 1) & 7): the 16 rows a fragment read touches then lie in 16 different 16-byte columns of the 256 bytes that all banks hold.
 //   columns  64 rows of ROWS elements.  32-byte granule g of row k holds the row's granule g ^ f(k), f out of bits 0, 1 and 3 of k
-//            (ROWS = 64: 1 and 3): the transposing read takes granules of 4 neighbouring rows in each group of 16 lanes and of
+//            (64 elements: 1 and 3, 32: 3): the transposing read takes granules of 4 neighbouring rows in each group of 16 lanes and of
 //            rows 8 further in the next, which then lie in different banks.
 // What lies outside the matrix: rows are clamped (their results are not stored), and beyond the end of the contraction zeros are fetched.
 // ---------------------------------------------------------------------------------------
@@ -96,7 +109,9 @@ struct Operand {
     unsigned off[kCopies];                                    // elements from the step's first, of this lane's pieces
 
     static __device__ __forceinline__ int swap(int r) { return (r >> 1) & 7; }
-    static __device__ __forceinline__ int turn(int k) { return ROWS == 64 ? ((k >> 1) & 1) | ((k >> 3) & 1) << 1 : (k & 3) | ((k >> 3) & 1) << 2; }
+    static __device__ __forceinline__ int turn(int k) {
+        return ROWS == 32 ? (k >> 3) & 1 : ROWS == 64 ? ((k >> 1) & 1) | ((k >> 3) & 1) << 1 : (k & 3) | ((k >> 3) & 1) << 2;
+    }
     // of the lane's j-th piece: its row and its first element along the row, in the tile
     static __device__ __forceinline__ int row_of(int i, int lane) { return COLUMNS ? i * (512 / ROWS) + lane / kPerRow : i * (64 / kPieces) + lane / kPieces; }
     static __device__ __forceinline__ int place_of(int row, int lane) {
@@ -163,9 +178,11 @@ struct Product {
     int64_t s_gate, ldr, ldz, ldo;
     T *out, *z;
     int per_sample, act;
-    int wide;                             // N and the pointers and strides of bias, gate and residual allow 16-byte accesses
-    int wide_out;                         // and those of out; or its rows are padded with zeros to a multiple of 8 elements (those of z always are)
-    // dW: pieces of the sum
+    // whether 16-byte accesses are allowed: to bias and gate; to the residual; to out, or its rows are padded with zeros to a multiple of 8 elements (those
+    // of z always are)
+    int wide, wide_side, wide_out;
+    // dW: pieces of the sum, or out and its sums of rows where there is one piece
+    T* sums;
     float *part, *part_sum;               // [sample][piece][M][ld_part], [sample][piece][M] or NULL
     int64_t ld_part;
 };
@@ -194,7 +211,7 @@ __device__ __forceinline__ void load8(float (&v)[8], const T* p, bool wide, int 
         for (int e = 0; e < 8; e++) v[e] = (float)a[e];
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = e < n ? (float)p[e] : 0.f;
+        for (int e = 0; e < 8; e++) v[e] = (float)p[min(e, n - 1)];          // (the last one again beyond the end: a branch for each would wait for each)
     }
 }
 // the same as they are; zeros of no memory
@@ -203,7 +220,11 @@ __device__ __forceinline__ vec8<T> take8(const T* p, bool wide, int n) {
     vec8<T> v;
     if (p != nullptr && wide) return *reinterpret_cast<const vec8<T>*>(p);
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = p != nullptr && e < n ? p[e] : (T)0.f;
+    for (int e = 0; e < 8; e++) v[e] = (T)0.f;
+    if (p != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = p[min(e, n - 1)];
+    }
     return v;
 }
 template <typename T>
@@ -234,7 +255,7 @@ template <int WAY, typename T>
 __device__ __forceinline__ vec8<T> way_out(const Product<T>& a, float (&v)[8], const vec8<T>& bias, const vec8<T>& gate, const vec8<T>& early, int64_t row, int col,
                                            const Lane& at, int left, vec8<T>& z) {
     constexpr bool any = WAY == kAnything;
-    const bool wide = any ? a.wide : true, slope = any ? a.slope_at != nullptr : WAY >= kSlope;
+    const bool slope = any ? a.slope_at != nullptr : WAY >= kSlope;
     const int act = any ? a.act : WAY & 3;
     if (!slope) {
 #pragma unroll
@@ -261,13 +282,13 @@ __device__ __forceinline__ vec8<T> way_out(const Product<T>& a, float (&v)[8], c
     }
     if (!slope && a.residual != nullptr) {
         float r[8];
-        if (any) load8(r, a.residual + (row * a.ldr + col) + at.residual, wide, left);
+        if (any) load8(r, a.residual + (row * a.ldr + col) + at.residual, a.wide_side, left);
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] += any ? r[e] : (float)early[e];
     }
     vec8<T> o;
 #pragma unroll
-    for (int e = 0; e < 8; e++) o[e] = (T)(any && e >= left ? 0.f : v[e]);
+    for (int e = 0; e < 8; e++) o[e] = (T)(e >= left ? 0.f : v[e]);
     return o;
 }
 
@@ -336,7 +357,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(cons
         k_left -= kStep;
     };
 
-    const bool sums = XC && a.part_sum != nullptr && here.tn == 0 && wn == 0;
+    const bool sums = XC && (a.part_sum != nullptr || a.sums != nullptr) && here.tn == 0 && wn == 0;
     f32x4 acc[NT][MT], sum[XC ? MT : 1];
 #pragma unroll
     for (int i = 0; i < NT; i++)
@@ -422,8 +443,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(cons
 #pragma unroll
         for (int h = 0; h < kPairs; h++) {
             const int n = col0 + lane_col + 32 * (p0 + h), left = cols_left - 32 * (p0 + h);
-            bias[h] = take8(!XC && a.bias != nullptr && left > 0 ? a.bias + n : nullptr, WAY != kAnything || a.wide, left);
-            gate[h] = take8(one_sample && left > 0 ? a.gate + sample * a.s_gate + n : nullptr, WAY != kAnything || a.wide, left);
+            bias[h] = take8(!XC && a.bias != nullptr && left > 0 ? a.bias + n : nullptr, a.wide, left);
+            gate[h] = take8(one_sample && left > 0 ? a.gate + sample * a.s_gate + n : nullptr, a.wide, left);
         }
 #pragma unroll
         for (int j = 0; j < MT; j++) {
@@ -445,12 +466,16 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(cons
                 const bool inside = 16 * j < rows_left && left > 0;
                 if constexpr (XC) {
                     if (!inside) continue;
+                    if (a.part == nullptr) {                  // (the whole sum)
+                        store8(a.out + (row * a.ldo + col) + at.out, v, a.wide_out, left);
+                        continue;
+                    }
                     float* const o = a.part + (((int64_t)here.split * a.M + row) * a.ld_part + col) + at.out;
                     *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
                     *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
                 } else {
                     if (inside) {
-                        if (gated && !one_sample) gate[h] = take8(a.gate + (int)(row + lane_row) / a.per_sample * a.s_gate + col + lane_col, WAY != kAnything || a.wide, left);
+                        if (gated && !one_sample) gate[h] = take8(a.gate + (int)(row + lane_row) / a.per_sample * a.s_gate + col + lane_col, a.wide, left);
                         o[h] = way_out<WAY>(a, v, bias[h], gate[h], early[h][j], row, col, at, left, z[h]);
                     }
                     if (whole || !inside) continue;
@@ -480,9 +505,114 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(cons
 #pragma unroll
             for (int j = 0; j < MT; j++) {
                 const int m = here.m0 + wm + 16 * j + lane;
-                if (m < here.m_end) a.part_sum[(int64_t)here.split * a.M + m] = sum[j][0];
+                if (m >= here.m_end) continue;
+                if (a.sums != nullptr) a.sums[m] = (T)sum[j][0];
+                else a.part_sum[(int64_t)here.split * a.M + m] = sum[j][0];
             }
         }
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Few rows (up to 64: single tokens, one vector for each image).  The weight is read once, and there is little else: a workgroup takes 32 columns of C, its
+// eight waves an eighth of the contraction each, through two stages of LDS of their own that nobody else waits for; the sums meet at the end.
+// 8 rows, 2304 > 384 (dx): 6 workgroups of 64 x 64 17.1 us.
+// ---------------------------------------------------------------------------------------
+constexpr int kFewWaves = 8, kFewColumns = 32, kFewStage = kFewColumns * kStep, kFewRows = 64;
+template <typename T, bool YC, int MT, int WAY>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(const Product<T> a) {
+    typedef Operand<T, YC, kFewColumns, 1> OperandY;
+    HIP_DYNAMIC_SHARED(char, shared)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
+    T* const stage = reinterpret_cast<T*>(shared) + wave * 2 * kFewStage;
+    const int n0 = (int)blockIdx.x * kFewColumns;
+    const int all = (int)((a.K + kStep - 1) / kStep), each = (all + kFewWaves - 1) / kFewWaves, first = min(all, wave * each), steps = min(all - first, each);
+
+    OperandY oy;
+    oy.init(0, lane, a.ldy, min(kFewColumns, (YC ? a.ny : a.N) - n0));
+    const int k0 = first * kStep, K = (int)a.K;
+    const T* py = a.y + (YC ? k0 * a.ldy + n0 : n0 * a.ldy + k0);
+    const T* px[MT];
+#pragma unroll
+    for (int j = 0; j < MT; j++) px[j] = a.x + min(16 * j + (lane & 15), a.M - 1) * a.ldx;
+    f32x4 acc[2][MT];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    vec8<T> next[MT][2];
+    auto request = [&](int s) {
+        const int k = k0 + s * kStep;
+        oy.request(py + (YC ? s * kStep * a.ldy : s * kStep), stage + (s & 1) * kFewStage, 0, lane, K - k);
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+                const int at = k + 32 * ks + 8 * quad;
+                next[j][ks] = *reinterpret_cast<const vec8<T>*>(at < K ? px[j] + at : reinterpret_cast<const T*>(kZeros));
+            }
+    };
+    if (steps > 0) request(0);
+    for (int s = 0; s < steps; s++) {
+        vec8<T> fx[MT][2];
+        wave_waits_for_copies();
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) fx[j][ks] = next[j][ks];
+        if (s + 1 < steps) request(s + 1);
+        const T* const ty = stage + (s & 1) * kFewStage;
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const vec8<T> fy = OperandY::fragment(ty, 16 * i, ks, lane);
+#pragma unroll
+                for (int j = 0; j < MT; j++) acc[i][j] = product16(fy, fx[j][ks], acc[i][j]);
+            }
+        wave_waits_for_reads();                               // (done, before the next request but one writes there)
+    }
+
+    // wave j adds up tile j of rows, in the order of the waves
+    __syncthreads();
+    f32x4* const sums = reinterpret_cast<f32x4*>(shared);     // [wave][tile][half][lane]
+#pragma unroll
+    for (int j = 0; j < MT; j++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) sums[((wave * MT + j) * 2 + i) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    if (wave >= MT) return;
+    f32x4 t[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        t[i] = sums[(wave * 2 + i) * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < kFewWaves; w++) t[i] += sums[((w * MT + wave) * 2 + i) * 64 + lane];
+    }
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const u32x2 w = __builtin_amdgcn_permlane16_swap(__float_as_uint(t[0][e]), __float_as_uint(t[1][e]), false, false);
+        v[e] = __uint_as_float(w[0]);
+        v[4 + e] = __uint_as_float(w[1]);
+    }
+    const int lane_col = 16 * (quad & 1) + 8 * (quad >> 1), lane_row = lane & 15, row = 16 * wave, left = a.N - n0 - lane_col, m = row + lane_row;
+    if (m >= a.M || left <= 0) return;
+    const Lane at = {(unsigned)(lane_row * a.ldo) + lane_col, (unsigned)(lane_row * a.ldz) + lane_col, (unsigned)(lane_row * a.ldr) + lane_col};
+    const T* const side = WAY == kAnything || (YC && WAY < kSlope) ? nullptr : WAY >= kSlope ? a.slope_at : a.residual;
+    vec8<T> early = take8<T>(nullptr, true, 0), z;
+    if (side != nullptr) early = *reinterpret_cast<const vec8<T>*>(side + ((int64_t)row * (WAY >= kSlope ? a.ldz : a.ldr) + n0) + (WAY >= kSlope ? at.z : at.residual));
+    const vec8<T> bias = take8(!YC && a.bias != nullptr ? a.bias + n0 + lane_col : nullptr, a.wide, left);
+    const vec8<T> gate = take8(!YC && a.gate != nullptr ? a.gate + m / a.per_sample * a.s_gate + n0 + lane_col : nullptr, a.wide, left);
+    const vec8<T> o = way_out<WAY>(a, v, bias, gate, early, row, n0, at, left, z);
+    if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + ((int64_t)row * a.ldz + n0) + at.z) = z;
+    T* const to = a.out + ((int64_t)row * a.ldo + n0) + at.out;
+    if (WAY != kAnything || a.wide_out) {
+        *reinterpret_cast<vec8<T>*>(to) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < left) to[e] = o[e];
     }
 }
 
@@ -649,17 +779,29 @@ __global__ __launch_bounds__(256) void dgate_kernel(const float* part, T* dgate,
     dgate[i] = (T)v;
 }
 
-// Rows of an odd length or at odd addresses, copied to rows that the products can read: 16-byte aligned, padded with zeros
-__global__ __launch_bounds__(256) void pad_kernel(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int64_t rows, int cols) {
-    const int64_t per = ldy / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * per) return;
-    const int64_t r = i / per;
+// Rows of an odd length or at odd addresses, copied to rows that the products can read: 16-byte aligned, padded with zeros.  Several matrices a launch.
+struct Pads {
+    llsa_pad_job job[LLSA_PAD_JOBS];
+    int64_t end[LLSA_PAD_JOBS];           // pieces of eight, of this and the jobs before it
+};
+__global__ __launch_bounds__(256) void pad_kernel(const Pads a) {
+    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    int k = 0;
+    while (k < LLSA_PAD_JOBS && i >= a.end[k]) k++;
+    if (k == LLSA_PAD_JOBS) return;
+    if (k > 0) i -= a.end[k - 1];
+    const llsa_pad_job q = a.job[k];
+    const int64_t per = q.ldy / 8, r = i / per;
     const int c = (int)(i - r * per) * 8;
+    const uint16_t* const x = static_cast<const uint16_t*>(q.x) + r * q.ldx;
     typedef __attribute__((ext_vector_type(8))) uint16_t u16x8;
     u16x8 v;
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = c + e < cols ? x[r * ldx + c + e] : (uint16_t)0;
-    *reinterpret_cast<u16x8*>(y + r * ldy + c) = v;
+    for (int e = 0; e < 8; e++) {
+        const uint16_t t = x[min(c + e, q.cols - 1)];
+        v[e] = c + e < q.cols ? t : (uint16_t)0;
+    }
+    *reinterpret_cast<u16x8*>(static_cast<uint16_t*>(q.y) + r * q.ldy + c) = v;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -702,6 +844,15 @@ Tiles tiles_for(int64_t M, int64_t N, int64_t K) {
     const double t128 = rounds(128, 128, 2 * kCus), t192 = 1.42 * rounds(192, 128, 2 * kCus), t256 = (1.75 + 160. / (double)K) * rounds(256, 256, kCus);
     return t256 < std::min(t128, t192) ? k256 : t192 < t128 ? k192 : k128;
 }
+template <typename T, bool YC, int WAY>
+int launch_few_rows(const Product<T>& a, hipStream_t stream) {
+    const dim3 grid((unsigned)ceil_div(a.N, kFewColumns)), block(64 * kFewWaves);
+    constexpr int lds = kFewWaves * 2 * kFewStage * (int)sizeof(T);                            // (the sums of up to 64 rows fit in it as well)
+    if (a.M <= 16) hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, YC, 1, WAY>), grid, block, lds, stream, a);
+    else if (a.M <= 32) hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, YC, 2, WAY>), grid, block, lds, stream, a);
+    else hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, YC, 4, WAY>), grid, block, lds, stream, a);
+    return 0;
+}
 template <typename T, bool XC, bool YC, int WAY>
 int launch_way(Product<T>& a, int splits, hipStream_t stream) {
     a.group = (int64_t)a.N * a.K <= (1 << 20) || XC ? 1 : 8;  // (rows of tiles that share y while it does not fit the L2 beside them)
@@ -709,6 +860,7 @@ int launch_way(Product<T>& a, int splits, hipStream_t stream) {
         if (ceil_div(a.M, 128) * ceil_div(a.N, 128) * splits >= kCus) return launch_tiles<T, XC, YC, 128, 128, 2, 2, WAY>(a, splits, stream);
         return launch_tiles<T, XC, YC, 64, 64, 2, 2, WAY>(a, splits, stream);
     } else {
+        if (a.M <= kFewRows && a.y_sample == 0) return launch_few_rows<T, YC, WAY>(a, stream);
         switch (tiles_for(a.M, a.N, a.K)) {
             case k64: return launch_tiles<T, XC, YC, 64, 64, 2, 2, WAY>(a, splits, stream);
             case k128: return launch_tiles<T, XC, YC, 128, 128, 2, 2, WAY>(a, splits, stream);
@@ -722,7 +874,7 @@ int launch_product(Product<T>& a, int splits, hipStream_t stream) {
     if constexpr (XC) {
         return launch_way<T, XC, YC, 0>(a, splits, stream);
     } else {
-        if (!a.wide || !a.wide_out) return launch_way<T, XC, YC, kAnything>(a, splits, stream);
+        if (!a.wide_side || !a.wide_out) return launch_way<T, XC, YC, kAnything>(a, splits, stream);
         if constexpr (YC) {
             switch (a.act) {
                 case LLSA_ACT_SILU: return launch_way<T, XC, YC, kSlope + LLSA_ACT_SILU>(a, splits, stream);
@@ -789,7 +941,8 @@ int linear_fwd(const llsa_linear_args& q, hipStream_t stream) {
     a.residual = (const T*)q.residual; a.ldr = q.ldr;
     a.out = (T*)q.out; a.ldo = q.ldo; a.z = (T*)q.z; a.ldz = q.ldz;
     a.act = q.act;
-    a.wide = q.N % 8 == 0 && wide8(q.bias, 0) && wide8(q.gate, q.s_gate) && wide8(q.residual, q.ldr);
+    a.wide = q.N % 8 == 0 && wide8(q.bias, 0) && wide8(q.gate, q.s_gate);
+    a.wide_side = q.residual == nullptr || (q.N % 8 == 0 && wide8(q.residual, q.ldr));
     a.wide_out = (q.N % 8 == 0 && wide8(q.out, q.ldo)) || q.padded;
     if (int rc = launch_product<T, false, false>(a, 1, stream)) return rc;
     return launch_status("linear_fwd");
@@ -804,7 +957,7 @@ int linear_dx(const llsa_linear_args& q, hipStream_t stream) {
     if (q.s_w != 0) a.rows = (int)q.per_sample;
     a.out = (T*)q.out; a.ldo = q.ldo;
     a.slope_at = (const T*)q.z; a.ldz = q.ldz; a.act = q.z != nullptr ? q.act : LLSA_ACT_NONE;
-    a.wide = q.K % 8 == 0;
+    a.wide = a.wide_side = 1;
     a.wide_out = (q.K % 8 == 0 && wide8(q.out, q.ldo)) || q.padded;
     if (int rc = launch_product<T, false, true>(a, 1, stream)) return rc;
     return launch_status("linear_dx");
@@ -819,6 +972,12 @@ int linear_dw(const llsa_linear_args& q, hipStream_t stream) {
     one_piece(a);
     a.k_sample = p.sample; a.k_piece = p.piece; a.pieces = p.pieces;
     a.ld_part = pad8(q.K);
+    if (q.gate == nullptr && p.count() == 1) {
+        a.out = (T*)q.out; a.ldo = q.ldo; a.sums = (T*)q.dbias;
+        a.wide_out = q.K % 8 == 0 && wide8(q.out, q.ldo);
+        if (int rc = launch_product<T, true, true>(a, 1, stream)) return rc;
+        return launch_status("linear_dw");
+    }
     a.part = (float*)q.workspace;
     a.ldo = a.ld_part;
     const bool sums = q.dbias != nullptr || (q.dgate != nullptr && q.bias != nullptr);
@@ -878,7 +1037,7 @@ using namespace llsa;
 
 extern "C" int64_t llsa_linear_dw_workspace_bytes(int64_t M, int64_t samples, int N, int K) {
     if (M <= 0 || samples <= 0 || N <= 0 || K <= 0) return 0;
-    return 4 * (int64_t)weight_pieces(M, samples, N, K).count() * N * (pad8(K) + 1);
+    return 4 * (int64_t)weight_pieces(M, samples, N, K).count() * N * (pad8(K) + 1);      // (also where the one piece of a layer without a gate goes straight to dW)
 }
 extern "C" int64_t llsa_linear_dz_workspace_bytes(int64_t M, int64_t per_sample, int N) {
     if (M <= 0 || N <= 0 || per_sample <= 0) return 0;
@@ -937,10 +1096,21 @@ extern "C" int llsa_linear_dz(const llsa_linear_args* a, void* stream) {
     LLSA_REQUIRE(a->dgate == nullptr || a->workspace != nullptr, "linear_dz: workspace");
     return BY_TYPE(linear_dz);
 }
-extern "C" int llsa_pad_rows(const void* x, int64_t ldx, void* y, int64_t ldy, int64_t rows, int cols, void* stream) {
-    LLSA_REQUIRE(rows >= 0 && cols > 0 && ldy >= cols && rows16(y, ldy) && x != nullptr, "pad_rows: bad arguments");
-    if (rows == 0) return 0;
-    LLSA_REQUIRE(ceil_div(rows * (ldy / 8), 256) <= kMaxGrid, "pad_rows: too many rows");
-    hipLaunchKernelGGL(pad_kernel, dim3((unsigned)ceil_div(rows * (ldy / 8), 256)), dim3(256), 0, (hipStream_t)stream, (const uint16_t*)x, ldx, (uint16_t*)y, ldy, rows, cols);
+extern "C" int llsa_pad_rows(const llsa_pad_job* jobs, int n, void* stream) {
+    LLSA_REQUIRE(jobs != nullptr && n >= 1 && n <= LLSA_PAD_JOBS, "pad_rows: 1 to %d matrices", LLSA_PAD_JOBS);
+    Pads a{};
+    int64_t total = 0;
+    for (int i = 0; i < LLSA_PAD_JOBS; i++) {
+        if (i < n) {
+            const llsa_pad_job& q = jobs[i];
+            LLSA_REQUIRE(q.rows >= 0 && q.cols > 0 && q.ldy >= q.cols && rows16(q.y, q.ldy) && (q.rows == 0 || q.x != nullptr), "pad_rows: bad arguments");
+            a.job[i] = q;
+            total += q.rows * (q.ldy / 8);
+        }
+        a.end[i] = total;
+    }
+    if (total == 0) return 0;
+    LLSA_REQUIRE(ceil_div(total, 256) <= kMaxGrid, "pad_rows: too many rows");
+    hipLaunchKernelGGL(pad_kernel, dim3((unsigned)ceil_div(total, 256)), dim3(256), 0, (hipStream_t)stream, a);
     return launch_status("pad_rows");
 }
