@@ -323,7 +323,7 @@ def bench_dit(args):
     N = side * side
     torch.manual_seed(0)
     model = PixelDiT(num_layers=layers, num_attention_heads=H, attention_head_dim=D, sample_size=side, sparse_topk=(t2, t1),
-                     fused_prologue=not args.unfused).to(dev)
+                     fused_prologue=not args.unfused, fused_layers=args.fused_layers).to(dev)
     step = FlowMatchingStep(model)
     # images: smooth fields in raster order scaled into [-1, 1]; timesteps uniform in [0, 1000); noise N(0,1)
     f = smooth_field(7, B, 1, N, 3, dtype=torch.float32, mix=(1.0, 0.0), zorder=False).reshape(B, side, side, 3).permute(0, 3, 1, 2)
@@ -367,6 +367,7 @@ def bench_dit(args):
         "config": {"workload": f"c4: DiT-S {layers} layers hidden {H * D} heads {H}x{D}, batch {B} of 3x{side}x{side} (N={N} tokens, "
                                f"Z-order), llsa_l2 topk {t1}/{t2}, qk RMS norm + RoPE "
                                + ("composed before the operator" if args.unfused else "inside the operator")
+                               + (", norms, linear layers and feed-forward blocks by llsa_amd" if args.fused_layers else "")
                                + ", bf16 autocast, AdamW, grad-norm clip 1.0",
                    "parameters": nparams},
         "images_per_s": B / (ms * 1e-3),
@@ -429,6 +430,7 @@ def main():
     ap.add_argument("--workload", default="c3", choices=sorted(WORKLOADS) + ["c4", "fwd_sweep"])
     ap.add_argument("--no-extras", action="store_true", help="skip stage profile, CPU baseline and dense SDPA")
     ap.add_argument("--unfused", action="store_true", help="use the reference's composition (separate pools, autograd adds)")
+    ap.add_argument("--fused-layers", action="store_true", help="c4: layer norms, linear layers and feed-forward blocks by this package's operators")
     ap.add_argument("--calibrate", action="store_true",
                     help="after the timed region also launch a plain elementwise copy of 256 MiB (fp32, read 256 MiB + "
                          "write 256 MiB) five times, so that a counter profile of this command holds a kernel of known "
