@@ -2,7 +2,7 @@
 // the autograd nodes.  Native for the reason operators.cpp is: a layer norm of 1024 tokens runs for a few microseconds.
 #include "block.h"
 
-#include <cstring>
+#include <c10/hip/HIPGraphsC10Utils.h>
 
 namespace {
 
@@ -123,6 +123,22 @@ struct BlockNode : public Node {
     void keep(const Tensor& t, const Tensor& input) { kept.emplace_back(t.is_same(input) ? input : t, false); }
 };
 
+// A graph that is being captured must not reach gradients that another graph on another stream holds: a leaf has one accumulator, tied to the stream
+// it was made on, and a captured backward that has to wait for that stream ends the process (of any operator).
+void refuse_foreign_accumulators(const Library& lib, std::initializer_list<const Tensor*> all) {
+    if (!lib.device || !at::GradMode::is_enabled()) return;
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const Tensor* t : all) {
+        if (t == nullptr || !t->requires_grad() || !t->is_leaf() || !t->is_cuda()) continue;
+        const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!accumulator) continue;
+        const std::optional<c10::Stream> made_on = accumulator->stream();
+        if (made_on.has_value() && *made_on != c10::hip::getCurrentHIPStream(t->device().index()).unwrap())
+            fail(Failure::kRuntime, "llsa_amd: a graph is being captured, and an input's gradient belongs to another graph that is still alive: let go of it first "
+                                    "(delete the outputs of earlier forward passes)");
+    }
+}
+
 // the checks all three begin with
 void begin(const Library& lib, const char* what, const Tensor& x, std::initializer_list<const Tensor*> all) {
     if (torch::jit::tracer::isTracing()) fail(Failure::kRuntime, std::string("llsa_amd ") + what + " cannot be recorded by torch.jit.trace");
@@ -133,6 +149,7 @@ void begin(const Library& lib, const char* what, const Tensor& x, std::initializ
         if (t->device() != x.device()) fail(Failure::kValue, std::string(what) + ": all tensors must be on one device");
     }
     lib.on_device(x);
+    refuse_foreign_accumulators(lib, all);
 }
 bool wants(std::initializer_list<const Tensor*> all) {
     if (!at::GradMode::is_enabled()) return false;
@@ -188,7 +205,7 @@ Tensor small_vector(const Tensor* t, at::ScalarType type) {
 
 struct LayerNormBackward : public BlockNode {
     std::vector<int64_t> sizes;
-    int64_t rows, per_sample, C;
+    int64_t rows, per_sample, samples, C;
     bool has[4];                          // weight, bias, scale, shift
     at::ScalarType types[4], vector_type;
     float eps;
@@ -215,7 +232,7 @@ struct LayerNormBackward : public BlockNode {
         const auto options = grad.options().dtype(vector_type);
         for (int i = 0; i < 4; i++)
             if (has[i] && task_should_compute_output(at_++)) {
-                d[i] = i < 2 ? at::empty({C}, options) : at::empty({rows / per_sample, C}, options);
+                d[i] = i < 2 ? at::empty({C}, options) : at::empty({samples, C}, options);
                 any = true;
             }
         if (rows > 0 && (dx.defined() || any)) {
@@ -285,7 +302,7 @@ Tensor layer_norm(const std::shared_ptr<Library>& lib, const Tensor& x_in, const
         if (grad) {
             node = make_node<LayerNormBackward>(lib);
             node->sizes = x_in.sizes().vec();
-            node->rows = x.count; node->per_sample = samples && B > 0 && x.count == 0 ? 0 : per_sample; node->C = C;
+            node->rows = x.count; node->per_sample = per_sample; node->samples = B; node->C = C;
             node->vector_type = vector_type;
             node->eps = static_cast<float>(eps);
             for (int i = 0; i < 4; i++) {

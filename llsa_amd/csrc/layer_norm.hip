@@ -164,7 +164,7 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const Norm a) {
             add[j][e] = fmaf(add[j][e], 1.f + t[e], u[e]);
         }
     }
-    const float per = 1.f / (float)a.C;
+    const float C = (float)a.C;
     for (int64_t first = share.first; first < share.last; first += kRows) {       // (the same count for all lanes: row sums may meet at barriers)
         const int64_t r = first + row;
         float v[CHUNKS][8], s = 0.f;
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const Norm a) {
                 s += v[j][e];
             }
         if (first + kRows < share.last) request(first + kRows);
-        const float mean = row_sum<LANES>(s, slots) * per;
+        const float mean = row_sum<LANES>(s, slots) / C;     // (divided: the mean of equal values is that value)
         s = 0.f;
 #pragma unroll
         for (int j = 0; j < CHUNKS; j++) {
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const Norm a) {
                 s = fmaf(v[j][e], v[j][e], s);
             }
         }
-        const float rstd = rsqrtf(row_sum<LANES>(s, slots) * per + a.eps);
+        const float rstd = rsqrtf(row_sum<LANES>(s, slots) / C + a.eps);
         if (r >= share.last) continue;
         if (a.stats != nullptr && lane == 0) {
             a.stats[2 * r] = mean;

@@ -625,6 +625,7 @@ __global__ __launch_bounds__(256) void product_join_kernel(const float* part, co
         const int64_t m = i / n4;
         const int n = (int)(i - m * n4) * 4;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
         for (int s = 0; s < splits; s++) v += *reinterpret_cast<const f32x4*>(part + ((int64_t)s * M + m) * ld_part + n);
 #pragma unroll
         for (int e = 0; e < 4; e++)
@@ -649,37 +650,47 @@ struct GatedJoin {
 };
 template <typename T>
 __global__ __launch_bounds__(256) void gated_join_kernel(const GatedJoin a) {
-    HIP_DYNAMIC_SHARED(float, dots)                           // [wave][sample]
+    constexpr int kColumns = 256;                             // of a wave at a time; the four waves take every fourth sample
+    __shared__ f32x4 rows[4][64];
+    HIP_DYNAMIC_SHARED(float, dots)                           // [sample]
     const int m = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const T* const gate = static_cast<const T*>(a.gate) + m;
     const T* const w = static_cast<const T*>(a.w);
-    float* const dot = dots + wave * a.samples;
     if (a.dgate != nullptr)
-        for (int b = lane; b < a.samples; b += 64) dot[b] = 0.f;
-    for (int first = 0; first < a.N; first += 1024) {         // (the same count for all lanes)
-        const int n = first + threadIdx.x * 4;
+        for (int b = threadIdx.x; b < a.samples; b += 256) dots[b] = 0.f;
+    for (int first = 0; first < a.N; first += kColumns) {
+        const int n = first + lane * 4;
         f32x4 v = {0.f, 0.f, 0.f, 0.f}, wn = {0.f, 0.f, 0.f, 0.f};
         if (a.dgate != nullptr)
 #pragma unroll
             for (int e = 0; e < 4; e++) wn[e] = n + e < a.N ? (float)w[m * a.ldw + n + e] : 0.f;
-        for (int b = 0; b < a.samples; b++) {
+        __syncthreads();                                      // (dots are cleared, and the rows of the columns before are read)
+        for (int b = wave; b < a.samples; b += 4) {
             f32x4 g = {0.f, 0.f, 0.f, 0.f};
-            if (n < a.N)
-                for (int p = 0; p < a.pieces; p++) g += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)(b * a.pieces + p) * a.M + m) * a.ld_part + n);
+            if (n < a.N) {
+                const float* part = a.part + ((int64_t)b * a.pieces * a.M + m) * a.ld_part + n;
+#pragma unroll 8
+                for (int p = 0; p < a.pieces; p++) g += *reinterpret_cast<const f32x4*>(part + (int64_t)p * a.M * a.ld_part);
+            }
             v += (float)gate[b * a.s_gate] * g;
             if (a.dgate != nullptr) {
                 float d = 0.f;
 #pragma unroll
                 for (int e = 0; e < 4; e++) d += n + e < a.N ? g[e] * wn[e] : 0.f;
-                d = quad_sum(octet_sum(d));
+                d = octet_sum(d);
                 d += across<8>(d);
-                if (lane == 0) dot[b] += d;
+                d = quad_sum(d);
+                if (lane == 0) dots[b] += d;                  // (a sample is one wave's)
             }
         }
-        if (a.out != nullptr)
+        rows[wave][lane] = v;
+        __syncthreads();
+        if (wave == 0 && a.out != nullptr) {
+            v += rows[1][lane] + rows[2][lane] + rows[3][lane];
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 if (n + e < a.N) static_cast<T*>(a.out)[m * a.ldo + n + e] = (T)v[e];
+        }
     }
     __syncthreads();
     if (wave > 0) return;
@@ -691,8 +702,7 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const GatedJoin a) {
             for (int p = 0; p < a.pieces; p++) s += a.part_sum[(int64_t)(b * a.pieces + p) * a.M + m];
         sum += (float)gate[b * a.s_gate] * s;
         if (a.dgate != nullptr) {
-            float d = bias * s;
-            for (int i = 0; i < 4; i++) d += dots[i * a.samples + b];
+            const float d = dots[b] + bias * s;
             static_cast<T*>(a.dgate)[(int64_t)b * a.M + m] = (T)d;
         }
     }
@@ -988,7 +998,7 @@ int linear_dw(const llsa_linear_args& q, hipStream_t stream) {
         j.part = a.part; j.part_sum = a.part_sum; j.gate = q.gate; j.s_gate = q.s_gate; j.w = q.w; j.ldw = q.ldw; j.bias = q.bias;
         j.out = q.out; j.ldo = q.ldo; j.sums = q.dbias; j.dgate = q.dgate;
         j.ld_part = a.ld_part; j.M = a.M; j.N = a.N; j.samples = p.samples; j.pieces = p.pieces;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_join_kernel<T>), dim3((unsigned)a.M), dim3(256), 4 * 4 * p.samples, stream, j);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_join_kernel<T>), dim3((unsigned)a.M), dim3(256), 4 * p.samples, stream, j);
     } else {
         const int64_t threads = (int64_t)a.M * (a.ld_part / 4) + (q.dbias != nullptr ? a.M : 0);
         hipLaunchKernelGGL(HIP_KERNEL_NAME(product_join_kernel<T>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, stream, a.part, a.part_sum, (T*)q.out, q.ldo,
