@@ -514,9 +514,11 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(cons
 }
 
 // ---------------------------------------------------------------------------------------
-// Few rows (up to 64: single tokens, one vector for each image).  The weight is read once, and there is little else: a workgroup takes 32 columns of C, its
-// eight waves an eighth of the contraction each, through two stages of LDS of their own that nobody else waits for; the sums meet at the end.
-// 8 rows, 2304 > 384 (dx): 6 workgroups of 64 x 64 17.1 us.
+// Few rows: single tokens, one vector for each image, a small image.  A workgroup takes 32 columns of up to 64 rows of C, its eight waves an eighth of the
+// contraction each, through two stages of LDS of their own that nobody else waits for; the sums meet at the end.  Where a row of tiles is all there is the
+// weight is read once, and there is little else.  us, tiles of 64 x 64 / this: 8 rows of 4096 > 4096 29.7 / 7.1 (33 MB of weights: 4.8 TB/s), its dx 40.5 /
+// 13.9; and with up to a workgroup for each CU: 512, 1024 > 1024 (256 workgroups) 10.4 / 7.5, 1024, 1536 > 384 (192) 13.5 / 9.5, 256, 2048 > 2048 (256) 16.8 /
+// 11.6;  beyond: 1024, 1024 > 1024 (512) 10.5 / 12.7, 256, 4096 > 4096 (512) 31 / 36.7, 512, 384 > 1536 (384) 5.9 / 7.3.
 // ---------------------------------------------------------------------------------------
 constexpr int kFewWaves = 8, kFewColumns = 32, kFewStage = kFewColumns * kStep, kFewRows = 64;
 template <typename T, bool YC, int MT, int WAY>
@@ -525,7 +527,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(const Produ
     HIP_DYNAMIC_SHARED(char, shared)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
     T* const stage = reinterpret_cast<T*>(shared) + wave * 2 * kFewStage;
-    const int n0 = (int)blockIdx.x * kFewColumns;
+    const int n0 = (int)blockIdx.x * kFewColumns, row0 = (int)blockIdx.y * 16 * MT;
     const int all = (int)((a.K + kStep - 1) / kStep), each = (all + kFewWaves - 1) / kFewWaves, first = min(all, wave * each), steps = min(all - first, each);
 
     OperandY oy;
@@ -534,7 +536,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(const Produ
     const T* py = a.y + (YC ? k0 * a.ldy + n0 : n0 * a.ldy + k0);
     const T* px[MT];
 #pragma unroll
-    for (int j = 0; j < MT; j++) px[j] = a.x + min(16 * j + (lane & 15), a.M - 1) * a.ldx;
+    for (int j = 0; j < MT; j++) px[j] = a.x + min(row0 + 16 * j + (lane & 15), a.M - 1) * a.ldx;
     f32x4 acc[2][MT];
 #pragma unroll
     for (int i = 0; i < 2; i++)
@@ -596,7 +598,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(const Produ
         v[e] = __uint_as_float(w[0]);
         v[4 + e] = __uint_as_float(w[1]);
     }
-    const int lane_col = 16 * (quad & 1) + 8 * (quad >> 1), lane_row = lane & 15, row = 16 * wave, left = a.N - n0 - lane_col, m = row + lane_row;
+    const int lane_col = 16 * (quad & 1) + 8 * (quad >> 1), lane_row = lane & 15, row = row0 + 16 * wave, left = a.N - n0 - lane_col, m = row + lane_row;
     if (m >= a.M || left <= 0) return;
     const Lane at = {(unsigned)(lane_row * a.ldo) + lane_col, (unsigned)(lane_row * a.ldz) + lane_col, (unsigned)(lane_row * a.ldr) + lane_col};
     const T* const side = WAY == kAnything || (YC && WAY < kSlope) ? nullptr : WAY >= kSlope ? a.slope_at : a.residual;
@@ -854,9 +856,10 @@ Tiles tiles_for(int64_t M, int64_t N, int64_t K) {
     const double t128 = rounds(128, 128, 2 * kCus), t192 = 1.42 * rounds(192, 128, 2 * kCus), t256 = (1.75 + 160. / (double)K) * rounds(256, 256, kCus);
     return t256 < std::min(t128, t192) ? k256 : t192 < t128 ? k192 : k128;
 }
+bool few_rows(int64_t M, int64_t N) { return M <= kFewRows || ceil_div(M, kFewRows) * ceil_div(N, kFewColumns) <= kCus; }
 template <typename T, bool YC, int WAY>
 int launch_few_rows(const Product<T>& a, hipStream_t stream) {
-    const dim3 grid((unsigned)ceil_div(a.N, kFewColumns)), block(64 * kFewWaves);
+    const dim3 grid((unsigned)ceil_div(a.N, kFewColumns), (unsigned)ceil_div(a.M, kFewRows)), block(64 * kFewWaves);
     constexpr int lds = kFewWaves * 2 * kFewStage * (int)sizeof(T);                            // (the sums of up to 64 rows fit in it as well)
     if (a.M <= 16) hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, YC, 1, WAY>), grid, block, lds, stream, a);
     else if (a.M <= 32) hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, YC, 2, WAY>), grid, block, lds, stream, a);
@@ -870,7 +873,7 @@ int launch_way(Product<T>& a, int splits, hipStream_t stream) {
         if (ceil_div(a.M, 128) * ceil_div(a.N, 128) * splits >= kCus) return launch_tiles<T, XC, YC, 128, 128, 2, 2, WAY>(a, splits, stream);
         return launch_tiles<T, XC, YC, 64, 64, 2, 2, WAY>(a, splits, stream);
     } else {
-        if (a.M <= kFewRows && a.y_sample == 0) return launch_few_rows<T, YC, WAY>(a, stream);
+        if (few_rows(a.M, a.N) && a.y_sample == 0) return launch_few_rows<T, YC, WAY>(a, stream);
         switch (tiles_for(a.M, a.N, a.K)) {
             case k64: return launch_tiles<T, XC, YC, 64, 64, 2, 2, WAY>(a, splits, stream);
             case k128: return launch_tiles<T, XC, YC, 128, 128, 2, 2, WAY>(a, splits, stream);

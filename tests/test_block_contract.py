@@ -490,6 +490,35 @@ def test_forward_in_a_captured_graph(op, shape):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("op", OPS)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_training_step_in_a_captured_graph(op, shape):
+    """Forward and backward captured once nothing of the warm-up lives, replayed with new inputs and eager work in between."""
+    dev = torch.device("cuda")
+    t = _inputs(op, dev, **shape)
+    dout = torch.randn(_call(op, t).shape, generator=torch.Generator().manual_seed(77)).to(BF16).to(dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            _grads(op, t, dout=dout)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = _grads(op, t, dout=dout)
+    for seed in (1, 2, 3):
+        new = _inputs(op, dev, seed=seed, **shape)
+        with torch.no_grad():
+            for n, v in new.items():
+                t[n].copy_(v)
+        eager = _grads(op, new, dout=dout)
+        graph.replay()
+        torch.cuda.synchronize()
+        _same(eager, captured)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", OPS)
 def test_capture_with_gradients_alive_is_refused(op):
     """Leaves whose gradients belong to a graph that still lives: a captured forward that would record their backward is an error, and the same without
     gradients is none."""

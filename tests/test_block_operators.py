@@ -89,6 +89,12 @@ def test_linear_gate_in_the_weights(dev, dtype, B, T, K, N):
     check_linear(dev, dtype, B, T, K, N, None, bias=False, gate=True, seed=N)
 
 
+@pytest.mark.parametrize("dtype,act", [(BF16, "silu"), (FP16, None)])
+def test_linear_tiles(dev, dtype, act):
+    """More than a workgroup of few rows for each CU: the smallest tiles."""
+    check_linear(dev, dtype, 2, 515, 8, 500, act, gate=act is None, residual=True)
+
+
 def check_ffn(dev, dtype, B, T, C, F, act="gelu_tanh", bias=True, gate=True, residual=True, N=None, seed=0):
     r = Draw(dev, dtype, seed)
     N = N or C
@@ -118,7 +124,7 @@ def test_feed_forward_gate_in_the_weights(dev, B, T, C, F, N):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-@pytest.mark.parametrize("B,T,K,N", [(3, 5459, 136, 264), (3, 32765, 40, 120), (1, 4090, 1032, 4090), (2, 2046, 1032, 4088), (5, 1639, 320, 1025)])
+@pytest.mark.parametrize("B,T,K,N", [(3, 5459, 136, 264), (3, 32765, 40, 120), (1, 4090, 1032, 4090), (2, 2046, 1032, 4088), (5, 1639, 320, 1025), (3, 1531, 77, 333)])
 def test_large_tiles(dtype, B, T, K, N):
     """Sizes at which the larger tiles are taken, with edges inside them in every direction: each activation once."""
     dev = torch.device("cuda")
