@@ -618,6 +618,140 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_kernel(const Produ
     }
 }
 
+// ---------------------------------------------------------------------------------------
+// Many rows, a short contraction: the weights stay in registers.  A workgroup of twelve waves keeps 384 columns' weights, 32 columns a wave, and takes its
+// rows of x through LDS, 32 at a time and two such tiles ahead: a row is read once for 384 columns of C, and no weight a second time.  131072 rows, us of the
+// tiles / this: 384 > 1536 with GELU and z kept 325 / 252, without 228 / 165 (0.94 PFLOP/s; without its stores 155), dx 384 > 1536 242 / 162, with act'(z) 329 /
+// 248 (3.7 TB/s), 384 > 384 with gate and residual 85 / 72 (4.2 TB/s).  What is left is the multiplication itself (96 registers of weights leave three waves a
+// SIMD and no fragments read ahead).  Eight waves of 48 columns, taking turns on a SIMD with C through LDS as whole rows, measured the same: 240, 164, 176, 283, 74.
+// ---------------------------------------------------------------------------------------
+constexpr int kResWaves = 12, kResColumns = 32 * kResWaves, kResRows = 32, kResStages = 3, kResOwn = 32 * kStep + 64;
+struct Resident { int blocks, slots, tiles, per_sample; };   // blocks of columns, workgroups for each, tiles of rows in all and of a sample
+template <typename T, bool YC, int WAY, int STEPS>
+__global__ __launch_bounds__(64 * kResWaves) void resident_kernel(const Product<T> a, const Resident q) {
+    typedef Operand<T, false, kResRows, 1> OperandX;          // of a step: 4 copies
+    typedef Operand<T, YC, 32, 1> OperandY;
+    constexpr int kStage = kResRows * kStep * STEPS;
+    static_assert(4 * STEPS <= 2 * kResWaves, "two copies of a wave take in a tile");
+    HIP_DYNAMIC_SHARED(char, shared)
+    T* const lds = reinterpret_cast<T*>(shared);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
+    // workgroups of an XCD: the blocks of columns of the same rows side by side
+    const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3, block = local % q.blocks, slot = (local / q.blocks) * 8 + xcd;
+    if (slot >= q.slots) return;
+    const int t0 = (int)((int64_t)q.tiles * slot / q.slots), t1 = (int)((int64_t)q.tiles * (slot + 1) / q.slots);
+    if (t0 >= t1) return;
+    const int n0 = block * kResColumns + 32 * wave;
+    const bool columns = n0 < a.N;                            // (a wave beyond the last column copies, and does no more)
+    const int lane_col = 16 * (quad & 1) + 8 * (quad >> 1), lane_row = lane & 15;
+    // LDS of the wave's own: its weights on their way, 64 of the contraction at a time; bias and gate of its columns, 32 of either
+    T* const own = lds + kResStages * kStage + wave * kResOwn;
+    T* const vectors = own + 32 * kStep;
+
+    vec8<T> fy[2 * STEPS][2];
+    auto weights = [&](const T* w) {
+        OperandY oy;
+        oy.init(0, lane, a.ldy, 32);
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            oy.request(w + (YC ? s * kStep * a.ldy + n0 : n0 * a.ldy + s * kStep), own, 0, lane, kStep);
+            wave_waits_for_copies();
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) fy[2 * s + ks][i] = OperandY::fragment(own, 16 * i, ks, lane);
+            wave_waits_for_reads();
+        }
+    };
+
+    unsigned off[2];                                          // of this wave's two copies of a tile
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        const int i = 2 * wave + c, r = OperandX::row_of(i & 3, lane);
+        off[c] = (unsigned)(r * a.ldx) + (i >> 2) * kStep + OperandX::place_of(r, lane);
+    }
+    // The last rows of a sample are a whole tile as well: it takes in rows of the one before, and stores the same values a second time.
+    auto row_of_tile = [&](int t, int sample) { return sample * a.rows + min((t - sample * q.per_sample) * kResRows, a.rows - kResRows); };
+    auto request = [&](int t) {
+        if (t >= t1 || wave >= 2 * STEPS) return;
+        T* const stage = lds + (t % kResStages) * kStage;
+        const T* const base = a.x + row_of_tile(t, t / q.per_sample) * a.ldx;
+#pragma unroll
+        for (int c = 0; c < 2; c++) copy_to_lds(base + off[c], stage + (2 * wave + c) * 512);
+    };
+    request(t0);
+    request(t0 + 1);
+    const Lane at = {(unsigned)(lane_row * a.ldo) + lane_col, (unsigned)(lane_row * a.ldz) + lane_col, (unsigned)(lane_row * a.ldr) + lane_col};
+    const T* const side = YC && WAY < kSlope ? nullptr : WAY >= kSlope ? a.slope_at : a.residual;
+    if (!YC && columns) {
+        if (lane_row == 0) *reinterpret_cast<vec8<T>*>(vectors + lane_col) = take8(a.bias != nullptr ? a.bias + n0 + lane_col : nullptr, true, 8);
+        weights(a.y);
+    }
+    wait_vm0();
+    for (int t = t0, have = -1; t < t1; t++) {
+        const int sample = t / q.per_sample, m0 = row_of_tile(t, sample);
+        if (sample != have && columns) {
+            if (YC && (have < 0 || a.y_sample != 0)) weights(a.y + sample * a.y_sample);
+            if (!YC && a.gate != nullptr && lane_row == 0) *reinterpret_cast<vec8<T>*>(vectors + 32 + lane_col) = *reinterpret_cast<const vec8<T>*>(a.gate + sample * a.s_gate + n0 + lane_col);
+        }
+        have = sample;
+        // this tile is there (every wave has waited for its copies before its last stores), and the one before it is read
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        request(t + 2);
+        if (!columns) {
+            wait_vm0();
+            continue;
+        }
+        vec8<T> early[2];                                     // what is read on the way out
+        if (side != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                early[j] = __builtin_nontemporal_load(
+                    reinterpret_cast<const vec8<T>*>(side + ((int64_t)(m0 + 16 * j) * (WAY >= kSlope ? a.ldz : a.ldr) + n0) + (WAY >= kSlope ? at.z : at.residual)));
+        }
+        f32x4 acc[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const T* const tx = lds + (t % kResStages) * kStage;
+#pragma unroll
+        for (int ks = 0; ks < 2 * STEPS; ks++) {
+            vec8<T> fx[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) fx[j] = OperandX::fragment(tx + (ks >> 1) * (kResRows * kStep), 16 * j, ks & 1, lane);
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) acc[i][j] = product16(fy[ks][i], fx[j], acc[i][j]);
+        }
+        wait_vm0();
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            __builtin_amdgcn_sched_barrier(0);                // (the weights leave no registers for both at once, nor for bias and gate but here)
+            vec8<T> bias = take8<T>(nullptr, true, 8), gate = bias, z;
+            if (!YC) {
+                bias = *reinterpret_cast<const vec8<T>*>(vectors + lane_col);
+                gate = *reinterpret_cast<const vec8<T>*>(vectors + 32 + lane_col);
+            }
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const u32x2 w = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[0][j][e]), __float_as_uint(acc[1][j][e]), false, false);
+                v[e] = __uint_as_float(w[0]);
+                v[4 + e] = __uint_as_float(w[1]);
+            }
+            const int64_t row = m0 + 16 * j;
+            const vec8<T> o = way_out<WAY>(a, v, bias, gate, early[j], row, n0, at, 8, z);
+            if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (row * a.ldz + n0) + at.z) = z;
+            *reinterpret_cast<vec8<T>*>(a.out + (row * a.ldo + n0) + at.out) = o;
+        }
+    }
+}
+
 // The pieces of dW and db added up
 template <typename T>
 __global__ __launch_bounds__(256) void product_join_kernel(const float* part, const float* part_sum, T* out, int64_t ldo, T* sums, int64_t M, int N, int64_t ld_part,
@@ -856,6 +990,33 @@ Tiles tiles_for(int64_t M, int64_t N, int64_t K) {
     const double t128 = rounds(128, 128, 2 * kCus), t192 = 1.42 * rounds(192, 128, 2 * kCus), t256 = (1.75 + 160. / (double)K) * rounds(256, 256, kCus);
     return t256 < std::min(t128, t192) ? k256 : t192 < t128 ? k192 : k128;
 }
+template <typename T, bool YC, int WAY, int STEPS>
+int launch_resident(const Product<T>& in, hipStream_t stream) {
+    Product<T> a = in;
+    if (!YC && a.gate != nullptr) a.rows = a.per_sample;     // (tiles of one sample)
+    Resident q{};
+    q.blocks = (int)ceil_div(a.N, kResColumns);
+    q.slots = kCus / 8 / q.blocks * 8;
+    q.per_sample = (int)ceil_div(a.rows, kResRows);
+    q.tiles = a.M / a.rows * q.per_sample;
+    constexpr int lds = (kResStages * kResRows * kStep * STEPS + kResWaves * kResOwn) * (int)sizeof(T);
+    auto kernel = resident_kernel<T, YC, WAY, STEPS>;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return fail(-101, "linear: %s", hipGetErrorString(e));
+    hipLaunchKernelGGL(kernel, dim3(kCus), dim3(64 * kResWaves), lds, stream, a, q);
+    return 0;
+}
+// Whether the weights stay in registers: a contraction of five or six steps (four measured no gain, more leave no registers), columns of which a wave has
+// 32 or none and at most a quarter of the waves none, and four tiles for each workgroup, which pay for the weights' way there.  us, tiles / this:
+//     131072, 384 > 384     70 / 52       16384, 384 > 1536    29 / 25      131072, 320 > 1280    161 / 137      samples of 256 rows, each with weights of its own
+//      32768, 384 > 384   17.1 / 17.2      8192, 384 > 1536    17 / 16       32768, 320 > 1280     47 / 39       (131072, dx 384 > 1536)   350 / 269
+//      16384, 384 > 384     11 / 12.5      4096, 384 > 1536    11 / 11.4    131072, 256 > 1024    109 / 109       32768, 384 > 480   21 / 23
+template <bool YC, typename T>
+bool resident(const Product<T>& a) {
+    const int64_t rows = YC ? a.rows : a.gate != nullptr ? a.per_sample : a.M, blocks = ceil_div(a.N, kResColumns);
+    if ((a.K != 5 * kStep && a.K != 6 * kStep) || a.N % 32 != 0 || !a.wide || 4 * a.N < 3 * kResColumns * blocks || blocks > kCus / 8) return false;
+    return rows >= 8 * kResRows && a.M % rows == 0 && (int64_t)a.M * a.N >= 4 * kResRows * kResColumns * blocks * (kCus / 8 / blocks * 8);
+}
 bool few_rows(int64_t M, int64_t N) { return M <= kFewRows || ceil_div(M, kFewRows) * ceil_div(N, kFewColumns) <= kCus; }
 template <typename T, bool YC, int WAY>
 int launch_few_rows(const Product<T>& a, hipStream_t stream) {
@@ -874,6 +1035,9 @@ int launch_way(Product<T>& a, int splits, hipStream_t stream) {
         return launch_tiles<T, XC, YC, 64, 64, 2, 2, WAY>(a, splits, stream);
     } else {
         if (few_rows(a.M, a.N) && a.y_sample == 0) return launch_few_rows<T, YC, WAY>(a, stream);
+        if constexpr (WAY != kAnything) {
+            if (resident<YC>(a)) return a.K == 5 * kStep ? launch_resident<T, YC, WAY, 5>(a, stream) : launch_resident<T, YC, WAY, 6>(a, stream);
+        }
         switch (tiles_for(a.M, a.N, a.K)) {
             case k64: return launch_tiles<T, XC, YC, 64, 64, 2, 2, WAY>(a, splits, stream);
             case k128: return launch_tiles<T, XC, YC, 128, 128, 2, 2, WAY>(a, splits, stream);

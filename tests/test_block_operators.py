@@ -138,3 +138,32 @@ def test_large_tiles(dtype, B, T, K, N):
 def test_large_feed_forward(dtype, B, T, C, F):
     for act in ("gelu_tanh", "gelu", "silu"):
         check_ffn(torch.device("cuda"), dtype, B, T, C, F, act, seed=F)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("B,T,K,N", [(3, 3221, 384, 1472), (2, 20011, 384, 320), (7, 1639, 320, 1184), (33, 289, 384, 1536), (3, 3301, 1536, 384), (2, 4099, 1600, 320)])
+def test_weights_in_registers(dtype, B, T, K, N):
+    """Many rows and a contraction of 320 or 384, forward (K) or back (N): a last tile that overlaps the one before it, columns that end inside a
+    workgroup's, samples that begin anywhere, weights of each sample."""
+    dev = torch.device("cuda")
+    for act, gate, residual in ((None, True, True), ("gelu_tanh", False, True), ("silu", True, False), ("gelu", False, False), (None, False, False)):
+        check_linear(dev, dtype, B, T, K, N, act, gate=gate, residual=residual, seed=N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("B,T,C,F", [(3, 3301, 384, 1536), (1, 8211, 320, 1600), (35, 257, 384, 1536)])
+def test_feed_forward_weights_in_registers(dtype, B, T, C, F):
+    for act in ("gelu_tanh", "gelu", "silu"):
+        check_ffn(torch.device("cuda"), dtype, B, T, C, F, act, seed=F)
+
+
+@pytest.mark.gpu
+def test_weights_in_registers_of_slices():
+    """Rows inside wider ones: the same bits as contiguous rows."""
+    r = Draw(torch.device("cuda"), BF16, 7)
+    x, w, res, g = r(2, 4111, 400).detach(), r(1536, 424).detach(), r(2, 4111, 1552).detach(), r(2, 1536).detach()
+    xs, ws, rs = x[..., 8:392], w[:, 16:400], res[..., 8:1544]
+    a = llsa_amd.linear(xs, ws, None, activation="silu", gate=g, residual=rs)
+    assert torch.equal(a, llsa_amd.linear(xs.contiguous(), ws.contiguous(), None, activation="silu", gate=g, residual=rs.contiguous()))
