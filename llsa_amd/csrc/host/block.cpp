@@ -75,6 +75,17 @@ public:
         if (n > 0) lib_.check(lib_.pad_rows(jobs, n, stream_), "pad_rows");
         copied_.clear();
     }
+    // Rows of a residual, which are read as they lie, up to 2^23 elements apart
+    Rows addend(const Tensor* t) const {
+        Rows r;
+        if (t == nullptr) return r;
+        r = rows_of(*t);
+        if (r.ld > (int64_t(1) << 23)) {
+            r.t = r.t.contiguous();
+            r.ld = r.cols;
+        }
+        return r;
+    }
     Rows operand(const Tensor& t) const {
         Rows r;
         operands({{&t, &r}});
@@ -533,7 +544,7 @@ Tensor linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, const Ten
         if (in.rows > 0) {
             call.operands({{&x_in, &x}, {&w_in, &w}});
             if ((act != LLSA_ACT_NONE && inner) || (gates && !gate_out)) z = call.rows(in.rows, N);
-            layer_fwd(call, x, w, dense_vector(bias_p), gate, residual_p != nullptr ? rows_of(*residual_p) : Rows(), z, out, N, false, in.per_sample(), act, dtype);
+            layer_fwd(call, x, w, dense_vector(bias_p), gate, call.addend(residual_p), z, out, N, false, in.per_sample(), act, dtype);
         } else {
             x.t = x_in;
             w.t = w_in;
@@ -666,7 +677,7 @@ Tensor feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_in, con
             if (inner) z = call.rows(in.rows, F);
             if (gates && !gate_out) y = call.rows(in.rows, N);
             layer_fwd(call, x, w1, dense_vector(b1), Tensor(), Rows(), z, h, hidden.ld, true, 1, act, dtype);
-            layer_fwd(call, hidden, w2, dense_vector(b2), gate, residual_p != nullptr ? rows_of(*residual_p) : Rows(), y, out, N, false, in.per_sample(),
+            layer_fwd(call, hidden, w2, dense_vector(b2), gate, call.addend(residual_p), y, out, N, false, in.per_sample(),
                       LLSA_ACT_NONE, dtype);
         }
         if (grad) {

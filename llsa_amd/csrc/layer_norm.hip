@@ -7,7 +7,8 @@
 // The gradients of all four vectors come out of two sums per sample and channel, S1 = sum of dy and S2 = sum of dy * h.
 //
 // A row is held in registers by LANES lanes, up to CHUNKS pieces of 8 channels each: it is read once, the variance is that of the
-// differences from the mean (no cancellation), and everything is fp32 in between.
+// differences from the mean (no cancellation), and everything is fp32 in between.  Bound by memory: 131072 x 384 in bf16, forward 39.5 us (201 MB, 5.1 TB/s;
+// a large copy 5.2), backward 62.6 (302 MB, 4.8 TB/s), the sums of its pieces 4.6.
 #include <algorithm>
 
 #include "llsa_device.h"
@@ -300,7 +301,7 @@ struct Join {
     const void *weight, *bias, *scale;
     void *dscale, *dshift, *dweight, *dbias;
     int64_t s_scale;
-    int C, pieces, samples;
+    int C, pieces, samples, groups;       // groups: of sixteen channels
     bool f32;
 };
 template <typename T>
@@ -315,7 +316,7 @@ constexpr int kJoinChannels = 16, kJoinLanes = 16;
 template <typename T>
 __global__ __launch_bounds__(256) void norm_join_kernel(const Join a) {
     __shared__ float sums[2][kJoinLanes][kJoinChannels];
-    const int k = threadIdx.x % kJoinChannels, lane = threadIdx.x / kJoinChannels, c = (int)blockIdx.x * kJoinChannels + k, sample = blockIdx.y;
+    const int k = threadIdx.x % kJoinChannels, lane = threadIdx.x / kJoinChannels, sample = (int)blockIdx.x / a.groups, c = ((int)blockIdx.x - sample * a.groups) * kJoinChannels + k;
     float s1 = 0.f, s2 = 0.f;
     if (c < a.C) {
         const float* const part = a.part + (int64_t)sample * a.pieces * 2 * a.C + c;
@@ -463,11 +464,11 @@ int backward(const llsa_layer_norm_args* a, hipStream_t stream) {
     if (sums) {
         Join j{};
         const int64_t samples = a->rows / a->per_sample;
-        j.part = n.part; j.pieces = n.pieces; j.samples = (int)samples; j.C = a->C; j.f32 = n.f32;
+        j.part = n.part; j.pieces = n.pieces; j.samples = (int)samples; j.groups = (int)ceil_div(a->C, kJoinChannels); j.C = a->C; j.f32 = n.f32;
         j.weight = a->weight; j.bias = a->bias; j.scale = a->scale; j.s_scale = a->s_scale;
         j.dscale = a->dscale; j.dshift = a->dshift; j.dweight = a->dweight; j.dbias = a->dbias;
         if (samples > 1 && (a->dweight != nullptr || a->dbias != nullptr)) j.per_sample = n.part + samples * n.pieces * 2 * a->C;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_join_kernel<T>), dim3((unsigned)ceil_div(a->C, kJoinChannels), (unsigned)samples), dim3(256), 0, stream, j);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_join_kernel<T>), dim3((unsigned)(samples * j.groups)), dim3(256), 0, stream, j);
         if (j.per_sample != nullptr) hipLaunchKernelGGL(HIP_KERNEL_NAME(norm_join_samples_kernel<T>), dim3((unsigned)ceil_div(a->C, 256)), dim3(256), 0, stream, j);
     }
     return launch_status("layer_norm_bwd");
@@ -497,7 +498,7 @@ extern "C" int llsa_layer_norm_bwd(const llsa_layer_norm_args* a, void* stream) 
     LLSA_REQUIRE(a->rows > 0, "layer_norm_bwd: no rows");
     LLSA_REQUIRE(a->dy != nullptr && a->stats != nullptr, "layer_norm_bwd: dy and the statistics are needed");
     LLSA_REQUIRE(a->workspace != nullptr || (a->dweight == nullptr && a->dbias == nullptr && a->dscale == nullptr && a->dshift == nullptr), "layer_norm_bwd: workspace");
-    LLSA_REQUIRE(a->rows / a->per_sample <= 65535, "layer_norm_bwd: at most 65535 samples (got %lld)", (long long)(a->rows / a->per_sample));
+    LLSA_REQUIRE(a->rows / a->per_sample <= kMaxGrid / ceil_div(a->C, kJoinChannels), "layer_norm_bwd: too many samples (%lld)", (long long)(a->rows / a->per_sample));
     const hipStream_t s = (hipStream_t)stream;
     return a->dtype == LLSA_DTYPE_BF16 ? backward<bf16>(a, s) : a->dtype == LLSA_DTYPE_F16 ? backward<_Float16>(a, s) : backward<float>(a, s);
 }

@@ -6,6 +6,10 @@
 //
 // All three products are one kernel, C[m][n] = sum over k of X[m,k] Y[n,k], whose operands lie in memory either with the contraction
 // along a row ("rows": x and W of the forward, dz of dx) or across the rows ("columns": W of dx, both operands of dW).
+//
+// Sums are fp32 and what is added, multiplied or activated on the way out is too.  Rounded to 16 bits, besides the results: z where it is kept, and what a
+// product takes in that another made, the hidden rows of a feed-forward block, dz, and gate * W.  The matrix instructions of 16-bit operands are 16 times as
+// fast as those of 32; each such rounding is off by up to 2^-8 of an element (bf16; fp16 2^-11), as a result's own does.
 #include <algorithm>
 #include <cmath>
 
@@ -325,6 +329,10 @@ __device__ __forceinline__ void arrange_lines(vec8<T>& first, vec8<T>& second, i
     second = __builtin_bit_cast(vec8<T>, upper ? high : theirs);
 }
 
+// Two stages of LDS and two workgroups a CU that fill each other's waits.  131072 rows of 384 and 1536 channels, us: forward 1536 > 384 203 (0.76 PFLOP/s), dx
+// 1536 > 384 215, dW 209 (0.74); 8192 x 4096 x 4096 230 (1.19; a library's 200), its dW 332.  What bounds it is the way of the operands from L2 (11 TB/s with 128 x
+// 128 tiles): without the copies 134, 118, 127 and 189, 198, while half of the LDS reads or of the products take off 1 to 9 %.  More stages of 32, three of 64
+// with 256 x 128, and for dW 256 x 192 tiles, with a third less to fetch, are one workgroup a CU or more barriers: dW 280, 270, 226.
 template <typename T, bool XC, bool YC, int BM, int BN, int WAVES_M, int WAVES_N, int WAY>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(const Product<T> a) {
     constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
@@ -752,31 +760,41 @@ __global__ __launch_bounds__(64 * kResWaves) void resident_kernel(const Product<
     }
 }
 
-// The pieces of dW and db added up
+// The pieces of dW and db added up.  Each of a workgroup's four waves takes every fourth piece, of the same 64 places: 56 pieces of 384 x 384 (33 MB) are seven
+// loads deep then, not 28.
 template <typename T>
 __global__ __launch_bounds__(256) void product_join_kernel(const float* part, const float* part_sum, T* out, int64_t ldo, T* sums, int64_t M, int N, int64_t ld_part,
                                                            int splits) {
-    const int64_t n4 = ld_part / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < M * n4) {
-        const int64_t m = i / n4;
-        const int n = (int)(i - m * n4) * 4;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    __shared__ f32x4 rest[3][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t n4 = ld_part / 4, i = (int64_t)blockIdx.x * 64 + lane, m = i < M * n4 ? i / n4 : i - M * n4;
+    const int n = (int)(i - m * n4) * 4;
+    const bool sum = i >= M * n4;                             // of dz's rows
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (!sum) {
 #pragma unroll 8
-        for (int s = 0; s < splits; s++) v += *reinterpret_cast<const f32x4*>(part + ((int64_t)s * M + m) * ld_part + n);
+        for (int s = wave; s < splits; s += 4) v += *reinterpret_cast<const f32x4*>(part + ((int64_t)s * M + m) * ld_part + n);
+    } else if (part_sum != nullptr && m < M) {
+        for (int s = wave; s < splits; s += 4) v[0] += part_sum[(int64_t)s * M + m];
+    }
+    if (wave > 0) rest[wave - 1][lane] = v;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int r = 0; r < 3; r++) v += rest[r][lane];
+    if (!sum) {
 #pragma unroll
         for (int e = 0; e < 4; e++)
             if (n + e < N) out[m * ldo + n + e] = (T)v[e];
-    } else if (part_sum != nullptr && i - M * n4 < M) {
-        const int64_t m = i - M * n4;
-        float v = 0.f;
-        for (int s = 0; s < splits; s++) v += part_sum[(int64_t)s * M + m];
-        sums[m] = (T)v;
+    } else if (part_sum != nullptr && m < M) {
+        sums[m] = (T)v[0];
     }
 }
 
 // The same for a layer whose gate was left out of the products: G_b = dout^T x of sample b, S_b = sum of its rows of dout, in pieces.
 //     dW = sum over b of gate_b G_b,   db = sum of gate_b S_b,   dgate_b = sum over k of W G_b + bias S_b
-// (the last is sum over the rows of dout (x W^T + bias), without those rows).  A workgroup takes a row of G.
+// (the last is sum over the rows of dout (x W^T + bias), without those rows).  A workgroup takes a row of G, in eight waves for every eighth sample of 256
+// columns and eight more for those of the next 256: that many loads are under way at a time (40 pieces of 384 x 1536, 94 MB: 32 us, 2.9 TB/s; four waves 40).
 struct GatedJoin {
     const float *part, *part_sum;
     const void *gate, *w, *bias;
@@ -784,24 +802,25 @@ struct GatedJoin {
     int64_t ld_part, s_gate, ldw, ldo;
     int M, N, samples, pieces;
 };
+constexpr int kJoinSamples = 8, kJoinGroups = 2, kJoinThreads = 64 * kJoinSamples * kJoinGroups;
 template <typename T>
-__global__ __launch_bounds__(256) void gated_join_kernel(const GatedJoin a) {
-    constexpr int kColumns = 256;                             // of a wave at a time; the four waves take every fourth sample
-    __shared__ f32x4 rows[4][64];
-    HIP_DYNAMIC_SHARED(float, dots)                           // [sample]
-    const int m = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(kJoinThreads) void gated_join_kernel(const GatedJoin a) {
+    constexpr int kColumns = 256;                             // of a wave at a time
+    __shared__ f32x4 rows[kJoinGroups][kJoinSamples][64];
+    HIP_DYNAMIC_SHARED(float, dots)                           // [group][sample]
+    const int m = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = wave / kJoinSamples, of = wave % kJoinSamples;
     const T* const gate = static_cast<const T*>(a.gate) + m;
     const T* const w = static_cast<const T*>(a.w);
     if (a.dgate != nullptr)
-        for (int b = threadIdx.x; b < a.samples; b += 256) dots[b] = 0.f;
-    for (int first = 0; first < a.N; first += kColumns) {
-        const int n = first + lane * 4;
+        for (int b = threadIdx.x; b < kJoinGroups * a.samples; b += kJoinThreads) dots[b] = 0.f;
+    for (int first = 0; first < a.N; first += kJoinGroups * kColumns) {
+        const int n = first + group * kColumns + lane * 4;
         f32x4 v = {0.f, 0.f, 0.f, 0.f}, wn = {0.f, 0.f, 0.f, 0.f};
         if (a.dgate != nullptr)
 #pragma unroll
             for (int e = 0; e < 4; e++) wn[e] = n + e < a.N ? (float)w[m * a.ldw + n + e] : 0.f;
         __syncthreads();                                      // (dots are cleared, and the rows of the columns before are read)
-        for (int b = wave; b < a.samples; b += 4) {
+        for (int b = of; b < a.samples; b += kJoinSamples) {
             f32x4 g = {0.f, 0.f, 0.f, 0.f};
             if (n < a.N) {
                 const float* part = a.part + ((int64_t)b * a.pieces * a.M + m) * a.ld_part + n;
@@ -816,13 +835,14 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const GatedJoin a) {
                 d = octet_sum(d);
                 d += across<8>(d);
                 d = quad_sum(d);
-                if (lane == 0) dots[b] += d;                  // (a sample is one wave's)
+                if (lane == 0) dots[group * a.samples + b] += d;      // (a sample is one wave's of each group)
             }
         }
-        rows[wave][lane] = v;
+        rows[group][of][lane] = v;
         __syncthreads();
-        if (wave == 0 && a.out != nullptr) {
-            v += rows[1][lane] + rows[2][lane] + rows[3][lane];
+        if (of == 0 && a.out != nullptr) {
+#pragma unroll
+            for (int r = 1; r < kJoinSamples; r++) v += rows[group][r][lane];
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 if (n + e < a.N) static_cast<T*>(a.out)[m * a.ldo + n + e] = (T)v[e];
@@ -838,7 +858,7 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const GatedJoin a) {
             for (int p = 0; p < a.pieces; p++) s += a.part_sum[(int64_t)(b * a.pieces + p) * a.M + m];
         sum += (float)gate[b * a.s_gate] * s;
         if (a.dgate != nullptr) {
-            const float d = dots[b] + bias * s;
+            const float d = dots[b] + dots[a.samples + b] + bias * s;
             static_cast<T*>(a.dgate)[(int64_t)b * a.M + m] = (T)d;
         }
     }
@@ -849,7 +869,7 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const GatedJoin a) {
     }
 }
 
-// The weights of every sample with its gate: gate_b[n] W[n][k].  Rounded to 16 bits, as dout * gate would be: the products take operands of that size.
+// The weights of every sample with its gate: gate_b[n] W[n][k] (8 samples of 384 x 1536: 5.7 us).  Rounded to 16 bits, as dout * gate would be: the products take operands of that size.
 template <typename T>
 __global__ __launch_bounds__(256) void gate_rows_kernel(const T* w, int64_t ldw, const T* gate, int64_t s_gate, T* out, int64_t ldo, int N, int64_t pieces) {
     const int64_t per = ldo / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -865,7 +885,7 @@ __global__ __launch_bounds__(256) void gate_rows_kernel(const T* w, int64_t ldw,
 
 // ---------------------------------------------------------------------------------------
 // dz = dout * gate * act'(z), and pieces of dgate = sum over a sample's rows of dout * act(z).  A workgroup takes 128 columns of up to `rows` rows
-// of one sample: 16 threads along a row, 16 rows at a time.
+// of one sample: 16 threads along a row, 16 rows at a time.  Bound by memory: it reads dout and z and writes dz once, and nothing here is reused.
 // ---------------------------------------------------------------------------------------
 constexpr int kDzColumns = 128;
 template <typename T>
@@ -1092,6 +1112,7 @@ int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - (1 << 16);
 constexpr int64_t kMaxLd = int64_t(1) << 23;                  // 128 rows of 16 bits then lie within 2^32 bytes
+bool offsets32(int64_t ld) { return ld >= 0 && ld <= kMaxLd; }
 bool rows16(const void* p, int64_t ld) { return p != nullptr && aligned16(p) && ld % 8 == 0 && ld > 0 && ld <= kMaxLd; }
 
 int check_sizes(const char* what, int64_t M, int N, int K, int dtype, int act) {
@@ -1165,10 +1186,10 @@ int linear_dw(const llsa_linear_args& q, hipStream_t stream) {
         j.part = a.part; j.part_sum = a.part_sum; j.gate = q.gate; j.s_gate = q.s_gate; j.w = q.w; j.ldw = q.ldw; j.bias = q.bias;
         j.out = q.out; j.ldo = q.ldo; j.sums = q.dbias; j.dgate = q.dgate;
         j.ld_part = a.ld_part; j.M = a.M; j.N = a.N; j.samples = p.samples; j.pieces = p.pieces;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_join_kernel<T>), dim3((unsigned)a.M), dim3(256), 4 * p.samples, stream, j);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(gated_join_kernel<T>), dim3((unsigned)a.M), dim3(kJoinThreads), 4 * kJoinGroups * p.samples, stream, j);
     } else {
-        const int64_t threads = (int64_t)a.M * (a.ld_part / 4) + (q.dbias != nullptr ? a.M : 0);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_join_kernel<T>), dim3((unsigned)ceil_div(threads, 256)), dim3(256), 0, stream, a.part, a.part_sum, (T*)q.out, q.ldo,
+        const int64_t places = (int64_t)a.M * (a.ld_part / 4) + (q.dbias != nullptr ? a.M : 0);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(product_join_kernel<T>), dim3((unsigned)ceil_div(places, 64)), dim3(256), 0, stream, a.part, a.part_sum, (T*)q.out, q.ldo,
                            (T*)q.dbias, a.M, a.N, a.ld_part, p.count());
     }
     return launch_status("linear_dw");
@@ -1228,7 +1249,8 @@ extern "C" int llsa_linear_fwd(const llsa_linear_args* a, void* stream) {
                  "linear_fwd: rows of x and w must be 16-byte aligned and a multiple of 8 long (zeros beyond the end)");
     LLSA_REQUIRE(a->out != nullptr && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->N))), "linear_fwd: output, padded rows 16-byte aligned and a multiple of 8 long");
     LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->N)), "linear_fwd: rows of z must be 16-byte aligned and padded to a multiple of 8");
-    LLSA_REQUIRE(a->gate == nullptr || a->per_sample > 0, "linear_fwd: rows of a sample");
+    LLSA_REQUIRE(a->gate == nullptr || (a->per_sample > 0 && a->M % a->per_sample == 0), "linear_fwd: rows of a sample, whole samples");
+    LLSA_REQUIRE(offsets32(a->ldo) && (a->residual == nullptr || offsets32(a->ldr)), "linear_fwd: rows of out and residual at most %lld apart", (long long)kMaxLd);
     return BY_TYPE(linear_fwd);
 }
 extern "C" int llsa_linear_dx(const llsa_linear_args* a, void* stream) {
@@ -1240,6 +1262,7 @@ extern "C" int llsa_linear_dx(const llsa_linear_args* a, void* stream) {
     LLSA_REQUIRE(a->s_w == 0 || (a->s_w % 8 == 0 && a->per_sample > 0 && a->M % a->per_sample == 0), "linear_dx: weights of each sample: whole samples, 16-byte aligned");
     LLSA_REQUIRE(a->out != nullptr && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->K))), "linear_dx: output, padded rows 16-byte aligned and a multiple of 8 long");
     LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->K)), "linear_dx: rows of z must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(offsets32(a->ldo), "linear_dx: rows of dx at most %lld apart", (long long)kMaxLd);
     return BY_TYPE(linear_dx);
 }
 extern "C" int llsa_linear_dw(const llsa_linear_args* a, void* stream) {
@@ -1248,7 +1271,7 @@ extern "C" int llsa_linear_dw(const llsa_linear_args* a, void* stream) {
     LLSA_REQUIRE(a->M > 0, "linear_dw: no rows");
     LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->x, a->ldx) && a->lddz >= pad8(a->N) && a->ldx >= pad8(a->K),
                  "linear_dw: rows of dz and x must be 16-byte aligned and padded to a multiple of 8");
-    LLSA_REQUIRE(a->out != nullptr && a->workspace != nullptr && aligned16(a->workspace), "linear_dw: output and workspace (16-byte aligned)");
+    LLSA_REQUIRE(a->out != nullptr && offsets32(a->ldo) && a->workspace != nullptr && aligned16(a->workspace), "linear_dw: output and workspace (16-byte aligned)");
     LLSA_REQUIRE(a->gate == nullptr || (a->per_sample > 0 && a->M % a->per_sample == 0 && a->M / a->per_sample <= LLSA_LINEAR_MAX_GATED_SAMPLES),
                  "linear_dw: a gate needs whole samples, at most %d", LLSA_LINEAR_MAX_GATED_SAMPLES);
     LLSA_REQUIRE(a->dgate == nullptr || (a->gate != nullptr && a->w != nullptr), "linear_dw: dgate needs the gate and the weight");

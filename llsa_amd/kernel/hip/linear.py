@@ -23,7 +23,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
     x is (..., K), weight (N, K), bias (N,), gate (B, N) for an x of (B, ..., K), one row for each sample, residual (..., N); all of
     them bf16 or all fp16.  Sums in fp32, one rounding.  activation: None, "silu", "gelu" (erf) or "gelu_tanh".  Differentiable in
-    all five (once); the backward keeps x, weight and, with an activation or a gate that wants a gradient, x @ weight.T + bias."""
+    all five (once); the backward keeps x, weight and, with an activation (or a gate that wants a gradient, on samples of less than
+    2 K rows), x @ weight.T + bias."""
     lib = current_lib()
     return lib.host.linear(lib.host_library, x, weight, bias, _activation(activation), gate, residual)
 

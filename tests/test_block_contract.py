@@ -564,3 +564,60 @@ def test_rows_beyond_32_bits():
     assert ((dw.double() - sw.double()).abs() <= 2 * 2.0 ** -8 * sw.abs() + 2.0 ** -10).all()
     back = llsa_amd.linear(y.detach(), w.detach().t().contiguous())           # rows of 1032 out
     assert torch.equal(back[at], llsa_amd.linear(y.detach()[at.repeat(20)], w.detach().t().contiguous())[:len(at)])
+
+
+def test_c_calls_check_distances():
+    """Rows so far apart that a kernel's 32-bit offsets would not hold, and a gate for part of a sample."""
+    import ctypes as C
+    from llsa_amd._lib import LIB_PATH, Lib, LinearArgs
+    lib = Lib(LIB_PATH)
+    bad = lambda fn, a, text: (fn(C.byref(a), None) != 0 and text in lib.last_error_string())
+    a = LinearArgs()
+    a.M, a.N, a.K = 8, 8, 8
+    a.x = a.w = a.out = a.dz = a.workspace = a.residual = 1 << 20
+    a.ldx = a.ldw = a.ldo = a.lddz = a.ldr = 8
+    for field in ("ldr", "ldo"):
+        for value in ((1 << 23) + 8, -8):
+            setattr(a, field, value)
+            assert bad(lib.linear_fwd, a, b"apart"), field
+        setattr(a, field, 8)
+    a.gate = 1 << 20
+    for per_sample in (3, 1 << 32):
+        a.per_sample = per_sample
+        assert bad(lib.linear_fwd, a, b"whole samples")
+    a.gate, a.ldo = None, (1 << 23) + 8
+    assert bad(lib.linear_dx, a, b"apart") and bad(lib.linear_dw, a, b"output")
+
+
+def test_residual_of_distant_rows(dev):
+    K, N, far = 16, 24, (1 << 23) + 8
+    g = torch.Generator().manual_seed(5)
+    draw = lambda *s: torch.randn(*s, generator=g).bfloat16().to(dev)
+    x, w, res = draw(3, K), draw(N, K), draw(3, N)
+    wide = torch.empty(2 * far + N, dtype=torch.bfloat16, device=dev).as_strided((3, N), (far, 1))
+    wide.copy_(res)
+    assert torch.equal(llsa_amd.linear(x, w, residual=wide), llsa_amd.linear(x, w, residual=res))
+    w2, short = draw(N, N), dict(activation="silu")
+    assert torch.equal(llsa_amd.feed_forward(x, w, None, w2, residual=wide, **short), llsa_amd.feed_forward(x, w, None, w2, residual=res, **short))
+
+
+@pytest.mark.gpu
+def test_norm_of_many_samples():
+    """More samples than a grid has rows, each with a scale and shift of its own."""
+    B, C = 70001, 24
+    g = torch.Generator().manual_seed(6)
+    x, scale, shift, dout = (torch.randn(*s, generator=g).cuda() for s in ((B, 1, C), (B, C), (B, C), (B, 1, C)))
+    w = torch.randn(C, generator=g).cuda()
+    leaves = [t.requires_grad_() for t in (x, w, scale, shift)]
+    got = torch.autograd.grad(llsa_amd.layer_norm(x, w, scale=scale, shift=shift), leaves, dout)
+    l64 = [t.detach().double().requires_grad_() for t in leaves]
+    d = l64[0] - l64[0].mean(-1, keepdim=True)
+    h = d * (d.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+    ref = torch.autograd.grad(h * l64[1] * (1 + l64[2][:, None]) + l64[3][:, None], l64, dout.double())
+    # in fp32: a few roundings an element; the weight's gradient adds up 70001 rows one after another, 70001 * 2^-24 of the sum of magnitudes
+    for a, b, bound in zip(got, ref, (2e-5, None, 2e-5, 1e-6)):
+        if bound is None:
+            sums = (dout.double() * (h * (1 + l64[2][:, None])).detach()).abs().sum((0, 1))
+            assert ((a - b).abs() <= (B + 64) * 2.0 ** -24 * sums).all()
+        else:
+            assert (a - b).norm() <= bound * b.norm()
