@@ -29,7 +29,8 @@ One JSON line is printed:
 
 --workload c4 times something else, one training step of the operator's caller (a pixel DiT-S with
 llsa_l2 in its 12 attention layers, batch 8 of 3x128x128, bf16 autocast, AdamW), and prints a line
-of its own kind: ms per step, images/s and the share of the step spent in the operator.
+of its own kind: ms per step, images/s and the share of the step spent in the operator.  With --fused-layers
+the layer norms, linear layers and feed-forward blocks around the attention are this package's operators too.
 """
 from __future__ import annotations
 
