@@ -329,9 +329,9 @@ __device__ __forceinline__ void arrange_lines(vec8<T>& first, vec8<T>& second, i
     second = __builtin_bit_cast(vec8<T>, upper ? high : theirs);
 }
 
-// Two stages of LDS and two workgroups a CU that fill each other's waits.  131072 rows of 384 and 1536 channels, us: forward 1536 > 384 203 (0.76 PFLOP/s), dx
-// 1536 > 384 215, dW 209 (0.74); 8192 x 4096 x 4096 230 (1.19; a library's 200), its dW 332.  What bounds it is the way of the operands from L2 (11 TB/s with 128 x
-// 128 tiles): without the copies 134, 118, 127 and 189, 198, while half of the LDS reads or of the products take off 1 to 9 %.  More stages of 32, three of 64
+// Two stages of LDS and two workgroups a CU that fill each other's waits.  131072 rows of 384 and 1536 channels, us: forward 1536 > 384 with gate and
+// residual 194 (0.80 PFLOP/s; 128 x 128 205), dx 1536 > 384 205 (213), dW 209 (0.74); 8192 x 4096 x 4096 230 (1.19; a library's 200), its dW 332.  What bounds it is the way of the operands from L2 (11 TB/s with 128 x
+// 128 tiles): without the copies 134, 118 (of 128 x 128), 127 and 189, 198, while half of the LDS reads or of the products take off 1 to 9 %.  More stages of 32, three of 64
 // with 256 x 128, and for dW 256 x 192 tiles, with a third less to fetch, are one workgroup a CU or more barriers: dW 280, 270, 226.
 template <typename T, bool XC, bool YC, int BM, int BN, int WAVES_M, int WAVES_N, int WAY>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(const Product<T> a) {
@@ -994,20 +994,22 @@ int launch_tiles(Product<T>& a, int splits, hipStream_t stream) {
     return 0;
 }
 // Which tiles.  Measured (us, forward of M rows, K channels in, N out), 64 x 64 / 128 x 128 / 192 x 128 / 256 x 256:
-//     2048, 1024 > 1024    9.6 / 14.6 / 18.7 / 31        32768, 384 > 1536    68 / 56 / 61 / 61
-//     4096, 1024 > 1024     15 / 15.2 / 19.1 / 32       131072, 384 > 1536     - / 214 / 203 / 220
-//     8192, 1024 > 1024     27 / 20.9 / 25.6 / 33       131072, 1536 > 384     - / 203 / 190 / 235
-//     8192, 2048 > 2048     98 / 70 / 78 / 64             8192, 4096 > 4096    - / 260 / 260 / 226
+//     2048, 1024 > 1024    9.6 / 14.6 / 18.7 / 31       131072, 1536 > 384     - / 208 / 197 / 259
+//     4096, 1024 > 1024     15 / 15.2 / 19.1 / 32        65536, 1024 > 1024    - / 188 / 177 / 189
+//     8192, 1024 > 1024     27 / 24.0 / 30.9 / 40        16384, 768 > 768      - / 34 / 41 / 36
+//     8192, 2048 > 2048     98 / 77 / 85 / 75             8192, 4096 > 4096    - / 260 / 260 / 226
 // Small tiles keep a grid of few tiles busy, up to four for each CU.  Beyond that it is rounds times the length of one: two workgroups of 128 x 128 or
-// 192 x 128 fit a CU, one of 256 x 256, and a round of these takes 1, 1.42 and (the longer the contraction, the less its ends weigh) 1.75 + 160 / K.
+// 192 x 128 fit a CU, one of 256 x 256, and a round of these takes 1, 1.3 and 1.8 + 220 / K forward (the shorter the contraction, the more weighs a way out with
+// gate and residual that no second workgroup fills), 1, 1.38 and 1.8 in dx.  Over 82 sizes of 384 to 4608 channels the choice costs 0.5 % more than the
+// best one on average, 9 % at most.
 enum Tiles { k64, k128, k192, k256 };
-Tiles tiles_for(int64_t M, int64_t N, int64_t K) {
+Tiles tiles_for(int64_t M, int64_t N, int64_t K, bool dx) {
     if (ceil_div(M, 64) * ceil_div(N, 64) <= 4 * kCus) return k64;
     const auto rounds = [&](int bm, int bn, int slots) {      // (many rounds run into one another: only the last one is not full)
         const double n = (double)(ceil_div(M, bm) * ceil_div(N, bn)) / slots;
-        return n > 8 ? n + 0.5 : std::ceil(n);
+        return n > 4 ? n + 0.5 : std::ceil(n);
     };
-    const double t128 = rounds(128, 128, 2 * kCus), t192 = 1.42 * rounds(192, 128, 2 * kCus), t256 = (1.75 + 160. / (double)K) * rounds(256, 256, kCus);
+    const double t128 = rounds(128, 128, 2 * kCus), t192 = (dx ? 1.38 : 1.3) * rounds(192, 128, 2 * kCus), t256 = (dx ? 1.8 : 1.8 + 220. / (double)K) * rounds(256, 256, kCus);
     return t256 < std::min(t128, t192) ? k256 : t192 < t128 ? k192 : k128;
 }
 template <typename T, bool YC, int WAY, int STEPS>
@@ -1058,7 +1060,7 @@ int launch_way(Product<T>& a, int splits, hipStream_t stream) {
         if constexpr (WAY != kAnything) {
             if (resident<YC>(a)) return a.K == 5 * kStep ? launch_resident<T, YC, WAY, 5>(a, stream) : launch_resident<T, YC, WAY, 6>(a, stream);
         }
-        switch (tiles_for(a.M, a.N, a.K)) {
+        switch (tiles_for(a.M, a.N, a.K, YC)) {
             case k64: return launch_tiles<T, XC, YC, 64, 64, 2, 2, WAY>(a, splits, stream);
             case k128: return launch_tiles<T, XC, YC, 128, 128, 2, 2, WAY>(a, splits, stream);
             case k192: return launch_tiles<T, XC, YC, 192, 128, 2, 2, WAY>(a, splits, stream);
