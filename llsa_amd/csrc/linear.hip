@@ -92,7 +92,7 @@ __device__ __forceinline__ float activate_slope(int act, float z) {
 // the order of its source pieces; it is the source address that is permuted, never the place in LDS.
 //   rows     ROWS rows of 64 elements.  Piece p (8 elements) of row r holds the row's piece p ^ ((r >> 1) & 7): the 16 rows a fragment read touches then lie in 16 different 16-byte columns of the 256 bytes that all banks hold.
 //   columns  64 rows of ROWS elements.  32-byte granule g of row k holds the row's granule g ^ f(k), f out of bits 0, 1 and 3 of k
-//            (64 elements: 1 and 3, 32: 3): the transposing read takes granules of 4 neighbouring rows in each group of 16 lanes and of
+//            (64 or 192 elements: 1 and 3, 32: 3): the transposing read takes granules of 4 neighbouring rows in each group of 16 lanes and of
 //            rows 8 further in the next, which then lie in different banks.
 // What lies outside the matrix: rows are clamped (their results are not stored), and beyond the end of the contraction zeros are fetched.
 // ---------------------------------------------------------------------------------------
@@ -114,13 +114,13 @@ struct Operand {
 
     static __device__ __forceinline__ int swap(int r) { return (r >> 1) & 7; }
     static __device__ __forceinline__ int turn(int k) {
-        return ROWS == 32 ? (k >> 3) & 1 : ROWS == 64 ? ((k >> 1) & 1) | ((k >> 3) & 1) << 1 : (k & 3) | ((k >> 3) & 1) << 2;
+        return ROWS == 32 ? (k >> 3) & 1 : ROWS % 128 == 64 ? ((k >> 1) & 1) | ((k >> 3) & 1) << 1 : (k & 3) | ((k >> 3) & 1) << 2;
     }
-    // of the lane's j-th piece: its row and its first element along the row, in the tile
-    static __device__ __forceinline__ int row_of(int i, int lane) { return COLUMNS ? i * (512 / ROWS) + lane / kPerRow : i * (64 / kPieces) + lane / kPieces; }
-    static __device__ __forceinline__ int place_of(int row, int lane) {
+    // of the lane's piece of copy i: its row and its first element along the row, in the tile
+    static __device__ __forceinline__ int row_of(int i, int lane) { return COLUMNS ? (i * 64 + lane) / kPerRow : i * (64 / kPieces) + lane / kPieces; }
+    static __device__ __forceinline__ int place_of(int i, int row, int lane) {
         if (!COLUMNS) return ((lane % kPieces) ^ swap(row)) * 8;
-        const int unit = lane % kPerRow;
+        const int unit = i * 64 + lane - row * kPerRow;
         return (((unit >> 1) ^ turn(row)) * 2 + (unit & 1)) * 8;
     }
 
@@ -128,7 +128,7 @@ struct Operand {
     __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int left) {
 #pragma unroll
         for (int j = 0; j < kCopies; j++) {
-            const int r = row_of(wave * kCopies + j, lane), e = place_of(r, lane);
+            const int i = wave * kCopies + j, r = row_of(i, lane), e = place_of(i, r, lane);
             off[j] = COLUMNS ? (unsigned)(r * ld) + (unsigned)min(e, left - 8) : (unsigned)(min(r, left - 1) * ld) + (unsigned)e;
         }
     }
@@ -140,7 +140,7 @@ struct Operand {
         } else {
 #pragma unroll
             for (int j = 0; j < kCopies; j++) {
-                const int r = row_of(wave * kCopies + j, lane), k = COLUMNS ? r : place_of(r, lane);
+                const int i = wave * kCopies + j, r = row_of(i, lane), k = COLUMNS ? r : place_of(i, r, lane);
                 copy_to_lds(k < k_left ? base + off[j] : reinterpret_cast<const T*>(kZeros), tile + (wave * kCopies + j) * 512);
             }
         }
@@ -330,9 +330,9 @@ __device__ __forceinline__ void arrange_lines(vec8<T>& first, vec8<T>& second, i
 }
 
 // Two stages of LDS and two workgroups a CU that fill each other's waits.  131072 rows of 384 and 1536 channels, us: forward 1536 > 384 with gate and
-// residual 194 (0.80 PFLOP/s; 128 x 128 205), dx 1536 > 384 205 (213), dW 209 (0.74); 8192 x 4096 x 4096 230 (1.19; a library's 200), its dW 332.  What bounds it is the way of the operands from L2 (11 TB/s with 128 x
-// 128 tiles): without the copies 134, 118 (of 128 x 128), 127 and 189, 198, while half of the LDS reads or of the products take off 1 to 9 %.  More stages of 32, three of 64
-// with 256 x 128, and for dW 256 x 192 tiles, with a third less to fetch, are one workgroup a CU or more barriers: dW 280, 270, 226.
+// residual 194 (0.80 PFLOP/s; 128 x 128 205), dx 1536 > 384 205 (213), dW 196 (0.79; 215); 8192 x 4096 x 4096 230 (1.19; a library's 200), its dW 332.  What bounds it is the way of the operands from L2 (11 TB/s with 128 x
+// 128 tiles): without the copies 134, 118, 127 (of 128 x 128) and 189, 198, while half of the LDS reads or of the products take off 1 to 9 %.  More stages of 32, three of 64
+// with 256 x 128, and 256 x 192 tiles, with a third less to fetch, are one workgroup a CU or more barriers: dW 280, 270, 226.
 template <typename T, bool XC, bool YC, int BM, int BN, int WAVES_M, int WAVES_N, int WAY>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(const Product<T> a) {
     constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
@@ -676,7 +676,7 @@ __global__ __launch_bounds__(64 * kResWaves) void resident_kernel(const Product<
 #pragma unroll
     for (int c = 0; c < 2; c++) {
         const int i = 2 * wave + c, r = OperandX::row_of(i & 3, lane);
-        off[c] = (unsigned)(r * a.ldx) + (i >> 2) * kStep + OperandX::place_of(r, lane);
+        off[c] = (unsigned)(r * a.ldx) + (i >> 2) * kStep + OperandX::place_of(i & 3, r, lane);
     }
     // The last rows of a sample are a whole tile as well: it takes in rows of the one before, and stores the same values a second time.
     auto row_of_tile = [&](int t, int sample) { return sample * a.rows + min((t - sample * q.per_sample) * kResRows, a.rows - kResRows); };
@@ -1049,10 +1049,14 @@ int launch_few_rows(const Product<T>& a, hipStream_t stream) {
     else hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, YC, 4, WAY>), grid, block, lds, stream, a);
     return 0;
 }
+// dW in tiles of 192 x 128 where they cover its rows with no more than those of 128 x 128 do: a fifth less to fetch for a product, and two of them fit a CU as well.  us, 128 / 192 rows:
+// 131072 rows of 384 and 1536 channels 215 / 196 either way round, of 8 gated samples 256 / 230, 384 x 384 73 / 73
+int dw_rows(int64_t N) { return ceil_div(N, 192) * 192 <= ceil_div(N, 128) * 128 ? 192 : 128; }
 template <typename T, bool XC, bool YC, int WAY>
 int launch_way(Product<T>& a, int splits, hipStream_t stream) {
     a.group = (int64_t)a.N * a.K <= (1 << 20) || XC ? 1 : 8;  // (rows of tiles that share y while it does not fit the L2 beside them)
     if constexpr (XC) {
+        if (dw_rows(a.M) == 192 && ceil_div(a.M, 192) * ceil_div(a.N, 128) * splits >= kCus) return launch_tiles<T, XC, YC, 192, 128, 2, 2, WAY>(a, splits, stream);
         if (ceil_div(a.M, 128) * ceil_div(a.N, 128) * splits >= kCus) return launch_tiles<T, XC, YC, 128, 128, 2, 2, WAY>(a, splits, stream);
         return launch_tiles<T, XC, YC, 64, 64, 2, 2, WAY>(a, splits, stream);
     } else {
@@ -1096,10 +1100,10 @@ bool wide8(const void* p, int64_t ld) { return p == nullptr || (aligned16(p) && 
 
 // The pieces of dW's contraction over the token rows, of which `samples` runs have to be kept apart.  More pieces fill the chip's workgroups more evenly
 // but are more sums to write and read: the products run at about 0.72 PFLOP/s where all workgroups are busy, the sums at 4 TB/s.  131072 rows of 1536 and
-// 384 channels: 14 pieces (504 workgroups of 512) 216 + 7 us; of 8 samples, 1 piece each (288 workgroups) 324 + 15.
+// 384 channels, in 128 x 128: 14 pieces (504 workgroups of 512) 216 + 7 us; of 8 samples, 1 piece each (288 workgroups) 324 + 15.
 struct Pieces { int samples, pieces; int64_t sample, piece; int count() const { return samples * pieces; } };
 Pieces weight_pieces(int64_t M, int64_t samples, int N, int K) {
-    const int64_t tiles = ceil_div(N, 128) * ceil_div(K, 128), rows = M / samples;
+    const int64_t tiles = ceil_div(N, dw_rows(N)) * ceil_div(K, 128), rows = M / samples;
     const double all = 2. * (double)M * N * K / 0.72e9, sums = 8. * (double)samples * N * K / 4e6;      // us
     int64_t best = 1;
     double least = 0;
