@@ -330,9 +330,10 @@ __device__ __forceinline__ void arrange_lines(vec8<T>& first, vec8<T>& second, i
 }
 
 // Two stages of LDS and two workgroups a CU that fill each other's waits.  131072 rows of 384 and 1536 channels, us: forward 1536 > 384 with gate and
-// residual 194 (0.80 PFLOP/s; 128 x 128 205), dx 1536 > 384 205 (213), dW 196 (0.79; 215); 8192 x 4096 x 4096 230 (1.19; a library's 200), its dW 332.  What bounds it is the way of the operands from L2 (11 TB/s with 128 x
-// 128 tiles): without the copies 134, 118, 127 (of 128 x 128) and 189, 198, while half of the LDS reads or of the products take off 1 to 9 %.  More stages of 32, three of 64
-// with 256 x 128, and 256 x 192 tiles, with a third less to fetch, are one workgroup a CU or more barriers: dW 280, 270, 226.
+// residual 194 (0.80 PFLOP/s; 128 x 128 205), dx 1536 > 384 205 (213), dW 196 (0.79; 215); 8192 x 4096 x 4096 230 (1.19; a library's 200), its dW 332.  What
+// bounds it is the way of the operands from L2 (11 TB/s with 128 x 128 tiles): without the copies 134, 118, 127 (of 128 x 128) and 189, 198, while half of
+// the LDS reads or of the products take off 1 to 9 %.  More stages of 32, three of 64 with 256 x 128, and 256 x 192 tiles, with a third less to fetch, are
+// one workgroup a CU or more barriers: dW 280, 270, 226.
 template <typename T, bool XC, bool YC, int BM, int BN, int WAVES_M, int WAVES_N, int WAY>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(const Product<T> a) {
     constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
@@ -1049,8 +1050,8 @@ int launch_few_rows(const Product<T>& a, hipStream_t stream) {
     else hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_kernel<T, YC, 4, WAY>), grid, block, lds, stream, a);
     return 0;
 }
-// dW in tiles of 192 x 128 where they cover its rows with no more than those of 128 x 128 do: a fifth less to fetch for a product, and two of them fit a CU as well.  us, 128 / 192 rows:
-// 131072 rows of 384 and 1536 channels 215 / 196 either way round, of 8 gated samples 256 / 230, 384 x 384 73 / 73
+// dW in tiles of 192 x 128 where they cover its rows with no more than those of 128 x 128 do: a fifth less to fetch for a product, and two of them fit a CU
+// as well.  us, 128 / 192 rows: 131072 rows of 384 and 1536 channels 215 / 196 either way round, of 8 gated samples 256 / 230, 384 x 384 73 / 73
 int dw_rows(int64_t N) { return ceil_div(N, 192) * 192 <= ceil_div(N, 128) * 128 ? 192 : 128; }
 template <typename T, bool XC, bool YC, int WAY>
 int launch_way(Product<T>& a, int splits, hipStream_t stream) {
