@@ -44,7 +44,7 @@ extern "C" {
 #define LLSA_DTYPE_F32 1
 #define LLSA_DTYPE_F16 2
 
-#define LLSA_ABI_VERSION 214     /* changes with every change of a signature or argument structure below */
+#define LLSA_ABI_VERSION 215     /* changes with every change of a signature or argument structure below */
 int llsa_version(void);          /* LLSA_ABI_VERSION of the built library                                    */
 const char* llsa_last_error_string(void);
 
@@ -393,6 +393,8 @@ typedef struct llsa_linear_args {
     void* dbias;            /* (N) or NULL: dw                                                         */
     void* dgate;            /* (M/per_sample, N) contiguous, or NULL: dz, dw                           */
     void* workspace;        /* dw, dz: llsa_linear_{dw,dz}_workspace_bytes                             */
+    void* scales;           /* gate_rows in fp16: written, (M/per_sample, K padded to 8) powers of two in
+                               bf16; dx: read unless NULL.  16-byte aligned                            */
     int64_t ldx, ldw, s_gate, ldr, ldo, ldz, lddout, lddz;
     int64_t s_w;            /* dx: unless 0, every sample has weights of its own, this far apart       */
     int64_t M, per_sample;
@@ -407,7 +409,8 @@ int llsa_linear_dx(const llsa_linear_args* a, void* stream);
 int llsa_linear_dw(const llsa_linear_args* a, void* stream);
 /* A gate without an activation can stay out of the rows.  With `gate` set, llsa_linear_dw takes dout itself as dz (its `samples` is then
  * M / per_sample, else 1) and returns dW and dbias of the gated layer, and dgate unless NULL; llsa_linear_dx takes dout with the gated
- * weights of every sample, which llsa_linear_gate_rows writes: out (M/per_sample, N, K) = gate * w, rows ldo = K padded to a multiple of 8. */
+ * weights of every sample, which llsa_linear_gate_rows writes: out (M/per_sample, N, K) = gate * w, rows ldo = K padded to a multiple of 8.
+ * In fp16 out is divided by the scales, one for each column of a sample, and llsa_linear_dx multiplies dx by them. */
 #define LLSA_LINEAR_MAX_GATED_SAMPLES 1024
 int llsa_linear_gate_rows(const llsa_linear_args* a, void* stream);
 int64_t llsa_linear_dw_workspace_bytes(int64_t M, int64_t samples, int N, int K);

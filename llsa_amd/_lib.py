@@ -85,7 +85,7 @@ class TransposeJob(C.Structure):
 
 
 class LinearArgs(C.Structure):
-    _fields_ = ([(n, c_void_p) for n in ("x", "w", "bias", "gate", "residual", "out", "z", "dout", "dz", "dz_out", "dbias", "dgate", "workspace")]
+    _fields_ = ([(n, c_void_p) for n in ("x", "w", "bias", "gate", "residual", "out", "z", "dout", "dz", "dz_out", "dbias", "dgate", "workspace", "scales")]
                 + [(n, c_int64) for n in ("ldx", "ldw", "s_gate", "ldr", "ldo", "ldz", "lddout", "lddz", "s_w", "M", "per_sample")]
                 + [(n, c_int32) for n in ("N", "K", "act", "dtype", "padded", "reserved")])
 
@@ -151,7 +151,7 @@ _SIGNATURES = {
 
 EXPORTS = tuple(_SIGNATURES)
 CHUNK_FINE_MAX = 256                                        # LLSA_CHUNK_FINE_MAX of include/llsa_hip.h
-ABI_VERSION = 214                                           # LLSA_ABI_VERSION
+ABI_VERSION = 215                                           # LLSA_ABI_VERSION
 STATIC_PARTIALS_MAX = 262144                                # LLSA_STATIC_PARTIALS_MAX
 
 

@@ -363,14 +363,17 @@ Rows layer_dz(const Call& call, const Rows& dout_any, const Tensor& dout, const 
 // Whether the gate of a layer without an activation stays out of the rows in the backward.  It then costs sums and weights of every sample, 12 N K bytes
 // each, in place of passes over its rows: dout and the kept x W^T + b in, dz out, that kept in the forward, 10 T N bytes.
 bool gate_in_weights(int64_t per_sample, int64_t samples, int64_t K) { return per_sample >= 2 * K && samples <= LLSA_LINEAR_MAX_GATED_SAMPLES; }
-// every sample's weights with its gate
+// every sample's weights with its gate; behind them, in fp16, a row of scales for each sample
+void* scales_of(const Rows& gated, int64_t samples, int dtype) {
+    return dtype == LLSA_DTYPE_F16 ? static_cast<char*>(gated.p()) + 2 * samples * gated.count * gated.ld : nullptr;
+}
 Rows gated_weights(const Call& call, const Rows& w, const Tensor& gate, int64_t samples, int dtype) {
     Rows r;
-    r.t = call.rows(samples * w.count, w.cols);
+    r.t = call.rows(samples * (w.count + (dtype == LLSA_DTYPE_F16)), w.cols);
     r.ld = r.t.size(1); r.count = w.count; r.cols = w.cols;
     llsa_linear_args a{};
     a.w = w.p(); a.ldw = w.ld; a.gate = gate.data_ptr(); a.s_gate = gate.size(0) > 1 ? gate.stride(0) : 0;
-    a.out = r.p(); a.ldo = r.ld;
+    a.out = r.p(); a.ldo = r.ld; a.scales = scales_of(r, samples, dtype);
     a.M = samples; a.per_sample = 1; a.N = static_cast<int32_t>(w.count); a.K = static_cast<int32_t>(w.cols); a.dtype = dtype;
     call.lib().check(call.lib().linear_gate_rows(&a, call.stream()), "linear_gate_rows");
     return r;
@@ -381,7 +384,10 @@ void layer_dx(const Call& call, const Rows& dz, const Rows& w, const Tensor& out
     a.dz = dz.p(); a.lddz = dz.ld; a.w = w.p(); a.ldw = w.ld;
     a.out = out.data_ptr(); a.ldo = ldo;
     if (z.defined()) { a.z = z.data_ptr(); a.ldz = z.size(1); a.act = act; a.padded = 1; }
-    if (per_sample > 0) a.s_w = w.count * w.ld;
+    if (per_sample > 0) {
+        a.s_w = w.count * w.ld;
+        a.scales = scales_of(w, dz.count / per_sample, dtype);
+    }
     a.M = dz.count; a.per_sample = std::max<int64_t>(1, per_sample); a.N = static_cast<int32_t>(dz.cols); a.K = static_cast<int32_t>(w.cols); a.dtype = dtype;
     call.lib().check(call.lib().linear_dx(&a, call.stream()), "linear_dx");
 }

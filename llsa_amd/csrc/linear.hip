@@ -9,9 +9,11 @@
 //
 // Sums are fp32 and what is added, multiplied or activated on the way out is too.  Rounded to 16 bits, besides the results: z where it is kept, and what a
 // product takes in that another made, the hidden rows of a feed-forward block, dz, and gate * W.  The matrix instructions of 16-bit operands are 16 times as
-// fast as those of 32; each such rounding is off by up to 2^-8 of an element (bf16; fp16 2^-11), as a result's own does.
+// fast as those of 32; each such rounding is off by up to 2^-8 of an element (bf16; fp16 2^-11), as a result's own is.  In fp16 that ends at 2^-14, below which
+// half a step is 2^-25: z, hidden rows and dz lie there as a result would, and a scale of the loss moves dz.  Of gate * W it does not, so that is scaled here.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "llsa_device.h"
 #include "llsa_host.h"
@@ -174,6 +176,8 @@ struct Product {
     // dx with weights of its own for each sample: rows and rows of tiles of a sample, elements from one sample's weights to the next's.  Else: one sample.
     int rows, tiles_rows;
     int64_t y_sample;
+    const bf16* scales;                   // fp16: powers of two that the columns of each sample's weights were divided by, rows s_scales apart, or NULL
+    int64_t s_scales;
     // dW: the contraction in pieces, `pieces` of k_piece rows (a multiple of 64) for every k_sample of them.  Else: one piece.
     int64_t k_piece, k_sample;
     int pieces;
@@ -252,6 +256,24 @@ enum Way { kSlope = 4, kAnything = 8 };
 // Where a lane's eight values of one row of C lie in the tensors of the way out.  Uniform parts are kept apart from the lane's (32 bits, the same for
 // all rows of its tile), so that one register a tensor addresses them all.
 struct Lane { unsigned out, z, residual; };
+
+// Those of a lane's eight columns, and the columns multiplied by them: nothing but in dx of fp16
+template <bool YC, typename T>
+__device__ __forceinline__ bf16x8 take_scales(const Product<T>& a, int sample, int n, bool inside) {
+    bf16x8 up = take8<bf16>(nullptr, true, 8);
+    if constexpr (YC && std::is_same_v<T, _Float16>) {
+        if (a.scales != nullptr && inside) up = *reinterpret_cast<const bf16x8*>(a.scales + sample * a.s_scales + n);
+    }
+    return up;
+}
+template <bool YC, typename T>
+__device__ __forceinline__ void put_back(const Product<T>& a, float (&v)[8], const bf16x8& up) {
+    if constexpr (YC && std::is_same_v<T, _Float16>) {
+        if (a.scales == nullptr) return;
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] *= (float)up[e];
+    }
+}
 
 // Eight values on their way out: columns n .. n + 7 of row m, `left` of them inside the matrix; row and col are the uniform parts of m and n.  Returns
 // what out gets, and in z what the backward wants of it.
@@ -449,11 +471,13 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(cons
     for (int p0 = 0; p0 < NT / 2; p0 += kPair) {
         constexpr int kPairs = kPair;
         vec8<T> bias[kPair], gate[kPair];
+        bf16x8 up[kPair];
 #pragma unroll
         for (int h = 0; h < kPairs; h++) {
             const int n = col0 + lane_col + 32 * (p0 + h), left = cols_left - 32 * (p0 + h);
             bias[h] = take8(!XC && a.bias != nullptr && left > 0 ? a.bias + n : nullptr, a.wide, left);
             gate[h] = take8(one_sample && left > 0 ? a.gate + sample * a.s_gate + n : nullptr, a.wide, left);
+            up[h] = take_scales<!XC && YC>(a, here.sample, n, left > 0);
         }
 #pragma unroll
         for (int j = 0; j < MT; j++) {
@@ -484,6 +508,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product_kernel(cons
                     *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
                 } else {
                     if (inside) {
+                        put_back<YC>(a, v, up[h]);
                         if (gated && !one_sample) gate[h] = take8(a.gate + (int)(row + lane_row) / a.per_sample * a.s_gate + col + lane_col, a.wide, left);
                         o[h] = way_out<WAY>(a, v, bias[h], gate[h], early[h][j], row, col, at, left, z[h]);
                     }
@@ -701,6 +726,9 @@ __global__ __launch_bounds__(64 * kResWaves) void resident_kernel(const Product<
         const int sample = t / q.per_sample, m0 = row_of_tile(t, sample);
         if (sample != have && columns) {
             if (YC && (have < 0 || a.y_sample != 0)) weights(a.y + sample * a.y_sample);
+            if constexpr (YC && std::is_same_v<T, _Float16>) {
+                if (lane_row == 0) *reinterpret_cast<bf16x8*>(vectors + lane_col) = take_scales<YC>(a, sample, n0 + lane_col, true);
+            }
             if (!YC && a.gate != nullptr && lane_row == 0) *reinterpret_cast<vec8<T>*>(vectors + 32 + lane_col) = *reinterpret_cast<const vec8<T>*>(a.gate + sample * a.s_gate + n0 + lane_col);
         }
         have = sample;
@@ -753,6 +781,7 @@ __global__ __launch_bounds__(64 * kResWaves) void resident_kernel(const Product<
                 v[e] = __uint_as_float(w[0]);
                 v[4 + e] = __uint_as_float(w[1]);
             }
+            if constexpr (YC) put_back<YC>(a, v, *reinterpret_cast<const bf16x8*>(vectors + lane_col));
             const int64_t row = m0 + 16 * j;
             const vec8<T> o = way_out<WAY>(a, v, bias, gate, early[j], row, n0, at, 8, z);
             if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (row * a.ldz + n0) + at.z) = z;
@@ -870,18 +899,68 @@ __global__ __launch_bounds__(kJoinThreads) void gated_join_kernel(const GatedJoi
     }
 }
 
-// The weights of every sample with its gate: gate_b[n] W[n][k] (8 samples of 384 x 1536: 5.7 us).  Rounded to 16 bits, as dout * gate would be: the products take operands of that size.
-template <typename T>
-__global__ __launch_bounds__(256) void gate_rows_kernel(const T* w, int64_t ldw, const T* gate, int64_t s_gate, T* out, int64_t ldo, int N, int64_t pieces) {
+// The weights of every sample with its gate: gate_b[n] W[n][k] (8 samples of 384 x 1536: 5.7 us).  Rounded to 16 bits, as dout * gate would be: the products
+// take operands of that size.  bf16 has fp32's range for it.
+__global__ __launch_bounds__(256) void gate_rows_kernel(const bf16* w, int64_t ldw, const bf16* gate, int64_t s_gate, bf16* out, int64_t ldo, int N, int64_t pieces) {
     const int64_t per = ldo / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= pieces) return;
     const int64_t r = i / per, b = r / N;
     const int n = (int)(r - b * N), c = (int)(i - r * per) * 8;
     const float g = (float)gate[b * s_gate + n];
-    vec8<T> v = *reinterpret_cast<const vec8<T>*>(w + n * ldw + c);
+    bf16x8 v = *reinterpret_cast<const bf16x8*>(w + n * ldw + c);
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = (T)((float)v[e] * g);
-    *reinterpret_cast<vec8<T>*>(out + r * ldo + c) = v;
+    for (int e = 0; e < 8; e++) v[e] = (bf16)((float)v[e] * g);
+    *reinterpret_cast<bf16x8*>(out + r * ldo + c) = v;
+}
+// fp16 has not: the gates of an adaLN-zero block begin at zero, and a product below 2^-14 loses its bits.  Every column of a sample is divided by a power of two
+// that brings the largest of its products to 2^14 .. 2^15, and dx is multiplied by it in fp32.  What is 2^-28 and less of that largest one is rounded by up to
+// 2^-39 of it, far below the 2^-24 that a sum in fp32 is off by.  A workgroup takes 64 columns of a sample, 32 rows at a time, and reads them twice.
+constexpr int kScaleColumns = 64, kScaleRows = 32;
+__global__ __launch_bounds__(256) void gate_rows_scaled_kernel(const _Float16* w, int64_t ldw, const _Float16* gate, int64_t s_gate, _Float16* out, int64_t ldo, bf16* scales,
+                                                               int N, int groups) {
+    __shared__ float most[kScaleRows][kScaleColumns + 8];
+    const int64_t b = (int)blockIdx.x / groups;
+    const int group = (int)blockIdx.x - (int)b * groups, lane = threadIdx.x & 7, row = threadIdx.x >> 3, c = group * kScaleColumns + lane * 8;
+    const bool inside = c < ldo;                              // (whole pieces of eight)
+    auto products = [&](int n, float (&v)[8]) {
+        const float g = (float)gate[b * s_gate + n];
+        const f16x8 a = *reinterpret_cast<const f16x8*>(w + n * ldw + c);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = (float)a[e] * g;   // (exact)
+    };
+    float top[8], v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) top[e] = 0.f;
+    if (inside)
+        for (int n = row; n < N; n += kScaleRows) {
+            products(n, v);
+#pragma unroll
+            for (int e = 0; e < 8; e++) top[e] = fmaxf(top[e], fabsf(v[e]));       // (of a NaN and a number the number)
+        }
+#pragma unroll
+    for (int e = 0; e < 8; e++) most[row][lane * 8 + e] = top[e];
+    __syncthreads();
+    if (!inside) return;
+    float down[8];
+    bf16x8 up;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        float m = 0.f;
+#pragma unroll 4
+        for (int r = 0; r < kScaleRows; r++) m = fmaxf(m, most[r][lane * 8 + e]);
+        // the exponent of m, which is 0 or in 2^-48 .. 2^32, or an infinity
+        const int exponent = (int)(__float_as_uint(m) >> 23), k = m == 0.f || exponent == 255 ? 0 : exponent - 127 - 14;
+        down[e] = __uint_as_float((unsigned)(127 - k) << 23);
+        up[e] = (bf16)__uint_as_float((unsigned)(127 + k) << 23);
+    }
+    if (row == 0) *reinterpret_cast<bf16x8*>(scales + b * ldo + c) = up;
+    for (int n = row; n < N; n += kScaleRows) {
+        products(n, v);
+        f16x8 o;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = (_Float16)(v[e] * down[e]);
+        *reinterpret_cast<f16x8*>(out + (b * N + n) * ldo + c) = o;
+    }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1157,6 +1236,7 @@ int linear_dx(const llsa_linear_args& q, hipStream_t stream) {
     Product<T> a{};
     a.x = (const T*)q.dz; a.ldx = q.lddz;
     a.y = (const T*)q.w; a.ldy = q.ldw; a.y_sample = q.s_w;
+    a.scales = (const bf16*)q.scales; a.s_scales = pad8(q.K);
     a.M = (int)q.M; a.N = q.K; a.ny = (int)pad8(q.K); a.K = q.N;
     one_piece(a);
     if (q.s_w != 0) a.rows = (int)q.per_sample;
@@ -1203,9 +1283,14 @@ int linear_dw(const llsa_linear_args& q, hipStream_t stream) {
 }
 template <typename T>
 int gate_rows(const llsa_linear_args& q, hipStream_t stream) {
-    const int64_t pieces = q.M / q.per_sample * q.N * (q.ldo / 8);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(gate_rows_kernel<T>), dim3((unsigned)ceil_div(pieces, 256)), dim3(256), 0, stream, (const T*)q.w, q.ldw, (const T*)q.gate, q.s_gate, (T*)q.out,
-                       q.ldo, q.N, pieces);
+    if constexpr (std::is_same_v<T, _Float16>) {
+        const int groups = (int)ceil_div(q.ldo, kScaleColumns);
+        hipLaunchKernelGGL(gate_rows_scaled_kernel, dim3((unsigned)(q.M / q.per_sample * groups)), dim3(256), 0, stream, (const T*)q.w, q.ldw, (const T*)q.gate, q.s_gate, (T*)q.out,
+                           q.ldo, (bf16*)q.scales, q.N, groups);
+    } else {
+        const int64_t pieces = q.M / q.per_sample * q.N * (q.ldo / 8);
+        hipLaunchKernelGGL(gate_rows_kernel, dim3((unsigned)ceil_div(pieces, 256)), dim3(256), 0, stream, (const T*)q.w, q.ldw, (const T*)q.gate, q.s_gate, (T*)q.out, q.ldo, q.N, pieces);
+    }
     return launch_status("linear_gate_rows");
 }
 struct DzPieces { int count, rows; };
@@ -1266,6 +1351,7 @@ extern "C" int llsa_linear_dx(const llsa_linear_args* a, void* stream) {
     if (a->M == 0) return 0;
     LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->w, a->ldw) && a->lddz >= pad8(a->N) && a->ldw >= pad8(a->K),
                  "linear_dx: rows of dz and w must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->scales == nullptr || (a->s_w != 0 && a->dtype == LLSA_DTYPE_F16 && aligned16(a->scales)), "linear_dx: scales go with fp16 weights of each sample");
     LLSA_REQUIRE(a->s_w == 0 || (a->s_w % 8 == 0 && a->per_sample > 0 && a->M % a->per_sample == 0), "linear_dx: weights of each sample: whole samples, 16-byte aligned");
     LLSA_REQUIRE(a->out != nullptr && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->K))), "linear_dx: output, padded rows 16-byte aligned and a multiple of 8 long");
     LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->K)), "linear_dx: rows of z must be 16-byte aligned and padded to a multiple of 8");
@@ -1290,7 +1376,9 @@ extern "C" int llsa_linear_gate_rows(const llsa_linear_args* a, void* stream) {
     if (a->M == 0) return 0;
     LLSA_REQUIRE(a->gate != nullptr && a->per_sample > 0 && a->M % a->per_sample == 0, "linear_gate_rows: gate, whole samples");
     LLSA_REQUIRE(rows16(a->w, a->ldw) && rows16(a->out, a->ldo) && a->ldo == pad8(a->K) && a->ldw >= a->ldo, "linear_gate_rows: rows 16-byte aligned and padded to a multiple of 8");
-    LLSA_REQUIRE(ceil_div(a->M / a->per_sample * a->N * (a->ldo / 8), 256) <= kMaxGrid, "linear_gate_rows: too many samples");
+    LLSA_REQUIRE(a->dtype != LLSA_DTYPE_F16 || (a->scales != nullptr && aligned16(a->scales)), "linear_gate_rows: fp16 needs room for the scales, 16-byte aligned");
+    LLSA_REQUIRE(ceil_div(a->M / a->per_sample * a->N * (a->ldo / 8), 256) <= kMaxGrid && a->M / a->per_sample * ceil_div(a->ldo, kScaleColumns) <= kMaxGrid,
+                 "linear_gate_rows: too many samples");
     return BY_TYPE(gate_rows);
 }
 extern "C" int llsa_linear_dz(const llsa_linear_args* a, void* stream) {
