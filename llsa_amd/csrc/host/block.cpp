@@ -101,8 +101,15 @@ private:
 
 // The node of an operator with one output: what is common to the three of them.  `kept` are the saved tensors in the order run() unpacks them.
 struct BlockNode : public Node {
+    struct Kind {                         // of a saved tensor, which its hooks have to give back: the kernels' sizes come from the node.  Strides may differ.
+        bool defined;
+        std::vector<int64_t> sizes;
+        at::ScalarType type;
+        at::Device device;
+    };
     std::shared_ptr<Library> lib;
     std::vector<SavedVariable> kept;
+    std::vector<Kind> kinds;
     bool released = false;
 
     void release_variables() override {
@@ -118,7 +125,13 @@ struct BlockNode : public Node {
             if (!grads[0].defined()) return variable_list(num_outputs());
             // (before the autograd keys are left out: a hook may run the forward again)
             std::vector<Tensor> saved;
-            for (SavedVariable& s : kept) saved.push_back(s.unpack(shared_from_this()));
+            for (size_t i = 0; i < kept.size(); i++) {
+                saved.push_back(kept[i].unpack(shared_from_this()));
+                const Tensor& t = saved.back();
+                const Kind& k = kinds[i];
+                if (t.defined() != k.defined || (k.defined && (t.layout() != at::kStrided || t.sizes() != k.sizes || t.scalar_type() != k.type || t.device() != k.device)))
+                    fail(Failure::kRuntime, "llsa_amd: a saved-tensor hook returned another tensor than it was given");
+            }
             at::AutoDispatchBelowADInplaceOrView below;
             c10::OptionalDeviceGuard guard(lib->device ? std::optional<at::Device>(grads[0].device()) : std::nullopt);
             return run(grads[0], saved);
@@ -126,12 +139,11 @@ struct BlockNode : public Node {
     }
     virtual variable_list run(const Tensor& grad, const std::vector<Tensor>& saved) = 0;
     // a tensor that only the kernels read, as they left it
-    static Tensor as_kept(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
-        if (!t.defined() || t.sizes() != sizes || t.scalar_type() != type)
-            fail(Failure::kRuntime, "llsa_amd: a saved-tensor hook returned another tensor than it was given");
-        return t.is_contiguous() && aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+    static Tensor as_kept(const Tensor& t) { return t.is_contiguous() && aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+    void keep(const Tensor& t, const Tensor& input) {
+        kinds.push_back(t.defined() ? Kind{true, t.sizes().vec(), t.scalar_type(), t.device()} : Kind{false, {}, at::kFloat, at::kCPU});
+        kept.emplace_back(t.is_same(input) ? input : t, false);
     }
-    void keep(const Tensor& t, const Tensor& input) { kept.emplace_back(t.is_same(input) ? input : t, false); }
 };
 
 // A graph that is being captured must not reach gradients that another graph on another stream holds: a leaf has one accumulator, tied to the stream
@@ -223,7 +235,7 @@ struct LayerNormBackward : public BlockNode {
     std::string name() const override { return "LayerNormBackward"; }
     variable_list run(const Tensor& grad, const std::vector<Tensor>& saved) override {
         Call call(*lib, grad);
-        const Tensor stats = as_kept(saved[1], {rows, 2}, at::kFloat);
+        const Tensor stats = as_kept(saved[1]);
         const Rows x = rows_of(saved[0]), dy = rows_of(grad);
         NormInputs v;
         v.vtype = vector_type == at::kFloat ? LLSA_DTYPE_F32 : dtype_of(saved[0], true, "layer_norm");
@@ -491,7 +503,7 @@ struct LinearBackward : public BlockNode {
         Tensor dx, dw, db, dg;
         if (want_x) dx = at::empty(sizes, grad.options());
         if (rows > 0) {
-            const Tensor z = has_z ? as_kept(saved[3], {rows, pad8(N)}, grad.scalar_type()) : Tensor();
+            const Tensor z = has_z ? as_kept(saved[3]) : Tensor();
             const Tensor gate = has_gate ? dense_vector(&saved[2]) : Tensor();
             if (want_x || want_w || want_b || want_g) {
                 const Rows dz = gate_out ? call.operand(grad) : layer_dz(call, rows_of(grad), grad, gate, z, per_sample, act, dtype, want_g ? &dg : nullptr);
@@ -597,14 +609,13 @@ struct FeedForwardBackward : public BlockNode {
         if (want_x) dx = at::empty(sizes, grad.options());
         const auto o = grad.options();
         if (rows > 0 && (inner || outer || want_g)) {
-            const auto type = grad.scalar_type();
             const Tensor gate = has_gate ? dense_vector(&saved[3]) : Tensor();
-            const Tensor y = has_y ? as_kept(saved[6], {rows, pad8(N)}, type) : Tensor();
+            const Tensor y = has_y ? as_kept(saved[6]) : Tensor();
             const Rows dz2 = gate_out ? call.operand(grad) : layer_dz(call, rows_of(grad), grad, gate, y, per_sample, LLSA_ACT_NONE, dtype, want_g ? &dg : nullptr);
             const Rows w2 = inner || (gate_out && want_g) ? kept_operand(call, saved[2], F) : Rows();
             if (outer || (gate_out && want_g)) {
                 Rows h;
-                h.t = as_kept(saved[5], {rows, pad8(F)}, type);
+                h.t = as_kept(saved[5]);
                 h.ld = h.t.size(1); h.count = rows; h.cols = F;
                 dw2 = at::empty({N, F}, o);
                 if (want_b2) db2 = at::empty({N}, o);
@@ -620,7 +631,7 @@ struct FeedForwardBackward : public BlockNode {
                 Rows dz1;
                 dz1.t = call.rows(rows, F);
                 dz1.ld = dz1.t.size(1); dz1.count = rows; dz1.cols = F;
-                layer_dx(call, dz2, gate_out ? gated_weights(call, w2, gate, samples, dtype) : w2, dz1.t, dz1.ld, as_kept(saved[4], {rows, pad8(F)}, type), act, dtype,
+                layer_dx(call, dz2, gate_out ? gated_weights(call, w2, gate, samples, dtype) : w2, dz1.t, dz1.ld, as_kept(saved[4]), act, dtype,
                          gate_out ? per_sample : 0);
                 if (want_x) layer_dx(call, dz1, kept_operand(call, saved[1], C), dx, C, Tensor(), act, dtype);
                 if (want_w1 || want_b1) {
