@@ -156,7 +156,9 @@ void refuse_foreign_accumulators(const Library& lib, std::initializer_list<const
         const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
         if (!accumulator) continue;
         const std::optional<c10::Stream> made_on = accumulator->stream();
-        if (made_on.has_value() && *made_on != c10::hip::getCurrentHIPStream(t->device().index()).unwrap())
+        const c10::Stream now = c10::hip::getCurrentHIPStream(t->device().index()).unwrap();
+        // (number and device alone: autograd's streams call their devices CUDA, these call them HIP, and so no two of them are equal)
+        if (made_on.has_value() && (made_on->id() != now.id() || made_on->device_index() != now.device_index()))
             fail(Failure::kRuntime, "llsa_amd: a graph is being captured, and an input's gradient belongs to another graph that is still alive: let go of it first "
                                     "(delete the outputs of earlier forward passes)");
     }
