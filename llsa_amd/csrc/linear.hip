@@ -47,8 +47,8 @@ __device__ __forceinline__ void wave_waits_for_reads() {
 
 // ---------------------------------------------------------------------------------------
 // activations, in fp32.  Written with the logistic function: 0.5 (1 + tanh u) = s(2u), which saturates to 0 and 1 without an
-// overflow.  The derivatives are taken at z held to +-16, where they are 0 and 1 to the last bit of fp32, so that a large z does not
-// multiply an infinite inner derivative by zero.
+// overflow.  The derivatives are taken at z held to +-128, where they are 0 and 1 in fp32 (SiLU's 128 e^-128 is below its smallest number), so that a large z
+// does not multiply an infinite inner derivative by zero.
 // ---------------------------------------------------------------------------------------
 constexpr float kGeluC = 0.7978845608028654f, kGeluA = 0.044715f, kRsqrt2 = 0.7071067811865476f, kRsqrt2Pi = 0.3989422804014327f;
 
@@ -73,7 +73,7 @@ __device__ __forceinline__ float activate(int act, float z) {
 }
 __device__ __forceinline__ float activate_slope(int act, float z) {
     if (act == LLSA_ACT_NONE) return 1.f;
-    z = z > 16.f ? 16.f : z < -16.f ? -16.f : z;              // (a NaN stays one)
+    z = z > 128.f ? 128.f : z < -128.f ? -128.f : z;            // (a NaN stays one)
     switch (act) {
         case LLSA_ACT_SILU: {
             const float s = logistic2(kLog2e * z);
