@@ -7,9 +7,10 @@
 // The gradients of all four vectors come out of two sums per sample and channel, S1 = sum of dy and S2 = sum of dy * h.
 //
 // A row is held in registers by LANES lanes, up to CHUNKS pieces of 8 channels each: it is read once, the variance is that of the
-// differences from the mean (no cancellation), and everything is fp32 in between.  Bound by memory: 131072 x 384 in bf16, forward 39.5 us (201 MB, 5.1 TB/s;
+// differences from the mean (no cancellation; fp32 rows are centred twice), and everything is fp32 in between.  Bound by memory: 131072 x 384 in bf16, forward 39.5 us (201 MB, 5.1 TB/s;
 // a large copy 5.2), backward 62.6 (302 MB, 4.8 TB/s), the sums of its pieces 4.6.
 #include <algorithm>
+#include <type_traits>
 
 #include "llsa_device.h"
 #include "llsa_host.h"
@@ -118,6 +119,27 @@ __device__ __forceinline__ float row_sum(float v, float* slots) {
     return v;
 }
 
+// The row's values v become their differences from `mean`, zeros beyond the row.  Of fp32 rows far from zero the mean is off by a part of their size, which
+// may be more than their spread: the differences, exact or nearly, are then centred a second time (`again`).  Returns what that adds to the mean.
+template <bool WIDE, int LANES, int CHUNKS>
+__device__ __forceinline__ float centre(float (&v)[CHUNKS][8], float mean, int C, int lane, float* slots, bool again) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            v[j][e] = channel<WIDE, LANES>(j, e, lane) < C ? v[j][e] - mean : 0.f;
+            s += v[j][e];
+        }
+    if (!again) return 0.f;
+    const float more = row_sum<LANES>(s, slots) / (float)C;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[j][e] = channel<WIDE, LANES>(j, e, lane) < C ? v[j][e] - more : 0.f;
+    return more;
+}
+
 struct Norm {
     const void *x, *dy;
     void *y, *dx;
@@ -177,16 +199,13 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(const Norm a) {
                 s += v[j][e];
             }
         if (first + kRows < share.last) request(first + kRows);
-        const float mean = row_sum<LANES>(s, slots) / C;     // (divided: the mean of equal values is that value)
+        float mean = row_sum<LANES>(s, slots) / C;           // (divided: the mean of equal values of 16 bits, whose sums are exact, is that value)
+        mean += centre<WIDE, LANES>(v, mean, a.C, lane, slots, std::is_same_v<T, float>);
         s = 0.f;
 #pragma unroll
-        for (int j = 0; j < CHUNKS; j++) {
+        for (int j = 0; j < CHUNKS; j++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                v[j][e] = channel<WIDE, LANES>(j, e, lane) < a.C ? v[j][e] - mean : 0.f;
-                s = fmaf(v[j][e], v[j][e], s);
-            }
-        }
+            for (int e = 0; e < 8; e++) s = fmaf(v[j][e], v[j][e], s);
         const float rstd = rsqrtf(row_sum<LANES>(s, slots) / C + a.eps);
         if (r >= share.last) continue;
         if (a.stats != nullptr && lane == 0) {
@@ -241,10 +260,17 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(const Norm a) {
         for (int j = 0; j < CHUNKS; j++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                h[j][e] = ((float)next_x.piece[j][e] - mean) * rstd;        // (beyond the row d is zero, and so is all that h enters)
-                d[j][e] = there ? (float)next_dy.piece[j][e] : 0.f;
+                h[j][e] = std::is_same_v<T, float> ? (float)next_x.piece[j][e] : ((float)next_x.piece[j][e] - mean) * rstd;
+                d[j][e] = there ? (float)next_dy.piece[j][e] : 0.f;         // (beyond the row d is zero, and so is all that h enters)
             }
         if (first + kRows < share.last) request(first + kRows);
+        if constexpr (std::is_same_v<T, float>) {             // (the mean that the forward left is rounded to fp32)
+            centre<WIDE, LANES>(h, mean, a.C, lane, slots, true);
+#pragma unroll
+            for (int j = 0; j < CHUNKS; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) h[j][e] *= rstd;
+        }
 #pragma unroll
         for (int j = 0; j < CHUNKS; j++)
 #pragma unroll
