@@ -30,7 +30,10 @@ struct Rows {
     int64_t ld = 0, count = 0, cols = 0;
     void* p() const { return t.defined() ? t.data_ptr() : nullptr; }
 };
-Rows rows_of(const Tensor& t) {
+// What the memory of a tensor has to hold for the kernels: its values, not those of a view that torch negates on reading
+Tensor in_memory(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Rows rows_of(const Tensor& given) {
+    const Tensor t = in_memory(given);
     Rows r;
     r.cols = t.size(-1);
     r.count = r.cols > 0 ? t.numel() / r.cols : 0;
@@ -139,7 +142,7 @@ struct BlockNode : public Node {
     }
     virtual variable_list run(const Tensor& grad, const std::vector<Tensor>& saved) = 0;
     // a tensor that only the kernels read, as they left it
-    static Tensor as_kept(const Tensor& t) { return t.is_contiguous() && aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+    static Tensor as_kept(const Tensor& t) { return t.is_contiguous() && aligned(t) && !t.is_neg() ? t : t.clone(at::MemoryFormat::Contiguous).resolve_neg(); }
     void keep(const Tensor& t, const Tensor& input) {
         kinds.push_back(t.defined() ? Kind{true, t.sizes().vec(), t.scalar_type(), t.device()} : Kind{false, {}, at::kFloat, at::kCPU});
         kept.emplace_back(t.is_same(input) ? input : t, false);
@@ -224,7 +227,7 @@ void norm_inputs(llsa_layer_norm_args& a, const NormInputs& v) {
 // elements next to each other, of type `type`; rows of samples may be any step apart
 Tensor small_vector(const Tensor* t, at::ScalarType type) {
     if (t == nullptr) return Tensor();
-    const Tensor v = t->scalar_type() == type ? *t : t->to(type);
+    const Tensor v = in_memory(t->scalar_type() == type ? *t : t->to(type));
     return v.size(-1) <= 1 || v.stride(-1) == 1 ? v : v.contiguous();
 }
 
@@ -474,7 +477,9 @@ void same_types(const char* what, const Tensor& x, std::initializer_list<const T
             fail(Failure::kValue, std::string(what) + ": all tensors must have x's dtype, " + name_of(x.scalar_type()) + " (got " + name_of(t->scalar_type()) + ")");
 }
 Tensor dense_vector(const Tensor* t) {                        // (N) or (samples, N) with elements next to each other
-    return t == nullptr ? Tensor() : t->size(-1) <= 1 || t->stride(-1) == 1 ? *t : t->contiguous();
+    if (t == nullptr) return Tensor();
+    const Tensor v = in_memory(*t);
+    return v.size(-1) <= 1 || v.stride(-1) == 1 ? v : v.contiguous();
 }
 int activation(const char* what, int64_t act) {
     if (act < LLSA_ACT_NONE || act > LLSA_ACT_GELU_TANH) fail(Failure::kValue, std::string(what) + ": unknown activation");
