@@ -914,13 +914,16 @@ __global__ __launch_bounds__(256) void gate_rows_kernel(const bf16* w, int64_t l
 }
 // fp16 has not: the gates of an adaLN-zero block begin at zero, and a product below 2^-14 loses its bits.  Every column of a sample is divided by a power of two
 // that brings the largest of its products to 2^14 .. 2^15, and dx is multiplied by it in fp32.  What is 2^-28 and less of that largest one is rounded by up to
-// 2^-39 of it, far below the 2^-24 that a sum in fp32 is off by.  A workgroup takes 64 columns of a sample, 32 rows at a time, and reads them twice.
-constexpr int kScaleColumns = 64, kScaleRows = 32;
-__global__ __launch_bounds__(256) void gate_rows_scaled_kernel(const _Float16* w, int64_t ldw, const _Float16* gate, int64_t s_gate, _Float16* out, int64_t ldo, bf16* scales,
+// 2^-39 of it, far below the 2^-24 that a sum in fp32 is off by.  A workgroup takes 32 columns of a sample, 256 rows at a time, and reads them twice, the second time
+// out of L2.  Bound by the latency of those reads: 8 samples of 384 x 1536 12.2 us, of 384 x 384 7.2 (256 threads with 64 columns, 32 rows at a time: 20).
+// The multiplication takes 3 to 11 us of dx (131072 rows 384 > 1536 behind act' 257 -> 268).
+constexpr int kScaleColumns = 32, kScaleThreads = 1024, kScaleRows = kScaleThreads * 8 / kScaleColumns;
+__global__ __launch_bounds__(kScaleThreads) void gate_rows_scaled_kernel(const _Float16* w, int64_t ldw, const _Float16* gate, int64_t s_gate, _Float16* out, int64_t ldo, bf16* scales,
                                                                int N, int groups) {
-    __shared__ float most[kScaleRows][kScaleColumns + 8];
+    constexpr int kLanes = kScaleColumns / 8, kWaves = kScaleThreads / 64;      // lanes of a row
+    __shared__ float most[kWaves][kScaleColumns];
     const int64_t b = (int)blockIdx.x / groups;
-    const int group = (int)blockIdx.x - (int)b * groups, lane = threadIdx.x & 7, row = threadIdx.x >> 3, c = group * kScaleColumns + lane * 8;
+    const int group = (int)blockIdx.x - (int)b * groups, lane = threadIdx.x % kLanes, row = threadIdx.x / kLanes, c = group * kScaleColumns + lane * 8;
     const bool inside = c < ldo;                              // (whole pieces of eight)
     auto products = [&](int n, float (&v)[8]) {
         const float g = (float)gate[b * s_gate + n];
@@ -938,7 +941,11 @@ __global__ __launch_bounds__(256) void gate_rows_scaled_kernel(const _Float16* w
             for (int e = 0; e < 8; e++) top[e] = fmaxf(top[e], fabsf(v[e]));       // (of a NaN and a number the number)
         }
 #pragma unroll
-    for (int e = 0; e < 8; e++) most[row][lane * 8 + e] = top[e];
+    for (int e = 0; e < 8; e++) {
+#pragma unroll
+        for (int step = kLanes; step < 64; step *= 2) top[e] = fmaxf(top[e], __shfl_xor(top[e], step));
+        if ((threadIdx.x & 63) < kLanes) most[threadIdx.x >> 6][lane * 8 + e] = top[e];
+    }
     __syncthreads();
     if (!inside) return;
     float down[8];
@@ -946,8 +953,8 @@ __global__ __launch_bounds__(256) void gate_rows_scaled_kernel(const _Float16* w
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         float m = 0.f;
-#pragma unroll 4
-        for (int r = 0; r < kScaleRows; r++) m = fmaxf(m, most[r][lane * 8 + e]);
+#pragma unroll
+        for (int wave = 0; wave < kWaves; wave++) m = fmaxf(m, most[wave][lane * 8 + e]);
         // the exponent of m, which is 0 or in 2^-48 .. 2^32, or an infinity
         const int exponent = (int)(__float_as_uint(m) >> 23), k = m == 0.f || exponent == 255 ? 0 : exponent - 127 - 14;
         down[e] = __uint_as_float((unsigned)(127 - k) << 23);
@@ -1285,7 +1292,7 @@ template <typename T>
 int gate_rows(const llsa_linear_args& q, hipStream_t stream) {
     if constexpr (std::is_same_v<T, _Float16>) {
         const int groups = (int)ceil_div(q.ldo, kScaleColumns);
-        hipLaunchKernelGGL(gate_rows_scaled_kernel, dim3((unsigned)(q.M / q.per_sample * groups)), dim3(256), 0, stream, (const T*)q.w, q.ldw, (const T*)q.gate, q.s_gate, (T*)q.out,
+        hipLaunchKernelGGL(gate_rows_scaled_kernel, dim3((unsigned)(q.M / q.per_sample * groups)), dim3(kScaleThreads), 0, stream, (const T*)q.w, q.ldw, (const T*)q.gate, q.s_gate, (T*)q.out,
                            q.ldo, (bf16*)q.scales, q.N, groups);
     } else {
         const int64_t pieces = q.M / q.per_sample * q.N * (q.ldo / 8);
