@@ -369,7 +369,7 @@ int llsa_attn_bwd(const llsa_attn_bwd_args* a, void* stream);
  * residuals and the feed-forward block, torch modules in the reference).  Rows of tokens x (M,K), weights W (N,K):
  *     z = x W^T + bias,   out = residual + gate * act(z),      gate: one row of N for every per_sample rows of x
  *     dz = dout * gate * act'(z),  dx = dz W,  dW = dz^T x,  dbias = sum over rows of dz,  dgate = sum over a sample's rows of dout * act(z)
- * bf16 or fp16 throughout, sums in fp32, one rounding where a tensor is written.  The products read rows that are 16-byte aligned
+ * bf16 or fp16 throughout, sums in fp32, one rounding where a tensor is written (z, dz and gate * w among them).  The products read rows that are 16-byte aligned
  * and hold a multiple of 8 elements, zeros beyond the end; llsa_pad_rows makes such rows out of any.  What is written overlaps nothing
  * that is read.  Activations: */
 #define LLSA_ACT_NONE 0

@@ -352,7 +352,7 @@ __device__ __forceinline__ void arrange_lines(vec8<T>& first, vec8<T>& second, i
 }
 
 // Two stages of LDS and two workgroups a CU that fill each other's waits.  131072 rows of 384 and 1536 channels, us: forward 1536 > 384 with gate and
-// residual 194 (0.80 PFLOP/s; 128 x 128 205), dx 1536 > 384 205 (213), dW 196 (0.79; 215); 8192 x 4096 x 4096 230 (1.19; a library's 200), its dW 332.  What
+// residual 194 (0.80 PFLOP/s; 128 x 128 205), dx 1536 > 384 205 (213), dW 196 (0.79; 215); 8192 x 4096 x 4096 229 to 250 by card (1.10 to 1.20; a library's 200), its dW 332.  What
 // bounds it is the way of the operands from L2 (11 TB/s with 128 x 128 tiles): without the copies 134, 118, 127 (of 128 x 128) and 189, 198, while half of
 // the LDS reads or of the products take off 1 to 9 %.  More stages of 32, three of 64 with 256 x 128, and 256 x 192 tiles, with a third less to fetch, are
 // one workgroup a CU or more barriers: dW 280, 270, 226.
@@ -1087,8 +1087,7 @@ int launch_tiles(Product<T>& a, int splits, hipStream_t stream) {
 //     8192, 2048 > 2048     98 / 77 / 85 / 75             8192, 4096 > 4096    - / 260 / 260 / 226
 // Small tiles keep a grid of few tiles busy, up to four for each CU.  Beyond that it is rounds times the length of one: two workgroups of 128 x 128 or
 // 192 x 128 fit a CU, one of 256 x 256, and a round of these takes 1, 1.3 and 1.8 + 220 / K forward (the shorter the contraction, the more weighs a way out with
-// gate and residual that no second workgroup fills), 1, 1.38 and 1.8 in dx.  Over 82 sizes of 384 to 4608 channels the choice costs 0.5 % more than the
-// best one on average, 9 % at most.
+// gate and residual that no second workgroup fills), 1, 1.38 and 1.8 in dx.
 enum Tiles { k64, k128, k192, k256 };
 Tiles tiles_for(int64_t M, int64_t N, int64_t K, bool dx) {
     if (ceil_div(M, 64) * ceil_div(N, 64) <= 4 * kCus) return k64;

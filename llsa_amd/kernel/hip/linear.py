@@ -22,8 +22,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     """residual + gate * activation(x @ weight.T + bias).
 
     x is (..., K), weight (N, K), bias (N,), gate (B, N) for an x of (B, ..., K), one row for each sample, residual (..., N); all of
-    them bf16 or all fp16.  Sums in fp32, one rounding.  activation: None, "silu", "gelu" (erf) or "gelu_tanh".  Differentiable in
-    all five (once); the backward keeps x, weight and, with an activation (or a gate that wants a gradient, on samples of less than
+    them bf16 or all fp16.  activation: None, "silu", "gelu" (erf) or "gelu_tanh".  Sums in fp32; the forward rounds once, the
+    backward, besides its results, what its products take in: the gradient behind gate and activation (or gate * weight in its place),
+    and x @ weight.T + bias where it is kept.  Differentiable in all five (once); the backward keeps x, weight and, with an activation (or a gate that wants a gradient, on samples of less than
     2 K rows), x @ weight.T + bias."""
     lib = current_lib()
     return lib.host.linear(lib.host_library, x, weight, bias, _activation(activation), gate, residual)
@@ -35,6 +36,7 @@ def feed_forward(x: torch.Tensor, w_in: torch.Tensor, b_in: Optional[torch.Tenso
     """residual + gate * (activation(x @ w_in.T + b_in) @ w_out.T + b_out).
 
     x is (..., C), w_in (F, C), b_in (F,), w_out (N, F), b_out (N,), gate (B, N) for an x of (B, ..., C), residual (..., N); all of
-    them bf16 or all fp16.  The hidden rows are rounded to that type between the two products.  Differentiable in all seven (once)."""
+    them bf16 or all fp16.  Sums in fp32; the hidden rows are rounded to that type between the two products, and so are what the backward keeps of them
+    and their gradient.  Differentiable in all seven (once)."""
     lib = current_lib()
     return lib.host.feed_forward(lib.host_library, x, w_in, b_in, w_out, b_out, _activation(activation), gate, residual)
