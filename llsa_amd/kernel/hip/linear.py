@@ -24,8 +24,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     x is (..., K), weight (N, K), bias (N,), gate (B, N) for an x of (B, ..., K), one row for each sample, residual (..., N); all of
     them bf16 or all fp16.  activation: None, "silu", "gelu" (erf) or "gelu_tanh".  Sums in fp32; the forward rounds once, the
     backward, besides its results, what its products take in: the gradient behind gate and activation (or gate * weight in its place),
-    and x @ weight.T + bias where it is kept.  Differentiable in all five (once); the backward keeps x, weight and, with an activation (or a gate that wants a gradient, on samples of less than
-    2 K rows), x @ weight.T + bias."""
+    and x @ weight.T + bias where it is kept.  Differentiable in all five (once); the backward keeps x, weight and, with an
+    activation (or a gate that wants a gradient, on samples of less than 2 K rows), x @ weight.T + bias."""
     lib = current_lib()
     return lib.host.linear(lib.host_library, x, weight, bias, _activation(activation), gate, residual)
 

@@ -125,3 +125,23 @@ def test_large_linear_dx_of_small_gates(T, K, N):
 @pytest.mark.parametrize("B,T,C,F", [(3, 3301, 384, 1536), (2, 2085, 264, 1040)])
 def test_large_feed_forward_of_small_gates(B, T, C, F):
     _check_ffn(torch.device("cuda"), B, T, C, F, 1e-5)
+
+
+def test_c_calls_check_scales():
+    """Gated weights in fp16 need room for their scales, and dx takes scales with such weights alone; nothing is launched."""
+    import ctypes as C
+    from llsa_amd._lib import LIB_PATH, Lib, LinearArgs
+    lib = Lib(LIB_PATH)
+    bad = lambda fn, a: fn(C.byref(a), None) != 0 and b"scales" in lib.last_error_string()
+    a = LinearArgs()
+    a.M, a.N, a.K, a.dtype, a.per_sample = 8, 8, 8, 2, 4
+    a.w = a.gate = a.out = a.dz = 1 << 20
+    a.ldw = a.ldo = a.lddz = a.s_gate = 8
+    assert bad(lib.linear_gate_rows, a)
+    a.scales = 8 + (1 << 20)
+    assert bad(lib.linear_gate_rows, a)
+    assert bad(lib.linear_dx, a)                              # (one set of weights for all rows)
+    a.s_w = 64
+    assert bad(lib.linear_dx, a)                              # (not aligned)
+    a.scales, a.dtype = 1 << 20, 0
+    assert bad(lib.linear_dx, a)                              # (bf16)
