@@ -44,7 +44,7 @@ extern "C" {
 #define LLSA_DTYPE_F32 1
 #define LLSA_DTYPE_F16 2
 
-#define LLSA_ABI_VERSION 215     /* changes with every change of a signature or argument structure below */
+#define LLSA_ABI_VERSION 216     /* changes with every change of a signature or argument structure below */
 int llsa_version(void);          /* LLSA_ABI_VERSION of the built library                                    */
 const char* llsa_last_error_string(void);
 
@@ -455,6 +455,36 @@ typedef struct llsa_layer_norm_args {
 int llsa_layer_norm_fwd(const llsa_layer_norm_args* a, void* stream);
 int llsa_layer_norm_bwd(const llsa_layer_norm_args* a, void* stream);
 int64_t llsa_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t per_sample, int C);
+
+/* ------------------------------------------------------------------------------------------
+ * The linear layer in 8-bit integers, for sampling.  Rows of x become whole numbers with a scale each,
+ *     scale = max |x| / 127 (fp32),   q = x / scale to the nearest whole number (halves to even; 0 in a row of zeros),
+ * a row that holds an infinity or a NaN gets a scale of NaN.  Products of such rows with weights kept the same way (N,K), exact in 32 bits:
+ *     out = residual + gate * act(q_scale[m] * w_scale[n] * sum over k of q[m,k] w[n,k] + bias[n])
+ * x: bf16, fp16 or fp32; bias, gate, residual and out: bf16 or fp16. */
+#define LLSA_INT8_MAX_K 131072
+typedef struct llsa_quantize_args {
+    const void* x;          /* (rows,K) ldx apart                                                      */
+    void* q;                /* (rows,K) ldq apart                                                      */
+    float* scale;           /* (rows)                                                                  */
+    int64_t ldx, ldq, rows;
+    int32_t K, dtype;
+    int32_t padded;         /* rows of q are 16-byte aligned and get zeros up to a multiple of 16      */
+    int32_t pads;           /* 0 to 2 matrices of 8-bit integers that are copied to rows like those, in the same launch */
+    llsa_pad_job pad[2];
+} llsa_quantize_args;
+int llsa_quantize_rows(const llsa_quantize_args* a, void* stream);
+typedef struct llsa_int8_args {
+    const void *q, *w;      /* (M,K) ldq apart, (N,K) ldw apart: 16-byte aligned rows, zeros up to a multiple of 16 */
+    const float *q_scale, *w_scale;      /* (M), (N)                                                   */
+    const void* bias;       /* (N) or NULL                                                             */
+    const void* gate;       /* (M/per_sample, N) rows s_gate apart, or NULL                            */
+    const void* residual;   /* (M,N) ldr apart, or NULL                                                */
+    void* out;              /* (M,N) ldo apart                                                         */
+    int64_t ldq, ldw, s_gate, ldr, ldo, M, per_sample;
+    int32_t N, K, act, dtype;
+} llsa_int8_args;
+int llsa_linear_int8(const llsa_int8_args* a, void* stream);
 
 #ifdef __cplusplus
 }

@@ -94,6 +94,17 @@ class PadJob(C.Structure):
     _fields_ = [("x", c_void_p), ("y", c_void_p), ("ldx", c_int64), ("ldy", c_int64), ("rows", c_int64), ("cols", c_int32), ("reserved", c_int32)]
 
 
+class QuantizeArgs(C.Structure):
+    _fields_ = [("x", c_void_p), ("q", c_void_p), ("scale", c_void_p), ("ldx", c_int64), ("ldq", c_int64), ("rows", c_int64),
+                ("K", c_int32), ("dtype", c_int32), ("padded", c_int32), ("pads", c_int32), ("pad", PadJob * 2)]
+
+
+class Int8Args(C.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("q", "w", "q_scale", "w_scale", "bias", "gate", "residual", "out")]
+                + [(n, c_int64) for n in ("ldq", "ldw", "s_gate", "ldr", "ldo", "M", "per_sample")]
+                + [(n, c_int32) for n in ("N", "K", "act", "dtype")])
+
+
 class LayerNormArgs(C.Structure):
     _fields_ = ([(n, c_void_p) for n in ("x", "y", "weight", "bias", "scale", "shift", "stats", "dy", "dx", "dweight", "dbias", "dscale", "dshift", "workspace")]
                 + [(n, c_int64) for n in ("ldx", "ldy", "s_scale", "s_shift", "lddy", "lddx", "rows", "per_sample")]
@@ -147,11 +158,13 @@ _SIGNATURES = {
     "llsa_linear_dw_workspace_bytes": (c_int64, [c_int64, c_int64, c_int, c_int]),
     "llsa_linear_dz_workspace_bytes": (c_int64, [c_int64, c_int64, c_int]),
     "llsa_pad_rows": (c_int, [C.POINTER(PadJob), c_int, c_void_p]),
+    "llsa_quantize_rows": (c_int, [C.POINTER(QuantizeArgs), c_void_p]),
+    "llsa_linear_int8": (c_int, [C.POINTER(Int8Args), c_void_p]),
 }
 
 EXPORTS = tuple(_SIGNATURES)
 CHUNK_FINE_MAX = 256                                        # LLSA_CHUNK_FINE_MAX of include/llsa_hip.h
-ABI_VERSION = 215                                           # LLSA_ABI_VERSION
+ABI_VERSION = 216                                           # LLSA_ABI_VERSION
 STATIC_PARTIALS_MAX = 262144                                # LLSA_STATIC_PARTIALS_MAX
 
 

@@ -3,3 +3,4 @@
 #include "common.h"
 
 void bind_block(pybind11::module_& m);
+void bind_int8(pybind11::module_& m);           // int8.cpp

@@ -8,11 +8,11 @@ namespace {
 
 using namespace llsa_host;
 
-int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
-bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
-std::string name_of(at::ScalarType t) { return "torch." + std::string(torch::getTHPDtype(t)->name); }
+inline int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+inline bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+inline std::string name_of(at::ScalarType t) { return "torch." + std::string(torch::getTHPDtype(t)->name); }
 
-int dtype_of(const Tensor& t, bool f32_too, const char* what) {
+inline int dtype_of(const Tensor& t, bool f32_too, const char* what) {
     switch (t.scalar_type()) {
         case at::kBFloat16: return LLSA_DTYPE_BF16;
         case at::kHalf: return LLSA_DTYPE_F16;
@@ -31,8 +31,8 @@ struct Rows {
     void* p() const { return t.defined() ? t.data_ptr() : nullptr; }
 };
 // What the memory of a tensor has to hold for the kernels: its values, not those of a view that torch negates on reading
-Tensor in_memory(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
-Rows rows_of(const Tensor& given) {
+inline Tensor in_memory(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+inline Rows rows_of(const Tensor& given) {
     const Tensor t = in_memory(given);
     Rows r;
     r.cols = t.size(-1);
@@ -151,7 +151,7 @@ struct BlockNode : public Node {
 
 // A graph that is being captured must not reach gradients that another graph on another stream holds: a leaf has one accumulator, tied to the stream
 // it was made on, and a captured backward that has to wait for that stream ends the process (of any operator).
-void refuse_foreign_accumulators(const Library& lib, std::initializer_list<const Tensor*> all) {
+inline void refuse_foreign_accumulators(const Library& lib, std::initializer_list<const Tensor*> all) {
     if (!lib.device || !at::GradMode::is_enabled()) return;
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
     for (const Tensor* t : all) {
@@ -168,7 +168,7 @@ void refuse_foreign_accumulators(const Library& lib, std::initializer_list<const
 }
 
 // the checks all three begin with
-void begin(const Library& lib, const char* what, const Tensor& x, std::initializer_list<const Tensor*> all) {
+inline void begin(const Library& lib, const char* what, const Tensor& x, std::initializer_list<const Tensor*> all) {
     if (torch::jit::tracer::isTracing()) fail(Failure::kRuntime, std::string("llsa_amd ") + what + " cannot be recorded by torch.jit.trace");
     refuse_transforms(all);
     for (const Tensor* t : all) {
@@ -179,7 +179,7 @@ void begin(const Library& lib, const char* what, const Tensor& x, std::initializ
     lib.on_device(x);
     refuse_foreign_accumulators(lib, all);
 }
-bool wants(std::initializer_list<const Tensor*> all) {
+inline bool wants(std::initializer_list<const Tensor*> all) {
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor* t : all)
         if (t != nullptr && t->requires_grad()) return true;
@@ -191,19 +191,19 @@ std::shared_ptr<N> make_node(const std::shared_ptr<Library>& lib) {
     node->lib = lib;
     return node;
 }
-variable_list present(std::initializer_list<const Tensor*> all) {
+inline variable_list present(std::initializer_list<const Tensor*> all) {
     variable_list v;
     for (const Tensor* t : all)
         if (t != nullptr) v.push_back(*t);
     return v;
 }
 
-void check_vector(const char* what, const char* name, const Tensor* t, at::IntArrayRef sizes) {
+inline void check_vector(const char* what, const char* name, const Tensor* t, at::IntArrayRef sizes) {
     if (t != nullptr && t->sizes() != sizes)
         fail(Failure::kValue, std::string(what) + ": " + name + " must be " + text_of(sizes) + " (got " + text_of(t->sizes()) + ")");
 }
 // samples: the first dimension, where there is one beside the channels
-int64_t samples_of(const char* what, const char* name, const Tensor& x) {
+inline int64_t samples_of(const char* what, const char* name, const Tensor& x) {
     if (x.dim() < 2) fail(Failure::kValue, std::string(what) + ": " + name + " needs a dimension of samples in front of the channels");
     return x.size(0);
 }
@@ -214,7 +214,7 @@ struct LayerInputs {
     int64_t rows, samples;
     int64_t per_sample() const { return std::max<int64_t>(1, samples > 0 ? rows / samples : rows); }
 };
-LayerInputs layer_inputs(const char* what, const Tensor& x, const Tensor* gate, const Tensor* residual, int64_t out) {
+inline LayerInputs layer_inputs(const char* what, const Tensor& x, const Tensor* gate, const Tensor* residual, int64_t out) {
     LayerInputs i{&x, gate, residual, 1, 1};
     for (int64_t d = 0; d + 1 < x.dim(); d++) i.rows *= x.size(d);
     if (gate != nullptr) {
@@ -227,29 +227,29 @@ LayerInputs layer_inputs(const char* what, const Tensor& x, const Tensor* gate, 
     if (i.rows >= (int64_t(1) << 31) - (1 << 16)) fail(Failure::kValue, std::string(what) + ": too many rows (" + std::to_string(i.rows) + ")");
     return i;
 }
-void check_weight(const char* what, const char* name, const Tensor& w, int64_t in, const Tensor& x) {
+inline void check_weight(const char* what, const char* name, const Tensor& w, int64_t in, const Tensor& x) {
     if (w.dim() != 2 || w.size(0) < 1 || w.size(1) < 1 || (in >= 0 && w.size(1) != in))
         fail(Failure::kValue, std::string(what) + ": " + name + " must be (channels out, " + (in >= 0 ? std::to_string(in) : std::string("channels in")) + ") (got " + text_of(w.sizes()) + ")");
     if (w.size(0) >= (1 << 23) || w.size(1) >= (1 << 23)) fail(Failure::kValue, std::string(what) + ": too many channels");
 }
-void same_types(const char* what, const Tensor& x, std::initializer_list<const Tensor*> all) {
+inline void same_types(const char* what, const Tensor& x, std::initializer_list<const Tensor*> all) {
     for (const Tensor* t : all)
         if (t != nullptr && t->scalar_type() != x.scalar_type())
             fail(Failure::kValue, std::string(what) + ": all tensors must have x's dtype, " + name_of(x.scalar_type()) + " (got " + name_of(t->scalar_type()) + ")");
 }
-Tensor dense_vector(const Tensor* t) {                        // (N) or (samples, N) with elements next to each other
+inline Tensor dense_vector(const Tensor* t) {                        // (N) or (samples, N) with elements next to each other
     if (t == nullptr) return Tensor();
     const Tensor v = in_memory(*t);
     return v.size(-1) <= 1 || v.stride(-1) == 1 ? v : v.contiguous();
 }
-int activation(const char* what, int64_t act) {
+inline int activation(const char* what, int64_t act) {
     if (act < LLSA_ACT_NONE || act > LLSA_ACT_GELU_TANH) fail(Failure::kValue, std::string(what) + ": unknown activation");
     return static_cast<int>(act);
 }
-Tensor zeros_like_weight(int64_t n, int64_t k, const Tensor& like) { return at::zeros({n, k}, like.options()); }
+inline Tensor zeros_like_weight(int64_t n, int64_t k, const Tensor& like) { return at::zeros({n, k}, like.options()); }
 
 // An operand of the forward, which may be a copy with padded rows, of which `cols` elements count
-Rows kept_operand(const Call& call, const Tensor& t, int64_t cols) {
+inline Rows kept_operand(const Call& call, const Tensor& t, int64_t cols) {
     Rows r = call.operand(t);
     r.cols = cols;
     return r;

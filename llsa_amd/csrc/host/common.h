@@ -110,6 +110,8 @@ struct Library {
     decltype(&llsa_linear_dw_workspace_bytes) linear_dw_workspace_bytes;
     decltype(&llsa_linear_dz_workspace_bytes) linear_dz_workspace_bytes;
     decltype(&llsa_pad_rows) pad_rows;
+    decltype(&llsa_quantize_rows) quantize_rows;
+    decltype(&llsa_linear_int8) linear_int8;
     bool device;                          // false: the CPU emulation build the tests install
 
     Library(const std::map<std::string, uintptr_t>& at_, bool device_) : device(device_) {
@@ -142,6 +144,8 @@ struct Library {
         get("llsa_linear_dw_workspace_bytes", linear_dw_workspace_bytes);
         get("llsa_linear_dz_workspace_bytes", linear_dz_workspace_bytes);
         get("llsa_pad_rows", pad_rows);
+        get("llsa_quantize_rows", quantize_rows);
+        get("llsa_linear_int8", linear_int8);
     }
     void check(int rc, const char* what) const {
         if (rc != 0) fail(Failure::kLibrary, std::string(what) + " failed (" + std::to_string(rc) + "): " + last_error_string());

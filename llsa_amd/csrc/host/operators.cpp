@@ -547,4 +547,5 @@ PYBIND11_MODULE(_llsa_host, m) {
         return without_interpreter([&] { return permute(lib, x, perm, inv); });
     }));
     bind_block(m);
+    bind_int8(m);
 }

@@ -140,6 +140,24 @@ f32x4_t mfma_16x16x32_f16(f16x8_t a, f16x8_t b, f32x4_t c) {
     return mfma_16x16x32(ws.ha, ws.hb, a, b, c);
 }
 
+// D = A(16x64) * B(64x16) + C in 8-bit integers: lane l holds A[row l%16][k = 16*(l/16) + e], B likewise, D as above
+i32x4_t mfma_16x16x64_i8(i32x4_t a, i32x4_t b, i32x4_t c) {
+    WaveSync& ws = waves[cur / kWave];
+    const int l = cur % kWave;
+    memcpy(&ws.a[l], &a, 16);
+    memcpy(&ws.b[l], &b, 16);
+    wave_barrier();
+    i32x4_t d = c;
+    for (int e = 0; e < 4; e++)
+        for (int q = 0; q < 4; q++) {
+            const int8_t* av = reinterpret_cast<const int8_t*>(&ws.a[4 * (l / 16) + e + 16 * q]);
+            const int8_t* bv = reinterpret_cast<const int8_t*>(&ws.b[l % 16 + 16 * q]);
+            for (int k = 0; k < 16; k++) d[e] += (int)av[k] * (int)bv[k];
+        }
+    wave_barrier();
+    return d;
+}
+
 // ds_read_b64_tr_b16: in each group of 16 lanes, lane i gets element i%4 of the 8-byte chunks
 // addressed by lanes i/4, 4 + i/4, 8 + i/4, 12 + i/4 (behaviour observed on gfx950 hardware).
 s16x4_t ds_read_tr16_b64(const void* p) {
