@@ -44,7 +44,7 @@ extern "C" {
 #define LLSA_DTYPE_F32 1
 #define LLSA_DTYPE_F16 2
 
-#define LLSA_ABI_VERSION 216     /* changes with every change of a signature or argument structure below */
+#define LLSA_ABI_VERSION 217     /* changes with every change of a signature or argument structure below */
 int llsa_version(void);          /* LLSA_ABI_VERSION of the built library                                    */
 const char* llsa_last_error_string(void);
 
@@ -485,6 +485,57 @@ typedef struct llsa_int8_args {
     int32_t N, K, act, dtype;
 } llsa_int8_args;
 int llsa_linear_int8(const llsa_int8_args* a, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Rows that choose their weights.  The router: of every token's logits l (M,E) the k largest (equal ones: the lowest index first; -inf is never chosen, a NaN
+ * counts as the largest number),
+ *     experts[m,j] or -1,   weights[m,j] = exp(l_j - max l) / sum, over the chosen ones (normalize) or over all;  0 where there is none
+ * and the order of the rows: slots m * k + j sorted by expert, in turn.
+ *     order[place] = slot, -1 behind the last;   offsets[e] .. offsets[e + 1] - 1: the places of expert e;   places[slot] = place or -1
+ * Back: dlogits out of dweights. */
+#define LLSA_MAX_EXPERTS 256
+#define LLSA_MAX_CHOICES 16
+#define LLSA_MAX_SLOTS 268435456          /* rows of the experts' products; tokens times choices        */
+typedef struct llsa_route_args {
+    const void* logits;     /* (M,E) ld apart: bf16, fp16 or fp32                                      */
+    float* weights;         /* (M,k)                                                                   */
+    int32_t *experts, *order, *offsets, *places;      /* (M,k), (M*k), (E+1), (M,k); back: experts is read */
+    const float* dweights;  /* back: (M,k)                                                             */
+    void* dlogits;          /* back: (M,E) contiguous                                                  */
+    void* workspace;        /* llsa_route_workspace_bytes                                              */
+    int64_t ld, M;
+    int32_t E, k, normalize, dtype;
+} llsa_route_args;
+int llsa_route_tokens(const llsa_route_args* a, void* stream);
+int llsa_route_tokens_bwd(const llsa_route_args* a, void* stream);
+int64_t llsa_route_workspace_bytes(int64_t M, int E, int k);
+
+/* The experts' products.  Rows stand sorted by expert, those of expert e at offsets[e] .. offsets[e + 1] - 1 (held to 0 .. rows, and not falling); weights
+ * (E,N,K).  Conventions of the linear layers above (rows 16-byte aligned and padded, sums in fp32).  With gather_x (gather_dz) the rows of x (dz) are those of
+ * tokens: the row at a place is token order[place] / k.  Numbers in order, places and experts out of range are held to it or skipped.
+ *     fwd       z = x W_e^T + bias_e, kept unless z is NULL; out = act(z).  weights (tokens * k): out is multiplied by weights[order[place]], which is also
+ *               written to sorted[place].  sorted without weights: bias_e is multiplied by sorted[place].  gaps: rows that no expert has get zeros
+ *     dx        t = dz W_e; out = t, or with z t * sorted[place] * act'(z) (sorted NULL: 1); dots: sums of act(z) t, llsa_experts_dot_parts of them a place
+ *     dw        out (E,N,K) = dz^T x and dbias (E,N) = sum of sorted[place] * dz (sorted NULL: 1) over an expert's rows
+ *     combine   out (tokens,N) = residual + gate * sum over j of x[places[m,j]]; the sum, rounded, to z unless NULL
+ *     dweights  dweights[m,j] = sum of the place's dots + dz[m] . bias_(experts[m,j]); N, K as for the dx that made the dots */
+typedef struct llsa_experts_args {
+    const void *x, *w, *bias, *dz, *gate, *residual;
+    void *out, *z, *dbias, *workspace;
+    const int32_t *offsets, *order, *places, *experts;
+    const float* weights;
+    float *sorted, *dots, *dweights;
+    int64_t ldx, ldw, lddz, ldr, ldo, ldz, s_gate;
+    int64_t rows, tokens, per_sample;
+    int32_t E, N, K, k, act, dtype, padded, gaps, gather_x, gather_dz;
+} llsa_experts_args;
+int llsa_experts_fwd(const llsa_experts_args* a, void* stream);
+int llsa_experts_dx(const llsa_experts_args* a, void* stream);
+int llsa_experts_dw(const llsa_experts_args* a, void* stream);
+int llsa_experts_combine(const llsa_experts_args* a, void* stream);
+int llsa_experts_dweights(const llsa_experts_args* a, void* stream);
+int64_t llsa_experts_dw_workspace_bytes(int64_t rows, int E, int N, int K);
+int64_t llsa_experts_dot_parts(int64_t rows, int E, int N, int K);
 
 #ifdef __cplusplus
 }

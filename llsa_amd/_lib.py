@@ -94,6 +94,18 @@ class PadJob(C.Structure):
     _fields_ = [("x", c_void_p), ("y", c_void_p), ("ldx", c_int64), ("ldy", c_int64), ("rows", c_int64), ("cols", c_int32), ("reserved", c_int32)]
 
 
+class RouteArgs(C.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("logits", "weights", "experts", "order", "offsets", "places", "dweights", "dlogits", "workspace")]
+                + [(n, c_int64) for n in ("ld", "M")] + [(n, c_int32) for n in ("E", "k", "normalize", "dtype")])
+
+
+class ExpertsArgs(C.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "w", "bias", "dz", "gate", "residual", "out", "z", "dbias", "workspace", "offsets", "order", "places", "experts",
+                                         "weights", "sorted", "dots", "dweights")]
+                + [(n, c_int64) for n in ("ldx", "ldw", "lddz", "ldr", "ldo", "ldz", "s_gate", "rows", "tokens", "per_sample")]
+                + [(n, c_int32) for n in ("E", "N", "K", "k", "act", "dtype", "padded", "gaps", "gather_x", "gather_dz")])
+
+
 class QuantizeArgs(C.Structure):
     _fields_ = [("x", c_void_p), ("q", c_void_p), ("scale", c_void_p), ("ldx", c_int64), ("ldq", c_int64), ("rows", c_int64),
                 ("K", c_int32), ("dtype", c_int32), ("padded", c_int32), ("pads", c_int32), ("pad", PadJob * 2)]
@@ -160,11 +172,21 @@ _SIGNATURES = {
     "llsa_pad_rows": (c_int, [C.POINTER(PadJob), c_int, c_void_p]),
     "llsa_quantize_rows": (c_int, [C.POINTER(QuantizeArgs), c_void_p]),
     "llsa_linear_int8": (c_int, [C.POINTER(Int8Args), c_void_p]),
+    "llsa_route_tokens": (c_int, [C.POINTER(RouteArgs), c_void_p]),
+    "llsa_route_tokens_bwd": (c_int, [C.POINTER(RouteArgs), c_void_p]),
+    "llsa_route_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
+    "llsa_experts_fwd": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
+    "llsa_experts_dx": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
+    "llsa_experts_dw": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
+    "llsa_experts_combine": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
+    "llsa_experts_dweights": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
+    "llsa_experts_dw_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int]),
+    "llsa_experts_dot_parts": (c_int64, [c_int64, c_int, c_int, c_int]),
 }
 
 EXPORTS = tuple(_SIGNATURES)
 CHUNK_FINE_MAX = 256                                        # LLSA_CHUNK_FINE_MAX of include/llsa_hip.h
-ABI_VERSION = 216                                           # LLSA_ABI_VERSION
+ABI_VERSION = 217                                           # LLSA_ABI_VERSION
 STATIC_PARTIALS_MAX = 262144                                # LLSA_STATIC_PARTIALS_MAX
 
 

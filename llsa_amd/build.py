@@ -38,7 +38,7 @@ def sources():
     return sorted(f for f in os.listdir(CSRC) if f.endswith(".hip"))
 
 
-BLOCK_SOURCES = ("layer_norm.hip", "linear.hip", "linear_int8.hip", "experts.hip", "product_device.h")     # the operators around the attention: no attention workload launches their kernels
+BLOCK_SOURCES = ("layer_norm.hip", "linear.hip", "linear_int8.hip", "experts.hip", "route.hip", "product_device.h", "experts_device.h")     # the operators around the attention: no attention workload launches their kernels
 
 
 def kernel_sources_digest() -> str:

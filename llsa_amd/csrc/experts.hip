@@ -1,0 +1,874 @@
+// Products of rows with the weights of the expert that each belongs to, and the feed-forward block made of two of them.  Rows stand sorted by expert,
+// those of expert e at offsets[e] .. offsets[e + 1] - 1; the offsets stay on the device, so a launch has a workgroup for every piece of rows there can be,
+// and each finds its expert by itself (experts_device.h).
+//
+//     forward   z = x W_e^T + b_e,   out = act(z)                    of a block: h' = w act(z),   y = h' W_out^T + w b_out,   out = residual + gate * sum of a token's y
+//     backward  dx = dz W_e,   dW_e = dz^T x,   db_e = sum dz
+//
+// A token's weight w goes into the hidden rows.  With t = dout W_out the block's backward is then
+//     dW_out = dout^T h',   db_out = sum w dout,   dz = w act'(z) t,   dw = sum over the hidden channels of act(z) t + dout . b_out
+// and takes dout's rows as they are, gathered: nothing is multiplied by w in memory, and no expert's output is kept for dw.
+//
+// Sums are fp32, and so is what happens on the way out.  Rounded to 16 bits besides the results: what a product takes in that another made or that is kept (z,
+// h', dz), as in the linear layers, and the rows y and dx of each expert, which are read once more and added up in fp32: half a step of each, 2^-8 of it in
+// bf16 (fp16 2^-11), for half the bytes.
+#include "experts_device.h"
+
+namespace llsa {
+namespace {
+
+// ---------------------------------------------------------------------------------------
+// forward and dx
+// ---------------------------------------------------------------------------------------
+enum Scaled { kUnscaled, kScaledRows, kScaledBias };          // what is multiplied by a row's weight: nothing, what act gives, the bias
+template <typename T>
+struct Grouped {
+    const T *x, *y;                       // rows of tokens (or of places, without an order), weights
+    int64_t ldx, ldy, y_expert;
+    const int32_t* offsets;
+    Order order;
+    int experts, rows, N, ny, K;          // rows: of places
+    int tiles_n, group, gaps;             // gaps: zeros go to the rows that no expert has
+    // way out
+    const T *bias, *slope_at;
+    const float* weights;                 // of slots; kScaledRows in the forward, which writes `sorted` too
+    float* sorted;                        // of places; read elsewhere
+    float* dots;                          // dx: [place][part] of sums of act(z) t, or NULL
+    int64_t ldo, ldz;
+    T *out, *z;
+    int scaled, wide, wide_out, parts;    // wide: 16-byte accesses to bias; wide_out: to out, or its rows are padded with zeros to a multiple of 8
+};
+struct Here { int expert, m0, m_end, n0, tn; };
+template <int BM, int BN, typename P>
+__device__ __forceinline__ bool find_tile(const P& a, Here& h, int lane) {
+    Runs runs;
+    runs.load(a.offsets, a.experts, a.rows, BM, a.gaps != 0, lane);
+    const int total = runs.total * a.tiles_n;
+    if ((int)blockIdx.x >= total) return false;
+    const int at = xcd_order((int)blockIdx.x, total), in_group = a.group * a.tiles_n, g = at / in_group, rest = at - g * in_group;
+    const int rows_here = min(a.group, runs.total - g * a.group), tn = rest / rows_here, t = g * a.group + rest - tn * rows_here;
+    const Piece p = runs.find(t);
+    h = {p.expert, p.begin + (t - p.first) * BM, p.end, tn * BN, tn};
+    return true;
+}
+template <int BM, int BN, typename T>
+__device__ __forceinline__ void write_zeros(const Grouped<T>& a, const Here& h) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = 0.f;
+    for (int i = threadIdx.x; i < BM * (BN / 8); i += blockDim.x) {
+        const int r = i / (BN / 8), n = h.n0 + (i - r * (BN / 8)) * 8;
+        if (h.m0 + r < h.m_end && n < a.N) store8(a.out + (int64_t)(h.m0 + r) * a.ldo + n, v, a.wide_out, a.N - n);
+    }
+}
+
+// Eight values of a row on their way out; scale: the row's weight.  z: what the forward keeps; early: z of the layer in front in dx
+template <bool YC, int ACT, typename T>
+__device__ __forceinline__ vec8<T> way_out(const Grouped<T>& a, float (&v)[8], const vec8<T>& bias, float scale, const vec8<T>& early, int left, vec8<T>& z, float& dot) {
+    if constexpr (!YC) {
+        const float b = a.scaled == kScaledBias ? scale : 1.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = fmaf(b, (float)bias[e], v[e]);
+        if (a.z != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) z[e] = (T)v[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = activate(ACT, v[e]);
+        if (a.scaled == kScaledRows) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] *= scale;
+        }
+    } else if constexpr (ACT != LLSA_ACT_NONE) {
+        if (a.dots != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) dot += e >= left ? 0.f : v[e] * activate(ACT, (float)early[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] *= scale * activate_slope(ACT, (float)early[e]);
+    }
+    vec8<T> o;
+#pragma unroll
+    for (int e = 0; e < 8; e++) o[e] = (T)(e >= left ? 0.f : v[e]);
+    return o;
+}
+template <typename T>
+__device__ __forceinline__ void put8(T* to, const vec8<T>& o, bool wide, int left) {
+    if (wide) {
+        *reinterpret_cast<vec8<T>*>(to) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < left) to[e] = o[e];
+    }
+}
+// A row's weight: where the forward scales its rows it comes with the order, and is kept in it
+template <typename T>
+__device__ __forceinline__ float weight_of(const Grouped<T>& a, int place) {
+    return a.scaled == kUnscaled ? 1.f : a.weights != nullptr ? a.weights[a.order.slot(place)] : a.sorted[place];
+}
+
+// The tiles of linear.hip's product_kernel, with rows gathered on their way into LDS and an expert's weights.
+template <typename T, bool YC, int BM, int BN, int WAVES_M, int WAVES_N, int ACT>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(const Grouped<T> a) {
+    constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
+    constexpr bool kSlope = YC && ACT != LLSA_ACT_NONE;
+    typedef Operand<T, false, BM, kWaves> OperandX;
+    typedef Operand<T, YC, BN, kWaves> OperandY;
+    HIP_DYNAMIC_SHARED(char, shared)
+    T* const lds = reinterpret_cast<T*>(shared);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int quad = lane >> 4, wm = (wave % WAVES_M) * WM, wn = (wave / WAVES_M) * WN;
+    Here here;
+    if (!find_tile<BM, BN>(a, here, lane)) return;
+    if (here.expert < 0) {
+        write_zeros<BM, BN>(a, here);
+        return;
+    }
+    GatheredRows<T, BM, kWaves> ox;
+    OperandY oy;
+    ox.init(a.x, a.ldx, a.order, here.m0, min(BM, here.m_end - here.m0), wave, lane);
+    oy.init(wave, lane, a.ldy, min(BN, (YC ? a.ny : a.N) - here.n0));
+    const T* py = a.y + here.expert * a.y_expert + (YC ? (int64_t)here.n0 : (int64_t)here.n0 * a.ldy);
+    const int64_t stepy = YC ? kStep * a.ldy : kStep;
+    int k = 0;
+    auto request = [&](int buffer) {
+        T* const t = lds + buffer * (kTileX + kTileY);
+        ox.request(k, t, wave, lane, a.K - k);
+        oy.request(py, t + kTileX, wave, lane, a.K - k);
+        py += stepy;
+        k += kStep;
+    };
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](int buffer) {
+        const T* const tx = lds + buffer * (kTileX + kTileY);
+        const T* const ty = tx + kTileX;
+#pragma unroll
+        for (int ks = 0; ks < kStep / 32; ks++) {
+            vec8<T> fx[MT], fy[NT];
+#pragma unroll
+            for (int j = 0; j < MT; j++) fx[j] = OperandX::fragment(tx, wm + 16 * j, ks, lane);
+#pragma unroll
+            for (int i = 0; i < NT; i++) fy[i] = OperandY::fragment(ty, wn + 16 * i, ks, lane);
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int j = 0; j < MT; j++) acc[i][j] = product16(fy[i], fx[j], acc[i][j]);
+        }
+    };
+
+    const int lane_row = lane & 15, lane_col = 16 * (quad & 1) + 8 * (quad >> 1);
+    const int row0 = here.m0 + wm, col0 = here.n0 + wn, rows_left = here.m_end - row0 - lane_row, cols_left = a.N - col0 - lane_col;
+    const unsigned at_out = (unsigned)(lane_row * a.ldo) + lane_col, at_z = (unsigned)(lane_row * a.ldz) + lane_col;
+    constexpr int kPair = NT % 4 == 0 ? 2 : 1;                // pieces of 32 columns that leave together
+    const bool whole = kPair == 2 && here.m0 + BM <= here.m_end && here.n0 + BN <= a.N && a.wide_out;
+    vec8<T> early[kPair][MT];
+    auto read_side = [&](int p0) {
+        if constexpr (kSlope) {
+            if constexpr (kPair == 2) {
+                if (whole) {
+#pragma unroll
+                    for (int j = 0; j < MT; j++)
+                        request_lines(early[0][j], early[1][j], a.slope_at + ((int64_t)(row0 + 16 * j) * a.ldz + (col0 + 32 * p0)), at_z, (unsigned)(8 * a.ldz), lane);
+                    return;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < MT; j++)
+#pragma unroll
+                for (int h = 0; h < kPair; h++)
+                    if (16 * j < rows_left && 32 * (p0 + h) < cols_left)
+                        early[h][j] = *reinterpret_cast<const vec8<T>*>(a.slope_at + ((int64_t)(row0 + 16 * j) * a.ldz + (col0 + 32 * (p0 + h))) + at_z);
+        }
+    };
+    const int steps = (a.K + kStep - 1) / kStep;
+    request(0);
+    for (int s = 0; s + 1 < steps; s++) {
+        wait_vm0();
+        __syncthreads();                                      // everyone's copies of this step are there, and everyone is done with the other buffer
+        request((s + 1) & 1);
+        multiply(s & 1);
+    }
+    wait_vm0();
+    __syncthreads();
+    read_side(0);                                             // (on its way during the last step's products)
+    float scale[MT], dot[MT];
+#pragma unroll
+    for (int j = 0; j < MT; j++) {
+        scale[j] = 16 * j < rows_left ? weight_of(a, row0 + 16 * j + lane_row) : 0.f;
+        dot[j] = 0.f;
+    }
+    multiply((steps - 1) & 1);
+
+    const T* const bias_row = !YC && a.bias != nullptr ? a.bias + (int64_t)here.expert * a.N + col0 + lane_col : nullptr;
+#pragma unroll
+    for (int p0 = 0; p0 < NT / 2; p0 += kPair) {
+        vec8<T> bias[kPair];
+#pragma unroll
+        for (int h = 0; h < kPair; h++) {
+            const int left = cols_left - 32 * (p0 + h);
+            bias[h] = take8(bias_row != nullptr && left > 0 ? bias_row + 32 * (p0 + h) : nullptr, a.wide, left);
+        }
+#pragma unroll
+        for (int j = 0; j < MT; j++) {
+            const int64_t row = row0 + 16 * j;
+            vec8<T> o[kPair], z[kPair];
+            if constexpr (kPair == 2 && kSlope) {
+                if (whole) arrange_lines<T>(early[0][j], early[1][j], lane);
+            }
+#pragma unroll
+            for (int h = 0; h < kPair; h++) {
+                const int p = p0 + h, col = col0 + 32 * p, left = cols_left - 32 * p;
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const u32x2 w = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[2 * p][j][e]), __float_as_uint(acc[2 * p + 1][j][e]), false, false);
+                    v[e] = __uint_as_float(w[0]);
+                    v[4 + e] = __uint_as_float(w[1]);
+                }
+                const bool inside = 16 * j < rows_left && left > 0;
+                if (inside) o[h] = way_out<YC, ACT>(a, v, bias[h], scale[j], early[h][j], left, z[h], dot[j]);
+                if (whole || !inside) continue;
+                if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (row * a.ldz + col) + at_z) = z[h];
+                put8(a.out + (row * a.ldo + col) + at_out, o[h], a.wide_out, left);
+            }
+            if constexpr (kPair == 2) {
+                if (whole) {
+                    if (!YC && a.z != nullptr) store_lines(a.z + (row * a.ldz + (col0 + 32 * p0)), at_z, (unsigned)(8 * a.ldz), z[0], z[1], lane);
+                    store_lines(a.out + (row * a.ldo + (col0 + 32 * p0)), at_out, (unsigned)(8 * a.ldo), o[0], o[1], lane);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);                // (rows one after another: all at once do not fit the registers)
+        }
+        if (p0 + kPair < NT / 2) read_side(p0 + kPair);
+    }
+    if constexpr (kSlope) {
+        if (a.dots != nullptr) {
+#pragma unroll
+            for (int j = 0; j < MT; j++) {
+                const float d = quad_sum(dot[j]);
+                if (quad == 0 && 16 * j < rows_left) a.dots[(int64_t)(row0 + 16 * j + lane_row) * a.parts + here.tn * WAVES_N + wave / WAVES_M] = d;
+            }
+        }
+    }
+    if (!YC && a.scaled == kScaledRows && here.tn == 0 && wn == 0 && quad == 0) {
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+            if (16 * j < rows_left) a.sorted[row0 + 16 * j + lane_row] = scale[j];
+    }
+}
+
+// Few rows for each expert: a workgroup takes 32 columns of up to 64 rows of one, its eight waves an eighth of the contraction each, through two stages of
+// LDS of their own; the sums meet at the end (linear.hip's few_rows_kernel).  An expert's weight is read once for them, and there is little else.
+constexpr int kFewWaves = 8, kFewColumns = 32, kFewStage = kFewColumns * kStep;
+template <typename T, bool YC, int MT, int ACT>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void grouped_few_kernel(const Grouped<T> a) {
+    constexpr bool kSlope = YC && ACT != LLSA_ACT_NONE;
+    typedef Operand<T, YC, kFewColumns, 1> OperandY;
+    HIP_DYNAMIC_SHARED(char, shared)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
+    T* const stage = reinterpret_cast<T*>(shared) + wave * 2 * kFewStage;
+    Here here;
+    if (!find_tile<16 * MT, kFewColumns>(a, here, lane)) return;
+    if (here.expert < 0) {
+        write_zeros<16 * MT, kFewColumns>(a, here);
+        return;
+    }
+    const int n0 = here.n0, row0 = here.m0, all = (a.K + kStep - 1) / kStep, each = (all + kFewWaves - 1) / kFewWaves, first = min(all, wave * each), steps = min(all - first, each);
+    OperandY oy;
+    oy.init(0, lane, a.ldy, min(kFewColumns, (YC ? a.ny : a.N) - n0));
+    const int k0 = first * kStep;
+    const T* py = a.y + here.expert * a.y_expert + (YC ? k0 * a.ldy + n0 : n0 * a.ldy + k0);
+    const T* px[MT];
+#pragma unroll
+    for (int j = 0; j < MT; j++) {
+        const int place = min(row0 + 16 * j + (lane & 15), here.m_end - 1);
+        px[j] = a.x + (a.order.slots != nullptr ? a.order.token(place) : place) * a.ldx;
+    }
+    f32x4 acc[2][MT];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    vec8<T> next[MT][2];
+    auto request = [&](int s) {
+        const int k = k0 + s * kStep;
+        oy.request(py + (YC ? s * kStep * a.ldy : s * kStep), stage + (s & 1) * kFewStage, 0, lane, a.K - k);
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+                const int at = k + 32 * ks + 8 * quad;
+                next[j][ks] = *reinterpret_cast<const vec8<T>*>(at < a.K ? px[j] + at : reinterpret_cast<const T*>(kZeros));
+            }
+    };
+    if (steps > 0) request(0);
+    for (int s = 0; s < steps; s++) {
+        vec8<T> fx[MT][2];
+        wave_waits_for_copies();
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) fx[j][ks] = next[j][ks];
+        if (s + 1 < steps) request(s + 1);
+        const T* const ty = stage + (s & 1) * kFewStage;
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const vec8<T> fy = OperandY::fragment(ty, 16 * i, ks, lane);
+#pragma unroll
+                for (int j = 0; j < MT; j++) acc[i][j] = product16(fy, fx[j][ks], acc[i][j]);
+            }
+        wave_waits_for_reads();                               // (done, before the next request but one writes there)
+    }
+
+    // wave j adds up tile j of rows, in the order of the waves
+    __syncthreads();
+    f32x4* const sums = reinterpret_cast<f32x4*>(shared);     // [wave][tile][half][lane]
+#pragma unroll
+    for (int j = 0; j < MT; j++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) sums[((wave * MT + j) * 2 + i) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    if (wave >= MT) return;
+    f32x4 t[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        t[i] = sums[(wave * 2 + i) * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < kFewWaves; w++) t[i] += sums[((w * MT + wave) * 2 + i) * 64 + lane];
+    }
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const u32x2 w = __builtin_amdgcn_permlane16_swap(__float_as_uint(t[0][e]), __float_as_uint(t[1][e]), false, false);
+        v[e] = __uint_as_float(w[0]);
+        v[4 + e] = __uint_as_float(w[1]);
+    }
+    const int lane_col = 16 * (quad & 1) + 8 * (quad >> 1), m = row0 + 16 * wave + (lane & 15), left = a.N - n0 - lane_col;
+    const bool row_there = m < here.m_end, inside = row_there && left > 0;
+    float dot = 0.f;
+    const float scale = row_there ? weight_of(a, m) : 0.f;
+    if (inside) {
+        vec8<T> early = take8<T>(nullptr, true, 0), z;
+        if (kSlope) early = *reinterpret_cast<const vec8<T>*>(a.slope_at + (int64_t)m * a.ldz + n0 + lane_col);
+        const vec8<T> bias = take8(!YC && a.bias != nullptr ? a.bias + (int64_t)here.expert * a.N + n0 + lane_col : nullptr, a.wide, left);
+        const vec8<T> o = way_out<YC, ACT>(a, v, bias, scale, early, left, z, dot);
+        if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (int64_t)m * a.ldz + n0 + lane_col) = z;
+        put8(a.out + (int64_t)m * a.ldo + n0 + lane_col, o, a.wide_out, left);
+    }
+    if (kSlope && a.dots != nullptr) {
+        dot = quad_sum(dot);
+        if (quad == 0 && row_there) a.dots[(int64_t)m * a.parts + here.tn] = dot;
+    }
+    if (!YC && a.scaled == kScaledRows && here.tn == 0 && quad == 0 && row_there) a.sorted[m] = scale;
+}
+
+// ---------------------------------------------------------------------------------------
+// dW: C_e[m][n] = sum over an expert's rows p of X[p][m] Y[p][n], either of them gathered.  The rows are taken in pieces; an expert of one piece is written
+// straight away, the sums of the others' pieces meet in a second launch, which also writes the zeros of an expert without rows.
+// ---------------------------------------------------------------------------------------
+template <typename T>
+struct GroupedWeights {
+    const T *x, *y;
+    int64_t ldx, ldy;
+    const int32_t* offsets;
+    Order order_x, order_y;
+    int experts, rows, piece;             // piece: rows of one, a multiple of 64
+    int M, N, nx, ny, tiles_m, tiles_n;
+    const float* sorted;                  // weights of the sums of x's rows, or NULL
+    T *out, *sums;                        // (experts, M, N), (experts, M) or NULL
+    float *part, *part_sum;               // [piece][M][ld_part], [piece][M]
+    int64_t ld_part;
+    int wide_out;
+};
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(const GroupedWeights<T> a) {
+    constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
+    typedef Operand<T, true, BM, kWaves> OperandX;
+    typedef Operand<T, true, BN, kWaves> OperandY;
+    HIP_DYNAMIC_SHARED(char, shared)
+    T* const lds = reinterpret_cast<T*>(shared);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int quad = lane >> 4, wm = (wave % WAVES_M) * WM, wn = (wave / WAVES_M) * WN;
+    Runs runs;
+    runs.load(a.offsets, a.experts, a.rows, a.piece, false, lane);
+    const int per_piece = a.tiles_m * a.tiles_n, total = runs.total * per_piece;
+    if ((int)blockIdx.x >= total) return;
+    const int at = xcd_order((int)blockIdx.x, total), number = at / per_piece, tile = at - number * per_piece, tn = tile / a.tiles_m, tm = tile - tn * a.tiles_m;
+    const Piece p = runs.find(number);
+    const int m0 = tm * BM, n0 = tn * BN, first = p.begin + (number - p.first) * a.piece, rows = min(a.piece, p.end - first), steps = (rows + kStep - 1) / kStep;
+
+    GatheredColumns<T, BM, kWaves> ox;
+    GatheredColumns<T, BN, kWaves> oy;
+    ox.init(min(BM, a.nx - m0), wave, lane);
+    oy.init(min(BN, a.ny - n0), wave, lane);
+    auto look_up = [&](int s) {
+        ox.look_up(a.order_x, first + s * kStep, rows - s * kStep, wave, lane);
+        oy.look_up(a.order_y, first + s * kStep, rows - s * kStep, wave, lane);
+    };
+    auto request = [&](int s) {
+        T* const t = lds + (s & 1) * (kTileX + kTileY);
+        ox.request(a.x + m0, a.ldx, t, wave, lane, rows - s * kStep);
+        oy.request(a.y + n0, a.ldy, t + kTileX, wave, lane, rows - s * kStep);
+    };
+    const bool sums = a.part_sum != nullptr && tn == 0 && wn == 0;
+    f32x4 acc[NT][MT], sum[MT];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < MT; j++) sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    vec8<T> ones;
+#pragma unroll
+    for (int e = 0; e < 8; e++) ones[e] = (T)1.f;
+    auto multiply = [&](int s) {
+        const T* const tx = lds + (s & 1) * (kTileX + kTileY);
+        const T* const ty = tx + kTileX;
+#pragma unroll
+        for (int ks = 0; ks < kStep / 32; ks++) {
+            vec8<T> fx[MT], fy[NT];
+#pragma unroll
+            for (int j = 0; j < MT; j++) fx[j] = OperandX::fragment(tx, wm + 16 * j, ks, lane);
+#pragma unroll
+            for (int i = 0; i < NT; i++) fy[i] = OperandY::fragment(ty, wn + 16 * i, ks, lane);
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+#pragma unroll
+                for (int j = 0; j < MT; j++) acc[i][j] = product16(fy[i], fx[j], acc[i][j]);
+            if (sums) {
+                if (a.sorted == nullptr) {
+#pragma unroll
+                    for (int j = 0; j < MT; j++) sum[j] = product16(ones, fx[j], sum[j]);
+                } else {
+                    // a weight in two parts of T, which hold 16 bits of it and more: sums of products with both.  (Those of tiny weights end at T's least number.)
+                    vec8<T> high, low;
+                    const int k = s * kStep + 32 * ks + 8 * quad;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float w = k + e < rows ? a.sorted[first + min(k + e, rows - 1)] : 0.f;
+                        high[e] = (T)w;
+                        low[e] = (T)(w - (float)high[e]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < MT; j++) sum[j] = product16(low, fx[j], product16(high, fx[j], sum[j]));
+                }
+            }
+        }
+    };
+    look_up(0);
+    request(0);
+    if (steps > 1) look_up(1);
+    for (int s = 0; s + 1 < steps; s++) {
+        wait_vm0();
+        __syncthreads();                                      // everyone's copies of this step are there, and everyone is done with the other buffer
+        request(s + 1);
+        if (s + 2 < steps) look_up(s + 2);
+        multiply(s);
+    }
+    wait_vm0();
+    __syncthreads();
+    multiply(steps - 1);
+
+    const int lane_row = lane & 15, lane_col = 16 * (quad & 1) + 8 * (quad >> 1);
+    const bool alone = p.count == 1;
+#pragma unroll
+    for (int c = 0; c < NT / 2; c++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) {
+            const int m = m0 + wm + 16 * j + lane_row, n = n0 + wn + 32 * c + lane_col, left = a.N - n;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const u32x2 w = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[2 * c][j][e]), __float_as_uint(acc[2 * c + 1][j][e]), false, false);
+                v[e] = __uint_as_float(w[0]);
+                v[4 + e] = __uint_as_float(w[1]);
+            }
+            if (m >= a.M || left <= 0) continue;
+            if (alone) {
+                store8(a.out + ((int64_t)p.expert * a.M + m) * a.N + n, v, a.wide_out, left);
+            } else {
+                float* const o = a.part + ((int64_t)number * a.M + m) * a.ld_part + n;
+                *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+                *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+            }
+        }
+    if (sums && quad == 0) {
+#pragma unroll
+        for (int j = 0; j < MT; j++) {
+            const int m = m0 + wm + 16 * j + lane;
+            if (m >= a.M) continue;
+            if (alone) a.sums[(int64_t)p.expert * a.M + m] = (T)sum[j][0];
+            else a.part_sum[(int64_t)number * a.M + m] = sum[j][0];
+        }
+    }
+}
+// The pieces of an expert added up, by four waves of which each takes every fourth piece of the same 64 places (of four elements); nothing to do where there was one.
+template <typename T>
+__global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<T> a, int blocks) {
+    __shared__ f32x4 rest[3][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, expert = (int)blockIdx.x / blocks;
+    Runs runs;
+    runs.load(a.offsets, a.experts, a.rows, a.piece, false, lane);
+    Piece p = {0, 0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < Runs::kLanes; i++)
+        if (expert / 64 == i) p = runs.of_expert(i, expert % 64);
+    if (p.count == 1) return;
+    const int64_t n4 = a.ld_part / 4, i = (int64_t)((int)blockIdx.x - expert * blocks) * 64 + lane, m = i < a.M * n4 ? i / n4 : i - a.M * n4;
+    const int n = (int)(i - m * n4) * 4;
+    const bool sum = i >= a.M * n4;                           // of the rows
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (!sum) {
+#pragma unroll 8
+        for (int s = wave; s < p.count; s += 4) v += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)(p.first + s) * a.M + m) * a.ld_part + n);
+    } else if (a.part_sum != nullptr && m < a.M) {
+        for (int s = wave; s < p.count; s += 4) v[0] += a.part_sum[(int64_t)(p.first + s) * a.M + m];
+    }
+    if (wave > 0) rest[wave - 1][lane] = v;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int r = 0; r < 3; r++) v += rest[r][lane];
+    if (!sum) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (n + e < a.N) a.out[((int64_t)expert * a.M + m) * a.N + n + e] = (T)v[e];
+    } else if (a.part_sum != nullptr && m < a.M) {
+        a.sums[(int64_t)expert * a.M + m] = (T)v[0];
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// A token's rows added up: out = residual + gate * sum over j of y[places[j]].  Bound by memory.
+// ---------------------------------------------------------------------------------------
+template <typename T>
+struct Combine {
+    const T *y, *gate, *residual;
+    const int32_t* places;
+    T *out, *sum;                         // sum: what the gate multiplies, or NULL
+    int64_t ldy, s_gate, ldr, ldo, lds, tokens, per_sample;
+    int k, rows, N, pieces, wide, wide_side, wide_out;       // pieces: of eight, of a row
+};
+template <typename T>
+__global__ __launch_bounds__(256) void combine_kernel(const Combine<T> a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / a.pieces;
+    if (m >= a.tokens) return;
+    const int n = (int)(i - m * a.pieces) * 8, left = a.N - n;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < a.k; j++) {
+        const int p = a.places[m * a.k + j];
+        if ((unsigned)p >= (unsigned)a.rows) continue;        // no expert
+        const vec8<T> y = *reinterpret_cast<const vec8<T>*>(a.y + p * a.ldy + n);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += (float)y[e];
+    }
+    if (a.sum != nullptr) store8(a.sum + m * a.lds + n, v, true, 8);
+    if (a.gate != nullptr) {
+        const vec8<T> g = take8(a.gate + m / a.per_sample * a.s_gate + n, a.wide, left);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] *= (float)g[e];
+    }
+    if (a.residual != nullptr) {
+        const vec8<T> r = take8(a.residual + m * a.ldr + n, a.wide_side, left);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += (float)r[e];
+    }
+    store8(a.out + m * a.ldo + n, v, a.wide_out, left);
+}
+
+// dweights[m][j] = the parts of its place added up, and dout[m] . b_out of the expert; 0 without one.  A wave a token.
+template <typename T>
+struct DWeights {
+    const float* dots;
+    const T *dout, *bias;
+    const int32_t *places, *experts;
+    float* dweights;
+    int64_t ldd, tokens;
+    int k, rows, parts, N, n_experts, wide;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void dweights_kernel(const DWeights<T> a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (m >= a.tokens) return;
+    for (int j = 0; j < a.k; j++) {
+        const int p = a.places[m * a.k + j];
+        float v = 0.f;
+        const bool there = (unsigned)p < (unsigned)a.rows;
+        if (there) {
+            for (int i = lane; i < a.parts; i += 64) v += a.dots[(int64_t)p * a.parts + i];
+            if (a.bias != nullptr) {
+                const T* const b = a.bias + (int64_t)clampi(a.experts[m * a.k + j], 0, a.n_experts - 1) * a.N;
+                for (int n = lane * 8; n < a.N; n += 512) {
+                    const vec8<T> x = *reinterpret_cast<const vec8<T>*>(a.dout + m * a.ldd + n), y = take8(b + n, a.wide, a.N - n);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v += n + e < a.N ? (float)x[e] * (float)y[e] : 0.f;
+                }
+            }
+        }
+        v = octet_sum(v);
+        v += across<8>(v);
+        v = quad_sum(v);
+        if (lane == 0) a.dweights[m * a.k + j] = v;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------------------
+Order order_of(const int32_t* slots, int k, int64_t tokens, int64_t rows) {
+    return Order{slots, k > 1 ? (unsigned)((((uint64_t)1 << 32) + k - 1) / k) : 0u, (int)tokens, (int)rows};
+}
+// Pieces there can be: the rows' whole ones, and one more for each expert (two more of rows that no expert has)
+int64_t pieces_of(int64_t rows, int64_t experts, int64_t size) { return rows / size + std::min<int64_t>(experts + 2, rows); }
+
+// Which tiles: few rows for each expert on the average, small tiles while there are few of them for each CU, large ones where the experts fill them
+enum GroupedTiles { kFew16, kFew32, kFew64, k64, k128, k256 };
+GroupedTiles grouped_tiles(int64_t rows, int64_t experts, int64_t N, int64_t K) {
+    const int64_t each = ceil_div(rows, experts);
+    if (each <= 64 || (rows / 64 + experts) * ceil_div(N, kFewColumns) <= kCus) return each <= 12 ? kFew16 : each <= 28 ? kFew32 : kFew64;
+    if ((rows / 64 + experts) * ceil_div(N, 64) <= 4 * kCus) return k64;
+    if (each >= 1024 && N >= 512 && K >= 1024 && (rows / 256 + experts) * ceil_div(N, 256) >= 2 * kCus) return k256;
+    return k128;
+}
+int columns_of(GroupedTiles t) { return t <= kFew64 ? kFewColumns : t == k64 ? 64 : t == k128 ? 128 : 256; }
+int waves_across(GroupedTiles t) { return t <= kFew64 ? 1 : t == k256 ? 4 : 2; }
+int64_t dot_parts(int64_t rows, int64_t experts, int64_t N, int64_t K) {
+    const GroupedTiles t = grouped_tiles(rows, experts, N, K);
+    return ceil_div(N, columns_of(t)) * waves_across(t);
+}
+template <typename T, bool YC, int BM, int BN, int WAVES_M, int WAVES_N, int ACT>
+int launch_grouped_tiles(Grouped<T>& a, hipStream_t stream) {
+    a.tiles_n = (int)ceil_div(a.N, BN);
+    const int64_t grid = pieces_of(a.rows, a.experts, BM) * a.tiles_n;
+    if (grid > kMaxGrid) return fail(-1, "experts: too many rows");
+    constexpr int lds = 2 * (BM + BN) * kStep * (int)sizeof(T);
+    auto kernel = grouped_kernel<T, YC, BM, BN, WAVES_M, WAVES_N, ACT>;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return fail(-101, "experts: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * WAVES_M * WAVES_N), lds, stream, a);
+    return 0;
+}
+template <typename T, bool YC, int MT, int ACT>
+int launch_grouped_few(Grouped<T>& a, hipStream_t stream) {
+    a.tiles_n = (int)ceil_div(a.N, kFewColumns);
+    a.group = 1;
+    const int64_t grid = pieces_of(a.rows, a.experts, 16 * MT) * a.tiles_n;
+    if (grid > kMaxGrid) return fail(-1, "experts: too many rows");
+    constexpr int lds = kFewWaves * 2 * kFewStage * (int)sizeof(T);                            // (the sums of up to 64 rows fit in it as well)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(grouped_few_kernel<T, YC, MT, ACT>), dim3((unsigned)grid), dim3(64 * kFewWaves), lds, stream, a);
+    return 0;
+}
+template <typename T, bool YC, int ACT>
+int launch_grouped(Grouped<T>& a, hipStream_t stream) {
+    a.group = (int64_t)a.N * a.K <= (1 << 20) ? 1 : 8;        // (rows of tiles that share y while it does not fit the L2 beside them)
+    const GroupedTiles t = grouped_tiles(a.rows, a.experts, a.N, a.K);
+    a.parts = (int)dot_parts(a.rows, a.experts, a.N, a.K);
+    switch (t) {
+        case kFew16: return launch_grouped_few<T, YC, 1, ACT>(a, stream);
+        case kFew32: return launch_grouped_few<T, YC, 2, ACT>(a, stream);
+        case kFew64: return launch_grouped_few<T, YC, 4, ACT>(a, stream);
+        case k64: return launch_grouped_tiles<T, YC, 64, 64, 2, 2, ACT>(a, stream);
+        case k128: return launch_grouped_tiles<T, YC, 128, 128, 2, 2, ACT>(a, stream);
+        default: return launch_grouped_tiles<T, YC, 256, 256, 2, 4, ACT>(a, stream);
+    }
+}
+template <typename T, bool YC>
+int launch_by_act(Grouped<T>& a, int act, hipStream_t stream) {
+    switch (act) {
+        case LLSA_ACT_SILU: return launch_grouped<T, YC, LLSA_ACT_SILU>(a, stream);
+        case LLSA_ACT_GELU: return launch_grouped<T, YC, LLSA_ACT_GELU>(a, stream);
+        case LLSA_ACT_GELU_TANH: return launch_grouped<T, YC, LLSA_ACT_GELU_TANH>(a, stream);
+        default: return launch_grouped<T, YC, LLSA_ACT_NONE>(a, stream);
+    }
+}
+template <typename T>
+int experts_fwd(const llsa_experts_args& q, hipStream_t stream) {
+    Grouped<T> a{};
+    a.x = (const T*)q.x; a.ldx = q.ldx; a.y = (const T*)q.w; a.ldy = q.ldw; a.y_expert = (int64_t)q.N * q.ldw;
+    a.offsets = q.offsets; a.order = order_of(q.gather_x ? q.order : nullptr, q.k, q.tokens, q.rows);
+    a.experts = q.E; a.rows = (int)q.rows; a.N = q.N; a.K = q.K; a.gaps = q.gaps;
+    a.bias = (const T*)q.bias; a.weights = q.weights; a.sorted = q.sorted;
+    a.scaled = q.weights != nullptr ? kScaledRows : q.sorted != nullptr ? kScaledBias : kUnscaled;
+    a.out = (T*)q.out; a.ldo = q.ldo; a.z = (T*)q.z; a.ldz = q.ldz;
+    a.wide = q.N % 8 == 0 && wide8(q.bias, 0);
+    a.wide_out = (q.N % 8 == 0 && wide8(q.out, q.ldo)) || q.padded;
+    if (int rc = launch_by_act<T, false>(a, q.act, stream)) return rc;
+    return launch_status("experts_fwd");
+}
+template <typename T>
+int experts_dx(const llsa_experts_args& q, hipStream_t stream) {
+    Grouped<T> a{};
+    a.x = (const T*)q.dz; a.ldx = q.lddz; a.y = (const T*)q.w; a.ldy = q.ldw; a.y_expert = (int64_t)q.N * q.ldw;
+    a.offsets = q.offsets; a.order = order_of(q.gather_dz ? q.order : nullptr, q.k, q.tokens, q.rows);
+    a.experts = q.E; a.rows = (int)q.rows; a.N = q.K; a.ny = (int)pad8(q.K); a.K = q.N; a.gaps = q.gaps;
+    a.out = (T*)q.out; a.ldo = q.ldo; a.slope_at = (const T*)q.z; a.ldz = q.ldz; a.dots = q.dots;
+    a.sorted = q.sorted;
+    a.scaled = q.z != nullptr && q.sorted != nullptr ? kScaledRows : kUnscaled;
+    a.wide_out = (q.K % 8 == 0 && wide8(q.out, q.ldo)) || q.padded;
+    if (int rc = launch_by_act<T, true>(a, q.z != nullptr ? q.act : LLSA_ACT_NONE, stream)) return rc;
+    return launch_status("experts_dx");
+}
+
+// Rows of a piece.  More pieces fill the chip's workgroups more evenly, and are more sums to write and read; experts of one piece need neither.
+int grouped_rows(int64_t N) { return ceil_div(N, 192) * 192 <= ceil_div(N, 128) * 128 ? 192 : 128; }
+bool small_tiles(int64_t rows, int64_t experts, int64_t N, int64_t K) { return experts * ceil_div(N, 128) * ceil_div(K, 128) < kCus && rows < 64 * 1024; }
+int64_t piece_rows(int64_t rows, int64_t experts, int64_t N, int64_t K) {
+    const bool small = small_tiles(rows, experts, N, K);
+    const int64_t bm = small ? 64 : grouped_rows(N), bn = small ? 64 : 128, tiles = ceil_div(N, bm) * ceil_div(K, bn);
+    const double all = 2. * (double)rows * N * K / 0.72e9, sums = 8. * (double)N * K / 4e6;    // us
+    int64_t best = 1;
+    double least = 0;
+    for (int64_t p = 1; p <= std::max<int64_t>(1, rows / experts / 256) && (p - 1) * tiles * experts < 8 * kCus; p++) {
+        const double n = (double)(tiles * experts * p) / (2 * kCus), t = all * std::ceil(n) / n + (p > 1 ? sums * experts * p : 0);
+        if (p == 1 || t < least) best = p, least = t;
+    }
+    // experts are not alike: with one piece each, the largest one's may be twice the average before it is cut
+    const int64_t length = best == 1 ? 2 * ceil_div(rows, experts) : ceil_div(ceil_div(rows, experts), best);
+    return std::max<int64_t>(256, ceil_div(length, kStep) * kStep);
+}
+template <typename T, int BM, int BN>
+int launch_grouped_dw(GroupedWeights<T>& a, hipStream_t stream) {
+    a.tiles_m = (int)ceil_div(a.M, BM);
+    a.tiles_n = (int)ceil_div(a.N, BN);
+    const int64_t grid = pieces_of(a.rows, a.experts, a.piece) * a.tiles_m * a.tiles_n;
+    if (grid > kMaxGrid) return fail(-1, "experts_dw: too many rows");
+    constexpr int lds = 2 * (BM + BN) * kStep * (int)sizeof(T);
+    auto kernel = grouped_dw_kernel<T, BM, BN, 2, 2>;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return fail(-101, "experts_dw: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), lds, stream, a);
+    return 0;
+}
+template <typename T>
+int experts_dw(const llsa_experts_args& q, hipStream_t stream) {
+    GroupedWeights<T> a{};
+    a.x = (const T*)q.dz; a.ldx = q.lddz; a.nx = (int)pad8(q.N);
+    a.y = (const T*)q.x; a.ldy = q.ldx; a.ny = (int)pad8(q.K);
+    a.offsets = q.offsets;
+    a.order_x = order_of(q.gather_dz ? q.order : nullptr, q.k, q.tokens, q.rows);
+    a.order_y = order_of(q.gather_x ? q.order : nullptr, q.k, q.tokens, q.rows);
+    a.experts = q.E; a.rows = (int)q.rows; a.M = q.N; a.N = q.K;
+    a.piece = (int)piece_rows(q.rows, q.E, q.N, q.K);
+    a.sorted = q.sorted;
+    a.out = (T*)q.out; a.sums = (T*)q.dbias;
+    a.ld_part = pad8(q.K);
+    a.part = (float*)q.workspace;
+    a.part_sum = q.dbias != nullptr ? a.part + pieces_of(q.rows, q.E, a.piece) * a.M * a.ld_part : nullptr;
+    a.wide_out = q.K % 8 == 0 && aligned16(q.out);
+    int rc;
+    if (small_tiles(q.rows, q.E, q.N, q.K)) rc = launch_grouped_dw<T, 64, 64>(a, stream);
+    else if (grouped_rows(q.N) == 192) rc = launch_grouped_dw<T, 192, 128>(a, stream);
+    else rc = launch_grouped_dw<T, 128, 128>(a, stream);
+    if (rc != 0) return rc;
+    const int64_t places = (int64_t)a.M * (a.ld_part / 4) + (q.dbias != nullptr ? a.M : 0), blocks = ceil_div(places, 64);
+    if (blocks * q.E > kMaxGrid) return fail(-1, "experts_dw: too many weights");
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(grouped_join_kernel<T>), dim3((unsigned)(blocks * q.E)), dim3(256), 0, stream, a, (int)blocks);
+    return launch_status("experts_dw");
+}
+template <typename T>
+int experts_combine(const llsa_experts_args& q, hipStream_t stream) {
+    Combine<T> a{};
+    a.y = (const T*)q.x; a.ldy = q.ldx; a.places = q.places; a.k = q.k; a.rows = (int)q.rows; a.N = q.N; a.tokens = q.tokens; a.per_sample = std::max<int64_t>(1, q.per_sample);
+    a.gate = (const T*)q.gate; a.s_gate = q.s_gate; a.residual = (const T*)q.residual; a.ldr = q.ldr;
+    a.out = (T*)q.out; a.ldo = q.ldo; a.sum = (T*)q.z; a.lds = q.ldz;
+    a.pieces = (int)(pad8(q.N) / 8);
+    a.wide = q.N % 8 == 0 && wide8(q.gate, q.s_gate);
+    a.wide_side = q.N % 8 == 0 && wide8(q.residual, q.ldr);
+    a.wide_out = q.N % 8 == 0 && wide8(q.out, q.ldo);
+    const int64_t grid = ceil_div(q.tokens * a.pieces, 256);
+    LLSA_REQUIRE(grid <= kMaxGrid, "experts_combine: too many rows");
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(combine_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+    return launch_status("experts_combine");
+}
+template <typename T>
+int experts_dweights(const llsa_experts_args& q, hipStream_t stream) {
+    DWeights<T> a{};
+    a.dots = q.dots; a.dout = (const T*)q.dz; a.ldd = q.lddz; a.bias = (const T*)q.bias; a.places = q.places; a.experts = q.experts; a.dweights = q.dweights;
+    a.tokens = q.tokens; a.k = q.k; a.rows = (int)q.rows; a.N = q.N; a.n_experts = q.E;
+    a.parts = (int)dot_parts(q.rows, q.E, q.K, q.N);          // (of the product that made them: N channels in, K out)
+    a.wide = q.N % 8 == 0 && wide8(q.bias, 0);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(dweights_kernel<T>), dim3((unsigned)ceil_div(q.tokens, 4)), dim3(256), 0, stream, a);
+    return launch_status("experts_dweights");
+}
+
+int check_experts(const char* what, const llsa_experts_args* a) {
+    LLSA_REQUIRE(a != nullptr, "%s: no arguments", what);
+    if (int rc = check_sizes(what, a->rows, a->N, a->K, a->dtype, a->act)) return rc;
+    LLSA_REQUIRE(a->E >= 1 && a->E <= LLSA_MAX_EXPERTS && a->rows <= LLSA_MAX_SLOTS && a->tokens >= 0 && a->tokens <= LLSA_MAX_SLOTS, "%s: 1 to %d experts, at most %d rows", what,
+                 LLSA_MAX_EXPERTS, LLSA_MAX_SLOTS);
+    LLSA_REQUIRE(a->k >= 1 && a->k <= LLSA_MAX_CHOICES, "%s: 1 to %d experts a token", what, LLSA_MAX_CHOICES);
+    LLSA_REQUIRE(a->rows == 0 || a->offsets != nullptr, "%s: offsets", what);
+    LLSA_REQUIRE(!((a->gather_x || a->gather_dz) && a->rows > 0) || (a->order != nullptr && a->tokens > 0), "%s: gathered rows need the order and tokens", what);
+    return 0;
+}
+}  // namespace
+}  // namespace llsa
+
+using namespace llsa;
+
+#define BY_TYPE(fn) (a->dtype == LLSA_DTYPE_BF16 ? fn<bf16>(*a, (hipStream_t)stream) : fn<_Float16>(*a, (hipStream_t)stream))
+
+extern "C" int64_t llsa_experts_dw_workspace_bytes(int64_t rows, int E, int N, int K) {
+    if (rows <= 0 || E <= 0 || N <= 0 || K <= 0) return 0;
+    return 4 * pieces_of(rows, E, piece_rows(rows, E, N, K)) * N * (pad8(K) + 1);
+}
+extern "C" int64_t llsa_experts_dot_parts(int64_t rows, int E, int N, int K) {
+    if (rows <= 0 || E <= 0 || N <= 0 || K <= 0) return 0;
+    return dot_parts(rows, E, K, N);
+}
+extern "C" int llsa_experts_fwd(const llsa_experts_args* a, void* stream) {
+    if (int rc = check_experts("experts_fwd", a)) return rc;
+    if (a->rows == 0) return 0;
+    LLSA_REQUIRE(rows16(a->x, a->ldx) && rows16(a->w, a->ldw) && a->K % 8 == 0 && a->ldx >= a->K && a->ldw >= a->K,
+                 "experts_fwd: rows of x and w must be 16-byte aligned and a multiple of 8 long (zeros beyond the end)");
+    LLSA_REQUIRE(a->out != nullptr && offsets32(a->ldo) && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->N))), "experts_fwd: output, padded rows 16-byte aligned and a multiple of 8 long");
+    LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->N)), "experts_fwd: rows of z must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->weights == nullptr || (a->sorted != nullptr && a->gather_x), "experts_fwd: weights go with gathered rows, and are kept sorted");
+    return BY_TYPE(experts_fwd);
+}
+extern "C" int llsa_experts_dx(const llsa_experts_args* a, void* stream) {
+    if (int rc = check_experts("experts_dx", a)) return rc;
+    if (a->rows == 0) return 0;
+    LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->w, a->ldw) && a->lddz >= pad8(a->N) && a->ldw >= pad8(a->K), "experts_dx: rows of dz and w must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->out != nullptr && offsets32(a->ldo) && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->K))), "experts_dx: output, padded rows 16-byte aligned and a multiple of 8 long");
+    LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->K) && a->act != LLSA_ACT_NONE), "experts_dx: rows of z must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->dots == nullptr || a->z != nullptr, "experts_dx: sums of act(z) dx need z");
+    return BY_TYPE(experts_dx);
+}
+extern "C" int llsa_experts_dw(const llsa_experts_args* a, void* stream) {
+    if (int rc = check_experts("experts_dw", a)) return rc;
+    LLSA_REQUIRE(a->rows > 0, "experts_dw: no rows");
+    LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->x, a->ldx) && a->lddz >= pad8(a->N) && a->ldx >= pad8(a->K), "experts_dw: rows of dz and x must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->out != nullptr && a->workspace != nullptr && aligned16(a->workspace), "experts_dw: output and workspace (16-byte aligned)");
+    return BY_TYPE(experts_dw);
+}
+extern "C" int llsa_experts_combine(const llsa_experts_args* a, void* stream) {
+    if (int rc = check_experts("experts_combine", a)) return rc;
+    if (a->tokens == 0) return 0;
+    LLSA_REQUIRE(a->places != nullptr && a->out != nullptr && (a->rows == 0 || (rows16(a->x, a->ldx) && a->ldx >= pad8(a->N))), "experts_combine: rows 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->N)), "experts_combine: rows of the sums must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->gate == nullptr || (a->per_sample > 0 && a->tokens % a->per_sample == 0), "experts_combine: rows of a sample, whole samples");
+    return BY_TYPE(experts_combine);
+}
+extern "C" int llsa_experts_dweights(const llsa_experts_args* a, void* stream) {
+    if (int rc = check_experts("experts_dweights", a)) return rc;
+    if (a->tokens == 0) return 0;
+    LLSA_REQUIRE(a->places != nullptr && a->dweights != nullptr && (a->rows == 0 || a->dots != nullptr), "experts_dweights: places, sums and result");
+    LLSA_REQUIRE(a->bias == nullptr || (a->experts != nullptr && rows16(a->dz, a->lddz) && a->lddz >= pad8(a->N)), "experts_dweights: the bias needs the experts and dout in padded rows");
+    return BY_TYPE(experts_dweights);
+}

@@ -548,4 +548,5 @@ PYBIND11_MODULE(_llsa_host, m) {
     }));
     bind_block(m);
     bind_int8(m);
+    bind_experts(m);
 }
