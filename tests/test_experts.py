@@ -95,7 +95,7 @@ def test_large_route(M, n, k):
     g = torch.Generator(device=dev).manual_seed(M)
     l = torch.randn(M, n, device=dev, generator=g)
     out = llsa_amd.route_tokens(l, k)
-    v, i = torch.sort(l, -1, descending=True, stable=True)
+    v, i = torch.sort(l, dim=-1, descending=True, stable=True)
     assert torch.equal(out.experts.long(), i[:, :k])
     by, order = torch.sort(i[:, :k].reshape(-1), stable=True)
     assert torch.equal(out.order.long(), order) and torch.equal(out.offsets.long(), torch.searchsorted(by, torch.arange(n + 1, device=dev)))
