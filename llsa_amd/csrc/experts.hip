@@ -369,55 +369,237 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void grouped_few_kernel(const Gr
     if (!YC && a.scaled == kScaledRows && here.tn == 0 && quad == 0 && row_there) a.sorted[m] = scale;
 }
 
+// Many rows for each expert, a short contraction: the weights stay in registers (linear.hip's resident_kernel).  A workgroup of twelve waves keeps 384 columns of
+// an expert's weights, 32 columns a wave, and takes its share of the rows through LDS, 32 at a time and two such tiles ahead; where the expert changes it takes
+// in the next one's weights.  The tokens of a tile are looked up three tiles ahead.
+constexpr int kResWaves = 12, kResColumns = 32 * kResWaves, kResRows = 32, kResStages = 3, kResOwn = 32 * kStep + 64;
+struct Entry { int expert, begin, end, first, upto; };       // upto: number of the first tile behind its own
+template <typename T, bool YC, int ACT, int STEPS>
+__global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const Grouped<T> a, int blocks, int slots) {
+    typedef Operand<T, false, kResRows, 1> OperandX;          // of a step: 4 copies
+    typedef Operand<T, YC, 32, 1> OperandY;
+    constexpr int kStage = kResRows * kStep * STEPS;
+    constexpr bool kSlope = YC && ACT != LLSA_ACT_NONE;
+    static_assert(4 * STEPS <= 2 * kResWaves, "two copies of a wave take in a tile");
+    HIP_DYNAMIC_SHARED(char, shared)
+    T* const lds = reinterpret_cast<T*>(shared);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
+    // workgroups of an XCD: the blocks of columns of the same rows side by side
+    const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3, block = local % blocks, slot = (local / blocks) * 8 + xcd;
+    if (slot >= slots) return;
+    // begin, end and upto of every expert, and of the rows before the first and behind the last
+    int* const table = reinterpret_cast<int*>(lds + kResStages * kStage + kResWaves * kResOwn);
+    int tiles;
+    {
+        Runs runs;
+        runs.load(a.offsets, a.experts, a.rows, kResRows, a.gaps != 0, lane);
+        tiles = runs.total;
+        if (wave == 0) {
+#pragma unroll
+            for (int i = 0; i < Runs::kLanes; i++)
+                if (64 * i + lane < a.experts) {
+                    int* const e = table + 3 * (64 * i + lane);
+                    e[0] = runs.begin[i];
+                    e[1] = runs.end[i];
+                    e[2] = runs.upto[i];
+                }
+            if (lane < 2) {
+                int* const e = table + 3 * (a.experts + lane);
+                e[0] = lane ? runs.back : 0;
+                e[1] = lane ? runs.rows : runs.front;
+                e[2] = lane ? runs.total : runs.of_experts + (runs.front + kResRows - 1) / kResRows;
+            }
+        }
+    }
+    __syncthreads();
+    const int t0 = (int)((int64_t)tiles * slot / slots), t1 = (int)((int64_t)tiles * (slot + 1) / slots);
+    if (t0 >= t1) return;
+    auto entry = [&](int e, int first) {
+        const int* const p = table + 3 * e;
+        return Entry{e, __builtin_amdgcn_readfirstlane(p[0]), __builtin_amdgcn_readfirstlane(p[1]), first, __builtin_amdgcn_readfirstlane(p[2])};
+    };
+    auto advance = [&](Entry& e, int t) {                     // to the entry of tile t < tiles
+        while (t >= e.upto) e = entry(e.expert + 1, e.upto);
+    };
+    const int n0 = block * kResColumns + 32 * wave;
+    const bool columns = n0 < a.N;                            // (a wave beyond the last column copies, and does no more)
+    const int lane_col = 16 * (quad & 1) + 8 * (quad >> 1), lane_row = lane & 15;
+    // LDS of the wave's own: its weights on their way, 64 of the contraction at a time; the bias of its columns
+    T* const own = lds + kResStages * kStage + wave * kResOwn;
+    T* const vectors = own + 32 * kStep;
+
+    vec8<T> fy[2 * STEPS][2];
+    auto weights = [&](const T* w) {
+        OperandY oy;
+        oy.init(0, lane, a.ldy, 32);
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            oy.request(w + (YC ? s * kStep * a.ldy + n0 : n0 * a.ldy + s * kStep), own, 0, lane, kStep);
+            wave_waits_for_copies();
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) fy[2 * s + ks][i] = OperandY::fragment(own, 16 * i, ks, lane);
+            wave_waits_for_reads();
+        }
+    };
+
+    // this wave's two copies of a tile: their rows, and the elements of a row from which they begin
+    const bool copies = wave < 2 * STEPS;
+    int from_row[2];
+    Entry ahead = entry(0, 0);
+    auto look_up = [&](int t) {
+        if (t >= t1 || !copies) return;
+        advance(ahead, t);
+        if (ahead.expert >= a.experts) return;
+        const int m0 = ahead.begin + (t - ahead.first) * kResRows;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int at = min(m0 + OperandX::row_of((2 * wave + c) & 3, lane), ahead.end - 1);
+            from_row[c] = a.order.slots != nullptr ? a.order.token(at) : at;
+        }
+    };
+    auto request = [&](int t) {
+        if (t >= t1 || !copies) return;
+        T* const stage = lds + (t % kResStages) * kStage;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int i = 2 * wave + c, r = OperandX::row_of(i & 3, lane);
+            copy_to_lds(a.x + (uint64_t)(unsigned)from_row[c] * (unsigned)a.ldx + ((i >> 2) * kStep + OperandX::place_of(i & 3, r, lane)), stage + i * 512);
+        }
+    };
+    from_row[0] = from_row[1] = 0;
+    look_up(t0);
+    request(t0);
+    look_up(t0 + 1);
+    request(t0 + 1);
+    look_up(t0 + 2);
+    const unsigned at_out = (unsigned)(lane_row * a.ldo) + lane_col, at_z = (unsigned)(lane_row * a.ldz) + lane_col;
+    Entry now = entry(0, 0);
+    wait_vm0();
+    for (int t = t0, have = -1; t < t1; t++) {
+        advance(now, t);
+        const int m0 = now.begin + (t - now.first) * kResRows;
+        if (now.expert != have && columns && now.expert < a.experts) {
+            weights(a.y + now.expert * a.y_expert);
+            if (!YC && lane_row == 0) *reinterpret_cast<vec8<T>*>(vectors + lane_col) = take8(a.bias != nullptr ? a.bias + (int64_t)now.expert * a.N + n0 + lane_col : nullptr, a.wide, 8);
+            have = now.expert;
+        }
+        // this tile is there (every wave has waited for its copies before its last stores), and the one before it is read
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        request(t + 2);
+        look_up(t + 3);
+        if (!columns) {
+            wait_vm0();
+            continue;
+        }
+        if (now.expert >= a.experts) {                        // no expert's rows
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                if (m0 + 16 * j + lane_row < now.end) *reinterpret_cast<vec8<T>*>(a.out + ((int64_t)(m0 + 16 * j) * a.ldo + n0) + at_out) = take8<T>(nullptr, true, 8);
+            wait_vm0();
+            continue;
+        }
+        vec8<T> early[2];                                     // what is read on the way out
+        float scale[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int row = min(m0 + 16 * j + lane_row, now.end - 1);
+            scale[j] = weight_of(a, row);
+            if (kSlope) early[j] = __builtin_nontemporal_load(reinterpret_cast<const vec8<T>*>(a.slope_at + (int64_t)row * a.ldz + n0 + lane_col));
+        }
+        f32x4 acc[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const T* const tx = lds + (t % kResStages) * kStage;
+#pragma unroll
+        for (int ks = 0; ks < 2 * STEPS; ks++) {
+            vec8<T> fx[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) fx[j] = OperandX::fragment(tx + (ks >> 1) * (kResRows * kStep), 16 * j, ks & 1, lane);
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) acc[i][j] = product16(fy[ks][i], fx[j], acc[i][j]);
+        }
+        wait_vm0();
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            __builtin_amdgcn_sched_barrier(0);                // (the weights leave no registers for both at once, nor for the bias but here)
+            vec8<T> bias = take8<T>(nullptr, true, 8), z;
+            if (!YC) bias = *reinterpret_cast<const vec8<T>*>(vectors + lane_col);
+            float v[8], dot = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const u32x2 w = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[0][j][e]), __float_as_uint(acc[1][j][e]), false, false);
+                v[e] = __uint_as_float(w[0]);
+                v[4 + e] = __uint_as_float(w[1]);
+            }
+            const int64_t row = m0 + 16 * j;
+            const bool inside = row + lane_row < now.end;
+            const vec8<T> o = way_out<YC, ACT>(a, v, bias, scale[j], early[j], 8, z, dot);
+            if (kSlope && a.dots != nullptr) {
+                dot = quad_sum(dot);
+                if (quad == 0 && inside) a.dots[(row + lane_row) * a.parts + (n0 >> 5)] = dot;
+            }
+            if (!inside) continue;
+            if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (row * a.ldz + n0) + at_z) = z;
+            *reinterpret_cast<vec8<T>*>(a.out + (row * a.ldo + n0) + at_out) = o;
+            if (!YC && a.scaled == kScaledRows && n0 == 0 && quad == 0) a.sorted[row + lane_row] = scale[j];
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------
-// dW: C_e[m][n] = sum over an expert's rows p of X[p][m] Y[p][n], either of them gathered.  The rows are taken in pieces; an expert of one piece is written
-// straight away, the sums of the others' pieces meet in a second launch, which also writes the zeros of an expert without rows.
+// dW: C_e[m][n] = sum over an expert's rows p of X[p][m] Y[p][n], either of them gathered.  All rows are taken in chunks of one length, whatever the
+// experts' are, so that the workgroups are alike; one that meets the end of an expert's rows writes its sums and goes on with the next expert's.  An expert
+// within one chunk is written straight away, the sums of the others meet in a second launch, which also writes the zeros of an expert without rows.  Expert
+// e's sums of chunk c are number c + e: with every next one either grows.
 // ---------------------------------------------------------------------------------------
 template <typename T>
 struct GroupedWeights {
     const T *x, *y;
     int64_t ldx, ldy;
     const int32_t* offsets;
-    Order order_x, order_y;
-    int experts, rows, piece;             // piece: rows of one, a multiple of 64
+    Order order;
+    int experts, rows, chunk;             // chunk: rows of one, a multiple of 64
     int M, N, nx, ny, tiles_m, tiles_n;
     const float* sorted;                  // weights of the sums of x's rows, or NULL
     T *out, *sums;                        // (experts, M, N), (experts, M) or NULL
-    float *part, *part_sum;               // [piece][M][ld_part], [piece][M]
+    float *part, *part_sum;               // [number][M][ld_part], [number][M]
     int64_t ld_part;
     int wide_out;
 };
-template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(const GroupedWeights<T> a) {
+// GX, GY: which of them is gathered.  Rows first .. end - 1 of an expert; alone: they are all it has
+template <typename T, bool GX, bool GY, int BM, int BN, int WAVES_M, int WAVES_N>
+__device__ __forceinline__ void grouped_dw_piece(const GroupedWeights<T>& a, T* lds, int expert, int first, int end, bool alone, int number, int m0, int n0, int lane, int wave) {
     constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
     typedef Operand<T, true, BM, kWaves> OperandX;
     typedef Operand<T, true, BN, kWaves> OperandY;
-    HIP_DYNAMIC_SHARED(char, shared)
-    T* const lds = reinterpret_cast<T*>(shared);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int quad = lane >> 4, wm = (wave % WAVES_M) * WM, wn = (wave / WAVES_M) * WN;
-    Runs runs;
-    runs.load(a.offsets, a.experts, a.rows, a.piece, false, lane);
-    const int per_piece = a.tiles_m * a.tiles_n, total = runs.total * per_piece;
-    if ((int)blockIdx.x >= total) return;
-    const int at = xcd_order((int)blockIdx.x, total), number = at / per_piece, tile = at - number * per_piece, tn = tile / a.tiles_m, tm = tile - tn * a.tiles_m;
-    const Piece p = runs.find(number);
-    const int m0 = tm * BM, n0 = tn * BN, first = p.begin + (number - p.first) * a.piece, rows = min(a.piece, p.end - first), steps = (rows + kStep - 1) / kStep;
-
-    GatheredColumns<T, BM, kWaves> ox;
-    GatheredColumns<T, BN, kWaves> oy;
-    ox.init(min(BM, a.nx - m0), wave, lane);
-    oy.init(min(BN, a.ny - n0), wave, lane);
+    const int quad = lane >> 4, wm = (wave % WAVES_M) * WM, wn = (wave / WAVES_M) * WN, rows = end - first, steps = (rows + kStep - 1) / kStep;
+    Columns<T, BM, kWaves, GX> ox;
+    Columns<T, BN, kWaves, GY> oy;
+    ox.init(a.x + m0, a.ldx, first, min(BM, a.nx - m0), wave, lane);
+    oy.init(a.y + n0, a.ldy, first, min(BN, a.ny - n0), wave, lane);
+    const bool sums = a.part_sum != nullptr && n0 == 0 && wn == 0;
+    float weight = 0.f, next_weight = 0.f;                    // of row `lane` of the step
     auto look_up = [&](int s) {
-        ox.look_up(a.order_x, first + s * kStep, rows - s * kStep, wave, lane);
-        oy.look_up(a.order_y, first + s * kStep, rows - s * kStep, wave, lane);
+        ox.look_up(a.order, first + s * kStep, rows - s * kStep, wave, lane);
+        oy.look_up(a.order, first + s * kStep, rows - s * kStep, wave, lane);
+    };
+    auto look_up_weight = [&](int s) {
+        if (sums && a.sorted != nullptr) next_weight = s * kStep + lane < rows ? a.sorted[first + s * kStep + lane] : 0.f;
     };
     auto request = [&](int s) {
         T* const t = lds + (s & 1) * (kTileX + kTileY);
-        ox.request(a.x + m0, a.ldx, t, wave, lane, rows - s * kStep);
-        oy.request(a.y + n0, a.ldy, t + kTileX, wave, lane, rows - s * kStep);
+        ox.request(t, wave, lane, rows - s * kStep);
+        oy.request(t + kTileX, wave, lane, rows - s * kStep);
     };
-    const bool sums = a.part_sum != nullptr && tn == 0 && wn == 0;
     f32x4 acc[NT][MT], sum[MT];
 #pragma unroll
     for (int i = 0; i < NT; i++)
@@ -449,10 +631,9 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(c
                 } else {
                     // a weight in two parts of T, which hold 16 bits of it and more: sums of products with both.  (Those of tiny weights end at T's least number.)
                     vec8<T> high, low;
-                    const int k = s * kStep + 32 * ks + 8 * quad;
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float w = k + e < rows ? a.sorted[first + min(k + e, rows - 1)] : 0.f;
+                        const float w = __shfl(weight, 32 * ks + 8 * quad + e);
                         high[e] = (T)w;
                         low[e] = (T)(w - (float)high[e]);
                     }
@@ -463,21 +644,24 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(c
         }
     };
     look_up(0);
+    look_up_weight(0);
     request(0);
     if (steps > 1) look_up(1);
     for (int s = 0; s + 1 < steps; s++) {
         wait_vm0();
         __syncthreads();                                      // everyone's copies of this step are there, and everyone is done with the other buffer
+        weight = next_weight;
         request(s + 1);
         if (s + 2 < steps) look_up(s + 2);
+        look_up_weight(s + 1);
         multiply(s);
     }
     wait_vm0();
     __syncthreads();
+    weight = next_weight;
     multiply(steps - 1);
 
     const int lane_row = lane & 15, lane_col = 16 * (quad & 1) + 8 * (quad >> 1);
-    const bool alone = p.count == 1;
 #pragma unroll
     for (int c = 0; c < NT / 2; c++)
 #pragma unroll
@@ -492,7 +676,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(c
             }
             if (m >= a.M || left <= 0) continue;
             if (alone) {
-                store8(a.out + ((int64_t)p.expert * a.M + m) * a.N + n, v, a.wide_out, left);
+                store8(a.out + ((int64_t)expert * a.M + m) * a.N + n, v, a.wide_out, left);
             } else {
                 float* const o = a.part + ((int64_t)number * a.M + m) * a.ld_part + n;
                 *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
@@ -504,44 +688,70 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(c
         for (int j = 0; j < MT; j++) {
             const int m = m0 + wm + 16 * j + lane;
             if (m >= a.M) continue;
-            if (alone) a.sums[(int64_t)p.expert * a.M + m] = (T)sum[j][0];
+            if (alone) a.sums[(int64_t)expert * a.M + m] = (T)sum[j][0];
             else a.part_sum[(int64_t)number * a.M + m] = sum[j][0];
         }
     }
 }
-// The pieces of an expert added up, by four waves of which each takes every fourth piece of the same 64 places (of four elements); nothing to do where there was one.
+template <typename T, bool GX, bool GY, int BM, int BN, int WAVES_M, int WAVES_N>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(const GroupedWeights<T> a) {
+    HIP_DYNAMIC_SHARED(char, shared)
+    T* const lds = reinterpret_cast<T*>(shared);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int per_chunk = a.tiles_m * a.tiles_n, at = xcd_order((int)blockIdx.x, (int)gridDim.x), chunk = at / per_chunk, tile = at - chunk * per_chunk, tn = tile / a.tiles_m;
+    const int m0 = (tile - tn * a.tiles_m) * BM, n0 = tn * BN, chunk0 = chunk * a.chunk, chunk1 = min(a.rows, chunk0 + a.chunk);
+    for (int first = chunk0; first < chunk1;) {
+        Piece p;
+        {                                                     // (looked up each time: where everyone's rows are does not stay in registers)
+            Runs runs;
+            runs.load(a.offsets, a.experts, a.rows, a.chunk, false, lane);
+            p = runs.among(first, chunk1);
+        }
+        if (p.expert < 0) return;
+        grouped_dw_piece<T, GX, GY, BM, BN, WAVES_M, WAVES_N>(a, lds, p.expert, max(p.begin, chunk0), min(p.end, chunk1), p.begin >= chunk0 && p.end <= chunk1, chunk + p.expert, m0, n0, lane, wave);
+        first = p.end;
+        __syncthreads();                                      // (everyone is done with what the next one's copies overwrite)
+    }
+}
+// The sums of an expert's chunks added up, by four waves of which each takes every fourth of the same 64 places (of four elements); nothing to do where there was one.
 template <typename T>
 __global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<T> a, int blocks) {
     __shared__ f32x4 rest[3][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, expert = (int)blockIdx.x / blocks;
     Runs runs;
-    runs.load(a.offsets, a.experts, a.rows, a.piece, false, lane);
+    runs.load(a.offsets, a.experts, a.rows, a.chunk, false, lane);
     Piece p = {0, 0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < Runs::kLanes; i++)
         if (expert / 64 == i) p = runs.of_expert(i, expert % 64);
-    if (p.count == 1) return;
-    const int64_t n4 = a.ld_part / 4, i = (int64_t)((int)blockIdx.x - expert * blocks) * 64 + lane, m = i < a.M * n4 ? i / n4 : i - a.M * n4;
-    const int n = (int)(i - m * n4) * 4;
-    const bool sum = i >= a.M * n4;                           // of the rows
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (!sum) {
+    const int chunk0 = p.begin / a.chunk, chunks = p.end > p.begin ? (p.end - 1) / a.chunk - chunk0 + 1 : 0, first = chunk0 + expert;
+    if (chunks == 1) return;
+    const int64_t n4 = a.ld_part / 4, places = a.M * n4 + (a.part_sum != nullptr ? a.M : 0);
+    for (int64_t i = (int64_t)((int)blockIdx.x - expert * blocks) * 64 + lane; i - lane < places; i += 64 * blocks) {
+        const bool sum = i >= a.M * n4;                       // of the rows
+        const int64_t m = sum ? i - a.M * n4 : i / n4;
+        const int n = sum ? 0 : (int)(i - m * n4) * 4;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (!sum) {
 #pragma unroll 8
-        for (int s = wave; s < p.count; s += 4) v += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)(p.first + s) * a.M + m) * a.ld_part + n);
-    } else if (a.part_sum != nullptr && m < a.M) {
-        for (int s = wave; s < p.count; s += 4) v[0] += a.part_sum[(int64_t)(p.first + s) * a.M + m];
-    }
-    if (wave > 0) rest[wave - 1][lane] = v;
-    __syncthreads();
-    if (wave > 0) return;
+            for (int s = wave; s < chunks; s += 4) v += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)(first + s) * a.M + m) * a.ld_part + n);
+        } else if (i < places) {
+            for (int s = wave; s < chunks; s += 4) v[0] += a.part_sum[(int64_t)(first + s) * a.M + m];
+        }
+        if (wave > 0) rest[wave - 1][lane] = v;
+        __syncthreads();
+        if (wave == 0) {
 #pragma unroll
-    for (int r = 0; r < 3; r++) v += rest[r][lane];
-    if (!sum) {
+            for (int r = 0; r < 3; r++) v += rest[r][lane];
+            if (!sum) {
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (n + e < a.N) a.out[((int64_t)expert * a.M + m) * a.N + n + e] = (T)v[e];
-    } else if (a.part_sum != nullptr && m < a.M) {
-        a.sums[(int64_t)expert * a.M + m] = (T)v[0];
+                for (int e = 0; e < 4; e++)
+                    if (n + e < a.N) a.out[((int64_t)expert * a.M + m) * a.N + n + e] = (T)v[e];
+            } else if (i < places) {
+                a.sums[(int64_t)expert * a.M + m] = (T)v[0];
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -632,17 +842,26 @@ Order order_of(const int32_t* slots, int k, int64_t tokens, int64_t rows) {
 // Pieces there can be: the rows' whole ones, and one more for each expert (two more of rows that no expert has)
 int64_t pieces_of(int64_t rows, int64_t experts, int64_t size) { return rows / size + std::min<int64_t>(experts + 2, rows); }
 
+// Whether the weights stay in registers: a contraction of five or six steps, columns of which a wave has 32 or none and at most a quarter of the waves none, and
+// tiles enough for each workgroup that they pay for the weights' way there, also where it meets the next expert.
+bool resident(int64_t rows, int64_t experts, int64_t N, int64_t K) {
+    const int64_t blocks = ceil_div(N, kResColumns);
+    if ((K != 5 * kStep && K != 6 * kStep) || N % 32 != 0 || 4 * N < 3 * kResColumns * blocks || blocks > kCus / 8) return false;
+    const int64_t slots = kCus / 8 / blocks * 8;
+    return rows >= 8 * kResRows * experts && rows >= 8 * kResRows * slots;
+}
 // Which tiles: few rows for each expert on the average, small tiles while there are few of them for each CU, large ones where the experts fill them
-enum GroupedTiles { kFew16, kFew32, kFew64, k64, k128, k256 };
+enum GroupedTiles { kFew16, kFew32, kFew64, k64, k128, k256, kResident };
 GroupedTiles grouped_tiles(int64_t rows, int64_t experts, int64_t N, int64_t K) {
     const int64_t each = ceil_div(rows, experts);
     if (each <= 64 || (rows / 64 + experts) * ceil_div(N, kFewColumns) <= kCus) return each <= 12 ? kFew16 : each <= 28 ? kFew32 : kFew64;
+    if (resident(rows, experts, N, K)) return kResident;
     if ((rows / 64 + experts) * ceil_div(N, 64) <= 4 * kCus) return k64;
     if (each >= 1024 && N >= 512 && K >= 1024 && (rows / 256 + experts) * ceil_div(N, 256) >= 2 * kCus) return k256;
     return k128;
 }
-int columns_of(GroupedTiles t) { return t <= kFew64 ? kFewColumns : t == k64 ? 64 : t == k128 ? 128 : 256; }
-int waves_across(GroupedTiles t) { return t <= kFew64 ? 1 : t == k256 ? 4 : 2; }
+int columns_of(GroupedTiles t) { return t <= kFew64 || t == kResident ? 32 : t == k64 ? 64 : t == k128 ? 128 : 256; }
+int waves_across(GroupedTiles t) { return t <= kFew64 || t == kResident ? 1 : t == k256 ? 4 : 2; }
 int64_t dot_parts(int64_t rows, int64_t experts, int64_t N, int64_t K) {
     const GroupedTiles t = grouped_tiles(rows, experts, N, K);
     return ceil_div(N, columns_of(t)) * waves_across(t);
@@ -671,6 +890,16 @@ int launch_grouped_few(Grouped<T>& a, hipStream_t stream) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(grouped_few_kernel<T, YC, MT, ACT>), dim3((unsigned)grid), dim3(64 * kFewWaves), lds, stream, a);
     return 0;
 }
+template <typename T, bool YC, int ACT, int STEPS>
+int launch_grouped_resident(Grouped<T>& a, hipStream_t stream) {
+    const int blocks = (int)ceil_div(a.N, kResColumns), slots = kCus / 8 / blocks * 8;
+    constexpr int lds = (kResStages * kResRows * kStep * STEPS + kResWaves * kResOwn) * (int)sizeof(T) + 3 * (LLSA_MAX_EXPERTS + 2) * 4;
+    auto kernel = grouped_resident_kernel<T, YC, ACT, STEPS>;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return fail(-101, "experts: %s", hipGetErrorString(e));
+    hipLaunchKernelGGL(kernel, dim3(kCus), dim3(64 * kResWaves), lds, stream, a, blocks, slots);
+    return 0;
+}
 template <typename T, bool YC, int ACT>
 int launch_grouped(Grouped<T>& a, hipStream_t stream) {
     a.group = (int64_t)a.N * a.K <= (1 << 20) ? 1 : 8;        // (rows of tiles that share y while it does not fit the L2 beside them)
@@ -682,6 +911,7 @@ int launch_grouped(Grouped<T>& a, hipStream_t stream) {
         case kFew64: return launch_grouped_few<T, YC, 4, ACT>(a, stream);
         case k64: return launch_grouped_tiles<T, YC, 64, 64, 2, 2, ACT>(a, stream);
         case k128: return launch_grouped_tiles<T, YC, 128, 128, 2, 2, ACT>(a, stream);
+        case kResident: return a.K == 5 * kStep ? launch_grouped_resident<T, YC, ACT, 5>(a, stream) : launch_grouped_resident<T, YC, ACT, 6>(a, stream);
         default: return launch_grouped_tiles<T, YC, 256, 256, 2, 4, ACT>(a, stream);
     }
 }
@@ -722,31 +952,30 @@ int experts_dx(const llsa_experts_args& q, hipStream_t stream) {
     return launch_status("experts_dx");
 }
 
-// Rows of a piece.  More pieces fill the chip's workgroups more evenly, and are more sums to write and read; experts of one piece need neither.
+// Rows of a chunk.  More chunks fill the chip's workgroups more evenly, and are more sums to write and read (linear.hip's weight_pieces).
 int grouped_rows(int64_t N) { return ceil_div(N, 192) * 192 <= ceil_div(N, 128) * 128 ? 192 : 128; }
-bool small_tiles(int64_t rows, int64_t experts, int64_t N, int64_t K) { return experts * ceil_div(N, 128) * ceil_div(K, 128) < kCus && rows < 64 * 1024; }
-int64_t piece_rows(int64_t rows, int64_t experts, int64_t N, int64_t K) {
-    const bool small = small_tiles(rows, experts, N, K);
-    const int64_t bm = small ? 64 : grouped_rows(N), bn = small ? 64 : 128, tiles = ceil_div(N, bm) * ceil_div(K, bn);
-    const double all = 2. * (double)rows * N * K / 0.72e9, sums = 8. * (double)N * K / 4e6;    // us
+bool small_tiles(int64_t rows, int64_t N, int64_t K) { return ceil_div(N, 128) * ceil_div(K, 128) * std::max<int64_t>(1, rows / 512) < kCus; }
+int64_t chunk_rows(int64_t rows, int64_t N, int64_t K) {
+    const bool small = small_tiles(rows, N, K);
+    const int64_t bm = small ? 64 : grouped_rows(N), bn = small ? 64 : 128, tiles = ceil_div(N, bm) * ceil_div(K, bn), slots = (small ? 4 : 2) * kCus;
+    const double all = 2. * (double)rows * N * K / 0.6e9, sums = 8. * (double)N * K / 4e6;     // us
     int64_t best = 1;
     double least = 0;
-    for (int64_t p = 1; p <= std::max<int64_t>(1, rows / experts / 256) && (p - 1) * tiles * experts < 8 * kCus; p++) {
-        const double n = (double)(tiles * experts * p) / (2 * kCus), t = all * std::ceil(n) / n + (p > 1 ? sums * experts * p : 0);
+    for (int64_t p = 1; p <= std::max<int64_t>(1, rows / 256) && (p - 1) * tiles < 4 * slots; p++) {
+        const double n = (double)(tiles * p) / (double)slots, t = all * std::ceil(n) / n + sums * (double)p;
         if (p == 1 || t < least) best = p, least = t;
     }
-    // experts are not alike: with one piece each, the largest one's may be twice the average before it is cut
-    const int64_t length = best == 1 ? 2 * ceil_div(rows, experts) : ceil_div(ceil_div(rows, experts), best);
-    return std::max<int64_t>(256, ceil_div(length, kStep) * kStep);
+    return ceil_div(ceil_div(rows, best), kStep) * kStep;
 }
-template <typename T, int BM, int BN>
+int64_t part_count(int64_t rows, int64_t experts, int64_t N, int64_t K) { return ceil_div(rows, chunk_rows(rows, N, K)) + experts; }
+template <typename T, bool GX, bool GY, int BM, int BN>
 int launch_grouped_dw(GroupedWeights<T>& a, hipStream_t stream) {
     a.tiles_m = (int)ceil_div(a.M, BM);
     a.tiles_n = (int)ceil_div(a.N, BN);
-    const int64_t grid = pieces_of(a.rows, a.experts, a.piece) * a.tiles_m * a.tiles_n;
+    const int64_t grid = ceil_div(a.rows, a.chunk) * a.tiles_m * a.tiles_n;
     if (grid > kMaxGrid) return fail(-1, "experts_dw: too many rows");
     constexpr int lds = 2 * (BM + BN) * kStep * (int)sizeof(T);
-    auto kernel = grouped_dw_kernel<T, BM, BN, 2, 2>;
+    auto kernel = grouped_dw_kernel<T, GX, GY, BM, BN, 2, 2>;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return fail(-101, "experts_dw: %s", hipGetErrorString(e));
@@ -754,29 +983,33 @@ int launch_grouped_dw(GroupedWeights<T>& a, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), lds, stream, a);
     return 0;
 }
+template <typename T, bool GX, bool GY>
+int launch_dw_tiles(GroupedWeights<T>& a, bool small, hipStream_t stream) {
+    if (small) return launch_grouped_dw<T, GX, GY, 64, 64>(a, stream);
+    if (grouped_rows(a.M) == 192) return launch_grouped_dw<T, GX, GY, 192, 128>(a, stream);
+    return launch_grouped_dw<T, GX, GY, 128, 128>(a, stream);
+}
 template <typename T>
 int experts_dw(const llsa_experts_args& q, hipStream_t stream) {
     GroupedWeights<T> a{};
     a.x = (const T*)q.dz; a.ldx = q.lddz; a.nx = (int)pad8(q.N);
     a.y = (const T*)q.x; a.ldy = q.ldx; a.ny = (int)pad8(q.K);
     a.offsets = q.offsets;
-    a.order_x = order_of(q.gather_dz ? q.order : nullptr, q.k, q.tokens, q.rows);
-    a.order_y = order_of(q.gather_x ? q.order : nullptr, q.k, q.tokens, q.rows);
+    a.order = order_of(q.order, q.k, q.tokens, q.rows);
     a.experts = q.E; a.rows = (int)q.rows; a.M = q.N; a.N = q.K;
-    a.piece = (int)piece_rows(q.rows, q.E, q.N, q.K);
+    a.chunk = (int)chunk_rows(q.rows, q.N, q.K);
     a.sorted = q.sorted;
     a.out = (T*)q.out; a.sums = (T*)q.dbias;
     a.ld_part = pad8(q.K);
     a.part = (float*)q.workspace;
-    a.part_sum = q.dbias != nullptr ? a.part + pieces_of(q.rows, q.E, a.piece) * a.M * a.ld_part : nullptr;
+    a.part_sum = q.dbias != nullptr ? a.part + part_count(q.rows, q.E, q.N, q.K) * a.M * a.ld_part : nullptr;
     a.wide_out = q.K % 8 == 0 && aligned16(q.out);
-    int rc;
-    if (small_tiles(q.rows, q.E, q.N, q.K)) rc = launch_grouped_dw<T, 64, 64>(a, stream);
-    else if (grouped_rows(q.N) == 192) rc = launch_grouped_dw<T, 192, 128>(a, stream);
-    else rc = launch_grouped_dw<T, 128, 128>(a, stream);
+    const bool small = small_tiles(q.rows, q.N, q.K);
+    const int rc = q.gather_dz ? launch_dw_tiles<T, true, false>(a, small, stream)
+                   : q.gather_x ? launch_dw_tiles<T, false, true>(a, small, stream) : launch_dw_tiles<T, false, false>(a, small, stream);
     if (rc != 0) return rc;
-    const int64_t places = (int64_t)a.M * (a.ld_part / 4) + (q.dbias != nullptr ? a.M : 0), blocks = ceil_div(places, 64);
-    if (blocks * q.E > kMaxGrid) return fail(-1, "experts_dw: too many weights");
+    // (as many workgroups as the chip holds: most experts have one piece, and nothing to add up)
+    const int64_t places = (int64_t)a.M * (a.ld_part / 4) + (q.dbias != nullptr ? a.M : 0), blocks = std::min(ceil_div(places, 64), ceil_div(8 * kCus, q.E));
     hipLaunchKernelGGL(HIP_KERNEL_NAME(grouped_join_kernel<T>), dim3((unsigned)(blocks * q.E)), dim3(256), 0, stream, a, (int)blocks);
     return launch_status("experts_dw");
 }
@@ -825,7 +1058,7 @@ using namespace llsa;
 
 extern "C" int64_t llsa_experts_dw_workspace_bytes(int64_t rows, int E, int N, int K) {
     if (rows <= 0 || E <= 0 || N <= 0 || K <= 0) return 0;
-    return 4 * pieces_of(rows, E, piece_rows(rows, E, N, K)) * N * (pad8(K) + 1);
+    return 4 * part_count(rows, E, N, K) * N * (pad8(K) + 1);
 }
 extern "C" int64_t llsa_experts_dot_parts(int64_t rows, int E, int N, int K) {
     if (rows <= 0 || E <= 0 || N <= 0 || K <= 0) return 0;
@@ -852,7 +1085,7 @@ extern "C" int llsa_experts_dx(const llsa_experts_args* a, void* stream) {
 }
 extern "C" int llsa_experts_dw(const llsa_experts_args* a, void* stream) {
     if (int rc = check_experts("experts_dw", a)) return rc;
-    LLSA_REQUIRE(a->rows > 0, "experts_dw: no rows");
+    LLSA_REQUIRE(a->rows > 0 && !(a->gather_x && a->gather_dz), "experts_dw: rows, of which x or dz may be gathered");
     LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->x, a->ldx) && a->lddz >= pad8(a->N) && a->ldx >= pad8(a->K), "experts_dw: rows of dz and x must be 16-byte aligned and padded to a multiple of 8");
     LLSA_REQUIRE(a->out != nullptr && a->workspace != nullptr && aligned16(a->workspace), "experts_dw: output and workspace (16-byte aligned)");
     return BY_TYPE(experts_dw);

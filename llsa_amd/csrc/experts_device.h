@@ -73,6 +73,16 @@ struct Runs {
         const int n = (e - b + size - 1) / size;
         return {64 * i + lane_, u - n, b, e, n};
     }
+    // the first expert with rows among first .. last - 1; -1: none
+    __device__ __forceinline__ Piece among(int first, int last) const {
+        Piece p = {-1, 0, last, last, 0};
+#pragma unroll
+        for (int i = 0; i < kLanes; i++) {
+            const uint64_t them = __ballot(end[i] > begin[i] && begin[i] < last && end[i] > first);
+            if (p.expert < 0 && them != 0) p = of_expert(i, __ffsll((unsigned long long)them) - 1);
+        }
+        return p;
+    }
     // piece t < total: its expert, and that expert's rows
     __device__ __forceinline__ Piece find(int t) const {
         if (t >= of_experts) {
@@ -128,31 +138,47 @@ struct GatheredRows {
         }
     }
 };
-// 64 rows of x across, as Operand<columns> lays them out: the tokens of a step are looked up a step ahead
-template <typename T, int ROWS, int WAVES>
-struct GatheredColumns {
+// 64 rows of x across, as Operand<columns> lays them out.  GATHERED: of tokens in the order, which are looked up a step ahead
+template <typename T, int ROWS, int WAVES, bool GATHERED>
+struct Columns {
     typedef Operand<T, true, ROWS, WAVES> Plain;
     static constexpr int kCopies = Plain::kCopies;
-    int row[kCopies], place[kCopies];
-    __device__ __forceinline__ void init(int left, int wave, int lane) {
+    Plain plain;
+    const T *x;
+    int64_t ld;
+    int row[GATHERED ? kCopies : 1], place[GATHERED ? kCopies : 1];
+    // left: elements of a row from x on.  first: the first row, where rows are not gathered
+    __device__ __forceinline__ void init(const T* x_, int64_t ld_, int first, int left, int wave, int lane) {
+        x = x_;
+        ld = ld_;
+        if constexpr (GATHERED) {
 #pragma unroll
-        for (int j = 0; j < kCopies; j++) {
-            const int i = wave * kCopies + j;
-            place[j] = min(Plain::place_of(i, Plain::row_of(i, lane), lane), left - 8);
+            for (int j = 0; j < kCopies; j++) {
+                const int i = wave * kCopies + j;
+                place[j] = min(Plain::place_of(i, Plain::row_of(i, lane), lane), left - 8);
+            }
+        } else {
+            x += first * ld;
+            plain.init(wave, lane, ld, left);
         }
     }
     __device__ __forceinline__ void look_up(const Order& order, int at, int k_left, int wave, int lane) {
+        if constexpr (GATHERED) {
 #pragma unroll
-        for (int j = 0; j < kCopies; j++) {
-            const int r = Plain::row_of(wave * kCopies + j, lane);
-            if (r < k_left) row[j] = order.slots != nullptr ? order.token(at + r) : at + r;
+            for (int j = 0; j < kCopies; j++) row[j] = order.token(at + min(Plain::row_of(wave * kCopies + j, lane), k_left - 1));
         }
     }
-    __device__ __forceinline__ void request(const T* x, int64_t ld, T* tile, int wave, int lane, int k_left) const {
+    __device__ __forceinline__ void request(T* tile, int wave, int lane, int k_left) {
+        if constexpr (GATHERED) {
 #pragma unroll
-        for (int j = 0; j < kCopies; j++) {
-            const int i = wave * kCopies + j;
-            copy_to_lds(Plain::row_of(i, lane) < k_left ? x + row[j] * ld + place[j] : reinterpret_cast<const T*>(kZeros), tile + i * 512);
+            for (int j = 0; j < kCopies; j++) {
+                const int i = wave * kCopies + j;
+                const T* const from = x + (uint64_t)(unsigned)row[j] * (unsigned)ld + place[j];
+                copy_to_lds(Plain::row_of(i, lane) < k_left ? from : reinterpret_cast<const T*>(kZeros), tile + i * 512);
+            }
+        } else {
+            plain.request(x, tile, wave, lane, k_left);
+            x += kStep * ld;
         }
     }
 };
