@@ -44,7 +44,7 @@ extern "C" {
 #define LLSA_DTYPE_F32 1
 #define LLSA_DTYPE_F16 2
 
-#define LLSA_ABI_VERSION 217     /* changes with every change of a signature or argument structure below */
+#define LLSA_ABI_VERSION 219     /* changes with every change of a signature or argument structure below */
 int llsa_version(void);          /* LLSA_ABI_VERSION of the built library                                    */
 const char* llsa_last_error_string(void);
 
@@ -511,31 +511,33 @@ int llsa_route_tokens_bwd(const llsa_route_args* a, void* stream);
 int64_t llsa_route_workspace_bytes(int64_t M, int E, int k);
 
 /* The experts' products.  Rows stand sorted by expert, those of expert e at offsets[e] .. offsets[e + 1] - 1 (held to 0 .. rows, and not falling); weights
- * (E,N,K).  Conventions of the linear layers above (rows 16-byte aligned and padded, sums in fp32).  With gather_x (gather_dz) the rows of x (dz) are those of
- * tokens: the row at a place is token order[place] / k.  Numbers in order, places and experts out of range are held to it or skipped.
- *     fwd       z = x W_e^T + bias_e, kept unless z is NULL; out = act(z).  weights (tokens * k): out is multiplied by weights[order[place]], which is also
- *               written to sorted[place].  sorted without weights: bias_e is multiplied by sorted[place].  gaps: rows that no expert has get zeros
- *     dx        t = dz W_e; out = t, or with z t * sorted[place] * act'(z) (sorted NULL: 1); dots: sums of act(z) t, llsa_experts_dot_parts of them a place
- *     dw        out (E,N,K) = dz^T x and dbias (E,N) = sum of sorted[place] * dz (sorted NULL: 1) over an expert's rows
- *     combine   out (tokens,N) = residual + gate * sum over j of x[places[m,j]]; the sum, rounded, to z unless NULL
- *     dweights  dweights[m,j] = sum of the place's dots + dz[m] . bias_(experts[m,j]); N, K as for the dx that made the dots */
+ * (E,N,K).  Conventions of the linear layers above (rows 16-byte aligned and padded, sums in fp32).  The row at a place is that of token order[place] / k.  Numbers
+ * in order, places and experts out of range are held to it or skipped.
+ *     gather    out[place] = x[token] (N channels) for places below offsets[E], times weights[order[place]] (and the gate of its sample) unless NULL
+ *     fwd       z = x W_e^T + bias_e, kept unless z is NULL; out = act(z).  gather_x: x has rows of tokens, where llsa_experts_gathers allows it.
+ *               gaps: rows that no expert has get zeros
+ *     dx        t = dz W_e; out = t, or with z t * act'(z); gaps as above
+ *     dw        out (E,N,K) = dz^T x and dbias (E,N) = sum of dz over an expert's rows
+ *     combine   out (tokens,N) = residual + gate * sum over j of weights[m,j] x[places[m,j]] (weights NULL: 1); the sum, rounded, to z unless NULL
+ *     dweights  dweights[m,j] = sum over n of gate * dz[m] * x[places[m,j]] */
 typedef struct llsa_experts_args {
     const void *x, *w, *bias, *dz, *gate, *residual;
     void *out, *z, *dbias, *workspace;
-    const int32_t *offsets, *order, *places, *experts;
+    const int32_t *offsets, *order, *places;
     const float* weights;
-    float *sorted, *dots, *dweights;
+    float* dweights;
     int64_t ldx, ldw, lddz, ldr, ldo, ldz, s_gate;
     int64_t rows, tokens, per_sample;
-    int32_t E, N, K, k, act, dtype, padded, gaps, gather_x, gather_dz;
+    int32_t E, N, K, k, act, dtype, padded, gaps, gather_x, reserved;
 } llsa_experts_args;
+int llsa_experts_gather(const llsa_experts_args* a, void* stream);
+int llsa_experts_gathers(int64_t rows, int E, int N, int K);
 int llsa_experts_fwd(const llsa_experts_args* a, void* stream);
 int llsa_experts_dx(const llsa_experts_args* a, void* stream);
 int llsa_experts_dw(const llsa_experts_args* a, void* stream);
 int llsa_experts_combine(const llsa_experts_args* a, void* stream);
 int llsa_experts_dweights(const llsa_experts_args* a, void* stream);
 int64_t llsa_experts_dw_workspace_bytes(int64_t rows, int E, int N, int K);
-int64_t llsa_experts_dot_parts(int64_t rows, int E, int N, int K);
 
 #ifdef __cplusplus
 }

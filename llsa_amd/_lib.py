@@ -100,10 +100,10 @@ class RouteArgs(C.Structure):
 
 
 class ExpertsArgs(C.Structure):
-    _fields_ = ([(n, c_void_p) for n in ("x", "w", "bias", "dz", "gate", "residual", "out", "z", "dbias", "workspace", "offsets", "order", "places", "experts",
-                                         "weights", "sorted", "dots", "dweights")]
+    _fields_ = ([(n, c_void_p) for n in ("x", "w", "bias", "dz", "gate", "residual", "out", "z", "dbias", "workspace", "offsets", "order", "places",
+                                         "weights", "dweights")]
                 + [(n, c_int64) for n in ("ldx", "ldw", "lddz", "ldr", "ldo", "ldz", "s_gate", "rows", "tokens", "per_sample")]
-                + [(n, c_int32) for n in ("E", "N", "K", "k", "act", "dtype", "padded", "gaps", "gather_x", "gather_dz")])
+                + [(n, c_int32) for n in ("E", "N", "K", "k", "act", "dtype", "padded", "gaps", "gather_x", "reserved")])
 
 
 class QuantizeArgs(C.Structure):
@@ -175,18 +175,19 @@ _SIGNATURES = {
     "llsa_route_tokens": (c_int, [C.POINTER(RouteArgs), c_void_p]),
     "llsa_route_tokens_bwd": (c_int, [C.POINTER(RouteArgs), c_void_p]),
     "llsa_route_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
+    "llsa_experts_gather": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
+    "llsa_experts_gathers": (c_int, [c_int64, c_int, c_int, c_int]),
     "llsa_experts_fwd": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
     "llsa_experts_dx": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
     "llsa_experts_dw": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
     "llsa_experts_combine": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
     "llsa_experts_dweights": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
     "llsa_experts_dw_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int]),
-    "llsa_experts_dot_parts": (c_int64, [c_int64, c_int, c_int, c_int]),
 }
 
 EXPORTS = tuple(_SIGNATURES)
 CHUNK_FINE_MAX = 256                                        # LLSA_CHUNK_FINE_MAX of include/llsa_hip.h
-ABI_VERSION = 217                                           # LLSA_ABI_VERSION
+ABI_VERSION = 219                                           # LLSA_ABI_VERSION
 STATIC_PARTIALS_MAX = 262144                                # LLSA_STATIC_PARTIALS_MAX
 
 

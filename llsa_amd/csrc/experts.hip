@@ -2,16 +2,19 @@
 // those of expert e at offsets[e] .. offsets[e + 1] - 1; the offsets stay on the device, so a launch has a workgroup for every piece of rows there can be,
 // and each finds its expert by itself (experts_device.h).
 //
-//     forward   z = x W_e^T + b_e,   out = act(z)                    of a block: h' = w act(z),   y = h' W_out^T + w b_out,   out = residual + gate * sum of a token's y
+//     forward   z = x W_e^T + b_e,   h = act(z)                     of a block: y = h W_out^T + b_out,   out = residual + gate * sum of a token's w y
 //     backward  dx = dz W_e,   dW_e = dz^T x,   db_e = sum dz
 //
-// A token's weight w goes into the hidden rows.  With t = dout W_out the block's backward is then
-//     dW_out = dout^T h',   db_out = sum w dout,   dz = w act'(z) t,   dw = sum over the hidden channels of act(z) t + dout . b_out
-// and takes dout's rows as they are, gathered: nothing is multiplied by w in memory, and no expert's output is kept for dw.
+// Of a block: with g = w gate dout, a row for each of a token's experts,   dz = act'(z) (g W_out),   dW_out = g^T h,   db_out = sum g,   dw = gate dout . y.
+// Rows of tokens (x, g) are brought into the order of the places once, where a product for each of a row's columns would gather them again (262144 rows of
+// 384 and 1536 channels, us: dW of gathered rows 573 and 530, of rows in order 376, and some 50 for the copy, which multiplies by w as well); few rows and the
+// smallest tiles of a forward without a backward gather them on their way into LDS.  The weight stays out of the products: in the hidden rows (h' = w act(z), so
+// that dout needs no factor) dw is a sum over act(z) (dout W_out) on the way out of that product, whose waves have no registers left for it (20 to 30
+// spilled: 1050 us instead of 560).
 //
 // Sums are fp32, and so is what happens on the way out.  Rounded to 16 bits besides the results: what a product takes in that another made or that is kept (z,
-// h', dz), as in the linear layers, and the rows y and dx of each expert, which are read once more and added up in fp32: half a step of each, 2^-8 of it in
-// bf16 (fp16 2^-11), for half the bytes.
+// h, g, dz), as in the linear layers, and the rows y and dx of each expert, which are read once or twice more and added up in fp32: half a step of each, 2^-8 of it
+// in bf16 (fp16 2^-11), for half the bytes.
 #include "experts_device.h"
 
 namespace llsa {
@@ -20,7 +23,6 @@ namespace {
 // ---------------------------------------------------------------------------------------
 // forward and dx
 // ---------------------------------------------------------------------------------------
-enum Scaled { kUnscaled, kScaledRows, kScaledBias };          // what is multiplied by a row's weight: nothing, what act gives, the bias
 template <typename T>
 struct Grouped {
     const T *x, *y;                       // rows of tokens (or of places, without an order), weights
@@ -31,12 +33,9 @@ struct Grouped {
     int tiles_n, group, gaps;             // gaps: zeros go to the rows that no expert has
     // way out
     const T *bias, *slope_at;
-    const float* weights;                 // of slots; kScaledRows in the forward, which writes `sorted` too
-    float* sorted;                        // of places; read elsewhere
-    float* dots;                          // dx: [place][part] of sums of act(z) t, or NULL
     int64_t ldo, ldz;
     T *out, *z;
-    int scaled, wide, wide_out, parts;    // wide: 16-byte accesses to bias; wide_out: to out, or its rows are padded with zeros to a multiple of 8
+    int wide, wide_out;                   // wide: 16-byte accesses to bias; wide_out: to out, or its rows are padded with zeros to a multiple of 8
 };
 struct Here { int expert, m0, m_end, n0, tn; };
 template <int BM, int BN, typename P>
@@ -62,30 +61,21 @@ __device__ __forceinline__ void write_zeros(const Grouped<T>& a, const Here& h) 
     }
 }
 
-// Eight values of a row on their way out; scale: the row's weight.  z: what the forward keeps; early: z of the layer in front in dx
+// Eight values of a row on their way out.  z: what the forward keeps; early: z of the layer in front in dx
 template <bool YC, int ACT, typename T>
-__device__ __forceinline__ vec8<T> way_out(const Grouped<T>& a, float (&v)[8], const vec8<T>& bias, float scale, const vec8<T>& early, int left, vec8<T>& z, float& dot) {
+__device__ __forceinline__ vec8<T> way_out(const Grouped<T>& a, float (&v)[8], const vec8<T>& bias, const vec8<T>& early, int left, vec8<T>& z) {
     if constexpr (!YC) {
-        const float b = a.scaled == kScaledBias ? scale : 1.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = fmaf(b, (float)bias[e], v[e]);
+        for (int e = 0; e < 8; e++) v[e] += (float)bias[e];
         if (a.z != nullptr) {
 #pragma unroll
             for (int e = 0; e < 8; e++) z[e] = (T)v[e];
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = activate(ACT, v[e]);
-        if (a.scaled == kScaledRows) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[e] *= scale;
-        }
     } else if constexpr (ACT != LLSA_ACT_NONE) {
-        if (a.dots != nullptr) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) dot += e >= left ? 0.f : v[e] * activate(ACT, (float)early[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] *= scale * activate_slope(ACT, (float)early[e]);
+        for (int e = 0; e < 8; e++) v[e] *= activate_slope(ACT, (float)early[e]);
     }
     vec8<T> o;
 #pragma unroll
@@ -102,14 +92,8 @@ __device__ __forceinline__ void put8(T* to, const vec8<T>& o, bool wide, int lef
             if (e < left) to[e] = o[e];
     }
 }
-// A row's weight: where the forward scales its rows it comes with the order, and is kept in it
-template <typename T>
-__device__ __forceinline__ float weight_of(const Grouped<T>& a, int place) {
-    return a.scaled == kUnscaled ? 1.f : a.weights != nullptr ? a.weights[a.order.slot(place)] : a.sorted[place];
-}
-
-// The tiles of linear.hip's product_kernel, with rows gathered on their way into LDS and an expert's weights.
-template <typename T, bool YC, int BM, int BN, int WAVES_M, int WAVES_N, int ACT>
+// The tiles of linear.hip's product_kernel, with an expert's weights; GATHERED: rows of tokens, brought into order on their way into LDS.
+template <typename T, bool YC, bool GATHERED, int BM, int BN, int WAVES_M, int WAVES_N, int ACT>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(const Grouped<T> a) {
     constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
     constexpr bool kSlope = YC && ACT != LLSA_ACT_NONE;
@@ -125,7 +109,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
         write_zeros<BM, BN>(a, here);
         return;
     }
-    GatheredRows<T, BM, kWaves> ox;
+    RowsAlong<T, BM, kWaves, GATHERED> ox;
     OperandY oy;
     ox.init(a.x, a.ldx, a.order, here.m0, min(BM, here.m_end - here.m0), wave, lane);
     oy.init(wave, lane, a.ldy, min(BN, (YC ? a.ny : a.N) - here.n0));
@@ -134,7 +118,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
     int k = 0;
     auto request = [&](int buffer) {
         T* const t = lds + buffer * (kTileX + kTileY);
-        ox.request(k, t, wave, lane, a.K - k);
+        ox.request(t, wave, lane, a.K - k);
         oy.request(py, t + kTileX, wave, lane, a.K - k);
         py += stepy;
         k += kStep;
@@ -196,12 +180,6 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
     wait_vm0();
     __syncthreads();
     read_side(0);                                             // (on its way during the last step's products)
-    float scale[MT], dot[MT];
-#pragma unroll
-    for (int j = 0; j < MT; j++) {
-        scale[j] = 16 * j < rows_left ? weight_of(a, row0 + 16 * j + lane_row) : 0.f;
-        dot[j] = 0.f;
-    }
     multiply((steps - 1) & 1);
 
     const T* const bias_row = !YC && a.bias != nullptr ? a.bias + (int64_t)here.expert * a.N + col0 + lane_col : nullptr;
@@ -231,7 +209,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
                     v[4 + e] = __uint_as_float(w[1]);
                 }
                 const bool inside = 16 * j < rows_left && left > 0;
-                if (inside) o[h] = way_out<YC, ACT>(a, v, bias[h], scale[j], early[h][j], left, z[h], dot[j]);
+                if (inside) o[h] = way_out<YC, ACT>(a, v, bias[h], early[h][j], left, z[h]);
                 if (whole || !inside) continue;
                 if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (row * a.ldz + col) + at_z) = z[h];
                 put8(a.out + (row * a.ldo + col) + at_out, o[h], a.wide_out, left);
@@ -245,20 +223,6 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
             __builtin_amdgcn_sched_barrier(0);                // (rows one after another: all at once do not fit the registers)
         }
         if (p0 + kPair < NT / 2) read_side(p0 + kPair);
-    }
-    if constexpr (kSlope) {
-        if (a.dots != nullptr) {
-#pragma unroll
-            for (int j = 0; j < MT; j++) {
-                const float d = quad_sum(dot[j]);
-                if (quad == 0 && 16 * j < rows_left) a.dots[(int64_t)(row0 + 16 * j + lane_row) * a.parts + here.tn * WAVES_N + wave / WAVES_M] = d;
-            }
-        }
-    }
-    if (!YC && a.scaled == kScaledRows && here.tn == 0 && wn == 0 && quad == 0) {
-#pragma unroll
-        for (int j = 0; j < MT; j++)
-            if (16 * j < rows_left) a.sorted[row0 + 16 * j + lane_row] = scale[j];
     }
 }
 
@@ -351,27 +315,18 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void grouped_few_kernel(const Gr
         v[4 + e] = __uint_as_float(w[1]);
     }
     const int lane_col = 16 * (quad & 1) + 8 * (quad >> 1), m = row0 + 16 * wave + (lane & 15), left = a.N - n0 - lane_col;
-    const bool row_there = m < here.m_end, inside = row_there && left > 0;
-    float dot = 0.f;
-    const float scale = row_there ? weight_of(a, m) : 0.f;
-    if (inside) {
-        vec8<T> early = take8<T>(nullptr, true, 0), z;
-        if (kSlope) early = *reinterpret_cast<const vec8<T>*>(a.slope_at + (int64_t)m * a.ldz + n0 + lane_col);
-        const vec8<T> bias = take8(!YC && a.bias != nullptr ? a.bias + (int64_t)here.expert * a.N + n0 + lane_col : nullptr, a.wide, left);
-        const vec8<T> o = way_out<YC, ACT>(a, v, bias, scale, early, left, z, dot);
-        if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (int64_t)m * a.ldz + n0 + lane_col) = z;
-        put8(a.out + (int64_t)m * a.ldo + n0 + lane_col, o, a.wide_out, left);
-    }
-    if (kSlope && a.dots != nullptr) {
-        dot = quad_sum(dot);
-        if (quad == 0 && row_there) a.dots[(int64_t)m * a.parts + here.tn] = dot;
-    }
-    if (!YC && a.scaled == kScaledRows && here.tn == 0 && quad == 0 && row_there) a.sorted[m] = scale;
+    if (m >= here.m_end || left <= 0) return;
+    vec8<T> early = take8<T>(nullptr, true, 0), z;
+    if (kSlope) early = *reinterpret_cast<const vec8<T>*>(a.slope_at + (int64_t)m * a.ldz + n0 + lane_col);
+    const vec8<T> bias = take8(!YC && a.bias != nullptr ? a.bias + (int64_t)here.expert * a.N + n0 + lane_col : nullptr, a.wide, left);
+    const vec8<T> o = way_out<YC, ACT>(a, v, bias, early, left, z);
+    if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (int64_t)m * a.ldz + n0 + lane_col) = z;
+    put8(a.out + (int64_t)m * a.ldo + n0 + lane_col, o, a.wide_out, left);
 }
 
 // Many rows for each expert, a short contraction: the weights stay in registers (linear.hip's resident_kernel).  A workgroup of twelve waves keeps 384 columns of
 // an expert's weights, 32 columns a wave, and takes its share of the rows through LDS, 32 at a time and two such tiles ahead; where the expert changes it takes
-// in the next one's weights.  The tokens of a tile are looked up three tiles ahead.
+// in the next one's weights.
 constexpr int kResWaves = 12, kResColumns = 32 * kResWaves, kResRows = 32, kResStages = 3, kResOwn = 32 * kStep + 64;
 struct Entry { int expert, begin, end, first, upto; };       // upto: number of the first tile behind its own
 template <typename T, bool YC, int ACT, int STEPS>
@@ -444,42 +399,31 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
         }
     };
 
-    // this wave's two copies of a tile: their rows, and the elements of a row from which they begin
-    const bool copies = wave < 2 * STEPS;
-    int from_row[2];
+    unsigned off[2];                                          // of this wave's two copies of a tile
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        const int i = 2 * wave + c, r = OperandX::row_of(i & 3, lane);
+        off[c] = (unsigned)(r * a.ldx) + (i >> 2) * kStep + OperandX::place_of(i & 3, r, lane);
+    }
     Entry ahead = entry(0, 0);
-    auto look_up = [&](int t) {
-        if (t >= t1 || !copies) return;
+    auto request = [&](int t) {
+        if (t >= t1 || wave >= 2 * STEPS) return;
         advance(ahead, t);
         if (ahead.expert >= a.experts) return;
-        const int m0 = ahead.begin + (t - ahead.first) * kResRows;
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const int at = min(m0 + OperandX::row_of((2 * wave + c) & 3, lane), ahead.end - 1);
-            from_row[c] = a.order.slots != nullptr ? a.order.token(at) : at;
-        }
-    };
-    auto request = [&](int t) {
-        if (t >= t1 || !copies) return;
         T* const stage = lds + (t % kResStages) * kStage;
+        // (the last tile of all begins early enough to be whole)
+        const T* const base = a.x + (int64_t)min(ahead.begin + (t - ahead.first) * kResRows, a.rows - kResRows) * a.ldx;
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const int i = 2 * wave + c, r = OperandX::row_of(i & 3, lane);
-            copy_to_lds(a.x + (uint64_t)(unsigned)from_row[c] * (unsigned)a.ldx + ((i >> 2) * kStep + OperandX::place_of(i & 3, r, lane)), stage + i * 512);
-        }
+        for (int c = 0; c < 2; c++) copy_to_lds(base + off[c], stage + (2 * wave + c) * 512);
     };
-    from_row[0] = from_row[1] = 0;
-    look_up(t0);
     request(t0);
-    look_up(t0 + 1);
     request(t0 + 1);
-    look_up(t0 + 2);
     const unsigned at_out = (unsigned)(lane_row * a.ldo) + lane_col, at_z = (unsigned)(lane_row * a.ldz) + lane_col;
     Entry now = entry(0, 0);
     wait_vm0();
     for (int t = t0, have = -1; t < t1; t++) {
         advance(now, t);
-        const int m0 = now.begin + (t - now.first) * kResRows;
+        const int first = now.begin + (t - now.first) * kResRows, m0 = min(first, a.rows - kResRows);
         if (now.expert != have && columns && now.expert < a.experts) {
             weights(a.y + now.expert * a.y_expert);
             if (!YC && lane_row == 0) *reinterpret_cast<vec8<T>*>(vectors + lane_col) = take8(a.bias != nullptr ? a.bias + (int64_t)now.expert * a.N + n0 + lane_col : nullptr, a.wide, 8);
@@ -491,7 +435,6 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         request(t + 2);
-        look_up(t + 3);
         if (!columns) {
             wait_vm0();
             continue;
@@ -499,17 +442,15 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
         if (now.expert >= a.experts) {                        // no expert's rows
 #pragma unroll
             for (int j = 0; j < 2; j++)
-                if (m0 + 16 * j + lane_row < now.end) *reinterpret_cast<vec8<T>*>(a.out + ((int64_t)(m0 + 16 * j) * a.ldo + n0) + at_out) = take8<T>(nullptr, true, 8);
+                if (first + 16 * j + lane_row < now.end) *reinterpret_cast<vec8<T>*>(a.out + ((int64_t)(first + 16 * j) * a.ldo + n0) + at_out) = take8<T>(nullptr, true, 8);
             wait_vm0();
             continue;
         }
         vec8<T> early[2];                                     // what is read on the way out
-        float scale[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const int row = min(m0 + 16 * j + lane_row, now.end - 1);
-            scale[j] = weight_of(a, row);
-            if (kSlope) early[j] = __builtin_nontemporal_load(reinterpret_cast<const vec8<T>*>(a.slope_at + (int64_t)row * a.ldz + n0 + lane_col));
+            const int64_t row = m0 + 16 * j;                  // (rows behind the expert's last are another's, or were never written: what comes of them is not kept)
+            if (kSlope) early[j] = __builtin_nontemporal_load(reinterpret_cast<const vec8<T>*>(a.slope_at + (row * a.ldz + n0) + at_z));
         }
         f32x4 acc[2][2];
 #pragma unroll
@@ -533,7 +474,7 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
             __builtin_amdgcn_sched_barrier(0);                // (the weights leave no registers for both at once, nor for the bias but here)
             vec8<T> bias = take8<T>(nullptr, true, 8), z;
             if (!YC) bias = *reinterpret_cast<const vec8<T>*>(vectors + lane_col);
-            float v[8], dot = 0.f;
+            float v[8];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const u32x2 w = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[0][j][e]), __float_as_uint(acc[1][j][e]), false, false);
@@ -541,22 +482,17 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
                 v[4 + e] = __uint_as_float(w[1]);
             }
             const int64_t row = m0 + 16 * j;
-            const bool inside = row + lane_row < now.end;
-            const vec8<T> o = way_out<YC, ACT>(a, v, bias, scale[j], early[j], 8, z, dot);
-            if (kSlope && a.dots != nullptr) {
-                dot = quad_sum(dot);
-                if (quad == 0 && inside) a.dots[(row + lane_row) * a.parts + (n0 >> 5)] = dot;
-            }
+            const bool inside = (int)row + lane_row >= first && (int)row + lane_row < now.end;
+            const vec8<T> o = way_out<YC, ACT>(a, v, bias, early[j], 8, z);
             if (!inside) continue;
             if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (row * a.ldz + n0) + at_z) = z;
             *reinterpret_cast<vec8<T>*>(a.out + (row * a.ldo + n0) + at_out) = o;
-            if (!YC && a.scaled == kScaledRows && n0 == 0 && quad == 0) a.sorted[row + lane_row] = scale[j];
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------
-// dW: C_e[m][n] = sum over an expert's rows p of X[p][m] Y[p][n], either of them gathered.  All rows are taken in chunks of one length, whatever the
+// dW: C_e[m][n] = sum over an expert's rows p of X[p][m] Y[p][n].  All rows are taken in chunks of one length, whatever the
 // experts' are, so that the workgroups are alike; one that meets the end of an expert's rows writes its sums and goes on with the next expert's.  An expert
 // within one chunk is written straight away, the sums of the others meet in a second launch, which also writes the zeros of an expert without rows.  Expert
 // e's sums of chunk c are number c + e: with every next one either grows.
@@ -566,47 +502,44 @@ struct GroupedWeights {
     const T *x, *y;
     int64_t ldx, ldy;
     const int32_t* offsets;
-    Order order;
     int experts, rows, chunk;             // chunk: rows of one, a multiple of 64
     int M, N, nx, ny, tiles_m, tiles_n;
-    const float* sorted;                  // weights of the sums of x's rows, or NULL
     T *out, *sums;                        // (experts, M, N), (experts, M) or NULL
-    float *part, *part_sum;               // [number][M][ld_part], [number][M]
+    float *part, *part_sum;               // [number][M][ld_part], [number][tiles_n][M]
     int64_t ld_part;
     int wide_out;
 };
-// GX, GY: which of them is gathered.  Rows first .. end - 1 of an expert; alone: they are all it has
-template <typename T, bool GX, bool GY, int BM, int BN, int WAVES_M, int WAVES_N>
+// Rows first .. end - 1 of an expert; alone: they are all it has
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __device__ __forceinline__ void grouped_dw_piece(const GroupedWeights<T>& a, T* lds, int expert, int first, int end, bool alone, int number, int m0, int n0, int lane, int wave) {
     constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
     typedef Operand<T, true, BM, kWaves> OperandX;
     typedef Operand<T, true, BN, kWaves> OperandY;
     const int quad = lane >> 4, wm = (wave % WAVES_M) * WM, wn = (wave / WAVES_M) * WN, rows = end - first, steps = (rows + kStep - 1) / kStep;
-    Columns<T, BM, kWaves, GX> ox;
-    Columns<T, BN, kWaves, GY> oy;
-    ox.init(a.x + m0, a.ldx, first, min(BM, a.nx - m0), wave, lane);
-    oy.init(a.y + n0, a.ldy, first, min(BN, a.ny - n0), wave, lane);
-    const bool sums = a.part_sum != nullptr && n0 == 0 && wn == 0;
-    float weight = 0.f, next_weight = 0.f;                    // of row `lane` of the step
-    auto look_up = [&](int s) {
-        ox.look_up(a.order, first + s * kStep, rows - s * kStep, wave, lane);
-        oy.look_up(a.order, first + s * kStep, rows - s * kStep, wave, lane);
-    };
-    auto look_up_weight = [&](int s) {
-        if (sums && a.sorted != nullptr) next_weight = s * kStep + lane < rows ? a.sorted[first + s * kStep + lane] : 0.f;
-    };
+    OperandX ox;
+    OperandY oy;
+    ox.init(wave, lane, a.ldx, min(BM, a.nx - m0));
+    oy.init(wave, lane, a.ldy, min(BN, a.ny - n0));
+    const T *px = a.x + (first * a.ldx + m0), *py = a.y + (first * a.ldy + n0);
+    // sums of x's rows: of every tiles_n-th step, the workgroups along a row of tiles take turns; each of the two waves that hold the same rows takes half of them
+    static_assert(WAVES_N == 2 && MT % 2 == 0, "halves");
+    const bool sums = a.part_sum != nullptr, upper = wave / WAVES_M != 0;
+    constexpr int kHalf = MT / 2;
+    const int tn = n0 / BN;
     auto request = [&](int s) {
         T* const t = lds + (s & 1) * (kTileX + kTileY);
-        ox.request(t, wave, lane, rows - s * kStep);
-        oy.request(t + kTileX, wave, lane, rows - s * kStep);
+        ox.request(px, t, wave, lane, rows - s * kStep);
+        oy.request(py, t + kTileX, wave, lane, rows - s * kStep);
+        px += kStep * a.ldx;
+        py += kStep * a.ldy;
     };
-    f32x4 acc[NT][MT], sum[MT];
+    f32x4 acc[NT][MT], sum[kHalf];
 #pragma unroll
     for (int i = 0; i < NT; i++)
 #pragma unroll
         for (int j = 0; j < MT; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < MT; j++) sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < kHalf; j++) sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     vec8<T> ones;
 #pragma unroll
     for (int e = 0; e < 8; e++) ones[e] = (T)1.f;
@@ -624,41 +557,21 @@ __device__ __forceinline__ void grouped_dw_piece(const GroupedWeights<T>& a, T* 
             for (int i = 0; i < NT; i++)
 #pragma unroll
                 for (int j = 0; j < MT; j++) acc[i][j] = product16(fy[i], fx[j], acc[i][j]);
-            if (sums) {
-                if (a.sorted == nullptr) {
+            if (sums && s % a.tiles_n == tn) {
 #pragma unroll
-                    for (int j = 0; j < MT; j++) sum[j] = product16(ones, fx[j], sum[j]);
-                } else {
-                    // a weight in two parts of T, which hold 16 bits of it and more: sums of products with both.  (Those of tiny weights end at T's least number.)
-                    vec8<T> high, low;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float w = __shfl(weight, 32 * ks + 8 * quad + e);
-                        high[e] = (T)w;
-                        low[e] = (T)(w - (float)high[e]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < MT; j++) sum[j] = product16(low, fx[j], product16(high, fx[j], sum[j]));
-                }
+                for (int j = 0; j < kHalf; j++) sum[j] = product16(ones, upper ? fx[j + kHalf] : fx[j], sum[j]);
             }
         }
     };
-    look_up(0);
-    look_up_weight(0);
     request(0);
-    if (steps > 1) look_up(1);
     for (int s = 0; s + 1 < steps; s++) {
         wait_vm0();
         __syncthreads();                                      // everyone's copies of this step are there, and everyone is done with the other buffer
-        weight = next_weight;
         request(s + 1);
-        if (s + 2 < steps) look_up(s + 2);
-        look_up_weight(s + 1);
         multiply(s);
     }
     wait_vm0();
     __syncthreads();
-    weight = next_weight;
     multiply(steps - 1);
 
     const int lane_row = lane & 15, lane_col = 16 * (quad & 1) + 8 * (quad >> 1);
@@ -685,15 +598,13 @@ __device__ __forceinline__ void grouped_dw_piece(const GroupedWeights<T>& a, T* 
         }
     if (sums && quad == 0) {
 #pragma unroll
-        for (int j = 0; j < MT; j++) {
-            const int m = m0 + wm + 16 * j + lane;
-            if (m >= a.M) continue;
-            if (alone) a.sums[(int64_t)expert * a.M + m] = (T)sum[j][0];
-            else a.part_sum[(int64_t)number * a.M + m] = sum[j][0];
+        for (int j = 0; j < kHalf; j++) {
+            const int m = m0 + wm + 16 * (j + (upper ? kHalf : 0)) + lane;
+            if (m < a.M) a.part_sum[((int64_t)number * a.tiles_n + tn) * a.M + m] = sum[j][0];
         }
     }
 }
-template <typename T, bool GX, bool GY, int BM, int BN, int WAVES_M, int WAVES_N>
+template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(const GroupedWeights<T> a) {
     HIP_DYNAMIC_SHARED(char, shared)
     T* const lds = reinterpret_cast<T*>(shared);
@@ -708,7 +619,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(c
             p = runs.among(first, chunk1);
         }
         if (p.expert < 0) return;
-        grouped_dw_piece<T, GX, GY, BM, BN, WAVES_M, WAVES_N>(a, lds, p.expert, max(p.begin, chunk0), min(p.end, chunk1), p.begin >= chunk0 && p.end <= chunk1, chunk + p.expert, m0, n0, lane, wave);
+        grouped_dw_piece<T, BM, BN, WAVES_M, WAVES_N>(a, lds, p.expert, max(p.begin, chunk0), min(p.end, chunk1), p.begin >= chunk0 && p.end <= chunk1, chunk + p.expert, m0, n0, fresh(lane), wave);
         first = p.end;
         __syncthreads();                                      // (everyone is done with what the next one's copies overwrite)
     }
@@ -725,29 +636,28 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<
     for (int i = 0; i < Runs::kLanes; i++)
         if (expert / 64 == i) p = runs.of_expert(i, expert % 64);
     const int chunk0 = p.begin / a.chunk, chunks = p.end > p.begin ? (p.end - 1) / a.chunk - chunk0 + 1 : 0, first = chunk0 + expert;
-    if (chunks == 1) return;
-    const int64_t n4 = a.ld_part / 4, places = a.M * n4 + (a.part_sum != nullptr ? a.M : 0);
-    for (int64_t i = (int64_t)((int)blockIdx.x - expert * blocks) * 64 + lane; i - lane < places; i += 64 * blocks) {
+    const int64_t n4 = a.ld_part / 4, places = a.M * n4 + (a.part_sum != nullptr ? a.M : 0), skipped = chunks == 1 ? a.M * n4 / 64 * 64 : 0;
+    for (int64_t i = skipped + (int64_t)((int)blockIdx.x - expert * blocks) * 64 + lane; i - lane < places; i += 64 * blocks) {
         const bool sum = i >= a.M * n4;                       // of the rows
         const int64_t m = sum ? i - a.M * n4 : i / n4;
         const int n = sum ? 0 : (int)(i - m * n4) * 4;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (!sum) {
+        if (!sum && chunks != 1) {
 #pragma unroll 8
             for (int s = wave; s < chunks; s += 4) v += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)(first + s) * a.M + m) * a.ld_part + n);
-        } else if (i < places) {
-            for (int s = wave; s < chunks; s += 4) v[0] += a.part_sum[(int64_t)(first + s) * a.M + m];
+        } else if (sum && i < places) {
+            for (int s = wave; s < chunks * a.tiles_n; s += 4) v[0] += a.part_sum[((int64_t)first * a.tiles_n + s) * a.M + m];
         }
         if (wave > 0) rest[wave - 1][lane] = v;
         __syncthreads();
         if (wave == 0) {
 #pragma unroll
             for (int r = 0; r < 3; r++) v += rest[r][lane];
-            if (!sum) {
+            if (!sum && chunks != 1) {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     if (n + e < a.N) a.out[((int64_t)expert * a.M + m) * a.N + n + e] = (T)v[e];
-            } else if (i < places) {
+            } else if (sum && i < places) {
                 a.sums[(int64_t)expert * a.M + m] = (T)v[0];
             }
         }
@@ -756,12 +666,51 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<
 }
 
 // ---------------------------------------------------------------------------------------
-// A token's rows added up: out = residual + gate * sum over j of y[places[j]].  Bound by memory.
+// Rows of tokens in the order of the places; with weights, multiplied by them (and by the gate of their sample) in fp32.  Bound by memory.
+// ---------------------------------------------------------------------------------------
+template <typename T>
+struct Gather {
+    const T *x, *gate;
+    T* out;
+    const float* weights;
+    const int32_t* offsets;
+    Order order;
+    int64_t ldx, ldo, s_gate, per_sample;
+    int rows, experts, N, pieces, wide, wide_gate;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void gather_kernel(const Gather<T> a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, place = i / a.pieces;
+    if (place >= min(a.rows, max(0, a.offsets[a.experts]))) return;
+    const int n = (int)(i - place * a.pieces) * 8, left = a.N - n, token = a.order.token((int)place);
+    vec8<T> v = take8(a.x + token * a.ldx + n, a.wide, left);
+    if (a.weights != nullptr) {
+        const float w = a.weights[a.order.slot((int)place)];
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = (float)v[e] * w;
+        if (a.gate != nullptr) {
+            const vec8<T> g = take8(a.gate + token / a.per_sample * a.s_gate + n, a.wide_gate, left);
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] *= (float)g[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = (T)f[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (e >= left) v[e] = (T)0.f;
+    *reinterpret_cast<vec8<T>*>(a.out + place * a.ldo + n) = v;
+}
+
+// ---------------------------------------------------------------------------------------
+// A token's rows added up: out = residual + gate * sum over j of w_j y[places[j]].  Bound by memory.
 // ---------------------------------------------------------------------------------------
 template <typename T>
 struct Combine {
     const T *y, *gate, *residual;
     const int32_t* places;
+    const float* weights;                 // or NULL: 1
     T *out, *sum;                         // sum: what the gate multiplies, or NULL
     int64_t ldy, s_gate, ldr, ldo, lds, tokens, per_sample;
     int k, rows, N, pieces, wide, wide_side, wide_out;       // pieces: of eight, of a row
@@ -779,8 +728,9 @@ __global__ __launch_bounds__(256) void combine_kernel(const Combine<T> a) {
         const int p = a.places[m * a.k + j];
         if ((unsigned)p >= (unsigned)a.rows) continue;        // no expert
         const vec8<T> y = *reinterpret_cast<const vec8<T>*>(a.y + p * a.ldy + n);
+        const float w = a.weights != nullptr ? a.weights[m * a.k + j] : 1.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += (float)y[e];
+        for (int e = 0; e < 8; e++) v[e] = fmaf(w, (float)y[e], v[e]);
     }
     if (a.sum != nullptr) store8(a.sum + m * a.lds + n, v, true, 8);
     if (a.gate != nullptr) {
@@ -796,41 +746,48 @@ __global__ __launch_bounds__(256) void combine_kernel(const Combine<T> a) {
     store8(a.out + m * a.ldo + n, v, a.wide_out, left);
 }
 
-// dweights[m][j] = the parts of its place added up, and dout[m] . b_out of the expert; 0 without one.  A wave a token.
+// dweights[m][j] = gate dout[m] . y of its place; 0 without one.  A wave a token.  Bound by memory.
 template <typename T>
 struct DWeights {
-    const float* dots;
-    const T *dout, *bias;
-    const int32_t *places, *experts;
+    const T *dout, *y, *gate;
+    const int32_t* places;
     float* dweights;
-    int64_t ldd, tokens;
-    int k, rows, parts, N, n_experts, wide;
+    int64_t ldd, ldy, s_gate, tokens, per_sample;
+    int k, rows, N, wide, wide_gate;
 };
 template <typename T>
 __global__ __launch_bounds__(256) void dweights_kernel(const DWeights<T> a) {
     const int lane = threadIdx.x & 63;
-    const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (m >= a.tokens) return;
-    for (int j = 0; j < a.k; j++) {
-        const int p = a.places[m * a.k + j];
-        float v = 0.f;
-        const bool there = (unsigned)p < (unsigned)a.rows;
-        if (there) {
-            for (int i = lane; i < a.parts; i += 64) v += a.dots[(int64_t)p * a.parts + i];
-            if (a.bias != nullptr) {
-                const T* const b = a.bias + (int64_t)clampi(a.experts[m * a.k + j], 0, a.n_experts - 1) * a.N;
-                for (int n = lane * 8; n < a.N; n += 512) {
-                    const vec8<T> x = *reinterpret_cast<const vec8<T>*>(a.dout + m * a.ldd + n), y = take8(b + n, a.wide, a.N - n);
+    const int64_t m = min((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), a.tokens - 1);
+    float v[LLSA_MAX_CHOICES];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) v += n + e < a.N ? (float)x[e] * (float)y[e] : 0.f;
+    for (int j = 0; j < LLSA_MAX_CHOICES; j++) v[j] = 0.f;
+    for (int n = lane * 8; n < a.N; n += 512) {
+        const int left = a.N - n;
+        const vec8<T> d = take8(a.dout + m * a.ldd + n, a.wide, left);
+        const vec8<T> g = take8(a.gate != nullptr ? a.gate + m / a.per_sample * a.s_gate + n : nullptr, a.wide_gate, left);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = e >= left ? 0.f : a.gate != nullptr ? (float)d[e] * (float)g[e] : (float)d[e];
+#pragma unroll
+        for (int j = 0; j < LLSA_MAX_CHOICES; j++)
+            if (j < a.k) {
+                const int p = a.places[m * a.k + j];
+                if ((unsigned)p < (unsigned)a.rows) {
+                    const vec8<T> y = *reinterpret_cast<const vec8<T>*>(a.y + p * a.ldy + n);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[j] = fmaf(x[e], e >= left ? 0.f : (float)y[e], v[j]);
                 }
             }
-        }
-        v = octet_sum(v);
-        v += across<8>(v);
-        v = quad_sum(v);
-        if (lane == 0) a.dweights[m * a.k + j] = v;
     }
+#pragma unroll
+    for (int j = 0; j < LLSA_MAX_CHOICES; j++)
+        if (j < a.k) {
+            float t = octet_sum(v[j]);
+            t += across<8>(t);
+            t = quad_sum(t);
+            if (lane == 0) a.dweights[m * a.k + j] = t;
+        }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -860,25 +817,26 @@ GroupedTiles grouped_tiles(int64_t rows, int64_t experts, int64_t N, int64_t K) 
     if (each >= 1024 && N >= 512 && K >= 1024 && (rows / 256 + experts) * ceil_div(N, 256) >= 2 * kCus) return k256;
     return k128;
 }
-int columns_of(GroupedTiles t) { return t <= kFew64 || t == kResident ? 32 : t == k64 ? 64 : t == k128 ? 128 : 256; }
-int waves_across(GroupedTiles t) { return t <= kFew64 || t == kResident ? 1 : t == k256 ? 4 : 2; }
-int64_t dot_parts(int64_t rows, int64_t experts, int64_t N, int64_t K) {
-    const GroupedTiles t = grouped_tiles(rows, experts, N, K);
-    return ceil_div(N, columns_of(t)) * waves_across(t);
-}
-template <typename T, bool YC, int BM, int BN, int WAVES_M, int WAVES_N, int ACT>
+template <typename T, bool YC, bool GATHERED, int BM, int BN, int WAVES_M, int WAVES_N, int ACT>
 int launch_grouped_tiles(Grouped<T>& a, hipStream_t stream) {
     a.tiles_n = (int)ceil_div(a.N, BN);
     const int64_t grid = pieces_of(a.rows, a.experts, BM) * a.tiles_n;
     if (grid > kMaxGrid) return fail(-1, "experts: too many rows");
     constexpr int lds = 2 * (BM + BN) * kStep * (int)sizeof(T);
-    auto kernel = grouped_kernel<T, YC, BM, BN, WAVES_M, WAVES_N, ACT>;
+    auto kernel = grouped_kernel<T, YC, GATHERED, BM, BN, WAVES_M, WAVES_N, ACT>;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return fail(-101, "experts: %s", hipGetErrorString(e));
     }
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * WAVES_M * WAVES_N), lds, stream, a);
     return 0;
+}
+template <typename T, bool YC, int ACT>
+int launch_grouped_64(Grouped<T>& a, hipStream_t stream) {
+    if constexpr (!YC) {
+        if (a.order.slots != nullptr) return launch_grouped_tiles<T, YC, true, 64, 64, 2, 2, ACT>(a, stream);
+    }
+    return launch_grouped_tiles<T, YC, false, 64, 64, 2, 2, ACT>(a, stream);
 }
 template <typename T, bool YC, int MT, int ACT>
 int launch_grouped_few(Grouped<T>& a, hipStream_t stream) {
@@ -904,15 +862,16 @@ template <typename T, bool YC, int ACT>
 int launch_grouped(Grouped<T>& a, hipStream_t stream) {
     a.group = (int64_t)a.N * a.K <= (1 << 20) ? 1 : 8;        // (rows of tiles that share y while it does not fit the L2 beside them)
     const GroupedTiles t = grouped_tiles(a.rows, a.experts, a.N, a.K);
-    a.parts = (int)dot_parts(a.rows, a.experts, a.N, a.K);
     switch (t) {
         case kFew16: return launch_grouped_few<T, YC, 1, ACT>(a, stream);
         case kFew32: return launch_grouped_few<T, YC, 2, ACT>(a, stream);
         case kFew64: return launch_grouped_few<T, YC, 4, ACT>(a, stream);
-        case k64: return launch_grouped_tiles<T, YC, 64, 64, 2, 2, ACT>(a, stream);
-        case k128: return launch_grouped_tiles<T, YC, 128, 128, 2, 2, ACT>(a, stream);
+        case k64: return launch_grouped_64<T, YC, ACT>(a, stream);
+        case k128: return launch_grouped_tiles<T, YC, false, 128, 128, 2, 2, ACT>(a, stream);
         case kResident: return a.K == 5 * kStep ? launch_grouped_resident<T, YC, ACT, 5>(a, stream) : launch_grouped_resident<T, YC, ACT, 6>(a, stream);
-        default: return launch_grouped_tiles<T, YC, 256, 256, 2, 4, ACT>(a, stream);
+        default:
+            if constexpr (!YC || ACT == LLSA_ACT_NONE) return launch_grouped_tiles<T, YC, false, 256, 256, 2, 4, ACT>(a, stream);
+            else return launch_grouped_tiles<T, YC, false, 128, 128, 2, 2, ACT>(a, stream);      // (with act'(z) besides, 256 x 256 does not fit the registers)
     }
 }
 template <typename T, bool YC>
@@ -930,8 +889,7 @@ int experts_fwd(const llsa_experts_args& q, hipStream_t stream) {
     a.x = (const T*)q.x; a.ldx = q.ldx; a.y = (const T*)q.w; a.ldy = q.ldw; a.y_expert = (int64_t)q.N * q.ldw;
     a.offsets = q.offsets; a.order = order_of(q.gather_x ? q.order : nullptr, q.k, q.tokens, q.rows);
     a.experts = q.E; a.rows = (int)q.rows; a.N = q.N; a.K = q.K; a.gaps = q.gaps;
-    a.bias = (const T*)q.bias; a.weights = q.weights; a.sorted = q.sorted;
-    a.scaled = q.weights != nullptr ? kScaledRows : q.sorted != nullptr ? kScaledBias : kUnscaled;
+    a.bias = (const T*)q.bias;
     a.out = (T*)q.out; a.ldo = q.ldo; a.z = (T*)q.z; a.ldz = q.ldz;
     a.wide = q.N % 8 == 0 && wide8(q.bias, 0);
     a.wide_out = (q.N % 8 == 0 && wide8(q.out, q.ldo)) || q.padded;
@@ -942,11 +900,9 @@ template <typename T>
 int experts_dx(const llsa_experts_args& q, hipStream_t stream) {
     Grouped<T> a{};
     a.x = (const T*)q.dz; a.ldx = q.lddz; a.y = (const T*)q.w; a.ldy = q.ldw; a.y_expert = (int64_t)q.N * q.ldw;
-    a.offsets = q.offsets; a.order = order_of(q.gather_dz ? q.order : nullptr, q.k, q.tokens, q.rows);
+    a.offsets = q.offsets;
     a.experts = q.E; a.rows = (int)q.rows; a.N = q.K; a.ny = (int)pad8(q.K); a.K = q.N; a.gaps = q.gaps;
-    a.out = (T*)q.out; a.ldo = q.ldo; a.slope_at = (const T*)q.z; a.ldz = q.ldz; a.dots = q.dots;
-    a.sorted = q.sorted;
-    a.scaled = q.z != nullptr && q.sorted != nullptr ? kScaledRows : kUnscaled;
+    a.out = (T*)q.out; a.ldo = q.ldo; a.slope_at = (const T*)q.z; a.ldz = q.ldz;
     a.wide_out = (q.K % 8 == 0 && wide8(q.out, q.ldo)) || q.padded;
     if (int rc = launch_by_act<T, true>(a, q.z != nullptr ? q.act : LLSA_ACT_NONE, stream)) return rc;
     return launch_status("experts_dx");
@@ -968,14 +924,14 @@ int64_t chunk_rows(int64_t rows, int64_t N, int64_t K) {
     return ceil_div(ceil_div(rows, best), kStep) * kStep;
 }
 int64_t part_count(int64_t rows, int64_t experts, int64_t N, int64_t K) { return ceil_div(rows, chunk_rows(rows, N, K)) + experts; }
-template <typename T, bool GX, bool GY, int BM, int BN>
+template <typename T, int BM, int BN>
 int launch_grouped_dw(GroupedWeights<T>& a, hipStream_t stream) {
     a.tiles_m = (int)ceil_div(a.M, BM);
     a.tiles_n = (int)ceil_div(a.N, BN);
     const int64_t grid = ceil_div(a.rows, a.chunk) * a.tiles_m * a.tiles_n;
     if (grid > kMaxGrid) return fail(-1, "experts_dw: too many rows");
     constexpr int lds = 2 * (BM + BN) * kStep * (int)sizeof(T);
-    auto kernel = grouped_dw_kernel<T, GX, GY, BM, BN, 2, 2>;
+    auto kernel = grouped_dw_kernel<T, BM, BN, 2, 2>;
     if (lds > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return fail(-101, "experts_dw: %s", hipGetErrorString(e));
@@ -983,30 +939,21 @@ int launch_grouped_dw(GroupedWeights<T>& a, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), lds, stream, a);
     return 0;
 }
-template <typename T, bool GX, bool GY>
-int launch_dw_tiles(GroupedWeights<T>& a, bool small, hipStream_t stream) {
-    if (small) return launch_grouped_dw<T, GX, GY, 64, 64>(a, stream);
-    if (grouped_rows(a.M) == 192) return launch_grouped_dw<T, GX, GY, 192, 128>(a, stream);
-    return launch_grouped_dw<T, GX, GY, 128, 128>(a, stream);
-}
 template <typename T>
 int experts_dw(const llsa_experts_args& q, hipStream_t stream) {
     GroupedWeights<T> a{};
     a.x = (const T*)q.dz; a.ldx = q.lddz; a.nx = (int)pad8(q.N);
     a.y = (const T*)q.x; a.ldy = q.ldx; a.ny = (int)pad8(q.K);
     a.offsets = q.offsets;
-    a.order = order_of(q.order, q.k, q.tokens, q.rows);
     a.experts = q.E; a.rows = (int)q.rows; a.M = q.N; a.N = q.K;
     a.chunk = (int)chunk_rows(q.rows, q.N, q.K);
-    a.sorted = q.sorted;
     a.out = (T*)q.out; a.sums = (T*)q.dbias;
     a.ld_part = pad8(q.K);
     a.part = (float*)q.workspace;
     a.part_sum = q.dbias != nullptr ? a.part + part_count(q.rows, q.E, q.N, q.K) * a.M * a.ld_part : nullptr;
     a.wide_out = q.K % 8 == 0 && aligned16(q.out);
     const bool small = small_tiles(q.rows, q.N, q.K);
-    const int rc = q.gather_dz ? launch_dw_tiles<T, true, false>(a, small, stream)
-                   : q.gather_x ? launch_dw_tiles<T, false, true>(a, small, stream) : launch_dw_tiles<T, false, false>(a, small, stream);
+    const int rc = small ? launch_grouped_dw<T, 64, 64>(a, stream) : grouped_rows(a.M) == 192 ? launch_grouped_dw<T, 192, 128>(a, stream) : launch_grouped_dw<T, 128, 128>(a, stream);
     if (rc != 0) return rc;
     // (as many workgroups as the chip holds: most experts have one piece, and nothing to add up)
     const int64_t places = (int64_t)a.M * (a.ld_part / 4) + (q.dbias != nullptr ? a.M : 0), blocks = std::min(ceil_div(places, 64), ceil_div(8 * kCus, q.E));
@@ -1014,9 +961,23 @@ int experts_dw(const llsa_experts_args& q, hipStream_t stream) {
     return launch_status("experts_dw");
 }
 template <typename T>
+int experts_gather(const llsa_experts_args& q, hipStream_t stream) {
+    Gather<T> a{};
+    a.x = (const T*)q.x; a.ldx = q.ldx; a.out = (T*)q.out; a.ldo = q.ldo; a.gate = (const T*)q.gate; a.s_gate = q.s_gate; a.per_sample = std::max<int64_t>(1, q.per_sample);
+    a.weights = q.weights; a.offsets = q.offsets; a.order = order_of(q.order, q.k, q.tokens, q.rows);
+    a.rows = (int)q.rows; a.experts = q.E; a.N = q.N; a.pieces = (int)(pad8(q.N) / 8);
+    a.wide = q.N % 8 == 0 && wide8(q.x, q.ldx);
+    a.wide_gate = q.N % 8 == 0 && wide8(q.gate, q.s_gate);
+    const int64_t grid = ceil_div(q.rows * a.pieces, 256);
+    LLSA_REQUIRE(grid <= kMaxGrid, "experts_gather: too many rows");
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(gather_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+    return launch_status("experts_gather");
+}
+template <typename T>
 int experts_combine(const llsa_experts_args& q, hipStream_t stream) {
     Combine<T> a{};
-    a.y = (const T*)q.x; a.ldy = q.ldx; a.places = q.places; a.k = q.k; a.rows = (int)q.rows; a.N = q.N; a.tokens = q.tokens; a.per_sample = std::max<int64_t>(1, q.per_sample);
+    a.y = (const T*)q.x; a.ldy = q.ldx; a.places = q.places; a.weights = q.weights; a.k = q.k; a.rows = (int)q.rows; a.N = q.N; a.tokens = q.tokens;
+    a.per_sample = std::max<int64_t>(1, q.per_sample);
     a.gate = (const T*)q.gate; a.s_gate = q.s_gate; a.residual = (const T*)q.residual; a.ldr = q.ldr;
     a.out = (T*)q.out; a.ldo = q.ldo; a.sum = (T*)q.z; a.lds = q.ldz;
     a.pieces = (int)(pad8(q.N) / 8);
@@ -1031,10 +992,10 @@ int experts_combine(const llsa_experts_args& q, hipStream_t stream) {
 template <typename T>
 int experts_dweights(const llsa_experts_args& q, hipStream_t stream) {
     DWeights<T> a{};
-    a.dots = q.dots; a.dout = (const T*)q.dz; a.ldd = q.lddz; a.bias = (const T*)q.bias; a.places = q.places; a.experts = q.experts; a.dweights = q.dweights;
-    a.tokens = q.tokens; a.k = q.k; a.rows = (int)q.rows; a.N = q.N; a.n_experts = q.E;
-    a.parts = (int)dot_parts(q.rows, q.E, q.K, q.N);          // (of the product that made them: N channels in, K out)
-    a.wide = q.N % 8 == 0 && wide8(q.bias, 0);
+    a.dout = (const T*)q.dz; a.ldd = q.lddz; a.y = (const T*)q.x; a.ldy = q.ldx; a.gate = (const T*)q.gate; a.s_gate = q.s_gate; a.per_sample = std::max<int64_t>(1, q.per_sample);
+    a.places = q.places; a.dweights = q.dweights; a.tokens = q.tokens; a.k = q.k; a.rows = (int)q.rows; a.N = q.N;
+    a.wide = q.N % 8 == 0 && wide8(q.dz, q.lddz);
+    a.wide_gate = q.N % 8 == 0 && wide8(q.gate, q.s_gate);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(dweights_kernel<T>), dim3((unsigned)ceil_div(q.tokens, 4)), dim3(256), 0, stream, a);
     return launch_status("experts_dweights");
 }
@@ -1046,7 +1007,7 @@ int check_experts(const char* what, const llsa_experts_args* a) {
                  LLSA_MAX_EXPERTS, LLSA_MAX_SLOTS);
     LLSA_REQUIRE(a->k >= 1 && a->k <= LLSA_MAX_CHOICES, "%s: 1 to %d experts a token", what, LLSA_MAX_CHOICES);
     LLSA_REQUIRE(a->rows == 0 || a->offsets != nullptr, "%s: offsets", what);
-    LLSA_REQUIRE(!((a->gather_x || a->gather_dz) && a->rows > 0) || (a->order != nullptr && a->tokens > 0), "%s: gathered rows need the order and tokens", what);
+    LLSA_REQUIRE(!a->gather_x || a->rows == 0 || (a->order != nullptr && a->tokens > 0), "%s: gathered rows need the order and tokens", what);
     return 0;
 }
 }  // namespace
@@ -1058,11 +1019,15 @@ using namespace llsa;
 
 extern "C" int64_t llsa_experts_dw_workspace_bytes(int64_t rows, int E, int N, int K) {
     if (rows <= 0 || E <= 0 || N <= 0 || K <= 0) return 0;
-    return 4 * part_count(rows, E, N, K) * N * (pad8(K) + 1);
+    return 4 * part_count(rows, E, N, K) * N * (pad8(K) + ceil_div(K, 64));
 }
-extern "C" int64_t llsa_experts_dot_parts(int64_t rows, int E, int N, int K) {
-    if (rows <= 0 || E <= 0 || N <= 0 || K <= 0) return 0;
-    return dot_parts(rows, E, K, N);
+extern "C" int llsa_experts_gathers(int64_t rows, int E, int N, int K) { return rows > 0 && E > 0 && N > 0 && K > 0 && grouped_tiles(rows, E, N, K) <= k64; }
+extern "C" int llsa_experts_gather(const llsa_experts_args* a, void* stream) {
+    if (int rc = check_experts("experts_gather", a)) return rc;
+    if (a->rows == 0) return 0;
+    LLSA_REQUIRE(a->order != nullptr && a->tokens > 0 && a->x != nullptr && rows16(a->out, a->ldo) && a->ldo >= pad8(a->N), "experts_gather: order, rows 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->gate == nullptr || (a->weights != nullptr && a->per_sample > 0), "experts_gather: a gate goes with the weights");
+    return BY_TYPE(experts_gather);
 }
 extern "C" int llsa_experts_fwd(const llsa_experts_args* a, void* stream) {
     if (int rc = check_experts("experts_fwd", a)) return rc;
@@ -1071,7 +1036,7 @@ extern "C" int llsa_experts_fwd(const llsa_experts_args* a, void* stream) {
                  "experts_fwd: rows of x and w must be 16-byte aligned and a multiple of 8 long (zeros beyond the end)");
     LLSA_REQUIRE(a->out != nullptr && offsets32(a->ldo) && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->N))), "experts_fwd: output, padded rows 16-byte aligned and a multiple of 8 long");
     LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->N)), "experts_fwd: rows of z must be 16-byte aligned and padded to a multiple of 8");
-    LLSA_REQUIRE(a->weights == nullptr || (a->sorted != nullptr && a->gather_x), "experts_fwd: weights go with gathered rows, and are kept sorted");
+    LLSA_REQUIRE(!a->gather_x || llsa_experts_gathers(a->rows, a->E, a->N, a->K), "experts_fwd: rows of this many tokens have to be gathered beforehand");
     return BY_TYPE(experts_fwd);
 }
 extern "C" int llsa_experts_dx(const llsa_experts_args* a, void* stream) {
@@ -1080,12 +1045,11 @@ extern "C" int llsa_experts_dx(const llsa_experts_args* a, void* stream) {
     LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->w, a->ldw) && a->lddz >= pad8(a->N) && a->ldw >= pad8(a->K), "experts_dx: rows of dz and w must be 16-byte aligned and padded to a multiple of 8");
     LLSA_REQUIRE(a->out != nullptr && offsets32(a->ldo) && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->K))), "experts_dx: output, padded rows 16-byte aligned and a multiple of 8 long");
     LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->K) && a->act != LLSA_ACT_NONE), "experts_dx: rows of z must be 16-byte aligned and padded to a multiple of 8");
-    LLSA_REQUIRE(a->dots == nullptr || a->z != nullptr, "experts_dx: sums of act(z) dx need z");
     return BY_TYPE(experts_dx);
 }
 extern "C" int llsa_experts_dw(const llsa_experts_args* a, void* stream) {
     if (int rc = check_experts("experts_dw", a)) return rc;
-    LLSA_REQUIRE(a->rows > 0 && !(a->gather_x && a->gather_dz), "experts_dw: rows, of which x or dz may be gathered");
+    LLSA_REQUIRE(a->rows > 0, "experts_dw: no rows");
     LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->x, a->ldx) && a->lddz >= pad8(a->N) && a->ldx >= pad8(a->K), "experts_dw: rows of dz and x must be 16-byte aligned and padded to a multiple of 8");
     LLSA_REQUIRE(a->out != nullptr && a->workspace != nullptr && aligned16(a->workspace), "experts_dw: output and workspace (16-byte aligned)");
     return BY_TYPE(experts_dw);
@@ -1101,7 +1065,8 @@ extern "C" int llsa_experts_combine(const llsa_experts_args* a, void* stream) {
 extern "C" int llsa_experts_dweights(const llsa_experts_args* a, void* stream) {
     if (int rc = check_experts("experts_dweights", a)) return rc;
     if (a->tokens == 0) return 0;
-    LLSA_REQUIRE(a->places != nullptr && a->dweights != nullptr && (a->rows == 0 || a->dots != nullptr), "experts_dweights: places, sums and result");
-    LLSA_REQUIRE(a->bias == nullptr || (a->experts != nullptr && rows16(a->dz, a->lddz) && a->lddz >= pad8(a->N)), "experts_dweights: the bias needs the experts and dout in padded rows");
+    LLSA_REQUIRE(a->places != nullptr && a->dweights != nullptr && a->dz != nullptr && (a->rows == 0 || (rows16(a->x, a->ldx) && a->ldx >= pad8(a->N))),
+                 "experts_dweights: places, dout, result, rows 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->gate == nullptr || (a->per_sample > 0 && a->tokens % a->per_sample == 0), "experts_dweights: rows of a sample, whole samples");
     return BY_TYPE(experts_dweights);
 }

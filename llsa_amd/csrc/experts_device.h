@@ -104,6 +104,14 @@ struct Runs {
     }
 };
 
+// A copy that the compiler takes for a new value: what is computed from it inside a loop is not kept in registers around the loop.
+__device__ __forceinline__ int fresh(int v) {
+#ifndef LLSA_CPU_EMU_BUILD
+    asm volatile("" : "+v"(v));
+#endif
+    return v;
+}
+
 // Which row of tokens stands at a place of the sorted order: slots are numbered token * per_token + choice
 struct Order {
     const int32_t* slots;                 // or NULL: rows are where they are
@@ -116,56 +124,24 @@ struct Order {
     }
 };
 
-// Rows of x as OperandX<rows> lays them out in LDS, of tokens in the order
-template <typename T, int ROWS, int WAVES>
-struct GatheredRows {
+// Rows of x as Operand<rows> lays them out in LDS.  GATHERED: of tokens in the order
+template <typename T, int ROWS, int WAVES, bool GATHERED>
+struct RowsAlong {
     typedef Operand<T, false, ROWS, WAVES> Plain;
     static constexpr int kCopies = Plain::kCopies;
-    const T* from[kCopies];
-    __device__ __forceinline__ void init(const T* x, int64_t ld, const Order& order, int place, int left, int wave, int lane) {
-#pragma unroll
-        for (int j = 0; j < kCopies; j++) {
-            const int i = wave * kCopies + j, r = Plain::row_of(i, lane), at = place + min(r, left - 1);
-            from[j] = x + (order.slots != nullptr ? order.token(at) : at) * ld + Plain::place_of(i, r, lane);
-        }
-    }
-    __device__ __forceinline__ void request(int k, T* tile, int wave, int lane, int k_left) const {
-#pragma unroll
-        for (int j = 0; j < kCopies; j++) {
-            const int i = wave * kCopies + j;
-            const bool inside = k_left >= kStep || Plain::place_of(i, Plain::row_of(i, lane), lane) < k_left;
-            copy_to_lds(inside ? from[j] + k : reinterpret_cast<const T*>(kZeros), tile + i * 512);
-        }
-    }
-};
-// 64 rows of x across, as Operand<columns> lays them out.  GATHERED: of tokens in the order, which are looked up a step ahead
-template <typename T, int ROWS, int WAVES, bool GATHERED>
-struct Columns {
-    typedef Operand<T, true, ROWS, WAVES> Plain;
-    static constexpr int kCopies = Plain::kCopies;
     Plain plain;
-    const T *x;
-    int64_t ld;
-    int row[GATHERED ? kCopies : 1], place[GATHERED ? kCopies : 1];
-    // left: elements of a row from x on.  first: the first row, where rows are not gathered
-    __device__ __forceinline__ void init(const T* x_, int64_t ld_, int first, int left, int wave, int lane) {
-        x = x_;
-        ld = ld_;
+    const T* x;
+    const T* from[GATHERED ? kCopies : 1];
+    __device__ __forceinline__ void init(const T* x_, int64_t ld, const Order& order, int first, int left, int wave, int lane) {
         if constexpr (GATHERED) {
 #pragma unroll
             for (int j = 0; j < kCopies; j++) {
-                const int i = wave * kCopies + j;
-                place[j] = min(Plain::place_of(i, Plain::row_of(i, lane), lane), left - 8);
+                const int i = wave * kCopies + j, r = Plain::row_of(i, lane);
+                from[j] = x_ + order.token(first + min(r, left - 1)) * ld + Plain::place_of(i, r, lane);
             }
         } else {
-            x += first * ld;
+            x = x_ + first * ld;
             plain.init(wave, lane, ld, left);
-        }
-    }
-    __device__ __forceinline__ void look_up(const Order& order, int at, int k_left, int wave, int lane) {
-        if constexpr (GATHERED) {
-#pragma unroll
-            for (int j = 0; j < kCopies; j++) row[j] = order.token(at + min(Plain::row_of(wave * kCopies + j, lane), k_left - 1));
         }
     }
     __device__ __forceinline__ void request(T* tile, int wave, int lane, int k_left) {
@@ -173,12 +149,13 @@ struct Columns {
 #pragma unroll
             for (int j = 0; j < kCopies; j++) {
                 const int i = wave * kCopies + j;
-                const T* const from = x + (uint64_t)(unsigned)row[j] * (unsigned)ld + place[j];
-                copy_to_lds(Plain::row_of(i, lane) < k_left ? from : reinterpret_cast<const T*>(kZeros), tile + i * 512);
+                const bool inside = k_left >= kStep || Plain::place_of(i, Plain::row_of(i, lane), lane) < k_left;
+                copy_to_lds(inside ? from[j] : reinterpret_cast<const T*>(kZeros), tile + i * 512);
+                from[j] += kStep;
             }
         } else {
             plain.request(x, tile, wave, lane, k_left);
-            x += kStep * ld;
+            x += kStep;
         }
     }
 };

@@ -115,13 +115,14 @@ struct Library {
     decltype(&llsa_route_tokens) route_tokens;
     decltype(&llsa_route_tokens_bwd) route_tokens_bwd;
     decltype(&llsa_route_workspace_bytes) route_workspace_bytes;
+    decltype(&llsa_experts_gather) experts_gather;
+    decltype(&llsa_experts_gathers) experts_gathers;
     decltype(&llsa_experts_fwd) experts_fwd;
     decltype(&llsa_experts_dx) experts_dx;
     decltype(&llsa_experts_dw) experts_dw;
     decltype(&llsa_experts_combine) experts_combine;
     decltype(&llsa_experts_dweights) experts_dweights;
     decltype(&llsa_experts_dw_workspace_bytes) experts_dw_workspace_bytes;
-    decltype(&llsa_experts_dot_parts) experts_dot_parts;
     bool device;                          // false: the CPU emulation build the tests install
 
     Library(const std::map<std::string, uintptr_t>& at_, bool device_) : device(device_) {
@@ -159,13 +160,14 @@ struct Library {
         get("llsa_route_tokens", route_tokens);
         get("llsa_route_tokens_bwd", route_tokens_bwd);
         get("llsa_route_workspace_bytes", route_workspace_bytes);
+        get("llsa_experts_gather", experts_gather);
+        get("llsa_experts_gathers", experts_gathers);
         get("llsa_experts_fwd", experts_fwd);
         get("llsa_experts_dx", experts_dx);
         get("llsa_experts_dw", experts_dw);
         get("llsa_experts_combine", experts_combine);
         get("llsa_experts_dweights", experts_dweights);
         get("llsa_experts_dw_workspace_bytes", experts_dw_workspace_bytes);
-        get("llsa_experts_dot_parts", experts_dot_parts);
     }
     void check(int rc, const char* what) const {
         if (rc != 0) fail(Failure::kLibrary, std::string(what) + " failed (" + std::to_string(rc) + "): " + last_error_string());

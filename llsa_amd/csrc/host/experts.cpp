@@ -116,7 +116,6 @@ void set_weights(llsa_experts_args& a, const Weights& w) {
     a.w = w.p(); a.ldw = w.rows.ld; a.E = static_cast<int32_t>(w.E); a.N = static_cast<int32_t>(w.N); a.K = static_cast<int32_t>(w.K);
 }
 const int32_t* ints(const Tensor& t) { return t.data_ptr<int32_t>(); }
-float* floats(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 Tensor dense_bias(const Tensor* t) { return t != nullptr ? contiguous(*t) : Tensor(); }
 
 struct GroupedLinearBackward : public BlockNode {
@@ -235,12 +234,23 @@ Tensor grouped_linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, c
 // ---------------------------------------------------------------------------------------
 // the routed feed-forward block
 // ---------------------------------------------------------------------------------------
+// Rows of tokens in the order of the places, multiplied by the router's weights and the gate unless they are NULL
+Rows gathered(const Call& call, const Rows& x, const llsa_experts_args& base, const float* weights, const Tensor& gate, int64_t per_sample) {
+    Rows r;
+    r.t = call.rows(base.rows, x.cols); r.ld = r.t.size(1); r.count = base.rows; r.cols = x.cols;
+    llsa_experts_args a = base;
+    a.act = LLSA_ACT_NONE;
+    a.x = x.p(); a.ldx = x.ld; a.out = r.p(); a.ldo = r.ld; a.weights = weights; a.N = static_cast<int32_t>(x.cols); a.K = 8;
+    if (gate.defined()) { a.gate = gate.data_ptr(); a.s_gate = gate.size(0) > 1 ? gate.stride(0) : 0; a.per_sample = per_sample; }
+    call.lib().check(call.lib().experts_gather(&a, call.stream()), "experts_gather");
+    return r;
+}
 struct ExpertFeedForwardBackward : public BlockNode {
     std::vector<int64_t> sizes, chosen;   // of x, of the router's weights
     int64_t tokens, k, per_sample, samples, E, C, F, N;
     bool has_b1, has_b2, has_gate, has_residual, has_sum;
     int act, dtype;
-    enum { kX, kW1, kW2, kGate, kOffsets, kOrder, kPlaces, kExperts, kSorted, kZ, kH, kSum, kB2 };
+    enum { kX, kW1, kW2, kGate, kOffsets, kOrder, kPlaces, kWeights, kZ, kH, kSum, kY };
     std::string name() const override { return "ExpertFeedForwardBackward"; }
     variable_list run(const Tensor& grad, const std::vector<Tensor>& saved) override {
         Call call(*lib, grad);
@@ -256,62 +266,47 @@ struct ExpertFeedForwardBackward : public BlockNode {
         if (want_x) dx = at::empty(sizes, o);
         if (want_p) dp = at::empty(chosen, o.dtype(at::kFloat));
         if (rows > 0 && (inner || outer || want_p || want_g)) {
-            // dout behind the gate: rows of tokens
-            Rows g;
-            if (has_gate) {
-                const Rows dout = rows_of(grad);
-                const Tensor gate = dense_vector(&saved[kGate]), sum = has_sum ? as_kept(saved[kSum]) : Tensor();
-                g.t = call.rows(tokens, N); g.ld = g.t.size(1); g.count = tokens; g.cols = N;
+            const Rows dout = rows_of(grad);
+            const Tensor gate = has_gate ? dense_vector(&saved[kGate]) : Tensor();
+            if (want_g) {
+                const Tensor sum = as_kept(saved[kSum]), unused = call.rows(tokens, N), workspace = call.bytes(lib->linear_dz_workspace_bytes(tokens, per_sample, static_cast<int>(N)));
+                dg = at::empty({samples, N}, o);
                 llsa_linear_args a{};
-                a.dout = dout.p(); a.lddout = dout.ld; a.gate = gate.data_ptr(); a.s_gate = gate.size(0) > 1 ? gate.stride(0) : 0;
-                if (has_sum) { a.z = sum.data_ptr(); a.ldz = sum.size(1); }
-                a.dz_out = g.p(); a.lddz = g.ld; a.M = tokens; a.per_sample = per_sample; a.N = static_cast<int32_t>(N); a.K = 1; a.act = LLSA_ACT_NONE; a.dtype = dtype;
-                Tensor workspace;
-                if (want_g) {
-                    dg = at::empty({samples, N}, o);
-                    workspace = call.bytes(lib->linear_dz_workspace_bytes(tokens, per_sample, a.N));
-                    a.dgate = dg.data_ptr(); a.workspace = workspace.data_ptr();
-                }
+                a.dout = dout.p(); a.lddout = dout.ld; a.z = sum.data_ptr(); a.ldz = sum.size(1); a.dz_out = unused.data_ptr(); a.lddz = unused.size(1);
+                a.M = tokens; a.per_sample = per_sample; a.N = static_cast<int32_t>(N); a.K = 1; a.act = LLSA_ACT_NONE; a.dtype = dtype;
+                a.dgate = dg.data_ptr(); a.workspace = workspace.data_ptr();
                 lib->check(lib->linear_dz(&a, call.stream()), "linear_dz");
-            } else {
-                g = call.operand(grad);
             }
             if (!inner && !outer && !want_p) return results(dx, dp, dw1, db1, dw2, db2, dg, grad, want_w1, want_w2, want_r);
-            const Tensor offsets = contiguous(saved[kOffsets]), order = contiguous(saved[kOrder]), places = contiguous(saved[kPlaces]), experts = contiguous(saved[kExperts]);
-            const Tensor sorted = as_kept(saved[kSorted]);
+            const Tensor offsets = contiguous(saved[kOffsets]), order = contiguous(saved[kOrder]), places = contiguous(saved[kPlaces]), weights = contiguous(saved[kWeights]);
             llsa_experts_args base{};
-            base.offsets = ints(offsets); base.order = ints(order); base.places = ints(places); base.experts = ints(experts); base.sorted = sorted.data_ptr<float>();
+            base.offsets = ints(offsets); base.order = ints(order); base.places = ints(places);
             base.rows = rows; base.tokens = tokens; base.k = static_cast<int32_t>(k); base.E = static_cast<int32_t>(E); base.dtype = dtype; base.act = act;
+            if (want_p) {
+                const Tensor y = as_kept(saved[kY]);
+                llsa_experts_args a = base;
+                a.dz = dout.p(); a.lddz = dout.ld; a.x = y.data_ptr(); a.ldx = y.size(1); a.dweights = dp.data_ptr<float>(); a.N = static_cast<int32_t>(N); a.K = 8;
+                if (has_gate) { a.gate = gate.data_ptr(); a.s_gate = gate.size(0) > 1 ? gate.stride(0) : 0; a.per_sample = per_sample; }
+                lib->check(lib->experts_dweights(&a, call.stream()), "experts_dweights");
+            }
+            if (!inner && !outer) return results(dx, dp, dw1, db1, dw2, db2, dg, grad, want_w1, want_w2, want_r);
+            const Rows g = gathered(call, dout, base, weights.data_ptr<float>(), gate, per_sample);      // w gate dout
             Rows dz;
-            Tensor dots;
-            if (inner || want_p) {                            // dz = w act'(z) (dout W_out), and the weights' sums
+            if (inner) {                                      // dz = act'(z) (g W_out)
                 const Weights w2 = weights_of(call, saved[kW2], E, N, F);
                 const Tensor z = as_kept(saved[kZ]);
                 dz.t = call.rows(rows, F); dz.ld = dz.t.size(1); dz.count = rows; dz.cols = F;
                 llsa_experts_args a = base;
                 set_weights(a, w2);
-                a.dz = g.p(); a.lddz = g.ld; a.gather_dz = 1;
+                a.dz = g.p(); a.lddz = g.ld;
                 a.out = dz.p(); a.ldo = dz.ld; a.padded = 1; a.z = z.data_ptr(); a.ldz = z.size(1);
-                if (want_p) {
-                    dots = at::empty({rows, lib->experts_dot_parts(rows, a.E, a.N, a.K)}, o.dtype(at::kFloat));
-                    a.dots = floats(dots);
-                }
                 lib->check(lib->experts_dx(&a, call.stream()), "experts_dx");
-                if (want_p) {
-                    const Tensor b2 = saved[kB2].defined() ? contiguous(saved[kB2]) : Tensor();
-                    llsa_experts_args d = a;
-                    d.z = nullptr; d.dweights = floats(dp);
-                    d.bias = b2.defined() ? b2.data_ptr() : nullptr;
-                    lib->check(lib->experts_dweights(&d, call.stream()), "experts_dweights");
-                }
             }
-            auto weights_back = [&](const void* dz_rows, int64_t lddz, bool gather_dz, const void* x, int64_t ldx, bool gather_x, int64_t n, int64_t kk, const float* scale, Tensor& dw, Tensor& db,
-                                    bool want_bias) {
+            auto weights_back = [&](const Rows& dz_rows, const Tensor& x, int64_t n, int64_t kk, Tensor& dw, Tensor& db, bool want_bias) {
                 dw = at::empty({E, n, kk}, o);
                 if (want_bias) db = at::empty({E, n}, o);
                 llsa_experts_args a = base;
-                a.sorted = const_cast<float*>(scale);
-                a.dz = dz_rows; a.lddz = lddz; a.gather_dz = gather_dz; a.x = x; a.ldx = ldx; a.gather_x = gather_x;
+                a.dz = dz_rows.p(); a.lddz = dz_rows.ld; a.x = x.data_ptr(); a.ldx = x.size(1);
                 a.N = static_cast<int32_t>(n); a.K = static_cast<int32_t>(kk); a.out = dw.data_ptr();
                 if (want_bias) a.dbias = db.data_ptr();
                 const Tensor workspace = call.bytes(lib->experts_dw_workspace_bytes(rows, a.E, a.N, a.K));
@@ -319,19 +314,17 @@ struct ExpertFeedForwardBackward : public BlockNode {
                 lib->check(lib->experts_dw(&a, call.stream()), "experts_dw");
             };
             if (outer) {
-                const Tensor h = as_kept(saved[kH]);
-                weights_back(g.p(), g.ld, true, h.data_ptr(), h.size(1), false, N, F, base.sorted, dw2, db2, want_b2);
+                weights_back(g, as_kept(saved[kH]), N, F, dw2, db2, want_b2);
             }
             if (want_w1 || want_b1) {
-                const Rows x = kept_operand(call, saved[kX], C);
-                weights_back(dz.p(), dz.ld, false, x.p(), x.ld, true, F, C, nullptr, dw1, db1, want_b1);
+                weights_back(dz, as_kept(saved[kX]), F, C, dw1, db1, want_b1);
             }
             if (want_x) {
                 const Weights w1 = weights_of(call, saved[kW1], E, F, C);
                 const Tensor each = call.rows(rows, C);
                 llsa_experts_args a = base;
                 set_weights(a, w1);
-                a.dz = dz.p(); a.lddz = dz.ld; a.out = each.data_ptr(); a.ldo = each.size(1); a.padded = 1; a.act = LLSA_ACT_NONE; a.sorted = nullptr;
+                a.dz = dz.p(); a.lddz = dz.ld; a.out = each.data_ptr(); a.ldo = each.size(1); a.padded = 1; a.act = LLSA_ACT_NONE;
                 lib->check(lib->experts_dx(&a, call.stream()), "experts_dx");
                 llsa_experts_args s = base;
                 s.x = each.data_ptr(); s.ldx = each.size(1); s.out = dx.data_ptr(); s.ldo = C; s.N = static_cast<int32_t>(C); s.K = 8; s.act = LLSA_ACT_NONE;
@@ -389,7 +382,7 @@ Tensor expert_feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_
     check_ints(what, "routing.offsets", offsets_in, {E + 1});
     const bool grad = wants({&x_in, &weights_in, &w1_in, b1, &w2_in, b2, gate_p, residual_p});
     const bool inner = grad && wants({&x_in, &w1_in, b1}), outer = grad && wants({&w2_in, b2}), gates = grad && wants({gate_p}), chooses = grad && wants({&weights_in});
-    Tensor out, z, h, sum, gate, sorted, order, offsets, places, experts;
+    Tensor out, z, h, y, sum, gate, weights, order, offsets, places;
     Rows x;
     Weights w1, w2;
     std::shared_ptr<ExpertFeedForwardBackward> node;
@@ -399,23 +392,28 @@ Tensor expert_feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_
         Call call(*lib, x_in);
         out = at::empty(with_last(x_in, N), x_in.options());
         gate = dense_vector(gate_p);
-        order = contiguous(order_in); offsets = contiguous(offsets_in); places = contiguous(places_in); experts = contiguous(experts_in);
+        order = contiguous(order_in); offsets = contiguous(offsets_in); places = contiguous(places_in); weights = contiguous(weights_in);
         x.t = x_in; w1.rows.t = w1_in; w2.rows.t = w2_in;
         if (tokens > 0) {
             call.operands({{&x_in, &x}, {&w1_in, &w1.rows}, {&w2_in, &w2.rows}});
             w1.E = w2.E = E; w1.N = F; w1.K = pad8(C); w2.N = N; w2.K = pad8(F);
-            const Tensor weights = contiguous(weights_in), bias1 = dense_bias(b1), bias2 = dense_bias(b2);
-            sorted = at::empty({rows}, x_in.options().dtype(at::kFloat));
+            const Tensor bias1 = dense_bias(b1), bias2 = dense_bias(b2);
             h = call.rows(rows, F);
-            if (inner || chooses) z = call.rows(rows, F);
+            if (inner) z = call.rows(rows, F);
             if (gates) sum = call.rows(tokens, N);
-            const Tensor y = call.rows(rows, N);
+            y = call.rows(rows, N);
             llsa_experts_args a{};
-            a.order = ints(order); a.offsets = ints(offsets); a.places = ints(places); a.sorted = floats(sorted);
+            a.order = ints(order); a.offsets = ints(offsets); a.places = ints(places);
             a.rows = rows; a.tokens = tokens; a.k = static_cast<int32_t>(k); a.dtype = dtype; a.padded = 1;
+            a.E = static_cast<int32_t>(E);
             llsa_experts_args one = a, two = a, all = a;
             set_weights(one, w1);
-            one.x = x.p(); one.ldx = x.ld; one.gather_x = 1; one.weights = weights.data_ptr<float>(); one.bias = bias1.defined() ? bias1.data_ptr() : nullptr;
+            // (what a backward wants in the order of the places is brought there once)
+            x.cols = C;
+            if (grad || !lib->experts_gathers(rows, one.E, one.N, one.K)) x = gathered(call, x, a, nullptr, Tensor(), 1);
+            else one.gather_x = 1;
+            one.x = x.p(); one.ldx = x.ld;
+                        one.bias = bias1.defined() ? bias1.data_ptr() : nullptr;
             one.out = h.data_ptr(); one.ldo = h.size(1); one.act = act;
             if (z.defined()) { one.z = z.data_ptr(); one.ldz = z.size(1); }
             lib->check(lib->experts_fwd(&one, call.stream()), "experts_fwd");
@@ -424,6 +422,7 @@ Tensor expert_feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_
             two.out = y.data_ptr(); two.ldo = y.size(1);
             lib->check(lib->experts_fwd(&two, call.stream()), "experts_fwd");
             const Rows residual = call.addend(residual_p);
+            all.weights = weights.data_ptr<float>();
             all.x = y.data_ptr(); all.ldx = y.size(1); all.E = static_cast<int32_t>(E); all.N = static_cast<int32_t>(N); all.K = 8; all.padded = 0;
             if (gate.defined()) { all.gate = gate.data_ptr(); all.s_gate = gate.size(0) > 1 ? gate.stride(0) : 0; }
             all.residual = residual.p(); all.ldr = residual.ld; all.per_sample = in.per_sample();
@@ -444,19 +443,18 @@ Tensor expert_feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_
         torch::autograd::set_history(out, node);
         auto keep = [&](bool needed, const Tensor& t, const Tensor& input) { node->keep(needed ? t : Tensor(), input); };
         const bool any = inner || outer || chooses;
-        keep(wants({&w1_in, b1}), x.t, x_in);
+        keep(wants({&w1_in, b1}), x.t, x.t);                  // (in the order of the places)
         keep(x_in.requires_grad(), w1.rows.t, w1_in);
-        keep(inner || chooses, w2.rows.t, w2_in);
+        keep(inner, w2.rows.t, w2_in);
         node->keep(gate, gate_p != nullptr ? *gate_p : gate);
         keep(any, offsets, offsets_in);
         keep(any, order, order_in);
         keep(any, places, places_in);
-        keep(any, experts, experts_in);
-        keep(any, sorted, sorted);
-        keep(inner || chooses, z, z);
+        keep(inner || outer, weights, weights_in);
+        keep(inner, z, z);
         keep(outer, h, h);
         node->keep(sum, sum);
-        keep(chooses && b2 != nullptr, b2 != nullptr ? *b2 : Tensor(), b2 != nullptr ? *b2 : Tensor());
+        keep(chooses, y, y);
     }
     return out;
 }

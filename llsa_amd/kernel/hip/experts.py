@@ -52,8 +52,8 @@ def expert_feed_forward(x: torch.Tensor, routing: Routing, w_in: torch.Tensor, b
 
     x is (..., C), routing what route_tokens returned for logits (..., experts) of the same tokens, w_in (experts, F, C), b_in (experts, F), w_out (experts, N, F),
     b_out (experts, N), gate (B, N) for an x of (B, ..., C), residual (..., N); all but the routing bf16 or all fp16.  A token without an expert gets its residual.
-    Sums in fp32; the hidden rows, with their expert's weight, and each expert's result are rounded to that type, and so are what the backward keeps of the hidden rows, their
-    gradient and each expert's part of x's.  Differentiable in x, routing.weights, the weights and biases, gate and residual (once)."""
+    Sums in fp32; the hidden rows and each expert's result are rounded to that type, and so are what the backward keeps of the hidden rows, the gradients of either
+    and each expert's part of x's.  Differentiable in x, routing.weights, the weights and biases, gate and residual (once)."""
     lib = current_lib()
     weights, experts, order, offsets, places = routing
     return lib.host.expert_feed_forward(lib.host_library, x, weights, experts, order, offsets, places, w_in, b_in, w_out, b_out, _activation(activation), gate, residual)

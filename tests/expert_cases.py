@@ -153,9 +153,7 @@ def check_experts(x, routing, w_in, b_in, w_out, b_out, act, gate, residual, dou
     per_row = lambda t: t.repeat_interleave(M // x.shape[0], 0)
     gt = per_row(c(gate)) if gate is not None else torch.ones(1, 1, dtype=torch.float64, device=where)
     d = c(dout).reshape(M, N)
-    G, dG = d * gt, zero(M, N)
-    if gate is not None:
-        dG = E * G.abs() + u * G.abs() + lo
+    G = d * gt
     s, ds, size = zero(M, N), zero(M, N), zero(M, N)
     dx, ddx, dp, ddp = zero(M, C), zero(M, C), zero(M, k), zero(M, k)
     for e in range(n_experts):
@@ -168,33 +166,29 @@ def check_experts(x, routing, w_in, b_in, w_out, b_out, act, gate, residual, dou
         dz = (C + 4) * E * (xe.abs() @ w1.abs().t() + b1.abs())
         a = act64(act, z)
         da = SLOPE * dz + FAST * (a.abs() + z.abs())
-        h, dh = w * a, w * da + E * (w * a).abs()
-        dh = dh + u * (h.abs() + dh) + lo                     # (the hidden rows, with their weight, are rounded)
-        y = h @ w2.t() + w * b2
-        dy = dh @ w2.abs().t() + (F + 4) * E * (h.abs() @ w2.abs().t() + w * b2.abs())
+        h, dh = a, da + u * (a.abs() + da) + lo               # (the hidden rows are rounded)
+        y = h @ w2.t() + b2
+        dy = dh @ w2.abs().t() + (F + 4) * E * (h.abs() @ w2.abs().t() + b2.abs())
         dy = dy + u * (y.abs() + dy) + lo                     # (and so is each expert's result)
-        s.index_add_(0, tok, y)
-        ds.index_add_(0, tok, dy)
-        size.index_add_(0, tok, y.abs())
+        s.index_add_(0, tok, w * y)
+        ds.index_add_(0, tok, w * dy)
+        size.index_add_(0, tok, (w * y).abs())
         # backward
-        ge, dge = G[tok], dG[tok]
+        dp[tok, j] = (G[tok] * y).sum(1)
+        ddp[tok, j] = (G[tok].abs() * dy).sum(1) + more(N) * (G[tok] * y).abs().sum(1)
+        ge = w * G[tok]
+        dge = (2 * E + u) * ge.abs() + lo                     # (dout with weight and gate is rounded)
         t = ge @ w2
         dt = dge @ w2.abs() + more(N) * (ge.abs() @ w2.abs())
         zk = u * (z.abs() + dz) + lo                          # (z is kept in 16 bits)
-        dak = SLOPE * (dz + zk) + FAST * (a.abs() + z.abs())
-        dp[tok, j] = (a * t).sum(1) + ge @ b2
-        ddp[tok, j] = (dak * (t.abs() + dt) + a.abs() * dt).sum(1) + dge @ b2.abs() + more(F + N) * ((a * t).abs().sum(1) + ge.abs() @ b2.abs())
-        sl = slope64(act, z)
-        g = w * t * sl
-        dg = w * (dt * SLOPE + t.abs() * (CURVE * (dz + zk) + FAST)) + 2 * E * g.abs()
+        g = t * slope64(act, z)
+        dg = dt * SLOPE + t.abs() * (CURVE * (dz + zk) + FAST) + 2 * E * g.abs()
         dg = dg + u * (g.abs() + dg) + lo
         r = ge.t() @ h
         within(got["w_out"][e].to(where), r, (dge.t() @ (h.abs() + dh) + ge.abs().t() @ dh + more(n) * (ge.abs().t() @ h.abs())) * (1 + u) + u * r.abs() + lo, f"dw_out, expert {e}")
         if b_out is not None:
-            r = (w * ge).sum(0)
-            # (a weight in two parts of 16 bits)
-            b = (w * dge + (u * u * w + lo + more(2 * n) * w) * (ge.abs() + dge)).sum(0)
-            within(got["b_out"][e].to(where), r, b * (1 + u) + u * r.abs() + lo, f"db_out, expert {e}")
+            r = ge.sum(0)
+            within(got["b_out"][e].to(where), r, (dge.sum(0) + more(n) * ge.abs().sum(0)) * (1 + u) + u * r.abs() + lo, f"db_out, expert {e}")
         r = g.t() @ xe
         within(got["w_in"][e].to(where), r, (dg.t() @ xe.abs() + more(n) * (g.abs().t() @ xe.abs())) * (1 + u) + u * r.abs() + lo, f"dw_in, expert {e}")
         if b_in is not None:
