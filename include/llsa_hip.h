@@ -44,7 +44,7 @@ extern "C" {
 #define LLSA_DTYPE_F32 1
 #define LLSA_DTYPE_F16 2
 
-#define LLSA_ABI_VERSION 219     /* changes with every change of a signature or argument structure below */
+#define LLSA_ABI_VERSION 220     /* changes with every change of a signature or argument structure below */
 int llsa_version(void);          /* LLSA_ABI_VERSION of the built library                                    */
 const char* llsa_last_error_string(void);
 
@@ -463,6 +463,7 @@ int64_t llsa_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t per_sample, in
  *     out = residual + gate * act(q_scale[m] * w_scale[n] * sum over k of q[m,k] w[n,k] + bias[n])
  * x: bf16, fp16 or fp32; bias, gate, residual and out: bf16 or fp16. */
 #define LLSA_INT8_MAX_K 131072
+#define LLSA_INT8_DIRECT_ROWS 16
 typedef struct llsa_quantize_args {
     const void* x;          /* (rows,K) ldx apart                                                      */
     void* q;                /* (rows,K) ldq apart                                                      */
@@ -481,7 +482,8 @@ typedef struct llsa_int8_args {
     const void* gate;       /* (M/per_sample, N) rows s_gate apart, or NULL                            */
     const void* residual;   /* (M,N) ldr apart, or NULL                                                */
     void* out;              /* (M,N) ldo apart                                                         */
-    int64_t ldq, ldw, s_gate, ldr, ldo, M, per_sample;
+    const void* x;          /* unless NULL: (M,K) ldx apart of dtype in the place of q and q_scale, up to LLSA_INT8_DIRECT_ROWS rows, K a multiple of 16 */
+    int64_t ldq, ldw, s_gate, ldr, ldo, M, per_sample, ldx;
     int32_t N, K, act, dtype;
 } llsa_int8_args;
 int llsa_linear_int8(const llsa_int8_args* a, void* stream);

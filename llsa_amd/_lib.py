@@ -112,8 +112,8 @@ class QuantizeArgs(C.Structure):
 
 
 class Int8Args(C.Structure):
-    _fields_ = ([(n, c_void_p) for n in ("q", "w", "q_scale", "w_scale", "bias", "gate", "residual", "out")]
-                + [(n, c_int64) for n in ("ldq", "ldw", "s_gate", "ldr", "ldo", "M", "per_sample")]
+    _fields_ = ([(n, c_void_p) for n in ("q", "w", "q_scale", "w_scale", "bias", "gate", "residual", "out", "x")]
+                + [(n, c_int64) for n in ("ldq", "ldw", "s_gate", "ldr", "ldo", "M", "per_sample", "ldx")]
                 + [(n, c_int32) for n in ("N", "K", "act", "dtype")])
 
 
@@ -187,7 +187,7 @@ _SIGNATURES = {
 
 EXPORTS = tuple(_SIGNATURES)
 CHUNK_FINE_MAX = 256                                        # LLSA_CHUNK_FINE_MAX of include/llsa_hip.h
-ABI_VERSION = 219                                           # LLSA_ABI_VERSION
+ABI_VERSION = 220                                           # LLSA_ABI_VERSION
 STATIC_PARTIALS_MAX = 262144                                # LLSA_STATIC_PARTIALS_MAX
 
 

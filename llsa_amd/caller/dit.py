@@ -6,7 +6,10 @@ trainers/ddpm_trainer.py:97-103).  Plain torch modules around this package's ope
 attention, the qk RMS norms, the RoPE rotation and the Z-order permutation run in the HIP kernels,
 everything else (linear layers, layer norms, GELU, AdamW) is torch's; with fused_layers=True the layer
 norms, the linear layers and the feed-forward blocks are this package's too (layer_norm, linear,
-feed_forward: modulation, bias, activation, gate and residual in the same passes).
+feed_forward: modulation, bias, activation, gate and residual in the same passes).  With num_experts every
+block's feed-forward is a mixture of that many (route_tokens, expert_feed_forward), which the reference does
+not have; quantize_for_sampling() keeps the blocks' projections and feed-forward weights in 8-bit integers
+(linear_int8).
 
 The reference builds its model from diffusers classes, which are neither part of its checkout nor
 installed here; the layer shapes below follow the arguments it passes to them (biases on q/k/v and
@@ -23,8 +26,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..kernel.hip.experts import expert_feed_forward, route_tokens
 from ..kernel.hip.layer_norm import layer_norm
 from ..kernel.hip.linear import feed_forward, linear
+from ..kernel.hip.linear_int8 import linear_int8, quantize_rows
 from ..kernel.hip.permute import permute_tokens
 from ..kernel.hip.rms_norm import my_rms_norm_fn
 from ..kernel.hip.rope import my_rope_fn
@@ -47,6 +52,21 @@ def timestep_channels(t: torch.Tensor, channels: int = 256, max_period: float = 
 def of(layer: nn.Linear, dtype: torch.dtype):
     """(weight, bias) of a layer in the dtype of the activations, as autocast would cast them."""
     return layer.weight.to(dtype), None if layer.bias is None else layer.bias.to(dtype)
+
+
+def keep_in_8_bits(layer: nn.Linear) -> None:
+    """The layer's weight as whole numbers with a scale for each channel out, beside the weight itself; project() then takes these."""
+    q, scale = quantize_rows(layer.weight.detach())
+    layer.register_buffer("weight_q", q, persistent=False)
+    layer.register_buffer("weight_scale", scale, persistent=False)
+
+
+def project(layer: nn.Linear, x: torch.Tensor, rows=None, **epilogue) -> torch.Tensor:
+    """The layer by this package's operators.  rows: x as quantize_rows gives it, for layers that share it."""
+    if hasattr(layer, "weight_q"):
+        bias = None if layer.bias is None else layer.bias.to(x.dtype)
+        return linear_int8(x if rows is None else rows, layer.weight_q, layer.weight_scale, bias, dtype=x.dtype, **epilogue)
+    return linear(x, *of(layer, x.dtype), **epilogue)
 
 
 class TimestepEmbedding(nn.Module):
@@ -115,8 +135,8 @@ class LlsaSelfAttention(nn.Module):
                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         B, N, _ = x.shape
         split = lambda y: y.view(B, N, self.heads, self.head_dim).transpose(1, 2)
-        project = (lambda layer: linear(x, *of(layer, x.dtype))) if self.fused_layers else (lambda layer: layer(x))
-        q, k, v = split(project(self.to_q)), split(project(self.to_k)), split(project(self.to_v))
+        rows = quantize_rows(x) if self.fused_layers and hasattr(self.to_q, "weight_q") else None
+        q, k, v = (split(project(layer, x, rows) if self.fused_layers else layer(x)) for layer in (self.to_q, self.to_k, self.to_v))
         norm = None
         if self.norm_q_weight is not None:
             norm = (self.norm_q_weight.float(), self.norm_k_weight.float(), self.eps)
@@ -135,29 +155,56 @@ class LlsaSelfAttention(nn.Module):
             o = llsa_l3(q, k, v, tk[-1], tk[-2], tk[-3], self.block_size, rope=rope, qk_norm=norm)
         o = o.transpose(1, 2).reshape(B, N, self.heads * self.head_dim)
         if self.fused_layers:
-            return linear(o, *of(self.to_out, o.dtype), gate=gate, residual=residual)
+            return project(self.to_out, o, gate=gate, residual=residual)
         o = self.to_out(o)
         if gate is not None:
             o = gate.unsqueeze(1) * o
         return o if residual is None else o + residual
 
 
+class Experts(nn.Module):
+    """A feed-forward block for each of num_experts, of which every token takes experts_per_token."""
+
+    def __init__(self, dim: int, hidden: int, num_experts: int, experts_per_token: int):
+        super().__init__()
+        self.experts_per_token = experts_per_token
+        self.router = nn.Linear(dim, num_experts, bias=False)
+        one = lambda n, k: nn.Parameter((torch.rand(num_experts, n, k) * 2 - 1) / math.sqrt(k))
+        self.w_in, self.w_out = one(hidden, dim), one(dim, hidden)
+        self.b_in, self.b_out = nn.Parameter(torch.zeros(num_experts, hidden)), nn.Parameter(torch.zeros(num_experts, dim))
+
+    def forward(self, x, gate, residual):
+        routing = route_tokens(linear(x, self.router.weight.to(x.dtype)), self.experts_per_token)
+        w = [p.to(x.dtype) for p in (self.w_in, self.b_in, self.w_out, self.b_out)]
+        return expert_feed_forward(x, routing, *w, activation="gelu_tanh", gate=gate, residual=residual)
+
+
 class RopeTransformerBlock(nn.Module):
     """:581-711 with norm_type 'ada_norm_zero' and no cross attention."""
 
-    def __init__(self, dim: int, heads: int, head_dim: int, fused_layers: bool = False, **attn):
+    def __init__(self, dim: int, heads: int, head_dim: int, fused_layers: bool = False, num_experts: int = 0, experts_per_token: int = 2, **attn):
         super().__init__()
+        if num_experts and not fused_layers:
+            raise ValueError("num_experts needs fused_layers=True")
         self.fused_layers = fused_layers
         self.norm1 = AdaLayerNormZero(dim, fused_layers)
         self.attn1 = LlsaSelfAttention(dim, heads, head_dim, fused_layers=fused_layers, **attn)
         self.norm3 = nn.LayerNorm(dim, eps=1e-5, elementwise_affine=False)
-        self.ff_in, self.ff_out = nn.Linear(dim, 4 * dim), nn.Linear(4 * dim, dim)
+        if num_experts:
+            self.experts = Experts(dim, 4 * dim, num_experts, experts_per_token)
+        else:
+            self.ff_in, self.ff_out = nn.Linear(dim, 4 * dim), nn.Linear(4 * dim, dim)
+        self.num_experts = num_experts
 
     def forward(self, x, t, freq):
         h, gate_msa, shift_mlp, scale_mlp, gate_mlp = self.norm1(x, t)
         x = self.attn1(h, freq, gate_msa, x)
         if self.fused_layers:
             h = layer_norm(x, scale=scale_mlp, shift=shift_mlp, eps=self.norm3.eps)
+            if self.num_experts:
+                return self.experts(h, gate_mlp, x)
+            if hasattr(self.ff_in, "weight_q"):
+                return project(self.ff_out, project(self.ff_in, h, activation="gelu_tanh"), gate=gate_mlp, residual=x)
             return feed_forward(h, *of(self.ff_in, h.dtype), *of(self.ff_out, h.dtype), activation="gelu_tanh", gate=gate_mlp, residual=x)
         h = self.norm3(x) * (1 + scale_mlp[:, None]) + shift_mlp[:, None]
         return gate_mlp.unsqueeze(1) * self.ff_out(F.gelu(self.ff_in(h), approximate="tanh")) + x
@@ -168,11 +215,13 @@ class PixelDiT(nn.Module):
     are configs/models/model_rope_dit_S_128_rms_llsa_l2.json (that file's sparse_topk is 8; the
     benchmark configuration uses 16).  fused_layers: layer norms, linear layers and feed-forward blocks
     by this package's operators, whose activations are bf16 or fp16 (autocast, or a model in that
-    dtype); the parameters are the same."""
+    dtype); the parameters are the same.  num_experts (with fused_layers): a mixture of that many feed-forward
+    blocks in each, of which a token takes experts_per_token."""
 
     def __init__(self, num_attention_heads: int = 6, attention_head_dim: int = 64, num_layers: int = 12, in_channels: int = 3,
                  out_channels: int = 3, sample_size: int = 128, axes_dims_rope: Sequence[int] = (32, 32), levels: int = 2,
-                 sparse_topk=16, qk_norm: bool = True, fused_prologue: bool = True, fused_layers: bool = False):
+                 sparse_topk=16, qk_norm: bool = True, fused_prologue: bool = True, fused_layers: bool = False, num_experts: int = 0,
+                 experts_per_token: int = 2):
         super().__init__()
         self.fused_layers = fused_layers
         dim = num_attention_heads * attention_head_dim
@@ -182,7 +231,8 @@ class PixelDiT(nn.Module):
         self.proj_in = nn.Conv2d(in_channels, dim, kernel_size=1)
         self.transformer_blocks = nn.ModuleList(
             RopeTransformerBlock(dim, num_attention_heads, attention_head_dim, levels=levels, sparse_topk=sparse_topk,
-                                 qk_norm=qk_norm, fused_prologue=fused_prologue, fused_layers=fused_layers) for _ in range(num_layers))
+                                 qk_norm=qk_norm, fused_prologue=fused_prologue, fused_layers=fused_layers, num_experts=num_experts,
+                                 experts_per_token=experts_per_token) for _ in range(num_layers))
         self.norm_out = nn.LayerNorm(dim, elementwise_affine=False, eps=1e-6)
         self.proj_out_1 = nn.Linear(dim, 2 * dim)
         self.proj_out_2 = nn.Linear(dim, out_channels)
@@ -191,6 +241,17 @@ class PixelDiT(nn.Module):
         self.register_buffer("fwd_perm", inv.to(torch.int32), persistent=False)      # raster -> Z-order
         # the table is kept in Z-order and in bf16, as register_rope_emb builds it (:153-173)
         self.register_buffer("freq", rope_table(sample_size, tuple(axes_dims_rope), dtype=torch.bfloat16), persistent=False)
+
+    def quantize_for_sampling(self) -> "PixelDiT":
+        """Keeps the blocks' projections and feed-forward weights (not an experts') as 8-bit integers, which the forward then multiplies with; call it
+        again after the weights have changed.  The model gives no gradients from then on: sample under torch.no_grad()."""
+        if not self.fused_layers:
+            raise ValueError("quantize_for_sampling needs fused_layers=True")
+        for block in self.transformer_blocks:
+            a = block.attn1
+            for layer in [a.to_q, a.to_k, a.to_v, a.to_out] + ([] if block.num_experts else [block.ff_in, block.ff_out]):
+                keep_in_8_bits(layer)
+        return self
 
     def forward(self, images: torch.Tensor, timestep: torch.Tensor) -> torch.Tensor:
         B, _, Hh, Ww = images.shape

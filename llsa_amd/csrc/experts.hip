@@ -624,44 +624,71 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(c
         __syncthreads();                                      // (everyone is done with what the next one's copies overwrite)
     }
 }
-// The sums of an expert's chunks added up, by four waves of which each takes every fourth of the same 64 places (of four elements); nothing to do where there was one.
+// The sums of the experts that are more than one chunk's, or none's, added up, and those of all experts' rows.  `ways` waves take every so many-th chunk of the
+// same places (of four elements): with few places a thread would wait for one chunk after another.
 template <typename T>
-__global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<T> a, int blocks) {
+__global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<T> a, int ways) {
     __shared__ f32x4 rest[3][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, expert = (int)blockIdx.x / blocks;
-    Runs runs;
-    runs.load(a.offsets, a.experts, a.rows, a.chunk, false, lane);
-    Piece p = {0, 0, 0, 0, 0};
+    __shared__ int first[LLSA_MAX_EXPERTS], chunks[LLSA_MAX_EXPERTS], cut[LLSA_MAX_EXPERTS], cuts;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    {
+        Runs runs;
+        runs.load(a.offsets, a.experts, a.rows, a.chunk, false, lane);
+        if (wave == 0) {
+            int n = 0;
 #pragma unroll
-    for (int i = 0; i < Runs::kLanes; i++)
-        if (expert / 64 == i) p = runs.of_expert(i, expert % 64);
-    const int chunk0 = p.begin / a.chunk, chunks = p.end > p.begin ? (p.end - 1) / a.chunk - chunk0 + 1 : 0, first = chunk0 + expert;
-    const int64_t n4 = a.ld_part / 4, places = a.M * n4 + (a.part_sum != nullptr ? a.M : 0), skipped = chunks == 1 ? a.M * n4 / 64 * 64 : 0;
-    for (int64_t i = skipped + (int64_t)((int)blockIdx.x - expert * blocks) * 64 + lane; i - lane < places; i += 64 * blocks) {
-        const bool sum = i >= a.M * n4;                       // of the rows
-        const int64_t m = sum ? i - a.M * n4 : i / n4;
-        const int n = sum ? 0 : (int)(i - m * n4) * 4;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (!sum && chunks != 1) {
-#pragma unroll 8
-            for (int s = wave; s < chunks; s += 4) v += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)(first + s) * a.M + m) * a.ld_part + n);
-        } else if (sum && i < places) {
-            for (int s = wave; s < chunks * a.tiles_n; s += 4) v[0] += a.part_sum[((int64_t)first * a.tiles_n + s) * a.M + m];
+            for (int i = 0; i < Runs::kLanes; i++) {
+                const int e = 64 * i + lane, c0 = runs.begin[i] / a.chunk, c = runs.end[i] > runs.begin[i] ? (runs.end[i] - 1) / a.chunk - c0 + 1 : 0;
+                const bool joins = e < a.experts && c != 1;
+                const uint64_t all = __ballot(joins);
+                if (e < a.experts) {
+                    first[e] = c0 + e;
+                    chunks[e] = c;
+                }
+                if (joins) cut[n + __popcll((unsigned long long)(all & (((uint64_t)1 << lane) - 1)))] = e;
+                n += __popcll((unsigned long long)all);
+            }
+            if (lane == 0) cuts = n;
         }
+    }
+    __syncthreads();
+    const int n4 = (int)(a.ld_part / 4), of_one = a.M * n4, at_once = 256 / ways, part = ways == 1 ? 0 : wave, mine = ways == 1 ? tid : lane, blocks = (of_one + at_once - 1) / at_once;
+    auto join = [&](f32x4 v) {
+        if (ways == 1) return v;
         if (wave > 0) rest[wave - 1][lane] = v;
         __syncthreads();
         if (wave == 0) {
 #pragma unroll
-            for (int r = 0; r < 3; r++) v += rest[r][lane];
-            if (!sum && chunks != 1) {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (n + e < a.N) a.out[((int64_t)expert * a.M + m) * a.N + n + e] = (T)v[e];
-            } else if (sum && i < places) {
-                a.sums[(int64_t)expert * a.M + m] = (T)v[0];
-            }
+            for (int w = 0; w < 3; w++) v += rest[w][lane];
         }
         __syncthreads();
+        return v;
+    };
+    for (int c = 0, turn = 0; c < cuts; c++) {
+        const int e = cut[c], from = first[e], count = chunks[e];
+        // (each expert's places begin at another workgroup)
+        for (int block = (int)((blockIdx.x + gridDim.x - (unsigned)turn) % gridDim.x); block < blocks; block += gridDim.x) {
+            const int i = block * at_once + mine, m = min(i, of_one - 1) / n4, n = (min(i, of_one - 1) - m * n4) * 4;
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+            for (int s = part; s < count; s += ways) v += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)(from + s) * a.M + m) * a.ld_part + n);
+            v = join(v);
+            if (part > 0 || i >= of_one) continue;
+            T* const out = a.out + ((int64_t)e * a.M + m) * a.N + n;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (n + k < a.N) out[k] = (T)v[k];
+        }
+        turn = (turn + blocks) % (int)gridDim.x;
+    }
+    if (a.part_sum == nullptr) return;
+    const int rows = a.experts * a.M;
+    for (int i0 = (int)blockIdx.x * at_once; i0 < rows; i0 += (int)gridDim.x * at_once) {
+        const int i = min(i0 + mine, rows - 1), e = i / a.M, m = i - e * a.M;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int s = part; s < chunks[e] * a.tiles_n; s += ways) v[0] += a.part_sum[((int64_t)first[e] * a.tiles_n + s) * a.M + m];
+        v = join(v);
+        if (part == 0 && i0 + mine < rows) a.sums[i] = (T)v[0];
     }
 }
 
@@ -770,14 +797,20 @@ __global__ __launch_bounds__(256) void dweights_kernel(const DWeights<T> a) {
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = e >= left ? 0.f : a.gate != nullptr ? (float)d[e] * (float)g[e] : (float)d[e];
 #pragma unroll
-        for (int j = 0; j < LLSA_MAX_CHOICES; j++)
-            if (j < a.k) {
-                const int p = a.places[m * a.k + j];
-                if ((unsigned)p < (unsigned)a.rows) {
-                    const vec8<T> y = *reinterpret_cast<const vec8<T>*>(a.y + p * a.ldy + n);
+        for (int j0 = 0; j0 < LLSA_MAX_CHOICES; j0 += 2)
+            if (j0 < a.k) {                                   // (two at a time, their loads in flight together)
+                vec8<T> y[2];
+                bool there[2];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) v[j] = fmaf(x[e], e >= left ? 0.f : (float)y[e], v[j]);
+                for (int h = 0; h < 2; h++) {
+                    const int p = a.places[m * a.k + min(j0 + h, a.k - 1)];
+                    there[h] = (unsigned)p < (unsigned)a.rows;
+                    y[h] = *reinterpret_cast<const vec8<T>*>(a.y + (there[h] ? p : 0) * a.ldy + n);
                 }
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[j0 + h] = fmaf(x[e], e >= left || !there[h] ? 0.f : (float)y[h][e], v[j0 + h]);
             }
     }
 #pragma unroll
@@ -808,14 +841,19 @@ bool resident(int64_t rows, int64_t experts, int64_t N, int64_t K) {
     return rows >= 8 * kResRows * experts && rows >= 8 * kResRows * slots;
 }
 // Which tiles: few rows for each expert on the average, small tiles while there are few of them for each CU, large ones where the experts fill them
-enum GroupedTiles { kFew16, kFew32, kFew64, k64, k128, k256, kResident };
-GroupedTiles grouped_tiles(int64_t rows, int64_t experts, int64_t N, int64_t K) {
+enum GroupedTiles { kFew16, kFew32, kFew64, k64, k128, k192, k256, kResident };
+GroupedTiles grouped_tiles(int64_t rows, int64_t experts, int64_t N, int64_t K, bool dx, bool slope) {
     const int64_t each = ceil_div(rows, experts);
     if (each <= 64 || (rows / 64 + experts) * ceil_div(N, kFewColumns) <= kCus) return each <= 12 ? kFew16 : each <= 28 ? kFew32 : kFew64;
     if (resident(rows, experts, N, K)) return kResident;
     if ((rows / 64 + experts) * ceil_div(N, 64) <= 4 * kCus) return k64;
-    if (each >= 1024 && N >= 512 && K >= 1024 && (rows / 256 + experts) * ceil_div(N, 256) >= 2 * kCus) return k256;
-    return k128;
+    // beyond, by linear.hip's lengths of a round, with half a tile more for each expert
+    const auto rounds = [&](int bm, int bn, int slots) {
+        const double n = ((double)rows / bm + 0.5 * (double)experts) * (double)ceil_div(N, bn) / slots;
+        return n > 4 ? n + 0.5 : std::ceil(n);
+    };
+    const double t128 = rounds(128, 128, 2 * kCus), t192 = (dx ? 1.38 : 1.3) * rounds(192, 128, 2 * kCus), t256 = slope ? 1e30 : (dx ? 1.8 : 1.8 + 220. / (double)K) * rounds(256, 256, kCus);
+    return t256 < std::min(t128, t192) ? k256 : t192 < t128 ? k192 : k128;      // (with act'(z) besides, 256 x 256 does not fit the registers)
 }
 template <typename T, bool YC, bool GATHERED, int BM, int BN, int WAVES_M, int WAVES_N, int ACT>
 int launch_grouped_tiles(Grouped<T>& a, hipStream_t stream) {
@@ -861,17 +899,18 @@ int launch_grouped_resident(Grouped<T>& a, hipStream_t stream) {
 template <typename T, bool YC, int ACT>
 int launch_grouped(Grouped<T>& a, hipStream_t stream) {
     a.group = (int64_t)a.N * a.K <= (1 << 20) ? 1 : 8;        // (rows of tiles that share y while it does not fit the L2 beside them)
-    const GroupedTiles t = grouped_tiles(a.rows, a.experts, a.N, a.K);
+    const GroupedTiles t = grouped_tiles(a.rows, a.experts, a.N, a.K, YC, YC && ACT != LLSA_ACT_NONE);
     switch (t) {
         case kFew16: return launch_grouped_few<T, YC, 1, ACT>(a, stream);
         case kFew32: return launch_grouped_few<T, YC, 2, ACT>(a, stream);
         case kFew64: return launch_grouped_few<T, YC, 4, ACT>(a, stream);
         case k64: return launch_grouped_64<T, YC, ACT>(a, stream);
         case k128: return launch_grouped_tiles<T, YC, false, 128, 128, 2, 2, ACT>(a, stream);
+        case k192: return launch_grouped_tiles<T, YC, false, 192, 128, 2, 2, ACT>(a, stream);
         case kResident: return a.K == 5 * kStep ? launch_grouped_resident<T, YC, ACT, 5>(a, stream) : launch_grouped_resident<T, YC, ACT, 6>(a, stream);
         default:
             if constexpr (!YC || ACT == LLSA_ACT_NONE) return launch_grouped_tiles<T, YC, false, 256, 256, 2, 4, ACT>(a, stream);
-            else return launch_grouped_tiles<T, YC, false, 128, 128, 2, 2, ACT>(a, stream);      // (with act'(z) besides, 256 x 256 does not fit the registers)
+            else return fail(-1, "experts: no such tiles");
     }
 }
 template <typename T, bool YC>
@@ -955,9 +994,9 @@ int experts_dw(const llsa_experts_args& q, hipStream_t stream) {
     const bool small = small_tiles(q.rows, q.N, q.K);
     const int rc = small ? launch_grouped_dw<T, 64, 64>(a, stream) : grouped_rows(a.M) == 192 ? launch_grouped_dw<T, 192, 128>(a, stream) : launch_grouped_dw<T, 128, 128>(a, stream);
     if (rc != 0) return rc;
-    // (as many workgroups as the chip holds: most experts have one piece, and nothing to add up)
-    const int64_t places = (int64_t)a.M * (a.ld_part / 4) + (q.dbias != nullptr ? a.M : 0), blocks = std::min(ceil_div(places, 64), ceil_div(8 * kCus, q.E));
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(grouped_join_kernel<T>), dim3((unsigned)(blocks * q.E)), dim3(256), 0, stream, a, (int)blocks);
+    const int64_t places = (int64_t)a.M * (a.ld_part / 4) * std::min<int64_t>(q.E, ceil_div(q.rows, a.chunk) + 1);
+    const int ways = ceil_div(q.rows, a.chunk) >= 2 * q.E ? 4 : 1;       // (three chunks of an expert on the average)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(grouped_join_kernel<T>), dim3((unsigned)std::min<int64_t>(8 * kCus, ceil_div(places, 256 / ways))), dim3(256), 0, stream, a, ways);
     return launch_status("experts_dw");
 }
 template <typename T>
@@ -1021,7 +1060,7 @@ extern "C" int64_t llsa_experts_dw_workspace_bytes(int64_t rows, int E, int N, i
     if (rows <= 0 || E <= 0 || N <= 0 || K <= 0) return 0;
     return 4 * part_count(rows, E, N, K) * N * (pad8(K) + ceil_div(K, 64));
 }
-extern "C" int llsa_experts_gathers(int64_t rows, int E, int N, int K) { return rows > 0 && E > 0 && N > 0 && K > 0 && grouped_tiles(rows, E, N, K) <= k64; }
+extern "C" int llsa_experts_gathers(int64_t rows, int E, int N, int K) { return rows > 0 && E > 0 && N > 0 && K > 0 && grouped_tiles(rows, E, N, K, false, false) <= k64; }
 extern "C" int llsa_experts_gather(const llsa_experts_args* a, void* stream) {
     if (int rc = check_experts("experts_gather", a)) return rc;
     if (a->rows == 0) return 0;
@@ -1050,6 +1089,7 @@ extern "C" int llsa_experts_dx(const llsa_experts_args* a, void* stream) {
 extern "C" int llsa_experts_dw(const llsa_experts_args* a, void* stream) {
     if (int rc = check_experts("experts_dw", a)) return rc;
     LLSA_REQUIRE(a->rows > 0, "experts_dw: no rows");
+    LLSA_REQUIRE((int64_t)a->N * pad8(a->K) < (int64_t(1) << 31) && (int64_t)a->E * a->N < (int64_t(1) << 31), "experts_dw: too many weights of an expert");
     LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->x, a->ldx) && a->lddz >= pad8(a->N) && a->ldx >= pad8(a->K), "experts_dw: rows of dz and x must be 16-byte aligned and padded to a multiple of 8");
     LLSA_REQUIRE(a->out != nullptr && a->workspace != nullptr && aligned16(a->workspace), "experts_dw: output and workspace (16-byte aligned)");
     return BY_TYPE(experts_dw);

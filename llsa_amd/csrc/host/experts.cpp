@@ -96,6 +96,7 @@ void check_expert_weight(const char* what, const char* name, const Tensor& w, in
                                   (in >= 0 ? std::to_string(in) : std::string("channels in")) + ") (got " + text_of(w.sizes()) + ")");
     if (w.size(0) > LLSA_MAX_EXPERTS) fail(Failure::kNotImplemented, std::string(what) + " takes at most " + std::to_string(LLSA_MAX_EXPERTS) + " experts (got " + std::to_string(w.size(0)) + ")");
     if (w.size(1) >= (1 << 23) || w.size(2) >= (1 << 23)) fail(Failure::kValue, std::string(what) + ": too many channels");
+    if (w.size(1) * pad8(w.size(2)) >= (int64_t(1) << 31)) fail(Failure::kValue, std::string(what) + ": too many weights of an expert");
     if (w.size(0) * w.size(1) >= (int64_t(1) << 31)) fail(Failure::kValue, std::string(what) + ": too many channels of all experts");
 }
 void check_ints(const char* what, const char* name, const Tensor& t, at::IntArrayRef sizes) {

@@ -105,11 +105,16 @@ Tensor linear_int8(const std::shared_ptr<Library>& lib, const Tensor& x_in, cons
     const Rows w = integers(w_in, q, copied);
     Rows x, from;
     Tensor scale;
+    bool direct = false;
     if (xs != nullptr) {
         x = integers(x_in, q, copied);
         scale = in_memory(*xs).contiguous();
     } else {
         from = rows_of(x_in);
+        // few rows: in one launch with the product, where nothing has to be copied
+        direct = q.pads == 0 && from.count <= LLSA_INT8_DIRECT_ROWS && K % 16 == 0 && aligned(from.t) && from.ld % 8 == 0 && from.ld <= (int64_t(1) << 23);
+    }
+    if (xs == nullptr && !direct) {
         x.t = at::empty({from.count, pad16(K)}, x_in.options().dtype(at::kChar));
         x.ld = pad16(K); x.count = from.count; x.cols = K;
         scale = at::empty({from.count}, x_in.options().dtype(at::kFloat));
@@ -119,7 +124,8 @@ Tensor linear_int8(const std::shared_ptr<Library>& lib, const Tensor& x_in, cons
     const Tensor w_scale = in_memory(w_scale_in).contiguous(), b = dense_vector(bias), gate = dense_vector(gate_p);
     const Rows residual = call.addend(residual_p);
     llsa_int8_args a{};
-    a.q = x.p(); a.ldq = x.ld; a.q_scale = scale.data_ptr<float>();
+    if (direct) { a.x = from.p(); a.ldx = from.ld; }
+    else { a.q = x.p(); a.ldq = x.ld; a.q_scale = scale.data_ptr<float>(); }
     a.w = w.p(); a.ldw = w.ld; a.w_scale = w_scale.data_ptr<float>();
     if (b.defined()) a.bias = b.data_ptr();
     if (gate.defined()) { a.gate = gate.data_ptr(); a.s_gate = gate.size(0) > 1 ? gate.stride(0) : 0; }

@@ -62,6 +62,29 @@ __device__ __forceinline__ int nearest(float x, float s, float inverse, float ha
     return (int)fmaxf(-127.f, fminf(127.f, q));
 }
 
+// A row's scale, out of its largest value's bits; NaN where that is no number
+template <typename T>
+__device__ __forceinline__ float step_of(unsigned top) {
+    typedef typename Bits<T>::type B;
+    const B bits = (B)top;
+    T value;
+    __builtin_memcpy(&value, &bits, sizeof(B));
+    return top < Bits<T>::kInf ? (float)value / 127.f : __uint_as_float(0x7fc00000u);
+}
+// What a row's elements are divided by.  (Steps near the least numbers are multiplied by a power of two beforehand: their inverse would be an infinity.)
+struct Steps { float lift, step, inverse, half; bool zero; };
+__device__ __forceinline__ Steps steps_for(float s) {
+    Steps t;
+    t.zero = !(s > 0.f);
+    t.lift = s < 0x1p-60f ? 0x1p80f : 1.f;
+    t.step = t.zero ? 1.f : s * t.lift;
+    t.inverse = __builtin_amdgcn_rcpf(t.step);
+    t.half = 0.5f * t.step;
+    return t;
+}
+template <typename T>
+__device__ __forceinline__ int8_t whole_number(T x, const Steps& t) { return (int8_t)(t.zero ? 0 : nearest((float)x * t.lift, t.step, t.inverse, t.half)); }
+
 // LANES lanes hold a row, PIECES pieces of 8 elements each; longer rows (256 lanes only) are read a second time.  Bound by memory.
 template <typename T, int LANES, int PIECES>
 __global__ __launch_bounds__(256) void quantize_kernel(const Quantize a) {
@@ -128,17 +151,9 @@ __global__ __launch_bounds__(256) void quantize_kernel(const Quantize a) {
         top = max_moved(max_moved(most[0], most[1]), max_moved(most[2], most[3]));
     }
     if (!there) return;
-    const bool finite = top < Bits<T>::kInf;
-    const B top_bits = (B)top;
-    T top_value;
-    __builtin_memcpy(&top_value, &top_bits, sizeof(B));
-    float s = finite ? (float)top_value / 127.f : __uint_as_float(0x7fc00000u);
+    const float s = step_of<T>(top);
     if (lane == 0) a.scale[row] = s;
-    // (steps near the least numbers are multiplied by a power of two beforehand: their inverse would be an infinity)
-    const float lift = s < 0x1p-60f ? 0x1p80f : 1.f;
-    const bool zero = !finite || top == 0;
-    s = zero ? 1.f : s * lift;
-    const float inverse = __builtin_amdgcn_rcpf(s), half = 0.5f * s;
+    const Steps st = steps_for(s);
     for (int run = 0; run < runs; run++) {
         if (runs > 1) read(run);
 #pragma unroll
@@ -146,7 +161,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const Quantize a) {
             const int c = ((run * PIECES + i) * LANES + lane) * 8;
             union { int8_t b[8]; u32x2 w; } o;
 #pragma unroll
-            for (int e = 0; e < 8; e++) o.b[e] = (int8_t)(zero ? 0 : nearest((float)v[i][e] * lift, s, inverse, half));
+            for (int e = 0; e < 8; e++) o.b[e] = whole_number(v[i][e], st);
             int8_t* const q = a.q + row * a.ldq + c;
             if (a.wide_q) {
                 if (c < (a.K + 15) / 16 * 16) *reinterpret_cast<u32x2*>(q) = o.w;
@@ -184,17 +199,27 @@ struct Product8 {
 
 // Eight values of a row: columns n .. n + 7, `left` of them inside the matrix
 template <int WAY, typename T>
-__device__ __forceinline__ void way_out8(const Product8<T>& a, const int (&sum)[8], float sx, const float (&sy)[8], const vec8<T>& bias, const vec8<T>& gate, const vec8<T>& side,
-                                         T* to, int left) {
+__device__ __forceinline__ vec8<T> way_out8(const Product8<T>& a, const int (&sum)[8], float sx, const float (&sy)[8], const vec8<T>& bias, const vec8<T>& gate, const vec8<T>& side) {
     const int act = WAY < 0 ? a.act : WAY;
-    float v[8];
+    vec8<T> o;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        v[e] = activate(act, (float)sum[e] * sx * sy[e] + (float)bias[e]);       // (the scales one after another: their product may be out of range)
-        if (a.gate != nullptr) v[e] *= (float)gate[e];
-        if (a.residual != nullptr) v[e] += (float)side[e];
+        float v = activate(act, (float)sum[e] * sx * sy[e] + (float)bias[e]);       // (the scales one after another: their product may be out of range)
+        if (a.gate != nullptr) v *= (float)gate[e];
+        if (a.residual != nullptr) v += (float)side[e];
+        o[e] = (T)v;
     }
-    store8(to, v, WAY >= 0 || (a.wide_out && left >= 8), left);
+    return o;
+}
+template <typename T>
+__device__ __forceinline__ void put8(T* to, const vec8<T>& o, bool wide, int left) {
+    if (wide) {
+        *reinterpret_cast<vec8<T>*>(to) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < left) to[e] = o[e];
+    }
 }
 template <typename T>
 __device__ __forceinline__ void scales8(float (&v)[8], const float* p, bool wide, int n) {
@@ -264,34 +289,82 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product8_kernel(con
     }
     wait_vm0();
     __syncthreads();
-    multiply((steps - 1) & 1);
 
-    // Lane l holds columns 4 (l/16) .. +3 of every 16, of row l%16; swapped between sixteens of lanes, a pair of tiles gives it eight neighbouring ones.
-    const int lane_row = lane & 15, lane_col = 16 * (quad & 1) + 8 * (quad >> 1), row0 = m0 + wm + lane_row, col0 = n0 + wn + lane_col;
+    // Lane l holds columns 4 (l/16) .. +3 of every 16, of row l%16; swapped between sixteens of lanes, a pair of tiles gives it eight neighbouring ones, and
+    // where the tile is whole two pairs leave as whole lines (linear.hip).  The residual is on its way during the last step's products.
+    const int lane_row = lane & 15, lane_col = 16 * (quad & 1) + 8 * (quad >> 1), row0 = m0 + wm, col0 = n0 + wn, rows_left = a.M - row0 - lane_row, cols_left = a.N - col0 - lane_col;
+    const unsigned at_out = (unsigned)(lane_row * a.ldo) + lane_col, at_side = (unsigned)(lane_row * a.ldr) + lane_col;
+    constexpr int kPair = NT % 4 == 0 ? 2 : 1;
+    const bool whole = kPair == 2 && WAY >= 0 && m0 + BM <= a.M && n0 + BN <= a.N;
+    constexpr bool kAhead = BM * BN < 256 * 256;              // (256 x 256 leave no registers for it: row by row)
+    constexpr int kEarly = kAhead ? MT : 1;
+    vec8<T> early[kPair][kEarly];
+    auto read_side = [&](int p0, int first) {
+        if (WAY < 0 || a.residual == nullptr) return;
+        if constexpr (kPair == 2) {
+            if (whole) {
+#pragma unroll
+                for (int i = 0, j = first; i < kEarly; i++, j++)
+                    request_lines(early[0][i], early[1][i], a.residual + ((int64_t)(row0 + 16 * j) * a.ldr + (col0 + 32 * p0)), at_side, (unsigned)(8 * a.ldr), lane);
+                return;
+            }
+        }
+#pragma unroll
+        for (int i = 0, j = first; i < kEarly; i++, j++)
+#pragma unroll
+            for (int h = 0; h < kPair; h++)
+                if (16 * j < rows_left && 32 * (p0 + h) < cols_left)
+                    early[h][i] = *reinterpret_cast<const vec8<T>*>(a.residual + ((int64_t)(row0 + 16 * j) * a.ldr + (col0 + 32 * (p0 + h))) + at_side);
+    };
+    if (kAhead) read_side(0, 0);
     float sx[MT];
 #pragma unroll
-    for (int j = 0; j < MT; j++) sx[j] = a.x_scale[min(row0 + 16 * j, a.M - 1)];
+    for (int j = 0; j < MT; j++) sx[j] = a.x_scale[min(row0 + lane_row + 16 * j, a.M - 1)];
+    multiply((steps - 1) & 1);
+    const int sample = a.gate != nullptr ? m0 / a.per_sample : 0;
+    const bool one_sample = a.gate != nullptr && min(m0 + BM, a.M) <= (int64_t)(sample + 1) * a.per_sample;
 #pragma unroll
-    for (int p = 0; p < NT / 2; p++) {
-        const int n = col0 + 32 * p, left = a.N - n;
-        float sy[8];
-        if (left > 0) scales8<T>(sy, a.y_scale + n, a.wide, left);
-        const vec8<T> bias = take8(a.bias != nullptr && left > 0 ? a.bias + n : nullptr, a.wide, left);
+    for (int p0 = 0; p0 < NT / 2; p0 += kPair) {
+        vec8<T> bias[kPair], gate[kPair];
+        float sy[kPair][8];
+#pragma unroll
+        for (int h = 0; h < kPair; h++) {
+            const int n = col0 + lane_col + 32 * (p0 + h), left = cols_left - 32 * (p0 + h);
+            if (left > 0) scales8<T>(sy[h], a.y_scale + n, a.wide, left);
+            bias[h] = take8(a.bias != nullptr && left > 0 ? a.bias + n : nullptr, a.wide, left);
+            gate[h] = take8(one_sample && left > 0 ? a.gate + sample * a.s_gate + n : nullptr, a.wide, left);
+        }
 #pragma unroll
         for (int j = 0; j < MT; j++) {
-            const int m = row0 + 16 * j;
-            int v[8];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const u32x2 w = __builtin_amdgcn_permlane16_swap((unsigned)acc[2 * p][j][e], (unsigned)acc[2 * p + 1][j][e], false, false);
-                v[e] = (int)w[0];
-                v[4 + e] = (int)w[1];
+            const int64_t row = row0 + 16 * j;
+            vec8<T> o[kPair];
+            const int i = kAhead ? j : 0;
+            if (!kAhead) read_side(p0, j);
+            if constexpr (kPair == 2) {
+                if (whole && a.residual != nullptr) arrange_lines<T>(early[0][i], early[1][i], lane);
             }
-            if (m >= a.M || left <= 0) continue;              // (not before the swap, which takes all lanes)
-            const vec8<T> gate = take8(a.gate != nullptr ? a.gate + m / a.per_sample * a.s_gate + n : nullptr, a.wide, left);
-            const vec8<T> side = take8(a.residual != nullptr ? a.residual + (int64_t)m * a.ldr + n : nullptr, WAY >= 0 || (a.wide_side && left >= 8), left);
-            way_out8<WAY>(a, v, sx[j], sy, bias, gate, side, a.out + (int64_t)m * a.ldo + n, left);
+#pragma unroll
+            for (int h = 0; h < kPair; h++) {
+                const int p = p0 + h, col = col0 + 32 * p, left = cols_left - 32 * p;
+                int v[8];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const u32x2 w = __builtin_amdgcn_permlane16_swap((unsigned)acc[2 * p][j][e], (unsigned)acc[2 * p + 1][j][e], false, false);
+                    v[e] = (int)w[0];
+                    v[4 + e] = (int)w[1];
+                }
+                if (16 * j >= rows_left || left <= 0) continue;      // (not before the swap, which takes all lanes)
+                if (a.gate != nullptr && !one_sample) gate[h] = take8(a.gate + (int)(row + lane_row) / a.per_sample * a.s_gate + col + lane_col, a.wide, left);
+                if (WAY < 0 && a.residual != nullptr) early[h][i] = take8(a.residual + (row + lane_row) * a.ldr + col + lane_col, a.wide_side && left >= 8, left);
+                o[h] = way_out8<WAY>(a, v, sx[j], sy[h], bias[h], gate[h], early[h][i]);
+                if (!whole) put8(a.out + (row * a.ldo + col) + at_out, o[h], WAY >= 0 || (a.wide_out && left >= 8), left);
+            }
+            if constexpr (kPair == 2) {
+                if (whole) store_lines(a.out + (row * a.ldo + (col0 + 32 * p0)), at_out, (unsigned)(8 * a.ldo), o[0], o[1], lane);
+            }
+            __builtin_amdgcn_sched_barrier(0);                // (rows one after another: all at once do not fit the registers)
         }
+        if (kAhead && p0 + kPair < NT / 2) read_side(p0 + kPair, 0);
     }
 }
 
@@ -379,7 +452,101 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows8_kernel(const Prod
     const vec8<T> bias = take8(a.bias != nullptr ? a.bias + n : nullptr, a.wide, left);
     const vec8<T> gate = take8(a.gate != nullptr ? a.gate + m / a.per_sample * a.s_gate + n : nullptr, a.wide, left);
     const vec8<T> side = take8(a.residual != nullptr ? a.residual + (int64_t)m * a.ldr + n : nullptr, WAY >= 0 || (a.wide_side && left >= 8), left);
-    way_out8<WAY>(a, v, a.x_scale[m], sy, bias, gate, side, a.out + (int64_t)m * a.ldo + n, left);
+    put8(a.out + (int64_t)m * a.ldo + n, way_out8<WAY>(a, v, a.x_scale[m], sy, bias, gate, side), WAY >= 0 || (a.wide_out && left >= 8), left);
+}
+
+// Up to sixteen rows of 16-bit elements, single tokens of a batch: brought to whole numbers here, by every workgroup for itself, in one launch with the product.
+// Each of the eight waves finds the largest values of two rows, and the rows' steps meet in LDS; the fragments are made of 32 bytes of a row as they are read.
+template <typename T, int WAY>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_direct8_kernel(const Product8<T> a, const T* rows, int64_t ld) {
+    typedef Operand<Pair, false, kFewColumns, 1> OperandY;
+    __shared__ float steps_of[16];
+    HIP_DYNAMIC_SHARED(char, shared)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4, lane_row = lane & 15;
+    Pair* const stage = reinterpret_cast<Pair*>(shared) + wave * 2 * kFewStage;
+    const int n0 = (int)blockIdx.x * kFewColumns;
+    const int all = (a.K + kStep - 1) / kStep, each = (all + kFewWaves - 1) / kFewWaves, first = min(all, wave * each), steps = min(all - first, each);
+    OperandY oy;
+    oy.init(0, lane, a.ldy, min(kFewColumns, a.N - n0));
+    const int k0 = first * kStep;                             // in pairs
+    const Pair* const py = a.y + (int64_t)n0 * a.ldy + k0;
+    auto request = [&](int s) { oy.request(py + s * kStep, stage + (s & 1) * kFewStage, 0, lane, a.K - k0 - s * kStep); };
+    if (steps > 0) request(0);                                // (weights on their way meanwhile)
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int r = 2 * wave + h;
+        const T* const x = rows + min(r, a.M - 1) * ld;
+        unsigned top = 0;
+        for (int c = lane * 8; c < 2 * a.K; c += 512) {
+            const vec8<T> v = *reinterpret_cast<const vec8<T>*>(x + c);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const T t = v[e];
+                uint16_t b;
+                __builtin_memcpy(&b, &t, 2);
+                top = max_moved(top, b & 0x7fffu);
+            }
+        }
+        top = lanes_max<64>(top);
+        if (lane == 0) steps_of[r] = step_of<T>(top);
+    }
+    __syncthreads();
+    const float own = steps_of[lane_row];
+    const Steps st = steps_for(own);
+    const T* const px = rows + min(lane_row, a.M - 1) * ld;
+    i32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    for (int s = 0; s < steps; s++) {
+        vec8<T> raw[2][2];
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            const int at = 2 * (k0 + s * kStep + 32 * ks + 8 * quad);         // (a multiple of 16 elements, as K is)
+#pragma unroll
+            for (int h = 0; h < 2; h++) raw[ks][h] = take8(at < 2 * a.K ? px + at + 8 * h : nullptr, true, 8);
+        }
+        wave_waits_for_copies();
+        if (s + 1 < steps) request(s + 1);
+        const Pair* const ty = stage + (s & 1) * kFewStage;
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            union { int8_t b[16]; i32x4 v; } q;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) q.b[8 * h + e] = whole_number(raw[ks][h][e], st);
+            const vec8<Pair> fx = __builtin_bit_cast(vec8<Pair>, q.v);
+#pragma unroll
+            for (int i = 0; i < 2; i++) acc[i] = product8(OperandY::fragment(ty, 16 * i, ks, lane), fx, acc[i]);
+        }
+        wave_waits_for_reads();
+    }
+    __syncthreads();
+    i32x4* const sums = reinterpret_cast<i32x4*>(shared);     // [wave][half][lane]
+#pragma unroll
+    for (int i = 0; i < 2; i++) sums[(wave * 2 + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    if (wave > 0) return;
+    i32x4 t[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        t[i] = sums[i * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < kFewWaves; w++) t[i] += sums[(w * 2 + i) * 64 + lane];
+    }
+    int v[8];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const u32x2 w = __builtin_amdgcn_permlane16_swap((unsigned)t[0][e], (unsigned)t[1][e], false, false);
+        v[e] = (int)w[0];
+        v[4 + e] = (int)w[1];
+    }
+    const int n = n0 + 16 * (quad & 1) + 8 * (quad >> 1), m = lane_row, left = a.N - n;
+    if (m >= a.M || left <= 0) return;
+    float sy[8];
+    scales8<T>(sy, a.y_scale + n, a.wide, left);
+    const vec8<T> bias = take8(a.bias != nullptr ? a.bias + n : nullptr, a.wide, left);
+    const vec8<T> gate = take8(a.gate != nullptr ? a.gate + m / a.per_sample * a.s_gate + n : nullptr, a.wide, left);
+    const vec8<T> side = take8(a.residual != nullptr ? a.residual + (int64_t)m * a.ldr + n : nullptr, WAY >= 0 || (a.wide_side && left >= 8), left);
+    put8(a.out + (int64_t)m * a.ldo + n, way_out8<WAY>(a, v, own, sy, bias, gate, side), WAY >= 0 || (a.wide_out && left >= 8), left);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -427,11 +594,23 @@ int launch_few8(const Product8<T>& a, hipStream_t stream) {
     return 0;
 }
 template <typename T, int WAY>
-int launch_way8(Product8<T>& a, hipStream_t stream) {
+int launch_way8(Product8<T>& a, const void* rows, int64_t ld, hipStream_t stream) {
+    if (rows != nullptr) {
+        constexpr int lds = kFewWaves * 2 * kFewStage * (int)sizeof(Pair);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(few_rows_direct8_kernel<T, WAY>), dim3((unsigned)ceil_div(a.N, kFewColumns)), dim3(64 * kFewWaves), lds, stream, a, (const T*)rows, ld);
+        return 0;
+    }
     a.group = (int64_t)a.N * a.K <= (1 << 20) ? 1 : 8;        // (rows of tiles that share y while it does not fit the L2 beside them)
     if (a.M <= kFewRows || ceil_div(a.M, kFewRows) * ceil_div(a.N, kFewColumns) <= kCus) return launch_few8<T, WAY>(a, stream);
     if (ceil_div(a.M, 64) * ceil_div(a.N, 64) <= 4 * kCus) return launch_tiles8<T, 64, 64, 2, 2, WAY>(a, stream);
-    if (ceil_div(a.M, 256) * ceil_div(a.N, 256) >= 2 * kCus) return launch_tiles8<T, 256, 256, 2, 4, WAY>(a, stream);
+    // (pairs of integers are half as many elements: linear.hip's lengths of a round, the way out weighing twice)
+    const auto rounds = [&](int bm, int bn, int slots) {
+        const double n = (double)(ceil_div(a.M, bm) * ceil_div(a.N, bn)) / slots;
+        return n > 4 ? n + 0.5 : std::ceil(n);
+    };
+    const double t128 = rounds(128, 128, 2 * kCus), t192 = 1.3 * rounds(192, 128, 2 * kCus), t256 = (1.8 + 220. / (double)a.K) * rounds(256, 256, kCus);
+    if (t256 < std::min(t128, t192)) return launch_tiles8<T, 256, 256, 2, 4, WAY>(a, stream);
+    if (t192 < t128) return launch_tiles8<T, 192, 128, 2, 2, WAY>(a, stream);
     return launch_tiles8<T, 128, 128, 2, 2, WAY>(a, stream);
 }
 template <typename T>
@@ -446,11 +625,11 @@ int linear_int8(const llsa_int8_args& q, hipStream_t stream) {
     a.wide_side = wide8(q.residual, q.ldr);
     a.wide_out = wide8(q.out, q.ldo);
     int rc;
-    if (!a.wide || !a.wide_side || !a.wide_out) rc = launch_way8<T, -1>(a, stream);
-    else if (a.act == LLSA_ACT_SILU) rc = launch_way8<T, LLSA_ACT_SILU>(a, stream);
-    else if (a.act == LLSA_ACT_GELU) rc = launch_way8<T, LLSA_ACT_GELU>(a, stream);
-    else if (a.act == LLSA_ACT_GELU_TANH) rc = launch_way8<T, LLSA_ACT_GELU_TANH>(a, stream);
-    else rc = launch_way8<T, LLSA_ACT_NONE>(a, stream);
+    if (!a.wide || !a.wide_side || !a.wide_out) rc = launch_way8<T, -1>(a, q.x, q.ldx, stream);
+    else if (a.act == LLSA_ACT_SILU) rc = launch_way8<T, LLSA_ACT_SILU>(a, q.x, q.ldx, stream);
+    else if (a.act == LLSA_ACT_GELU) rc = launch_way8<T, LLSA_ACT_GELU>(a, q.x, q.ldx, stream);
+    else if (a.act == LLSA_ACT_GELU_TANH) rc = launch_way8<T, LLSA_ACT_GELU_TANH>(a, q.x, q.ldx, stream);
+    else rc = launch_way8<T, LLSA_ACT_NONE>(a, q.x, q.ldx, stream);
     return rc != 0 ? rc : launch_status("linear_int8");
 }
 bool rows8(const void* p, int64_t ld, int64_t K) { return p != nullptr && aligned16(p) && ld % 16 == 0 && ld >= K && ld <= kMaxLd; }
@@ -494,8 +673,11 @@ extern "C" int llsa_linear_int8(const llsa_int8_args* a, void* stream) {
     LLSA_REQUIRE(a->K <= LLSA_INT8_MAX_K, "linear_int8: at most %d channels in (sums of 32 bits)", LLSA_INT8_MAX_K);
     if (a->M == 0) return 0;
     const int64_t K = (a->K + 15) / 16 * 16;
-    LLSA_REQUIRE(rows8(a->q, a->ldq, K) && rows8(a->w, a->ldw, K), "linear_int8: rows of q and w must be 16-byte aligned and filled with zeros to a multiple of 16");
-    LLSA_REQUIRE(a->q_scale != nullptr && a->w_scale != nullptr && a->out != nullptr, "linear_int8: scales and output");
+    LLSA_REQUIRE(rows8(a->w, a->ldw, K) && (a->x != nullptr || rows8(a->q, a->ldq, K)), "linear_int8: rows of q and w must be 16-byte aligned and filled with zeros to a multiple of 16");
+    LLSA_REQUIRE(a->x == nullptr || (a->M <= LLSA_INT8_DIRECT_ROWS && a->K % 16 == 0 && rows16(a->x, a->ldx) && a->ldx >= a->K),
+                 "linear_int8: at most %d rows of x itself, 16-byte aligned and a multiple of 16 long", LLSA_INT8_DIRECT_ROWS);
+    LLSA_REQUIRE((a->x != nullptr || a->q_scale != nullptr) && a->w_scale != nullptr && a->out != nullptr, "linear_int8: scales and output");
     LLSA_REQUIRE(a->gate == nullptr || (a->per_sample > 0 && a->M % a->per_sample == 0), "linear_int8: rows of a sample, whole samples");
+    LLSA_REQUIRE(offsets32(a->ldo) && (a->residual == nullptr || offsets32(a->ldr)), "linear_int8: rows of out and residual at most %lld apart", (long long)kMaxLd);
     return a->dtype == LLSA_DTYPE_BF16 ? linear_int8<bf16>(*a, (hipStream_t)stream) : linear_int8<_Float16>(*a, (hipStream_t)stream);
 }

@@ -225,20 +225,31 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(const Route a) {
     take_logits<T, PER>(v, logits, part * PER, a.E, a.wide);
 #pragma unroll
     for (int i = 0; i < PER; i++) g[i] = 0.f, chosen[i] = false;
+    // (all loads in flight together)
+    int e[LLSA_MAX_CHOICES];
+    float d[LLSA_MAX_CHOICES], l[LLSA_MAX_CHOICES];
+#pragma unroll
+    for (int j = 0; j < LLSA_MAX_CHOICES; j++) e[j] = j < a.k ? a.experts[m * a.k + j] : -1;
+#pragma unroll
+    for (int j = 0; j < LLSA_MAX_CHOICES; j++) {
+        const bool there = (unsigned)e[j] < (unsigned)a.E;
+        d[j] = there ? a.dweights[m * a.k + j] : 0.f;
+        l[j] = there ? (float)logits[e[j]] : 0.f;
+    }
     float top = 0.f, sum = 0.f, dot = 0.f;
     bool any = false;
-    for (int j = 0; j < a.k; j++) {
-        const int e = a.experts[m * a.k + j];
-        if ((unsigned)e >= (unsigned)a.E) continue;
-        const float l = (float)logits[e], d = a.dweights[m * a.k + j];
-        if (!any) top = l;                                    // (the largest is the first)
-        any = true;
-        const float x = expf(l - top);
-        sum += x;
-        dot += d * x;
 #pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (e == part * PER + i) g[i] = d, chosen[i] = true;
+    for (int j = 0; j < LLSA_MAX_CHOICES; j++) {
+        if ((unsigned)e[j] < (unsigned)a.E) {
+            if (!any) top = l[j];                             // (the largest is the first)
+            any = true;
+            const float x = expf(l[j] - top);
+            sum += x;
+            dot += d[j] * x;
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (e[j] == part * PER + i) g[i] = d[j], chosen[i] = true;
+        }
     }
     if (!a.normalize && any) {
         sum = 0.f;
