@@ -44,7 +44,7 @@ extern "C" {
 #define LLSA_DTYPE_F32 1
 #define LLSA_DTYPE_F16 2
 
-#define LLSA_ABI_VERSION 220     /* changes with every change of a signature or argument structure below */
+#define LLSA_ABI_VERSION 221     /* changes with every change of a signature or argument structure below */
 int llsa_version(void);          /* LLSA_ABI_VERSION of the built library                                    */
 const char* llsa_last_error_string(void);
 
@@ -516,30 +516,35 @@ int64_t llsa_route_workspace_bytes(int64_t M, int E, int k);
  * (E,N,K).  Conventions of the linear layers above (rows 16-byte aligned and padded, sums in fp32).  The row at a place is that of token order[place] / k.  Numbers
  * in order, places and experts out of range are held to it or skipped.
  *     gather    out[place] = x[token] (N channels) for places below offsets[E], times weights[order[place]] (and the gate of its sample) unless NULL
- *     fwd       z = x W_e^T + bias_e, kept unless z is NULL; out = act(z).  gather_x: x has rows of tokens, where llsa_experts_gathers allows it.
- *               gaps: rows that no expert has get zeros
- *     dx        t = dz W_e; out = t, or with z t * act'(z); gaps as above
+ *     fwd       z = x W_e^T + bias_e, out = act(z); act'(z) is kept in `slopes` unless that is NULL.  gather_x: x has rows of tokens, where llsa_experts_gathers
+ *               allows it.  gaps: rows that no expert has get zeros.  wide: out is fp32 (padded rows)
+ *     dx        t = dz W_e; out = t, or with slopes t * act'(z); gaps, wide as above
+ *     dz        out = dz * act'(z), of all rows
  *     dw        out (E,N,K) = dz^T x and dbias (E,N) = sum of dz over an expert's rows
- *     combine   out (tokens,N) = residual + gate * sum over j of weights[m,j] x[places[m,j]] (weights NULL: 1); the sum, rounded, to z unless NULL
- *     dweights  dweights[m,j] = sum over n of gate * dz[m] * x[places[m,j]] */
+ *     combine   out (tokens,N) = residual + gate * sum over j of weights[m,j] x[places[m,j]] (weights NULL: 1), x fp32
+ *     dweights  dweights[m,j] = sum over n of gate * dz[m] * x[places[m,j]], x fp32; dgate = sum over a sample's tokens of dz[m] * sum over j of weights[m,j] x[places[m,j]];
+ *               either unless NULL
+ * slopes: act'(z) in steps of 2^-14, 16-bit integers, -32768 for a NaN. */
 typedef struct llsa_experts_args {
     const void *x, *w, *bias, *dz, *gate, *residual;
-    void *out, *z, *dbias, *workspace;
+    void *out, *slopes, *dbias, *dgate, *workspace;
     const int32_t *offsets, *order, *places;
     const float* weights;
     float* dweights;
     int64_t ldx, ldw, lddz, ldr, ldo, ldz, s_gate;
     int64_t rows, tokens, per_sample;
-    int32_t E, N, K, k, act, dtype, padded, gaps, gather_x, reserved;
+    int32_t E, N, K, k, act, dtype, padded, gaps, gather_x, wide;
 } llsa_experts_args;
 int llsa_experts_gather(const llsa_experts_args* a, void* stream);
 int llsa_experts_gathers(int64_t rows, int E, int N, int K);
 int llsa_experts_fwd(const llsa_experts_args* a, void* stream);
 int llsa_experts_dx(const llsa_experts_args* a, void* stream);
+int llsa_experts_dz(const llsa_experts_args* a, void* stream);
 int llsa_experts_dw(const llsa_experts_args* a, void* stream);
 int llsa_experts_combine(const llsa_experts_args* a, void* stream);
 int llsa_experts_dweights(const llsa_experts_args* a, void* stream);
 int64_t llsa_experts_dw_workspace_bytes(int64_t rows, int E, int N, int K);
+int64_t llsa_experts_dweights_workspace_bytes(int64_t tokens, int64_t per_sample, int N);
 
 #ifdef __cplusplus
 }

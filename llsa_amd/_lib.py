@@ -100,10 +100,10 @@ class RouteArgs(C.Structure):
 
 
 class ExpertsArgs(C.Structure):
-    _fields_ = ([(n, c_void_p) for n in ("x", "w", "bias", "dz", "gate", "residual", "out", "z", "dbias", "workspace", "offsets", "order", "places",
+    _fields_ = ([(n, c_void_p) for n in ("x", "w", "bias", "dz", "gate", "residual", "out", "slopes", "dbias", "dgate", "workspace", "offsets", "order", "places",
                                          "weights", "dweights")]
                 + [(n, c_int64) for n in ("ldx", "ldw", "lddz", "ldr", "ldo", "ldz", "s_gate", "rows", "tokens", "per_sample")]
-                + [(n, c_int32) for n in ("E", "N", "K", "k", "act", "dtype", "padded", "gaps", "gather_x", "reserved")])
+                + [(n, c_int32) for n in ("E", "N", "K", "k", "act", "dtype", "padded", "gaps", "gather_x", "wide")])
 
 
 class QuantizeArgs(C.Structure):
@@ -179,6 +179,8 @@ _SIGNATURES = {
     "llsa_experts_gathers": (c_int, [c_int64, c_int, c_int, c_int]),
     "llsa_experts_fwd": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
     "llsa_experts_dx": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
+    "llsa_experts_dz": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
+    "llsa_experts_dweights_workspace_bytes": (c_int64, [c_int64, c_int64, c_int]),
     "llsa_experts_dw": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
     "llsa_experts_combine": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
     "llsa_experts_dweights": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
@@ -187,7 +189,7 @@ _SIGNATURES = {
 
 EXPORTS = tuple(_SIGNATURES)
 CHUNK_FINE_MAX = 256                                        # LLSA_CHUNK_FINE_MAX of include/llsa_hip.h
-ABI_VERSION = 220                                           # LLSA_ABI_VERSION
+ABI_VERSION = 221                                           # LLSA_ABI_VERSION
 STATIC_PARTIALS_MAX = 262144                                # LLSA_STATIC_PARTIALS_MAX
 
 

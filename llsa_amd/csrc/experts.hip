@@ -12,9 +12,9 @@
 // that dout needs no factor) dw is a sum over act(z) (dout W_out) on the way out of that product, whose waves have no registers left for it (20 to 30
 // spilled: 1050 us instead of 560).
 //
-// Sums are fp32, and so is what happens on the way out.  Rounded to 16 bits besides the results: what a product takes in that another made or that is kept (z,
-// h, g, dz), as in the linear layers, and the rows y and dx of each expert, which are read once or twice more and added up in fp32: half a step of each, 2^-8 of it
-// in bf16 (fp16 2^-11), for half the bytes.
+// Sums are fp32, and so are what happens on the way out and the rows that each expert gives a token (y, and dx of each), which are added up.  Rounded to 16 bits
+// besides the results is what a product takes in that another made (h, g, dz), as in the linear layers: half a step of each, 2^-8 of it in bf16 (fp16 2^-11).  What a
+// backward wants of z is act'(z), which lies between -0.13 and 1.13: 16 bits hold it in steps of 2^-14, where z itself would be half a step of bf16 off.
 #include "experts_device.h"
 
 namespace llsa {
@@ -32,12 +32,16 @@ struct Grouped {
     int experts, rows, N, ny, K;          // rows: of places
     int tiles_n, group, gaps;             // gaps: zeros go to the rows that no expert has
     // way out
-    const T *bias, *slope_at;
+    const T* bias;
+    const int16_t* slope_at;              // dx
     int64_t ldo, ldz;
-    T *out, *z;
+    void* out;                            // T, or fp32 (kWide)
+    int16_t* slopes;                      // forward: kept unless NULL
     int wide, wide_out;                   // wide: 16-byte accesses to bias; wide_out: to out, or its rows are padded with zeros to a multiple of 8
 };
 struct Here { int expert, m0, m_end, n0, tn; };
+// What is on the way out: in the forward an activation (its LLSA_ACT_ number), in dx the slopes that the forward kept; neither, to T or (kWide) to fp32
+enum { kBySlope = 1, kWide = 4 };
 template <int BM, int BN, typename P>
 __device__ __forceinline__ bool find_tile(const P& a, Here& h, int lane) {
     Runs runs;
@@ -57,26 +61,43 @@ __device__ __forceinline__ void write_zeros(const Grouped<T>& a, const Here& h) 
     for (int e = 0; e < 8; e++) v[e] = 0.f;
     for (int i = threadIdx.x; i < BM * (BN / 8); i += blockDim.x) {
         const int r = i / (BN / 8), n = h.n0 + (i - r * (BN / 8)) * 8;
-        if (h.m0 + r < h.m_end && n < a.N) store8(a.out + (int64_t)(h.m0 + r) * a.ldo + n, v, a.wide_out, a.N - n);
+        if (h.m0 + r < h.m_end && n < a.N) store8(static_cast<T*>(a.out) + (int64_t)(h.m0 + r) * a.ldo + n, v, a.wide_out, a.N - n);
     }
 }
 
-// Eight values of a row on their way out.  z: what the forward keeps; early: z of the layer in front in dx
-template <bool YC, int ACT, typename T>
-__device__ __forceinline__ vec8<T> way_out(const Grouped<T>& a, float (&v)[8], const vec8<T>& bias, const vec8<T>& early, int left, vec8<T>& z) {
+// act'(z) in 16 bits: steps of 2^-14, which hold 0 and 1; one number is left for a NaN
+typedef __attribute__((ext_vector_type(8))) int16_t s16x8;
+__device__ __forceinline__ int16_t slope_kept(float slope) { return slope != slope ? (int16_t)-32768 : (int16_t)(int)__builtin_rintf(slope * 16384.f); }
+__device__ __forceinline__ float slope_of(int16_t kept) { return kept == -32768 ? __uint_as_float(0x7fc00000u) : (float)kept * 0x1p-14f; }
+
+// Eight values of a row on their way out.  kept: the slopes, in the forward; early: those of the layer in front, in dx
+template <bool YC, int ACT, bool TIGHT = false, typename T>
+__device__ __forceinline__ void way_out(const Grouped<T>& a, float (&v)[8], const vec8<T>& bias, const s16x8& early, s16x8& kept) {
     if constexpr (!YC) {
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] += (float)bias[e];
-        if (a.z != nullptr) {
+        if constexpr (ACT != LLSA_ACT_NONE && ACT != kWide) {
+            if (a.slopes != nullptr) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) z[e] = (T)v[e];
+                for (int e = 0; e < 8; e++) {
+                    float value, slope;
+                    activate_both(ACT, v[e], value, slope);
+                    v[e] = value;
+                    kept[e] = slope_kept(slope);
+                    if (TIGHT && e % 2 == 1) __builtin_amdgcn_sched_barrier(0);      // (two at a time: there are no registers for more)
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = activate(ACT, v[e]);
+            }
         }
+    } else if constexpr (ACT == kBySlope) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = activate(ACT, v[e]);
-    } else if constexpr (ACT != LLSA_ACT_NONE) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] *= activate_slope(ACT, (float)early[e]);
+        for (int e = 0; e < 8; e++) v[e] *= slope_of(early[e]);
     }
+}
+template <typename T>
+__device__ __forceinline__ vec8<T> rounded(const float (&v)[8], int left) {
     vec8<T> o;
 #pragma unroll
     for (int e = 0; e < 8; e++) o[e] = (T)(e >= left ? 0.f : v[e]);
@@ -92,11 +113,17 @@ __device__ __forceinline__ void put8(T* to, const vec8<T>& o, bool wide, int lef
             if (e < left) to[e] = o[e];
     }
 }
+__device__ __forceinline__ void put8_wide(float* to, const float (&v)[8]) {
+    *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4*>(to + 4) = f32x4{v[4], v[5], v[6], v[7]};
+}
+
 // The tiles of linear.hip's product_kernel, with an expert's weights; GATHERED: rows of tokens, brought into order on their way into LDS.
 template <typename T, bool YC, bool GATHERED, int BM, int BN, int WAVES_M, int WAVES_N, int ACT>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(const Grouped<T> a) {
     constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
-    constexpr bool kSlope = YC && ACT != LLSA_ACT_NONE;
+    constexpr bool kSlope = YC && ACT == kBySlope;
+    constexpr bool kKeeps = !YC && ACT != LLSA_ACT_NONE && ACT != kWide;
     typedef Operand<T, false, BM, kWaves> OperandX;
     typedef Operand<T, YC, BN, kWaves> OperandY;
     HIP_DYNAMIC_SHARED(char, shared)
@@ -150,14 +177,15 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
     const unsigned at_out = (unsigned)(lane_row * a.ldo) + lane_col, at_z = (unsigned)(lane_row * a.ldz) + lane_col;
     constexpr int kPair = NT % 4 == 0 ? 2 : 1;                // pieces of 32 columns that leave together
     const bool whole = kPair == 2 && here.m0 + BM <= here.m_end && here.n0 + BN <= a.N && a.wide_out;
-    vec8<T> early[kPair][MT];
+    s16x8 early[kPair][MT];
     auto read_side = [&](int p0) {
         if constexpr (kSlope) {
             if constexpr (kPair == 2) {
                 if (whole) {
 #pragma unroll
                     for (int j = 0; j < MT; j++)
-                        request_lines(early[0][j], early[1][j], a.slope_at + ((int64_t)(row0 + 16 * j) * a.ldz + (col0 + 32 * p0)), at_z, (unsigned)(8 * a.ldz), lane);
+                        request_lines(reinterpret_cast<vec8<T>&>(early[0][j]), reinterpret_cast<vec8<T>&>(early[1][j]),
+                                      reinterpret_cast<const T*>(a.slope_at) + ((int64_t)(row0 + 16 * j) * a.ldz + (col0 + 32 * p0)), at_z, (unsigned)(8 * a.ldz), lane);
                     return;
                 }
             }
@@ -166,7 +194,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
 #pragma unroll
                 for (int h = 0; h < kPair; h++)
                     if (16 * j < rows_left && 32 * (p0 + h) < cols_left)
-                        early[h][j] = *reinterpret_cast<const vec8<T>*>(a.slope_at + ((int64_t)(row0 + 16 * j) * a.ldz + (col0 + 32 * (p0 + h))) + at_z);
+                        early[h][j] = *reinterpret_cast<const s16x8*>(a.slope_at + ((int64_t)(row0 + 16 * j) * a.ldz + (col0 + 32 * (p0 + h))) + at_z);
         }
     };
     const int steps = (a.K + kStep - 1) / kStep;
@@ -194,9 +222,10 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
 #pragma unroll
         for (int j = 0; j < MT; j++) {
             const int64_t row = row0 + 16 * j;
-            vec8<T> o[kPair], z[kPair];
+            vec8<T> o[kPair];
+            s16x8 kept[kPair];
             if constexpr (kPair == 2 && kSlope) {
-                if (whole) arrange_lines<T>(early[0][j], early[1][j], lane);
+                if (whole) arrange_lines<T>(reinterpret_cast<vec8<T>&>(early[0][j]), reinterpret_cast<vec8<T>&>(early[1][j]), lane);
             }
 #pragma unroll
             for (int h = 0; h < kPair; h++) {
@@ -208,16 +237,23 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
                     v[e] = __uint_as_float(w[0]);
                     v[4 + e] = __uint_as_float(w[1]);
                 }
-                const bool inside = 16 * j < rows_left && left > 0;
-                if (inside) o[h] = way_out<YC, ACT>(a, v, bias[h], early[h][j], left, z[h]);
-                if (whole || !inside) continue;
-                if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (row * a.ldz + col) + at_z) = z[h];
-                put8(a.out + (row * a.ldo + col) + at_out, o[h], a.wide_out, left);
+                if (16 * j >= rows_left || left <= 0) continue;
+                way_out<YC, ACT>(a, v, bias[h], early[h][j], kept[h]);
+                if constexpr (ACT == kWide) {
+                    put8_wide(static_cast<float*>(a.out) + (row * a.ldo + col) + at_out, v);
+                } else {
+                    o[h] = rounded<T>(v, left);
+                    if (whole) continue;
+                    if (kKeeps && a.slopes != nullptr) *reinterpret_cast<s16x8*>(a.slopes + (row * a.ldz + col) + at_z) = kept[h];
+                    put8(static_cast<T*>(a.out) + (row * a.ldo + col) + at_out, o[h], a.wide_out, left);
+                }
             }
-            if constexpr (kPair == 2) {
+            if constexpr (kPair == 2 && ACT != kWide) {
                 if (whole) {
-                    if (!YC && a.z != nullptr) store_lines(a.z + (row * a.ldz + (col0 + 32 * p0)), at_z, (unsigned)(8 * a.ldz), z[0], z[1], lane);
-                    store_lines(a.out + (row * a.ldo + (col0 + 32 * p0)), at_out, (unsigned)(8 * a.ldo), o[0], o[1], lane);
+                    if (kKeeps && a.slopes != nullptr)
+                        store_lines(reinterpret_cast<T*>(a.slopes) + (row * a.ldz + (col0 + 32 * p0)), at_z, (unsigned)(8 * a.ldz), __builtin_bit_cast(vec8<T>, kept[0]),
+                                    __builtin_bit_cast(vec8<T>, kept[1]), lane);
+                    store_lines(static_cast<T*>(a.out) + (row * a.ldo + (col0 + 32 * p0)), at_out, (unsigned)(8 * a.ldo), o[0], o[1], lane);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);                // (rows one after another: all at once do not fit the registers)
@@ -231,7 +267,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
 constexpr int kFewWaves = 8, kFewColumns = 32, kFewStage = kFewColumns * kStep;
 template <typename T, bool YC, int MT, int ACT>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void grouped_few_kernel(const Grouped<T> a) {
-    constexpr bool kSlope = YC && ACT != LLSA_ACT_NONE;
+    constexpr bool kSlope = YC && ACT == kBySlope;
+    constexpr bool kKeeps = !YC && ACT != LLSA_ACT_NONE && ACT != kWide;
     typedef Operand<T, YC, kFewColumns, 1> OperandY;
     HIP_DYNAMIC_SHARED(char, shared)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
@@ -316,12 +353,13 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void grouped_few_kernel(const Gr
     }
     const int lane_col = 16 * (quad & 1) + 8 * (quad >> 1), m = row0 + 16 * wave + (lane & 15), left = a.N - n0 - lane_col;
     if (m >= here.m_end || left <= 0) return;
-    vec8<T> early = take8<T>(nullptr, true, 0), z;
-    if (kSlope) early = *reinterpret_cast<const vec8<T>*>(a.slope_at + (int64_t)m * a.ldz + n0 + lane_col);
+    s16x8 early = {0, 0, 0, 0, 0, 0, 0, 0}, kept;
+    if (kSlope) early = *reinterpret_cast<const s16x8*>(a.slope_at + (int64_t)m * a.ldz + n0 + lane_col);
     const vec8<T> bias = take8(!YC && a.bias != nullptr ? a.bias + (int64_t)here.expert * a.N + n0 + lane_col : nullptr, a.wide, left);
-    const vec8<T> o = way_out<YC, ACT>(a, v, bias, early, left, z);
-    if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (int64_t)m * a.ldz + n0 + lane_col) = z;
-    put8(a.out + (int64_t)m * a.ldo + n0 + lane_col, o, a.wide_out, left);
+    way_out<YC, ACT>(a, v, bias, early, kept);
+    if (kKeeps && a.slopes != nullptr) *reinterpret_cast<s16x8*>(a.slopes + (int64_t)m * a.ldz + n0 + lane_col) = kept;
+    if constexpr (ACT == kWide) put8_wide(static_cast<float*>(a.out) + (int64_t)m * a.ldo + n0 + lane_col, v);
+    else put8(static_cast<T*>(a.out) + (int64_t)m * a.ldo + n0 + lane_col, rounded<T>(v, left), a.wide_out, left);
 }
 
 // Many rows for each expert, a short contraction: the weights stay in registers (linear.hip's resident_kernel).  A workgroup of twelve waves keeps 384 columns of
@@ -334,7 +372,8 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
     typedef Operand<T, false, kResRows, 1> OperandX;          // of a step: 4 copies
     typedef Operand<T, YC, 32, 1> OperandY;
     constexpr int kStage = kResRows * kStep * STEPS;
-    constexpr bool kSlope = YC && ACT != LLSA_ACT_NONE;
+    constexpr bool kSlope = YC && ACT == kBySlope;
+    constexpr bool kKeeps = !YC && ACT != LLSA_ACT_NONE && ACT != kWide;
     static_assert(4 * STEPS <= 2 * kResWaves, "two copies of a wave take in a tile");
     HIP_DYNAMIC_SHARED(char, shared)
     T* const lds = reinterpret_cast<T*>(shared);
@@ -442,15 +481,15 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
         if (now.expert >= a.experts) {                        // no expert's rows
 #pragma unroll
             for (int j = 0; j < 2; j++)
-                if (first + 16 * j + lane_row < now.end) *reinterpret_cast<vec8<T>*>(a.out + ((int64_t)(first + 16 * j) * a.ldo + n0) + at_out) = take8<T>(nullptr, true, 8);
+                if (first + 16 * j + lane_row < now.end) *reinterpret_cast<vec8<T>*>(static_cast<T*>(a.out) + ((int64_t)(first + 16 * j) * a.ldo + n0) + at_out) = take8<T>(nullptr, true, 8);
             wait_vm0();
             continue;
         }
-        vec8<T> early[2];                                     // what is read on the way out
+        s16x8 early[2];                                       // what is read on the way out
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const int64_t row = m0 + 16 * j;                  // (rows behind the expert's last are another's, or were never written: what comes of them is not kept)
-            if (kSlope) early[j] = __builtin_nontemporal_load(reinterpret_cast<const vec8<T>*>(a.slope_at + (row * a.ldz + n0) + at_z));
+            if (kSlope) early[j] = __builtin_nontemporal_load(reinterpret_cast<const s16x8*>(a.slope_at + (row * a.ldz + n0) + at_z));
         }
         f32x4 acc[2][2];
 #pragma unroll
@@ -472,7 +511,8 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             __builtin_amdgcn_sched_barrier(0);                // (the weights leave no registers for both at once, nor for the bias but here)
-            vec8<T> bias = take8<T>(nullptr, true, 8), z;
+            vec8<T> bias = take8<T>(nullptr, true, 8);
+            s16x8 kept;
             if (!YC) bias = *reinterpret_cast<const vec8<T>*>(vectors + lane_col);
             float v[8];
 #pragma unroll
@@ -483,10 +523,11 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
             }
             const int64_t row = m0 + 16 * j;
             const bool inside = (int)row + lane_row >= first && (int)row + lane_row < now.end;
-            const vec8<T> o = way_out<YC, ACT>(a, v, bias, early[j], 8, z);
+            way_out<YC, ACT, true>(a, v, bias, early[j], kept);
             if (!inside) continue;
-            if (!YC && a.z != nullptr) *reinterpret_cast<vec8<T>*>(a.z + (row * a.ldz + n0) + at_z) = z;
-            *reinterpret_cast<vec8<T>*>(a.out + (row * a.ldo + n0) + at_out) = o;
+            if (kKeeps && a.slopes != nullptr) *reinterpret_cast<s16x8*>(a.slopes + (row * a.ldz + n0) + at_z) = kept;
+            if constexpr (ACT == kWide) put8_wide(static_cast<float*>(a.out) + (row * a.ldo + n0) + at_out, v);
+            else *reinterpret_cast<vec8<T>*>(static_cast<T*>(a.out) + (row * a.ldo + n0) + at_out) = rounded<T>(v, 8);
         }
     }
 }
@@ -735,11 +776,12 @@ __global__ __launch_bounds__(256) void gather_kernel(const Gather<T> a) {
 // ---------------------------------------------------------------------------------------
 template <typename T>
 struct Combine {
-    const T *y, *gate, *residual;
+    const float* y;
+    const T *gate, *residual;
     const int32_t* places;
     const float* weights;                 // or NULL: 1
-    T *out, *sum;                         // sum: what the gate multiplies, or NULL
-    int64_t ldy, s_gate, ldr, ldo, lds, tokens, per_sample;
+    T* out;
+    int64_t ldy, s_gate, ldr, ldo, tokens, per_sample;
     int k, rows, N, pieces, wide, wide_side, wide_out;       // pieces: of eight, of a row
 };
 template <typename T>
@@ -754,12 +796,11 @@ __global__ __launch_bounds__(256) void combine_kernel(const Combine<T> a) {
     for (int j = 0; j < a.k; j++) {
         const int p = a.places[m * a.k + j];
         if ((unsigned)p >= (unsigned)a.rows) continue;        // no expert
-        const vec8<T> y = *reinterpret_cast<const vec8<T>*>(a.y + p * a.ldy + n);
+        const f32x4 y0 = *reinterpret_cast<const f32x4*>(a.y + p * a.ldy + n), y1 = *reinterpret_cast<const f32x4*>(a.y + p * a.ldy + n + 4);
         const float w = a.weights != nullptr ? a.weights[m * a.k + j] : 1.f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = fmaf(w, (float)y[e], v[e]);
+        for (int e = 0; e < 4; e++) v[e] = fmaf(w, y0[e], v[e]), v[4 + e] = fmaf(w, y1[e], v[4 + e]);
     }
-    if (a.sum != nullptr) store8(a.sum + m * a.lds + n, v, true, 8);
     if (a.gate != nullptr) {
         const vec8<T> g = take8(a.gate + m / a.per_sample * a.s_gate + n, a.wide, left);
 #pragma unroll
@@ -773,54 +814,104 @@ __global__ __launch_bounds__(256) void combine_kernel(const Combine<T> a) {
     store8(a.out + m * a.ldo + n, v, a.wide_out, left);
 }
 
-// dweights[m][j] = gate dout[m] . y of its place; 0 without one.  A wave a token.  Bound by memory.
+// dweights[m][j] = gate dout[m] . y of its place, 0 without one; pieces of dgate = sum over a sample's tokens of dout[m] * sum over j of w_j y.  A workgroup
+// takes up to `piece` tokens of one sample, each of its waves every fourth, 512 columns at a time.  Bound by memory: dout and y are read once for both.
 template <typename T>
 struct DWeights {
-    const T *dout, *y, *gate;
+    const T *dout, *gate;
+    const float *y, *weights;
     const int32_t* places;
-    float* dweights;
-    int64_t ldd, ldy, s_gate, tokens, per_sample;
-    int k, rows, N, wide, wide_gate;
+    float *dweights, *part;               // either may be NULL; part: [sample][piece][N]
+    int64_t ldd, ldy, s_gate, per_sample;
+    int k, rows, N, wide, wide_gate, piece, pieces;
 };
 template <typename T>
 __global__ __launch_bounds__(256) void dweights_kernel(const DWeights<T> a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t m = min((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), a.tokens - 1);
-    float v[LLSA_MAX_CHOICES];
+    __shared__ float sums[4][512];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sample = (int)blockIdx.x / a.pieces, piece = (int)blockIdx.x - sample * a.pieces;
+    const int64_t t0 = sample * a.per_sample + (int64_t)piece * a.piece, t1 = min((int64_t)(sample + 1) * a.per_sample, t0 + a.piece);
+    for (int n0 = 0; n0 < a.N; n0 += 512) {
+        const int n = n0 + lane * 8, left = a.N - n;
+        const bool inside = left > 0;
+        const vec8<T> g = take8(a.gate != nullptr && inside ? a.gate + sample * a.s_gate + n : nullptr, a.wide_gate, left);
+        float acc[8];
 #pragma unroll
-    for (int j = 0; j < LLSA_MAX_CHOICES; j++) v[j] = 0.f;
-    for (int n = lane * 8; n < a.N; n += 512) {
-        const int left = a.N - n;
-        const vec8<T> d = take8(a.dout + m * a.ldd + n, a.wide, left);
-        const vec8<T> g = take8(a.gate != nullptr ? a.gate + m / a.per_sample * a.s_gate + n : nullptr, a.wide_gate, left);
-        float x[8];
+        for (int e = 0; e < 8; e++) acc[e] = 0.f;
+        for (int64_t m = t0 + wave; m < t1; m += 4) {
+            const vec8<T> dout = take8(inside ? a.dout + m * a.ldd + n : nullptr, a.wide, left);
+            float d[8], s[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = e >= left ? 0.f : a.gate != nullptr ? (float)d[e] * (float)g[e] : (float)d[e];
-#pragma unroll
-        for (int j0 = 0; j0 < LLSA_MAX_CHOICES; j0 += 2)
-            if (j0 < a.k) {                                   // (two at a time, their loads in flight together)
-                vec8<T> y[2];
+            for (int e = 0; e < 8; e++) d[e] = e >= left ? 0.f : (float)dout[e], s[e] = 0.f;
+            for (int j0 = 0; j0 < a.k; j0 += 2) {             // (two at a time, their loads in flight together)
+                f32x4 y[2][2];
+                float w[2];
                 bool there[2];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int p = a.places[m * a.k + min(j0 + h, a.k - 1)];
-                    there[h] = (unsigned)p < (unsigned)a.rows;
-                    y[h] = *reinterpret_cast<const vec8<T>*>(a.y + (there[h] ? p : 0) * a.ldy + n);
+                    const int64_t slot = m * a.k + min(j0 + h, a.k - 1);
+                    const int p = a.places[slot];
+                    there[h] = (unsigned)p < (unsigned)a.rows && j0 + h < a.k;
+                    const float* const at = a.y + (there[h] ? p : 0) * a.ldy + (inside ? n : 0);
+                    y[h][0] = *reinterpret_cast<const f32x4*>(at);
+                    y[h][1] = *reinterpret_cast<const f32x4*>(at + 4);
+                    w[h] = a.weights[slot];
                 }
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int h = 0; h < 2; h++) {
+                    float dot = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) v[j0 + h] = fmaf(x[e], e >= left || !there[h] ? 0.f : (float)y[h][e], v[j0 + h]);
+                    for (int e = 0; e < 8; e++) {
+                        const float v = e >= left || !there[h] ? 0.f : y[h][e >> 2][e & 3];
+                        s[e] = fmaf(there[h] ? w[h] : 0.f, v, s[e]);
+                        dot = fmaf(a.gate != nullptr ? d[e] * (e >= left ? 0.f : (float)g[e]) : d[e], v, dot);
+                    }
+                    if (a.dweights != nullptr && j0 + h < a.k) {
+                        dot = octet_sum(dot);
+                        dot += across<8>(dot);
+                        dot = quad_sum(dot);
+                        if (lane == 0) a.dweights[m * a.k + j0 + h] = n0 == 0 ? dot : a.dweights[m * a.k + j0 + h] + dot;
+                    }
+                }
             }
-    }
 #pragma unroll
-    for (int j = 0; j < LLSA_MAX_CHOICES; j++)
-        if (j < a.k) {
-            float t = octet_sum(v[j]);
-            t += across<8>(t);
-            t = quad_sum(t);
-            if (lane == 0) a.dweights[m * a.k + j] = t;
+            for (int e = 0; e < 8; e++) acc[e] = fmaf(d[e], s[e], acc[e]);
         }
+        if (a.part == nullptr) continue;
+#pragma unroll
+        for (int e = 0; e < 8; e++) sums[wave][lane * 8 + e] = acc[e];
+        __syncthreads();
+        for (int c = threadIdx.x; c < 512; c += 256)
+            if (n0 + c < a.N) a.part[(int64_t)blockIdx.x * a.N + n0 + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+        __syncthreads();
+    }
+}
+// The pieces of dgate added up: four waves take every fourth of the same 64 columns' (a thread alone would wait for one after another)
+template <typename T>
+__global__ __launch_bounds__(256) void expert_gate_kernel(const float* part, T* dgate, int N, int pieces, int groups) {
+    __shared__ float rest[3][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sample = (int)blockIdx.x / groups, n = ((int)blockIdx.x - sample * groups) * 64 + lane;
+    float v = 0.f;
+    if (n < N) {
+#pragma unroll 8
+        for (int p = wave; p < pieces; p += 4) v += part[((int64_t)sample * pieces + p) * N + n];
+    }
+    if (wave > 0) rest[wave - 1][lane] = v;
+    __syncthreads();
+    if (wave == 0 && n < N) dgate[(int64_t)sample * N + n] = (T)(v + rest[0][lane] + rest[1][lane] + rest[2][lane]);
+}
+
+// dz = dout * slope, of all rows.  Bound by memory.
+template <typename T>
+__global__ __launch_bounds__(256) void slope_rows_kernel(const T* dout, int64_t ldd, const int16_t* slopes, int64_t lds, T* dz, int64_t ldz, int64_t rows, int N, int pieces, int wide) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / pieces;
+    if (m >= rows) return;
+    const int n = (int)(i - m * pieces) * 8, left = N - n;
+    const vec8<T> d = take8(dout + m * ldd + n, wide, left);
+    const s16x8 k = *reinterpret_cast<const s16x8*>(slopes + m * lds + n);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = (float)d[e] * slope_of(k[e]);
+    *reinterpret_cast<vec8<T>*>(dz + m * ldz + n) = rounded<T>(v, left);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -871,7 +962,7 @@ int launch_grouped_tiles(Grouped<T>& a, hipStream_t stream) {
 }
 template <typename T, bool YC, int ACT>
 int launch_grouped_64(Grouped<T>& a, hipStream_t stream) {
-    if constexpr (!YC) {
+    if constexpr (!YC && ACT != kWide) {
         if (a.order.slots != nullptr) return launch_grouped_tiles<T, YC, true, 64, 64, 2, 2, ACT>(a, stream);
     }
     return launch_grouped_tiles<T, YC, false, 64, 64, 2, 2, ACT>(a, stream);
@@ -899,7 +990,7 @@ int launch_grouped_resident(Grouped<T>& a, hipStream_t stream) {
 template <typename T, bool YC, int ACT>
 int launch_grouped(Grouped<T>& a, hipStream_t stream) {
     a.group = (int64_t)a.N * a.K <= (1 << 20) ? 1 : 8;        // (rows of tiles that share y while it does not fit the L2 beside them)
-    const GroupedTiles t = grouped_tiles(a.rows, a.experts, a.N, a.K, YC, YC && ACT != LLSA_ACT_NONE);
+    const GroupedTiles t = grouped_tiles(a.rows, a.experts, a.N, a.K, YC, YC && ACT == kBySlope);
     switch (t) {
         case kFew16: return launch_grouped_few<T, YC, 1, ACT>(a, stream);
         case kFew32: return launch_grouped_few<T, YC, 2, ACT>(a, stream);
@@ -909,17 +1000,18 @@ int launch_grouped(Grouped<T>& a, hipStream_t stream) {
         case k192: return launch_grouped_tiles<T, YC, false, 192, 128, 2, 2, ACT>(a, stream);
         case kResident: return a.K == 5 * kStep ? launch_grouped_resident<T, YC, ACT, 5>(a, stream) : launch_grouped_resident<T, YC, ACT, 6>(a, stream);
         default:
-            if constexpr (!YC || ACT == LLSA_ACT_NONE) return launch_grouped_tiles<T, YC, false, 256, 256, 2, 4, ACT>(a, stream);
+            if constexpr (!YC || ACT != kBySlope) return launch_grouped_tiles<T, YC, false, 256, 256, 2, 4, ACT>(a, stream);
             else return fail(-1, "experts: no such tiles");
     }
 }
-template <typename T, bool YC>
-int launch_by_act(Grouped<T>& a, int act, hipStream_t stream) {
+template <typename T>
+int launch_forward(Grouped<T>& a, int act, bool wide, hipStream_t stream) {
+    if (wide) return launch_grouped<T, false, kWide>(a, stream);
     switch (act) {
-        case LLSA_ACT_SILU: return launch_grouped<T, YC, LLSA_ACT_SILU>(a, stream);
-        case LLSA_ACT_GELU: return launch_grouped<T, YC, LLSA_ACT_GELU>(a, stream);
-        case LLSA_ACT_GELU_TANH: return launch_grouped<T, YC, LLSA_ACT_GELU_TANH>(a, stream);
-        default: return launch_grouped<T, YC, LLSA_ACT_NONE>(a, stream);
+        case LLSA_ACT_SILU: return launch_grouped<T, false, LLSA_ACT_SILU>(a, stream);
+        case LLSA_ACT_GELU: return launch_grouped<T, false, LLSA_ACT_GELU>(a, stream);
+        case LLSA_ACT_GELU_TANH: return launch_grouped<T, false, LLSA_ACT_GELU_TANH>(a, stream);
+        default: return launch_grouped<T, false, LLSA_ACT_NONE>(a, stream);
     }
 }
 template <typename T>
@@ -929,10 +1021,10 @@ int experts_fwd(const llsa_experts_args& q, hipStream_t stream) {
     a.offsets = q.offsets; a.order = order_of(q.gather_x ? q.order : nullptr, q.k, q.tokens, q.rows);
     a.experts = q.E; a.rows = (int)q.rows; a.N = q.N; a.K = q.K; a.gaps = q.gaps;
     a.bias = (const T*)q.bias;
-    a.out = (T*)q.out; a.ldo = q.ldo; a.z = (T*)q.z; a.ldz = q.ldz;
+    a.out = q.out; a.ldo = q.ldo; a.slopes = (int16_t*)q.slopes; a.ldz = q.ldz;
     a.wide = q.N % 8 == 0 && wide8(q.bias, 0);
     a.wide_out = (q.N % 8 == 0 && wide8(q.out, q.ldo)) || q.padded;
-    if (int rc = launch_by_act<T, false>(a, q.act, stream)) return rc;
+    if (int rc = launch_forward<T>(a, q.act, q.wide, stream)) return rc;
     return launch_status("experts_fwd");
 }
 template <typename T>
@@ -941,9 +1033,10 @@ int experts_dx(const llsa_experts_args& q, hipStream_t stream) {
     a.x = (const T*)q.dz; a.ldx = q.lddz; a.y = (const T*)q.w; a.ldy = q.ldw; a.y_expert = (int64_t)q.N * q.ldw;
     a.offsets = q.offsets;
     a.experts = q.E; a.rows = (int)q.rows; a.N = q.K; a.ny = (int)pad8(q.K); a.K = q.N; a.gaps = q.gaps;
-    a.out = (T*)q.out; a.ldo = q.ldo; a.slope_at = (const T*)q.z; a.ldz = q.ldz;
+    a.out = q.out; a.ldo = q.ldo; a.slope_at = (const int16_t*)q.slopes; a.ldz = q.ldz;
     a.wide_out = (q.K % 8 == 0 && wide8(q.out, q.ldo)) || q.padded;
-    if (int rc = launch_by_act<T, true>(a, q.z != nullptr ? q.act : LLSA_ACT_NONE, stream)) return rc;
+    const int rc = q.wide ? launch_grouped<T, true, kWide>(a, stream) : q.slopes != nullptr ? launch_grouped<T, true, kBySlope>(a, stream) : launch_grouped<T, true, LLSA_ACT_NONE>(a, stream);
+    if (rc != 0) return rc;
     return launch_status("experts_dx");
 }
 
@@ -1015,10 +1108,10 @@ int experts_gather(const llsa_experts_args& q, hipStream_t stream) {
 template <typename T>
 int experts_combine(const llsa_experts_args& q, hipStream_t stream) {
     Combine<T> a{};
-    a.y = (const T*)q.x; a.ldy = q.ldx; a.places = q.places; a.weights = q.weights; a.k = q.k; a.rows = (int)q.rows; a.N = q.N; a.tokens = q.tokens;
+    a.y = (const float*)q.x; a.ldy = q.ldx; a.places = q.places; a.weights = q.weights; a.k = q.k; a.rows = (int)q.rows; a.N = q.N; a.tokens = q.tokens;
     a.per_sample = std::max<int64_t>(1, q.per_sample);
     a.gate = (const T*)q.gate; a.s_gate = q.s_gate; a.residual = (const T*)q.residual; a.ldr = q.ldr;
-    a.out = (T*)q.out; a.ldo = q.ldo; a.sum = (T*)q.z; a.lds = q.ldz;
+    a.out = (T*)q.out; a.ldo = q.ldo;
     a.pieces = (int)(pad8(q.N) / 8);
     a.wide = q.N % 8 == 0 && wide8(q.gate, q.s_gate);
     a.wide_side = q.N % 8 == 0 && wide8(q.residual, q.ldr);
@@ -1028,15 +1121,38 @@ int experts_combine(const llsa_experts_args& q, hipStream_t stream) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(combine_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, a);
     return launch_status("experts_combine");
 }
+// About 1024 workgroups, each of at least 16 tokens
+struct TokenPieces { int count, tokens; };
+TokenPieces token_pieces(int64_t tokens, int64_t per_sample) {
+    const int64_t samples = tokens / per_sample, want = std::max<int64_t>(1, 4 * kCus / samples), each = std::max<int64_t>(16, ceil_div(per_sample, want));
+    return {(int)ceil_div(per_sample, each), (int)each};
+}
 template <typename T>
 int experts_dweights(const llsa_experts_args& q, hipStream_t stream) {
+    const int64_t per_sample = q.per_sample > 0 ? q.per_sample : q.tokens, samples = q.tokens / per_sample;
+    const TokenPieces p = token_pieces(q.tokens, per_sample);
     DWeights<T> a{};
-    a.dout = (const T*)q.dz; a.ldd = q.lddz; a.y = (const T*)q.x; a.ldy = q.ldx; a.gate = (const T*)q.gate; a.s_gate = q.s_gate; a.per_sample = std::max<int64_t>(1, q.per_sample);
-    a.places = q.places; a.dweights = q.dweights; a.tokens = q.tokens; a.k = q.k; a.rows = (int)q.rows; a.N = q.N;
+    a.dout = (const T*)q.dz; a.ldd = q.lddz; a.y = (const float*)q.x; a.ldy = q.ldx; a.gate = (const T*)q.gate; a.s_gate = q.s_gate; a.per_sample = per_sample;
+    a.weights = q.weights; a.places = q.places; a.dweights = q.dweights; a.k = q.k; a.rows = (int)q.rows; a.N = q.N;
+    a.part = q.dgate != nullptr ? (float*)q.workspace : nullptr;
+    a.piece = p.tokens; a.pieces = p.count;
     a.wide = q.N % 8 == 0 && wide8(q.dz, q.lddz);
     a.wide_gate = q.N % 8 == 0 && wide8(q.gate, q.s_gate);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(dweights_kernel<T>), dim3((unsigned)ceil_div(q.tokens, 4)), dim3(256), 0, stream, a);
+    const int64_t groups = ceil_div(q.N, 64);
+    LLSA_REQUIRE(samples * p.count <= kMaxGrid && samples * groups <= kMaxGrid, "experts_dweights: too many samples");
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(dweights_kernel<T>), dim3((unsigned)(samples * p.count)), dim3(256), 0, stream, a);
+    if (q.dgate != nullptr)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(expert_gate_kernel<T>), dim3((unsigned)(samples * groups)), dim3(256), 0, stream, a.part, (T*)q.dgate, q.N, p.count, (int)groups);
     return launch_status("experts_dweights");
+}
+template <typename T>
+int experts_dz(const llsa_experts_args& q, hipStream_t stream) {
+    const int pieces = (int)(pad8(q.N) / 8);
+    const int64_t grid = ceil_div(q.rows * pieces, 256);
+    LLSA_REQUIRE(grid <= kMaxGrid, "experts_dz: too many rows");
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(slope_rows_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, (const T*)q.dz, q.lddz, (const int16_t*)q.slopes, q.ldz, (T*)q.out, q.ldo, q.rows, q.N,
+                       pieces, q.N % 8 == 0 && wide8(q.dz, q.lddz));
+    return launch_status("experts_dz");
 }
 
 int check_experts(const char* what, const llsa_experts_args* a) {
@@ -1074,7 +1190,8 @@ extern "C" int llsa_experts_fwd(const llsa_experts_args* a, void* stream) {
     LLSA_REQUIRE(rows16(a->x, a->ldx) && rows16(a->w, a->ldw) && a->K % 8 == 0 && a->ldx >= a->K && a->ldw >= a->K,
                  "experts_fwd: rows of x and w must be 16-byte aligned and a multiple of 8 long (zeros beyond the end)");
     LLSA_REQUIRE(a->out != nullptr && offsets32(a->ldo) && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->N))), "experts_fwd: output, padded rows 16-byte aligned and a multiple of 8 long");
-    LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->N)), "experts_fwd: rows of z must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->slopes == nullptr || (rows16(a->slopes, a->ldz) && a->ldz >= pad8(a->N) && a->act != LLSA_ACT_NONE), "experts_fwd: rows of slopes must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(!a->wide || (a->padded && a->act == LLSA_ACT_NONE && !a->gaps && !a->gather_x), "experts_fwd: rows of fp32 are padded, without an activation, gaps or gathered rows");
     LLSA_REQUIRE(!a->gather_x || llsa_experts_gathers(a->rows, a->E, a->N, a->K), "experts_fwd: rows of this many tokens have to be gathered beforehand");
     return BY_TYPE(experts_fwd);
 }
@@ -1083,7 +1200,8 @@ extern "C" int llsa_experts_dx(const llsa_experts_args* a, void* stream) {
     if (a->rows == 0) return 0;
     LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->w, a->ldw) && a->lddz >= pad8(a->N) && a->ldw >= pad8(a->K), "experts_dx: rows of dz and w must be 16-byte aligned and padded to a multiple of 8");
     LLSA_REQUIRE(a->out != nullptr && offsets32(a->ldo) && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->K))), "experts_dx: output, padded rows 16-byte aligned and a multiple of 8 long");
-    LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->K) && a->act != LLSA_ACT_NONE), "experts_dx: rows of z must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->slopes == nullptr || (rows16(a->slopes, a->ldz) && a->ldz >= pad8(a->K)), "experts_dx: rows of slopes must be 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(!a->wide || (a->padded && a->slopes == nullptr && !a->gaps), "experts_dx: rows of fp32 are padded, without slopes or gaps");
     return BY_TYPE(experts_dx);
 }
 extern "C" int llsa_experts_dw(const llsa_experts_args* a, void* stream) {
@@ -1098,15 +1216,24 @@ extern "C" int llsa_experts_combine(const llsa_experts_args* a, void* stream) {
     if (int rc = check_experts("experts_combine", a)) return rc;
     if (a->tokens == 0) return 0;
     LLSA_REQUIRE(a->places != nullptr && a->out != nullptr && (a->rows == 0 || (rows16(a->x, a->ldx) && a->ldx >= pad8(a->N))), "experts_combine: rows 16-byte aligned and padded to a multiple of 8");
-    LLSA_REQUIRE(a->z == nullptr || (rows16(a->z, a->ldz) && a->ldz >= pad8(a->N)), "experts_combine: rows of the sums must be 16-byte aligned and padded to a multiple of 8");
     LLSA_REQUIRE(a->gate == nullptr || (a->per_sample > 0 && a->tokens % a->per_sample == 0), "experts_combine: rows of a sample, whole samples");
     return BY_TYPE(experts_combine);
 }
 extern "C" int llsa_experts_dweights(const llsa_experts_args* a, void* stream) {
     if (int rc = check_experts("experts_dweights", a)) return rc;
     if (a->tokens == 0) return 0;
-    LLSA_REQUIRE(a->places != nullptr && a->dweights != nullptr && a->dz != nullptr && (a->rows == 0 || (rows16(a->x, a->ldx) && a->ldx >= pad8(a->N))),
-                 "experts_dweights: places, dout, result, rows 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->places != nullptr && a->weights != nullptr && a->dz != nullptr && rows16(a->x, a->ldx) && a->ldx >= pad8(a->N), "experts_dweights: places, weights, dout, rows of fp32 16-byte aligned and padded to a multiple of 8");
+    LLSA_REQUIRE(a->dgate == nullptr || (a->gate != nullptr && a->workspace != nullptr), "experts_dweights: dgate needs the gate and a workspace");
     LLSA_REQUIRE(a->gate == nullptr || (a->per_sample > 0 && a->tokens % a->per_sample == 0), "experts_dweights: rows of a sample, whole samples");
     return BY_TYPE(experts_dweights);
+}
+extern "C" int64_t llsa_experts_dweights_workspace_bytes(int64_t tokens, int64_t per_sample, int N) {
+    if (tokens <= 0 || per_sample <= 0 || N <= 0) return 0;
+    return 4 * (tokens / per_sample) * token_pieces(tokens, per_sample).count * N;
+}
+extern "C" int llsa_experts_dz(const llsa_experts_args* a, void* stream) {
+    if (int rc = check_experts("experts_dz", a)) return rc;
+    if (a->rows == 0) return 0;
+    LLSA_REQUIRE(a->dz != nullptr && rows16(a->slopes, a->ldz) && rows16(a->out, a->ldo) && a->ldz >= pad8(a->N) && a->ldo >= pad8(a->N), "experts_dz: rows of slopes and dz must be 16-byte aligned and padded to a multiple of 8");
+    return BY_TYPE(experts_dz);
 }

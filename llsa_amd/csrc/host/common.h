@@ -119,7 +119,9 @@ struct Library {
     decltype(&llsa_experts_gathers) experts_gathers;
     decltype(&llsa_experts_fwd) experts_fwd;
     decltype(&llsa_experts_dx) experts_dx;
+    decltype(&llsa_experts_dz) experts_dz;
     decltype(&llsa_experts_dw) experts_dw;
+    decltype(&llsa_experts_dweights_workspace_bytes) experts_dweights_workspace_bytes;
     decltype(&llsa_experts_combine) experts_combine;
     decltype(&llsa_experts_dweights) experts_dweights;
     decltype(&llsa_experts_dw_workspace_bytes) experts_dw_workspace_bytes;
@@ -164,7 +166,9 @@ struct Library {
         get("llsa_experts_gathers", experts_gathers);
         get("llsa_experts_fwd", experts_fwd);
         get("llsa_experts_dx", experts_dx);
+        get("llsa_experts_dz", experts_dz);
         get("llsa_experts_dw", experts_dw);
+        get("llsa_experts_dweights_workspace_bytes", experts_dweights_workspace_bytes);
         get("llsa_experts_combine", experts_combine);
         get("llsa_experts_dweights", experts_dweights);
         get("llsa_experts_dw_workspace_bytes", experts_dw_workspace_bytes);

@@ -117,6 +117,16 @@ void set_weights(llsa_experts_args& a, const Weights& w) {
     a.w = w.p(); a.ldw = w.rows.ld; a.E = static_cast<int32_t>(w.E); a.N = static_cast<int32_t>(w.N); a.K = static_cast<int32_t>(w.K);
 }
 const int32_t* ints(const Tensor& t) { return t.data_ptr<int32_t>(); }
+// act'(z) as a forward keeps it
+Tensor slopes_of(const Call& call, int64_t rows, int64_t cols) {
+    const Tensor like = call.rows(0, 8);
+    return at::empty({rows, pad8(cols)}, like.options().dtype(at::kShort));
+}
+// rows of fp32 that are added up
+Tensor wide_rows(const Call& call, int64_t rows, int64_t cols) {
+    const Tensor like = call.rows(0, 8);
+    return at::empty({rows, pad8(cols)}, like.options().dtype(at::kFloat));
+}
 Tensor dense_bias(const Tensor* t) { return t != nullptr ? contiguous(*t) : Tensor(); }
 
 struct GroupedLinearBackward : public BlockNode {
@@ -138,12 +148,12 @@ struct GroupedLinearBackward : public BlockNode {
                 dz = call.operand(grad);
             } else {
                 const Rows dout = rows_of(grad);
-                const Tensor z = as_kept(saved[3]);
+                const Tensor slopes = as_kept(saved[3]);
                 dz.t = call.rows(rows, N); dz.ld = dz.t.size(1); dz.count = rows; dz.cols = N;
-                llsa_linear_args a{};
-                a.dout = dout.p(); a.lddout = dout.ld; a.z = z.data_ptr(); a.ldz = z.size(1); a.dz_out = dz.p(); a.lddz = dz.ld;
-                a.M = rows; a.per_sample = rows; a.N = static_cast<int32_t>(N); a.K = 1; a.act = act; a.dtype = dtype;
-                lib->check(lib->linear_dz(&a, call.stream()), "linear_dz");
+                llsa_experts_args a{};
+                a.dz = dout.p(); a.lddz = dout.ld; a.slopes = slopes.data_ptr(); a.ldz = slopes.size(1); a.out = dz.p(); a.ldo = dz.ld; a.offsets = ints(offsets);
+                a.rows = rows; a.tokens = rows; a.k = 1; a.E = static_cast<int32_t>(E); a.N = static_cast<int32_t>(N); a.K = 8; a.dtype = dtype;
+                lib->check(lib->experts_dz(&a, call.stream()), "experts_dz");
             }
             llsa_experts_args a{};
             a.offsets = ints(offsets); a.rows = rows; a.tokens = rows; a.k = 1; a.dtype = dtype; a.act = LLSA_ACT_NONE;
@@ -190,7 +200,7 @@ Tensor grouped_linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, c
     check_vector(what, "bias", bias_p, {E, N});
     check_rows(what, rows);
     const bool grad = wants({&x_in, &w_in, bias_p});
-    Tensor out, z, offsets;
+    Tensor out, slopes, offsets;
     Rows x;
     Weights w;
     std::shared_ptr<GroupedLinearBackward> node;
@@ -205,13 +215,13 @@ Tensor grouped_linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, c
         if (rows > 0) {
             call.operands({{&x_in, &x}, {&w_in, &w.rows}});
             w.E = E; w.N = N; w.K = pad8(K);
-            if (act != LLSA_ACT_NONE && grad) z = call.rows(rows, N);
+            if (act != LLSA_ACT_NONE && grad) slopes = slopes_of(call, rows, N);
             const Tensor bias = dense_bias(bias_p);
             llsa_experts_args a{};
             set_weights(a, w);
             a.x = x.p(); a.ldx = x.ld; a.offsets = ints(offsets); a.bias = bias.defined() ? bias.data_ptr() : nullptr;
             a.out = out.data_ptr(); a.ldo = N; a.gaps = 1;
-            if (z.defined()) { a.z = z.data_ptr(); a.ldz = z.size(1); }
+            if (slopes.defined()) { a.slopes = slopes.data_ptr(); a.ldz = slopes.size(1); }
             a.rows = rows; a.tokens = rows; a.k = 1; a.act = act; a.dtype = dtype;
             lib->check(lib->experts_fwd(&a, call.stream()), what);
         }
@@ -227,7 +237,7 @@ Tensor grouped_linear(const std::shared_ptr<Library>& lib, const Tensor& x_in, c
         node->keep(wants({&w_in, bias_p}) ? x.t : Tensor(), x_in);
         node->keep(x_in.requires_grad() ? w.rows.t : Tensor(), w_in);
         node->keep(offsets, offsets_in);
-        node->keep(z, z);
+        node->keep(slopes, slopes);
     }
     return out;
 }
@@ -249,9 +259,9 @@ Rows gathered(const Call& call, const Rows& x, const llsa_experts_args& base, co
 struct ExpertFeedForwardBackward : public BlockNode {
     std::vector<int64_t> sizes, chosen;   // of x, of the router's weights
     int64_t tokens, k, per_sample, samples, E, C, F, N;
-    bool has_b1, has_b2, has_gate, has_residual, has_sum;
-    int act, dtype;
-    enum { kX, kW1, kW2, kGate, kOffsets, kOrder, kPlaces, kWeights, kZ, kH, kSum, kY };
+    bool has_b1, has_b2, has_gate, has_residual;
+    int dtype;
+    enum { kX, kW1, kW2, kGate, kOffsets, kOrder, kPlaces, kWeights, kSlopes, kH, kY };
     std::string name() const override { return "ExpertFeedForwardBackward"; }
     variable_list run(const Tensor& grad, const std::vector<Tensor>& saved) override {
         Call call(*lib, grad);
@@ -269,25 +279,23 @@ struct ExpertFeedForwardBackward : public BlockNode {
         if (rows > 0 && (inner || outer || want_p || want_g)) {
             const Rows dout = rows_of(grad);
             const Tensor gate = has_gate ? dense_vector(&saved[kGate]) : Tensor();
-            if (want_g) {
-                const Tensor sum = as_kept(saved[kSum]), unused = call.rows(tokens, N), workspace = call.bytes(lib->linear_dz_workspace_bytes(tokens, per_sample, static_cast<int>(N)));
-                dg = at::empty({samples, N}, o);
-                llsa_linear_args a{};
-                a.dout = dout.p(); a.lddout = dout.ld; a.z = sum.data_ptr(); a.ldz = sum.size(1); a.dz_out = unused.data_ptr(); a.lddz = unused.size(1);
-                a.M = tokens; a.per_sample = per_sample; a.N = static_cast<int32_t>(N); a.K = 1; a.act = LLSA_ACT_NONE; a.dtype = dtype;
-                a.dgate = dg.data_ptr(); a.workspace = workspace.data_ptr();
-                lib->check(lib->linear_dz(&a, call.stream()), "linear_dz");
-            }
-            if (!inner && !outer && !want_p) return results(dx, dp, dw1, db1, dw2, db2, dg, grad, want_w1, want_w2, want_r);
-            const Tensor offsets = contiguous(saved[kOffsets]), order = contiguous(saved[kOrder]), places = contiguous(saved[kPlaces]), weights = contiguous(saved[kWeights]);
+            const Tensor places = contiguous(saved[kPlaces]), weights = contiguous(saved[kWeights]);
             llsa_experts_args base{};
-            base.offsets = ints(offsets); base.order = ints(order); base.places = ints(places);
-            base.rows = rows; base.tokens = tokens; base.k = static_cast<int32_t>(k); base.E = static_cast<int32_t>(E); base.dtype = dtype; base.act = act;
-            if (want_p) {
+            base.places = ints(places); base.rows = rows; base.tokens = tokens; base.k = static_cast<int32_t>(k); base.E = static_cast<int32_t>(E); base.dtype = dtype;
+            const Tensor offsets = contiguous(saved[kOffsets]), order = contiguous(saved[kOrder]);
+            base.offsets = ints(offsets); base.order = ints(order);
+            if (want_p || want_g) {
                 const Tensor y = as_kept(saved[kY]);
+                Tensor workspace;
                 llsa_experts_args a = base;
-                a.dz = dout.p(); a.lddz = dout.ld; a.x = y.data_ptr(); a.ldx = y.size(1); a.dweights = dp.data_ptr<float>(); a.N = static_cast<int32_t>(N); a.K = 8;
+                a.dz = dout.p(); a.lddz = dout.ld; a.x = y.data_ptr(); a.ldx = y.size(1); a.weights = weights.data_ptr<float>(); a.N = static_cast<int32_t>(N); a.K = 8;
+                if (want_p) a.dweights = dp.data_ptr<float>();
                 if (has_gate) { a.gate = gate.data_ptr(); a.s_gate = gate.size(0) > 1 ? gate.stride(0) : 0; a.per_sample = per_sample; }
+                if (want_g) {
+                    dg = at::empty({samples, N}, o);
+                    workspace = call.bytes(lib->experts_dweights_workspace_bytes(tokens, per_sample, a.N));
+                    a.dgate = dg.data_ptr(); a.workspace = workspace.data_ptr();
+                }
                 lib->check(lib->experts_dweights(&a, call.stream()), "experts_dweights");
             }
             if (!inner && !outer) return results(dx, dp, dw1, db1, dw2, db2, dg, grad, want_w1, want_w2, want_r);
@@ -295,12 +303,12 @@ struct ExpertFeedForwardBackward : public BlockNode {
             Rows dz;
             if (inner) {                                      // dz = act'(z) (g W_out)
                 const Weights w2 = weights_of(call, saved[kW2], E, N, F);
-                const Tensor z = as_kept(saved[kZ]);
+                const Tensor slopes = as_kept(saved[kSlopes]);
                 dz.t = call.rows(rows, F); dz.ld = dz.t.size(1); dz.count = rows; dz.cols = F;
                 llsa_experts_args a = base;
                 set_weights(a, w2);
                 a.dz = g.p(); a.lddz = g.ld;
-                a.out = dz.p(); a.ldo = dz.ld; a.padded = 1; a.z = z.data_ptr(); a.ldz = z.size(1);
+                a.out = dz.p(); a.ldo = dz.ld; a.padded = 1; a.slopes = slopes.data_ptr(); a.ldz = slopes.size(1);
                 lib->check(lib->experts_dx(&a, call.stream()), "experts_dx");
             }
             auto weights_back = [&](const Rows& dz_rows, const Tensor& x, int64_t n, int64_t kk, Tensor& dw, Tensor& db, bool want_bias) {
@@ -322,13 +330,13 @@ struct ExpertFeedForwardBackward : public BlockNode {
             }
             if (want_x) {
                 const Weights w1 = weights_of(call, saved[kW1], E, F, C);
-                const Tensor each = call.rows(rows, C);
+                const Tensor each = wide_rows(call, rows, C);
                 llsa_experts_args a = base;
                 set_weights(a, w1);
-                a.dz = dz.p(); a.lddz = dz.ld; a.out = each.data_ptr(); a.ldo = each.size(1); a.padded = 1; a.act = LLSA_ACT_NONE;
+                a.dz = dz.p(); a.lddz = dz.ld; a.out = each.data_ptr(); a.ldo = each.size(1); a.padded = 1; a.wide = 1;
                 lib->check(lib->experts_dx(&a, call.stream()), "experts_dx");
                 llsa_experts_args s = base;
-                s.x = each.data_ptr(); s.ldx = each.size(1); s.out = dx.data_ptr(); s.ldo = C; s.N = static_cast<int32_t>(C); s.K = 8; s.act = LLSA_ACT_NONE;
+                s.x = each.data_ptr(); s.ldx = each.size(1); s.out = dx.data_ptr(); s.ldo = C; s.N = static_cast<int32_t>(C); s.K = 8;
                 lib->check(lib->experts_combine(&s, call.stream()), "experts_combine");
             }
         } else if (rows == 0) {
@@ -383,7 +391,7 @@ Tensor expert_feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_
     check_ints(what, "routing.offsets", offsets_in, {E + 1});
     const bool grad = wants({&x_in, &weights_in, &w1_in, b1, &w2_in, b2, gate_p, residual_p});
     const bool inner = grad && wants({&x_in, &w1_in, b1}), outer = grad && wants({&w2_in, b2}), gates = grad && wants({gate_p}), chooses = grad && wants({&weights_in});
-    Tensor out, z, h, y, sum, gate, weights, order, offsets, places;
+    Tensor out, slopes, h, y, gate, weights, order, offsets, places;
     Rows x;
     Weights w1, w2;
     std::shared_ptr<ExpertFeedForwardBackward> node;
@@ -400,9 +408,8 @@ Tensor expert_feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_
             w1.E = w2.E = E; w1.N = F; w1.K = pad8(C); w2.N = N; w2.K = pad8(F);
             const Tensor bias1 = dense_bias(b1), bias2 = dense_bias(b2);
             h = call.rows(rows, F);
-            if (inner) z = call.rows(rows, F);
-            if (gates) sum = call.rows(tokens, N);
-            y = call.rows(rows, N);
+            if (inner) slopes = slopes_of(call, rows, F);
+            y = wide_rows(call, rows, N);
             llsa_experts_args a{};
             a.order = ints(order); a.offsets = ints(offsets); a.places = ints(places);
             a.rows = rows; a.tokens = tokens; a.k = static_cast<int32_t>(k); a.dtype = dtype; a.padded = 1;
@@ -416,11 +423,11 @@ Tensor expert_feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_
             one.x = x.p(); one.ldx = x.ld;
                         one.bias = bias1.defined() ? bias1.data_ptr() : nullptr;
             one.out = h.data_ptr(); one.ldo = h.size(1); one.act = act;
-            if (z.defined()) { one.z = z.data_ptr(); one.ldz = z.size(1); }
+            if (slopes.defined()) { one.slopes = slopes.data_ptr(); one.ldz = slopes.size(1); }
             lib->check(lib->experts_fwd(&one, call.stream()), "experts_fwd");
             set_weights(two, w2);
             two.x = h.data_ptr(); two.ldx = h.size(1); two.bias = bias2.defined() ? bias2.data_ptr() : nullptr;
-            two.out = y.data_ptr(); two.ldo = y.size(1);
+            two.out = y.data_ptr(); two.ldo = y.size(1); two.wide = 1;
             lib->check(lib->experts_fwd(&two, call.stream()), "experts_fwd");
             const Rows residual = call.addend(residual_p);
             all.weights = weights.data_ptr<float>();
@@ -428,22 +435,21 @@ Tensor expert_feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_
             if (gate.defined()) { all.gate = gate.data_ptr(); all.s_gate = gate.size(0) > 1 ? gate.stride(0) : 0; }
             all.residual = residual.p(); all.ldr = residual.ld; all.per_sample = in.per_sample();
             all.out = out.data_ptr(); all.ldo = N;
-            if (sum.defined()) { all.z = sum.data_ptr(); all.ldz = sum.size(1); }
             lib->check(lib->experts_combine(&all, call.stream()), "experts_combine");
         }
         if (grad) {
             node = make_node<ExpertFeedForwardBackward>(lib);
             node->sizes = x_in.sizes().vec(); node->chosen = weights_in.sizes().vec();
             node->tokens = tokens; node->k = k; node->per_sample = in.per_sample(); node->samples = in.samples; node->E = E; node->C = C; node->F = F; node->N = N;
-            node->has_b1 = b1 != nullptr; node->has_b2 = b2 != nullptr; node->has_gate = gate_p != nullptr; node->has_residual = residual_p != nullptr; node->has_sum = sum.defined();
-            node->act = act; node->dtype = dtype;
+            node->has_b1 = b1 != nullptr; node->has_b2 = b2 != nullptr; node->has_gate = gate_p != nullptr; node->has_residual = residual_p != nullptr;
+            node->dtype = dtype;
         }
     }
     if (node) {
         node->set_next_edges(torch::autograd::collect_next_edges(present({&x_in, &weights_in, &w1_in, b1, &w2_in, b2, gate_p, residual_p})));
         torch::autograd::set_history(out, node);
         auto keep = [&](bool needed, const Tensor& t, const Tensor& input) { node->keep(needed ? t : Tensor(), input); };
-        const bool any = inner || outer || chooses;
+        const bool any = inner || outer || chooses || gates;
         keep(wants({&w1_in, b1}), x.t, x.t);                  // (in the order of the places)
         keep(x_in.requires_grad(), w1.rows.t, w1_in);
         keep(inner, w2.rows.t, w2_in);
@@ -451,11 +457,10 @@ Tensor expert_feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_
         keep(any, offsets, offsets_in);
         keep(any, order, order_in);
         keep(any, places, places_in);
-        keep(inner || outer, weights, weights_in);
-        keep(inner, z, z);
+        keep(any, weights, weights_in);
+        keep(inner, slopes, slopes);
         keep(outer, h, h);
-        node->keep(sum, sum);
-        keep(chooses, y, y);
+        keep(chooses || gates, y, y);
     }
     return out;
 }

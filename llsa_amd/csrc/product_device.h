@@ -77,6 +77,34 @@ __device__ __forceinline__ float activate_slope(int act, float z) {
     }
 }
 
+// Both at once, with one exponential and one reciprocal
+__device__ __forceinline__ void activate_both(int act, float z, float& value, float& slope) {
+    const float t = z > 128.f ? 128.f : z < -128.f ? -128.f : z;
+    switch (act) {
+        case LLSA_ACT_SILU: {
+            const float s = logistic2(kLog2e * t);
+            value = z * s;
+            slope = fmaf(t * s, 1.f - s, s);
+            break;
+        }
+        case LLSA_ACT_GELU: {
+            const float x = fabsf(t) * kRsqrt2, r = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f)), bell = exp2_fast(-0.5f * kLog2e * t * t);
+            const float p = r * fmaf(r, fmaf(r, fmaf(r, fmaf(r, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f), tail = 0.5f * p * bell;
+            const float cdf = t > 0.f ? 1.f - tail : tail;
+            value = z * cdf;
+            slope = fmaf(t * kRsqrt2Pi, bell, cdf);
+            break;
+        }
+        case LLSA_ACT_GELU_TANH: {
+            const float q = t * t, s = logistic2(t * fmaf(kTanh3, q, kTanh1));
+            value = z * s;
+            slope = fmaf(t * fmaf(6.f * kGeluC * kGeluA, q, 2.f * kGeluC) * s, 1.f - s, s);
+            break;
+        }
+        default: value = z, slope = 1.f;
+    }
+}
+
 // ---------------------------------------------------------------------------------------
 // operands in LDS
 //

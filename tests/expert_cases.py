@@ -10,6 +10,9 @@ def more(n):
     return (n + 32) * E
 
 
+KEPT = 2.0 ** -15                                             # half a step of a kept act'(z)
+
+
 def slope64(act, z):
     return torch.autograd.functional.jvp(lambda t: act64(act, t), z, torch.ones_like(z))[1] if act else torch.ones_like(z)
 
@@ -122,7 +125,7 @@ def check_grouped(x, weight, offsets, bias, act, dout):
         within(out[a:b].detach().to(where), v, dv + u * (v.abs() + dv) + lo, f"out, expert {e}")
         g, dg = d * slope64(act, z), 0 * d
         if act:
-            dg = d.abs() * (CURVE * (dz + u * (z.abs() + dz) + lo) + FAST)
+            dg = d.abs() * (CURVE * dz + FAST + KEPT)
             dg = dg + E * g.abs() + u * (g.abs() + dg) + lo
         n = b - a
         r = g.t() @ xe
@@ -169,7 +172,6 @@ def check_experts(x, routing, w_in, b_in, w_out, b_out, act, gate, residual, dou
         h, dh = a, da + u * (a.abs() + da) + lo               # (the hidden rows are rounded)
         y = h @ w2.t() + b2
         dy = dh @ w2.abs().t() + (F + 4) * E * (h.abs() @ w2.abs().t() + b2.abs())
-        dy = dy + u * (y.abs() + dy) + lo                     # (and so is each expert's result)
         s.index_add_(0, tok, w * y)
         ds.index_add_(0, tok, w * dy)
         size.index_add_(0, tok, (w * y).abs())
@@ -180,9 +182,8 @@ def check_experts(x, routing, w_in, b_in, w_out, b_out, act, gate, residual, dou
         dge = (2 * E + u) * ge.abs() + lo                     # (dout with weight and gate is rounded)
         t = ge @ w2
         dt = dge @ w2.abs() + more(N) * (ge.abs() @ w2.abs())
-        zk = u * (z.abs() + dz) + lo                          # (z is kept in 16 bits)
         g = t * slope64(act, z)
-        dg = dt * SLOPE + t.abs() * (CURVE * (dz + zk) + FAST) + 2 * E * g.abs()
+        dg = dt * SLOPE + t.abs() * (CURVE * dz + FAST + KEPT) + 2 * E * g.abs()
         dg = dg + u * (g.abs() + dg) + lo
         r = ge.t() @ h
         within(got["w_out"][e].to(where), r, (dge.t() @ (h.abs() + dh) + ge.abs().t() @ dh + more(n) * (ge.abs().t() @ h.abs())) * (1 + u) + u * r.abs() + lo, f"dw_out, expert {e}")
@@ -197,7 +198,7 @@ def check_experts(x, routing, w_in, b_in, w_out, b_out, act, gate, residual, dou
         r = g @ w1
         b = dg @ w1.abs() + more(F) * (g.abs() @ w1.abs())
         dx.index_add_(0, tok, r)
-        ddx.index_add_(0, tok, b + (u + k * E) * (r.abs() + b) + lo)
+        ddx.index_add_(0, tok, b + k * E * (r.abs() + b))
     ds = ds + k * E * size
     res = c(residual).reshape(M, N) if residual is not None else zero(1, 1)
     ref = res + gt * s
@@ -208,7 +209,7 @@ def check_experts(x, routing, w_in, b_in, w_out, b_out, act, gate, residual, dou
         T = M // x.shape[0]
         each = lambda t: t.reshape(x.shape[0], -1, N).sum(1)
         r = each(d * s)
-        b = each(d.abs() * (ds + u * (s.abs() + ds) + lo) + (T + 32) * E * (d * s).abs())
+        b = each(d.abs() * ds + (T + 32) * E * d.abs() * size)
         within(got["gate"].to(where), r, b * (1 + u) + u * r.abs() + lo, "dgate")
     if residual is not None:
         assert torch.equal(got["residual"], dout)
