@@ -67,7 +67,8 @@ __device__ __forceinline__ void write_zeros(const Grouped<T>& a, const Here& h) 
 
 // act'(z) in 16 bits: steps of 2^-14, which hold 0 and 1; one number is left for a NaN
 typedef __attribute__((ext_vector_type(8))) int16_t s16x8;
-__device__ __forceinline__ int16_t slope_kept(float slope) { return slope != slope ? (int16_t)-32768 : (int16_t)(int)__builtin_rintf(slope * 16384.f); }
+// (added to 1.5 2^23 a number's last bits are its whole part, rounded)
+__device__ __forceinline__ int16_t slope_kept(float z, float slope) { return z != z ? (int16_t)-32768 : (int16_t)__float_as_uint(fmaf(slope, 16384.f, 12582912.f)); }
 __device__ __forceinline__ float slope_of(int16_t kept) { return kept == -32768 ? __uint_as_float(0x7fc00000u) : (float)kept * 0x1p-14f; }
 
 // Eight values of a row on their way out.  kept: the slopes, in the forward; early: those of the layer in front, in dx
@@ -82,8 +83,8 @@ __device__ __forceinline__ void way_out(const Grouped<T>& a, float (&v)[8], cons
                 for (int e = 0; e < 8; e++) {
                     float value, slope;
                     activate_both(ACT, v[e], value, slope);
+                    kept[e] = slope_kept(v[e], slope);
                     v[e] = value;
-                    kept[e] = slope_kept(slope);
                     if (TIGHT && e % 2 == 1) __builtin_amdgcn_sched_barrier(0);      // (two at a time: there are no registers for more)
                 }
             } else {
@@ -422,7 +423,9 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
     T* const own = lds + kResStages * kStage + wave * kResOwn;
     T* const vectors = own + 32 * kStep;
 
-    vec8<T> fy[2 * STEPS][2];
+    // (with slopes besides, the registers are 16 short of six steps' weights: the last step's stay in LDS, where they came through)
+    constexpr int kHeld = kKeeps && STEPS == 6 ? STEPS - 1 : STEPS;
+    vec8<T> fy[2 * kHeld][2];
     auto weights = [&](const T* w) {
         OperandY oy;
         oy.init(0, lane, a.ldy, 32);
@@ -430,6 +433,7 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
         for (int s = 0; s < STEPS; s++) {
             oy.request(w + (YC ? s * kStep * a.ldy + n0 : n0 * a.ldy + s * kStep), own, 0, lane, kStep);
             wave_waits_for_copies();
+            if (s >= kHeld) break;
 #pragma unroll
             for (int ks = 0; ks < 2; ks++)
 #pragma unroll
@@ -505,7 +509,10 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) acc[i][j] = product16(fy[ks][i], fx[j], acc[i][j]);
+                for (int j = 0; j < 2; j++) {
+                    if (ks < 2 * kHeld) acc[i][j] = product16(fy[ks < 2 * kHeld ? ks : 0][i], fx[j], acc[i][j]);
+                    else acc[i][j] = product16(OperandY::fragment(own, 16 * i, ks & 1, lane), fx[j], acc[i][j]);
+                }
         }
         wait_vm0();
 #pragma unroll

@@ -77,9 +77,9 @@ __device__ __forceinline__ float activate_slope(int act, float z) {
     }
 }
 
-// Both at once, with one exponential and one reciprocal
+// Both at once, with one exponential and one reciprocal.  The slope is that of a number: whoever keeps it looks at z for a NaN
 __device__ __forceinline__ void activate_both(int act, float z, float& value, float& slope) {
-    const float t = z > 128.f ? 128.f : z < -128.f ? -128.f : z;
+    const float t = __builtin_amdgcn_fmed3f(z, -128.f, 128.f);        // (of a NaN some number: the slope is then no number's)
     switch (act) {
         case LLSA_ACT_SILU: {
             const float s = logistic2(kLog2e * t);
