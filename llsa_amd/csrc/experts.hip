@@ -10,7 +10,7 @@
 // 384 and 1536 channels, us: dW of gathered rows 573 and 530, of rows in order 376, and some 50 for the copy, which multiplies by w as well); few rows and the
 // smallest tiles of a forward without a backward gather them on their way into LDS.  The weight stays out of the products: in the hidden rows (h' = w act(z), so
 // that dout needs no factor) dw is a sum over act(z) (dout W_out) on the way out of that product, whose waves have no registers left for it (20 to 30
-// spilled: 1050 us instead of 560).
+// spilled: 1050 us instead of 490).
 //
 // Sums are fp32, and so are what happens on the way out and the rows that each expert gives a token (y, and dx of each), which are added up.  Rounded to 16 bits
 // besides the results is what a product takes in that another made (h, g, dz), as in the linear layers: half a step of each, 2^-8 of it in bf16 (fp16 2^-11).  What a
@@ -748,15 +748,14 @@ struct Gather {
     const T *x, *gate;
     T* out;
     const float* weights;
-    const int32_t* offsets;
     Order order;
     int64_t ldx, ldo, s_gate, per_sample;
-    int rows, experts, N, pieces, wide, wide_gate;
+    int rows, N, pieces, wide, wide_gate;
 };
 template <typename T>
 __global__ __launch_bounds__(256) void gather_kernel(const Gather<T> a) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, place = i / a.pieces;
-    if (place >= min(a.rows, max(0, a.offsets[a.experts]))) return;
+    if (place >= a.rows) return;                              // (places behind the last expert's hold a row as well, whichever: it is not read)
     const int n = (int)(i - place * a.pieces) * 8, left = a.N - n, token = a.order.token((int)place);
     vec8<T> v = take8(a.x + token * a.ldx + n, a.wide, left);
     if (a.weights != nullptr) {
@@ -1103,8 +1102,8 @@ template <typename T>
 int experts_gather(const llsa_experts_args& q, hipStream_t stream) {
     Gather<T> a{};
     a.x = (const T*)q.x; a.ldx = q.ldx; a.out = (T*)q.out; a.ldo = q.ldo; a.gate = (const T*)q.gate; a.s_gate = q.s_gate; a.per_sample = std::max<int64_t>(1, q.per_sample);
-    a.weights = q.weights; a.offsets = q.offsets; a.order = order_of(q.order, q.k, q.tokens, q.rows);
-    a.rows = (int)q.rows; a.experts = q.E; a.N = q.N; a.pieces = (int)(pad8(q.N) / 8);
+    a.weights = q.weights; a.order = order_of(q.order, q.k, q.tokens, q.rows);
+    a.rows = (int)q.rows; a.N = q.N; a.pieces = (int)(pad8(q.N) / 8);
     a.wide = q.N % 8 == 0 && wide8(q.x, q.ldx);
     a.wide_gate = q.N % 8 == 0 && wide8(q.gate, q.s_gate);
     const int64_t grid = ceil_div(q.rows * a.pieces, 256);

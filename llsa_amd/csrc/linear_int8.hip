@@ -84,6 +84,24 @@ __device__ __forceinline__ Steps steps_for(float s) {
 }
 template <typename T>
 __device__ __forceinline__ int8_t whole_number(T x, const Steps& t) { return (int8_t)(t.zero ? 0 : nearest((float)x * t.lift, t.step, t.inverse, t.half)); }
+// Eight of them.  Without the cases that hardly a row has (halves that are exact, steps near the least numbers, no numbers), which are looked at once more: it is
+// these instructions that bound the pass (131072 rows of 1536: 136 us with all of nearest() for each, 112 % of the vector units' time by their counter).
+template <typename T>
+__device__ __forceinline__ u32x2 whole_numbers(const vec8any<T>& x, const Steps& t) {
+    union { int8_t b[8]; u32x2 w; } o;
+    bool rare = t.zero || t.lift != 1.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float v = (float)x[e], q = __builtin_rintf(v * t.inverse), left = fmaf(-q, t.step, v), size = fabsf(left);
+        rare |= size == t.half;
+        o.b[e] = (int8_t)(int)(size > t.half ? q + __builtin_copysignf(1.f, left) : q);
+    }
+    if (rare) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) o.b[e] = whole_number(x[e], t);
+    }
+    return o.w;
+}
 
 // LANES lanes hold a row, PIECES pieces of 8 elements each; longer rows (256 lanes only) are read a second time.  Bound by memory.
 template <typename T, int LANES, int PIECES>
@@ -160,8 +178,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const Quantize a) {
         for (int i = 0; i < PIECES; i++) {
             const int c = ((run * PIECES + i) * LANES + lane) * 8;
             union { int8_t b[8]; u32x2 w; } o;
-#pragma unroll
-            for (int e = 0; e < 8; e++) o.b[e] = whole_number(v[i][e], st);
+            o.w = whole_numbers<T>(v[i], st);
             int8_t* const q = a.q + row * a.ldq + c;
             if (a.wide_q) {
                 if (c < (a.K + 15) / 16 * 16) *reinterpret_cast<u32x2*>(q) = o.w;
@@ -508,12 +525,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_direct8_kernel(con
         const Pair* const ty = stage + (s & 1) * kFewStage;
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
-            union { int8_t b[16]; i32x4 v; } q;
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) q.b[8 * h + e] = whole_number(raw[ks][h][e], st);
-            const vec8<Pair> fx = __builtin_bit_cast(vec8<Pair>, q.v);
+            const u32x2 lo = whole_numbers<T>(raw[ks][0], st), hi = whole_numbers<T>(raw[ks][1], st);
+            const vec8<Pair> fx = __builtin_bit_cast(vec8<Pair>, u32x4{lo[0], lo[1], hi[0], hi[1]});
 #pragma unroll
             for (int i = 0; i < 2; i++) acc[i] = product8(OperandY::fragment(ty, 16 * i, ks, lane), fx, acc[i]);
         }

@@ -163,16 +163,22 @@ def test_largest_sums(dev):
     assert ((y.double().cpu() - ref).abs() <= ref.abs() * (half_step(BF16) + 4 * E)).all()
 
 
-def test_rows_that_are_no_numbers(dev):
-    x, w, ws, b, g, r = layer(dev, BF16, 2, 9, 40, 24, True, True, True)
+@pytest.mark.parametrize("K,T", [(40, 9), (48, 7)])
+def test_rows_that_are_no_numbers(dev, K, T):
+    """Quantised beforehand, and (up to sixteen rows, a multiple of sixteen long) in one launch with the product."""
+    x, w, ws, b, g, r = layer(dev, BF16, 2, T, K, 24, True, True, True)
     plain = llsa_amd.linear_int8(x, w, ws, b, gate=g, residual=r)
     for bad in (float("nan"), float("inf"), -float("inf")):
         v = x.clone()
         v[1, 4, 3] = bad
         got = llsa_amd.linear_int8(v, w, ws, b, gate=g, residual=r)
-        keep = torch.ones(2, 9, dtype=torch.bool)
+        keep = torch.ones(2, T, dtype=torch.bool)
         keep[1, 4] = False
         assert torch.equal(got[keep.to(dev)], plain[keep.to(dev)]) and got[1, 4].isnan().all()
+    v = x.clone()
+    v[0, 2] = 0
+    zero = llsa_amd.linear_int8(v, w, ws, b)[0, 2]
+    assert torch.equal(zero, b)
 
 
 def _layouts(v):
