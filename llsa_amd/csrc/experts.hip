@@ -119,7 +119,10 @@ __device__ __forceinline__ void put8_wide(float* to, const float (&v)[8]) {
     *reinterpret_cast<f32x4*>(to + 4) = f32x4{v[4], v[5], v[6], v[7]};
 }
 
-// The tiles of linear.hip's product_kernel, with an expert's weights; GATHERED: rows of tokens, brought into order on their way into LDS.
+// The tiles of linear.hip's product_kernel, with an expert's weights; GATHERED: rows of tokens, brought into order on their way into LDS.  Bound as those are by the
+// operands' way from L2, and by the last tile of each expert, half of it empty on the average.  us, rows of eight experts: 16384, 2048 > 2048 171 (0.81 PFLOP/s;
+// 256 x 256 181), its dx 168 to 180; 262144, 1536 > 384 to fp32 385 to 396 (0.78; a library's product of as many rows with one weight, to bf16, 324), dx 1536 > 384 428 to
+// 447; the matrix units work 28 to 32 % of the last two's time.
 template <typename T, bool YC, bool GATHERED, int BM, int BN, int WAVES_M, int WAVES_N, int ACT>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(const Grouped<T> a) {
     constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
@@ -264,7 +267,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
 }
 
 // Few rows for each expert: a workgroup takes 32 columns of up to 64 rows of one, its eight waves an eighth of the contraction each, through two stages of
-// LDS of their own; the sums meet at the end (linear.hip's few_rows_kernel).  An expert's weight is read once for them, and there is little else.
+// LDS of their own; the sums meet at the end (linear.hip's few_rows_kernel).  An expert's weight is read once for them, and there is little else: 16 rows of eight
+// experts 384 > 1536, 9.5 MB of weights, 5.2 us.  With up to a workgroup for each CU; at two for each (2048 rows 1536 > 384) the smallest tiles take 14 and this 19.5.
 constexpr int kFewWaves = 8, kFewColumns = 32, kFewStage = kFewColumns * kStep;
 template <typename T, bool YC, int MT, int ACT>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void grouped_few_kernel(const Grouped<T> a) {
@@ -365,7 +369,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void grouped_few_kernel(const Gr
 
 // Many rows for each expert, a short contraction: the weights stay in registers (linear.hip's resident_kernel).  A workgroup of twelve waves keeps 384 columns of
 // an expert's weights, 32 columns a wave, and takes its share of the rows through LDS, 32 at a time and two such tiles ahead; where the expert changes it takes
-// in the next one's weights.
+// in the next one's weights.  262144 rows 384 > 1536, us, tiles of 128 x 128 / this: GELU with slopes kept 823 / 535, back by the slopes 950 / 455 (501 and
+// 443 on another card).  Back it moves 1.9 GB at 4.1 to 4.3 TB/s, most of what a copy reaches; the forward writes 1.6 GB and has its vector units at work 52 % of the time.
 constexpr int kResWaves = 12, kResColumns = 32 * kResWaves, kResRows = 32, kResStages = 3, kResOwn = 32 * kStep + 64;
 struct Entry { int expert, begin, end, first, upto; };       // upto: number of the first tile behind its own
 template <typename T, bool YC, int ACT, int STEPS>
@@ -543,7 +548,9 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
 // dW: C_e[m][n] = sum over an expert's rows p of X[p][m] Y[p][n].  All rows are taken in chunks of one length, whatever the
 // experts' are, so that the workgroups are alike; one that meets the end of an expert's rows writes its sums and goes on with the next expert's.  An expert
 // within one chunk is written straight away, the sums of the others meet in a second launch, which also writes the zeros of an expert without rows.  Expert
-// e's sums of chunk c are number c + e: with every next one either grows.
+// e's sums of chunk c are number c + e: with every next one either grows.  us: 262144 rows of eight experts, 384 and 1536 channels, 376 to 390 (0.8 PFLOP/s, the matrix units
+// at work 33 % of the time; a library's product of one weight 950 to 990), the sums 20; 16384 rows of 2048 and 2048 channels 180 to 203 and 12, where pieces of every
+// expert's own took 303 and 70.
 // ---------------------------------------------------------------------------------------
 template <typename T>
 struct GroupedWeights {
@@ -734,6 +741,7 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<
     for (int i0 = (int)blockIdx.x * at_once; i0 < rows; i0 += (int)gridDim.x * at_once) {
         const int i = min(i0 + mine, rows - 1), e = i / a.M, m = i - e * a.M;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
         for (int s = part; s < chunks[e] * a.tiles_n; s += ways) v[0] += a.part_sum[((int64_t)first[e] * a.tiles_n + s) * a.M + m];
         v = join(v);
         if (part == 0 && i0 + mine < rows) a.sums[i] = (T)v[0];
@@ -741,7 +749,7 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<
 }
 
 // ---------------------------------------------------------------------------------------
-// Rows of tokens in the order of the places; with weights, multiplied by them (and by the gate of their sample) in fp32.  Bound by memory.
+// Rows of tokens in the order of the places; with weights, multiplied by them (and by the gate of their sample) in fp32.  Bound by memory: 262144 rows of 384, 403 MB, 79 us.
 // ---------------------------------------------------------------------------------------
 template <typename T>
 struct Gather {
@@ -778,7 +786,7 @@ __global__ __launch_bounds__(256) void gather_kernel(const Gather<T> a) {
 }
 
 // ---------------------------------------------------------------------------------------
-// A token's rows added up: out = residual + gate * sum over j of w_j y[places[j]].  Bound by memory.
+// A token's rows added up: out = residual + gate * sum over j of w_j y[places[j]].  Bound by memory: 131072 tokens of 384, two experts each, 106 us with the residual (5.7 TB/s).
 // ---------------------------------------------------------------------------------------
 template <typename T>
 struct Combine {
@@ -821,7 +829,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const Combine<T> a) {
 }
 
 // dweights[m][j] = gate dout[m] . y of its place, 0 without one; pieces of dgate = sum over a sample's tokens of dout[m] * sum over j of w_j y.  A workgroup
-// takes up to `piece` tokens of one sample, each of its waves every fourth, 512 columns at a time.  Bound by memory: dout and y are read once for both.
+// takes up to `piece` tokens of one sample, each of its waves every fourth, 512 columns at a time.  Bound by memory: dout and y are read once for both, 503 MB in 117 us.
 template <typename T>
 struct DWeights {
     const T *dout, *gate;
@@ -929,15 +937,16 @@ Order order_of(const int32_t* slots, int k, int64_t tokens, int64_t rows) {
 // Pieces there can be: the rows' whole ones, and one more for each expert (two more of rows that no expert has)
 int64_t pieces_of(int64_t rows, int64_t experts, int64_t size) { return rows / size + std::min<int64_t>(experts + 2, rows); }
 
-// Whether the weights stay in registers: a contraction of five or six steps, columns of which a wave has 32 or none and at most a quarter of the waves none, and
-// tiles enough for each workgroup that they pay for the weights' way there, also where it meets the next expert.
+// Whether the weights stay in registers: a contraction of five or six steps, columns of which a wave has 32 or none and at most a quarter of the waves none (as
+// linear.hip's resident() has it, with both sides' times), and tiles enough for each workgroup that they pay for the weights' way there, also where it meets the next expert.
 bool resident(int64_t rows, int64_t experts, int64_t N, int64_t K) {
     const int64_t blocks = ceil_div(N, kResColumns);
     if ((K != 5 * kStep && K != 6 * kStep) || N % 32 != 0 || 4 * N < 3 * kResColumns * blocks || blocks > kCus / 8) return false;
     const int64_t slots = kCus / 8 / blocks * 8;
     return rows >= 8 * kResRows * experts && rows >= 8 * kResRows * slots;
 }
-// Which tiles: few rows for each expert on the average, small tiles while there are few of them for each CU, large ones where the experts fill them
+// Which tiles: few rows for each expert on the average (64 and less are one workgroup's), small tiles while there are few of them for each CU, large ones beyond.
+// us, 16384 rows of eight experts 2048 > 2048: 256 x 256 181, 192 x 128 161 to 171; 262144 rows 1536 > 384: 128 x 128 425, 192 x 128 389; back 498 and 428 to 447.
 enum GroupedTiles { kFew16, kFew32, kFew64, k64, k128, k192, k256, kResident };
 GroupedTiles grouped_tiles(int64_t rows, int64_t experts, int64_t N, int64_t K, bool dx, bool slope) {
     const int64_t each = ceil_div(rows, experts);
@@ -1046,7 +1055,8 @@ int experts_dx(const llsa_experts_args& q, hipStream_t stream) {
     return launch_status("experts_dx");
 }
 
-// Rows of a chunk.  More chunks fill the chip's workgroups more evenly, and are more sums to write and read (linear.hip's weight_pieces).
+// Rows of a chunk.  More chunks fill the chip's workgroups more evenly, and are more sums to write and read (linear.hip's weight_pieces).  4593 rows of 777 and 333
+// channels, tiles of 64 x 64: 19.6 us and the sums 10.
 int grouped_rows(int64_t N) { return ceil_div(N, 192) * 192 <= ceil_div(N, 128) * 128 ? 192 : 128; }
 bool small_tiles(int64_t rows, int64_t N, int64_t K) { return ceil_div(N, 128) * ceil_div(K, 128) * std::max<int64_t>(1, rows / 512) < kCus; }
 int64_t chunk_rows(int64_t rows, int64_t N, int64_t K) {

