@@ -421,7 +421,7 @@ Tensor expert_feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_
             if (grad || !lib->experts_gathers(rows, one.E, one.N, one.K)) x = gathered(call, x, a, nullptr, Tensor(), 1);
             else one.gather_x = 1;
             one.x = x.p(); one.ldx = x.ld;
-                        one.bias = bias1.defined() ? bias1.data_ptr() : nullptr;
+            one.bias = bias1.defined() ? bias1.data_ptr() : nullptr;
             one.out = h.data_ptr(); one.ldo = h.size(1); one.act = act;
             if (slopes.defined()) { one.slopes = slopes.data_ptr(); one.ldz = slopes.size(1); }
             lib->check(lib->experts_fwd(&one, call.stream()), "experts_fwd");

@@ -103,7 +103,8 @@ __device__ __forceinline__ u32x2 whole_numbers(const vec8any<T>& x, const Steps&
     return o.w;
 }
 
-// LANES lanes hold a row, PIECES pieces of 8 elements each; longer rows (256 lanes only) are read a second time.  Bound by memory: 131072 rows of 1536 106 to 128 us by card (5.7 to 4.7 TB/s).
+// LANES lanes hold a row, PIECES pieces of 8 elements each; longer rows (256 lanes only) are read a second time.  Bound by memory and, still, by
+// its vector instructions (107 % by that counter): 131072 rows of 1536 106 to 128 us by card (5.7 to 4.7 TB/s).
 template <typename T, int LANES, int PIECES>
 __global__ __launch_bounds__(256) void quantize_kernel(const Quantize a) {
     typedef typename Bits<T>::type B;
