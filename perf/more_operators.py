@@ -19,7 +19,7 @@ Formulas, for a row l of logits, a row x of a sample b:
            expert's begin in it; places (token, j): where that number stands in it, or -1
   grouped  y = act(W_e x + bias_e) for rows offsets[e] .. offsets[e + 1] - 1, 0 for rows that no expert has
   experts  y = residual + gate_b * sum over the chosen e of w_e (W_out,e act(W_in,e x + b_in,e) + b_out,e)
-  int8     s = max |x| / 127 in fp32, q = x / s rounded to the nearest whole number (halves to even),  y = residual + gate_b * act(s s_n sum q q_n + bias)
+  int8     s = max |x| / 127, q = x / s rounded to the nearest whole number (halves to even),  y = residual + gate_b * act(s s_n sum q q_n + bias)
 """
 import math
 
@@ -130,15 +130,10 @@ def draw(rng):
 # ---------------------------------------------------------------------------------------
 # inputs
 # ---------------------------------------------------------------------------------------
-def _steps(x):
-    """max |x| / 127 of each row to the nearest fp32, which whole numbers hang on (a division by a number in 32 bits is a product with its inverse)."""
-    return (x.double().abs().amax(-1, keepdim=True) / 127).float()
-
-
 def _small_integers(w):
     """A weight (N, K) as it is kept for sampling: whole numbers from -127 to 127, and a scale for each channel out."""
-    scale = _steps(w)
-    return torch.round(w.double() / scale.double()).to(torch.int8), scale[:, 0]
+    scale = w.float().abs().amax(-1) / 127
+    return torch.round(w.double() / scale.double()[:, None]).to(torch.int8), scale
 
 
 def prepare(case, seed):
@@ -339,7 +334,7 @@ def _plain_experts(s):
 
 def _plain_int8(s):
     c, x = s["case"], s["x"]
-    scale = _steps(x)
+    scale = x.float().abs().amax(-1, keepdim=True) / 127
     q = torch.where(scale > 0, torch.round(x.double() / torch.where(scale > 0, scale, 1).double()), 0.0)
     z = (q @ s["weight"].double().t()).float() * scale * s["scale"]
     if c["bias"]:
@@ -486,7 +481,7 @@ def exact(case, seed):
             y = y + v["residual"]
     else:
         x = s["x"].double()
-        step = (x.abs().max(-1, keepdim=True).values / 127).float().double()
+        step = (x.abs().max(-1, keepdim=True).values.float() / 127).double()
         q = torch.where(step > 0, (x / torch.where(step > 0, step, 1.0)).round(), 0.0)
         z = step * s["scale"].double() * torch.matmul(q, s["weight"].double().transpose(0, 1))
         y = act(z + s["bias"].double() if case["bias"] else z)
