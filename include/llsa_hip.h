@@ -524,7 +524,7 @@ int64_t llsa_route_workspace_bytes(int64_t M, int E, int k);
  *     combine   out (tokens,N) = residual + gate * sum over j of weights[m,j] x[places[m,j]] (weights NULL: 1), x fp32
  *     dweights  dweights[m,j] = sum over n of gate * dz[m] * x[places[m,j]], x fp32; dgate = sum over a sample's tokens of dz[m] * sum over j of weights[m,j] x[places[m,j]];
  *               either unless NULL
- * slopes: act'(z) in steps of 2^-14, 16-bit integers, -32768 for a NaN. */
+ * slopes: act'(z) in 16 bits: steps of 2^-14, negative ones above -2^-4 with an exponent (ten bits behind the leading one, above -2^-19 seven). */
 typedef struct llsa_experts_args {
     const void *x, *w, *bias, *dz, *gate, *residual;
     void *out, *slopes, *dbias, *dgate, *workspace;

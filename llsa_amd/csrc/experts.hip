@@ -14,7 +14,8 @@
 //
 // Sums are fp32, and so are what happens on the way out and the rows that each expert gives a token (y, and dx of each), which are added up.  Rounded to 16 bits
 // besides the results is what a product takes in that another made (h, g, dz), as in the linear layers: half a step of each, 2^-8 of it in bf16 (fp16 2^-11).  What a
-// backward wants of z is act'(z), which lies between -0.13 and 1.13: 16 bits hold it in steps of 2^-14, where z itself would be half a step of bf16 off.
+// backward wants of z is act'(z), which lies between -0.13 and 1.13: 16 bits hold it in steps of 2^-14, and to seven bits and more where it is small, far below zero; z
+// itself would be half a step of bf16 off.
 #include "experts_device.h"
 
 namespace llsa {
@@ -65,11 +66,25 @@ __device__ __forceinline__ void write_zeros(const Grouped<T>& a, const Here& h) 
     }
 }
 
-// act'(z) in 16 bits: steps of 2^-14, which hold 0 and 1; one number is left for a NaN
+// act'(z) in 16 bits.  What matters for the products is its error beside 1: from -0.13 to 1.13 steps of 2^-14.  What matters to a unit far below zero, where all three
+// activations' slopes are negative and shrink to the least numbers, is its error beside itself: negative ones above -2^-4 are kept with an exponent.  Of the numbers of
+// 16 bits the steps take -2130 (-0.13) to 18500, so that 0x8000 to 0xf200 are left for those: from -0 on the upper half of the float (seven bits behind the leading one),
+// and from 2^-19 to 2^-4 ten bits behind it.  The two meet where they are equal, and above it the second, below it the first is the larger.  (Positive ones below
+// 2^-4 lie where act' crosses zero, and are no better known than z.)
 typedef __attribute__((ext_vector_type(8))) int16_t s16x8;
-// (added to 1.5 2^23 a number's last bits are its whole part, rounded)
-__device__ __forceinline__ int16_t slope_kept(float z, float slope) { return z != z ? (int16_t)-32768 : (int16_t)__float_as_uint(fmaf(slope, 16384.f, 12582912.f)); }
-__device__ __forceinline__ float slope_of(int16_t kept) { return kept == -32768 ? __uint_as_float(0x7fc00000u) : (float)kept * 0x1p-14f; }
+constexpr int16_t kNoSlope = 32767;       // of a NaN
+constexpr unsigned kSlopeJoin = (108u << 23) - (108u << 20);          // 2^-19: number 108 << 7 of either kind
+__device__ __forceinline__ int16_t slope_kept(float z, float slope) {
+    const unsigned bits = __float_as_uint(slope);
+    const int seven = (int)((bits + 0x8000u) >> 16), ten = (int)(bits + 0x1000u - 0x80000000u - kSlopeJoin + (0x8000u << 13)) >> 13;
+    // (added to 1.5 2^23 a number's last bits are its whole part, rounded)
+    const int step = (int)__float_as_uint(fmaf(slope, 16384.f, 12582912.f));
+    return z != z ? kNoSlope : (int16_t)((int)bits < (int)0xbd800000u ? max(seven, ten) : step);      // (0xbd800000: -2^-4; as integers negative floats are the lowest)
+}
+__device__ __forceinline__ float slope_of(int16_t kept) {
+    const unsigned k = (uint16_t)kept, seven = k << 16, ten = (k << 13) + (kSlopeJoin + 0x80000000u - (0x8000u << 13));
+    return kept == kNoSlope ? __uint_as_float(0x7fc00000u) : kept < -2304 ? __uint_as_float(min(seven, ten)) : (float)kept * 0x1p-14f;
+}
 
 // Eight values of a row on their way out.  kept: the slopes, in the forward; early: those of the layer in front, in dx
 template <bool YC, int ACT, bool TIGHT = false, typename T>

@@ -41,7 +41,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     x is (rows, K), weight (experts, N, K), bias (experts, N), all bf16 or all fp16; offsets (experts + 1) int32 on x's device, which stays there: experts may have any
     number of rows, none among them, and rows that no expert has (in front of the first or behind the last) come out as zeros, as does their gradient.  Offsets are
     held to 0 .. rows and made not to fall.  1 to 256 experts.  activation: None, "silu", "gelu" (erf) or "gelu_tanh".  Sums in fp32; besides the results, the backward rounds the
-    gradient behind the activation, whose slopes it keeps in 16 bits (steps of 2^-14).  Differentiable in x, weight and bias (once)."""
+    gradient behind the activation, whose slopes it keeps in 16 bits: off by up to 2^-15, and where they are small, far below zero, by up to a 2^-8th part of themselves
+    (below 2^-19, a 2^-11th above).  Differentiable in x, weight and bias (once)."""
     lib = current_lib()
     return lib.host.grouped_linear(lib.host_library, x, weight, offsets, bias, _activation(activation))
 
@@ -53,7 +54,7 @@ def expert_feed_forward(x: torch.Tensor, routing: Routing, w_in: torch.Tensor, b
     x is (..., C), routing what route_tokens returned for logits (..., experts) of the same tokens, w_in (experts, F, C), b_in (experts, F), w_out (experts, N, F),
     b_out (experts, N), gate (B, N) for an x of (B, ..., C), residual (..., N); all but the routing bf16 or all fp16.  A token without an expert gets its residual.
     Sums in fp32, each expert's result among them; the hidden rows and the gradients of either product's result are rounded to that type, and the backward keeps the activation's slopes in
-    16 bits (steps of 2^-14).  Differentiable in x, routing.weights, the weights and biases, gate and residual (once)."""
+    16 bits as grouped_linear does.  Differentiable in x, routing.weights, the weights and biases, gate and residual (once)."""
     lib = current_lib()
     weights, experts, order, offsets, places = routing
     return lib.host.expert_feed_forward(lib.host_library, x, weights, experts, order, offsets, places, w_in, b_in, w_out, b_out, _activation(activation), gate, residual)
