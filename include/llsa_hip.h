@@ -514,7 +514,7 @@ int64_t llsa_route_workspace_bytes(int64_t M, int E, int k);
 
 /* The experts' products.  Rows stand sorted by expert, those of expert e at offsets[e] .. offsets[e + 1] - 1 (held to 0 .. rows, and not falling); weights
  * (E,N,K).  Conventions of the linear layers above (rows 16-byte aligned and padded, sums in fp32).  The row at a place is that of token order[place] / k.  Numbers
- * in order, places and experts out of range are held to it or skipped.
+ * in order, places and experts out of range are held to it or skipped; products with `gaps` make places that no expert has rows of zeros.
  *     gather    out[place] = x[token] (N channels), times weights[order[place]] (and the gate of its sample) unless NULL
  *     fwd       z = x W_e^T + bias_e, out = act(z); act'(z) is kept in `slopes` unless that is NULL.  gather_x: x has rows of tokens, where llsa_experts_gathers
  *               allows it.  gaps: rows that no expert has get zeros.  wide: out is fp32 (padded rows)

@@ -55,16 +55,6 @@ __device__ __forceinline__ bool find_tile(const P& a, Here& h, int lane) {
     h = {p.expert, p.begin + (t - p.first) * BM, p.end, tn * BN, tn};
     return true;
 }
-template <int BM, int BN, typename T>
-__device__ __forceinline__ void write_zeros(const Grouped<T>& a, const Here& h) {
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = 0.f;
-    for (int i = threadIdx.x; i < BM * (BN / 8); i += blockDim.x) {
-        const int r = i / (BN / 8), n = h.n0 + (i - r * (BN / 8)) * 8;
-        if (h.m0 + r < h.m_end && n < a.N) store8(static_cast<T*>(a.out) + (int64_t)(h.m0 + r) * a.ldo + n, v, a.wide_out, a.N - n);
-    }
-}
 
 // act'(z) in 16 bits.  What matters for the products is its error beside 1: from -0.13 to 1.13 steps of 2^-14.  What matters to a unit far below zero, where all three
 // activations' slopes are negative and shrink to the least numbers, is its error beside itself: negative ones above -2^-4 are kept with an exponent.  Of the numbers of
@@ -133,6 +123,19 @@ __device__ __forceinline__ void put8_wide(float* to, const float (&v)[8]) {
     *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
     *reinterpret_cast<f32x4*>(to + 4) = f32x4{v[4], v[5], v[6], v[7]};
 }
+template <int BM, int BN, int ACT, typename T>
+__device__ __forceinline__ void write_zeros(const Grouped<T>& a, const Here& h) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = 0.f;
+    for (int i = threadIdx.x; i < BM * (BN / 8); i += blockDim.x) {
+        const int r = i / (BN / 8), n = h.n0 + (i - r * (BN / 8)) * 8;
+        if (h.m0 + r >= h.m_end || n >= a.N) continue;
+        const int64_t at = (int64_t)(h.m0 + r) * a.ldo + n;
+        if constexpr (ACT == kWide) put8_wide(static_cast<float*>(a.out) + at, v);
+        else store8(static_cast<T*>(a.out) + at, v, a.wide_out, a.N - n);
+    }
+}
 
 // The tiles of linear.hip's product_kernel, with an expert's weights; GATHERED: rows of tokens, brought into order on their way into LDS.  Bound as those are by the
 // operands' way from L2, and by the last tile of each expert, half of it empty on the average.  us, rows of eight experts: 16384, 2048 > 2048 171 (0.81 PFLOP/s;
@@ -152,7 +155,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_kernel(cons
     Here here;
     if (!find_tile<BM, BN>(a, here, lane)) return;
     if (here.expert < 0) {
-        write_zeros<BM, BN>(a, here);
+        write_zeros<BM, BN, ACT>(a, here);
         return;
     }
     RowsAlong<T, BM, kWaves, GATHERED> ox;
@@ -296,7 +299,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void grouped_few_kernel(const Gr
     Here here;
     if (!find_tile<16 * MT, kFewColumns>(a, here, lane)) return;
     if (here.expert < 0) {
-        write_zeros<16 * MT, kFewColumns>(a, here);
+        write_zeros<16 * MT, kFewColumns, ACT>(a, here);
         return;
     }
     const int n0 = here.n0, row0 = here.m0, all = (a.K + kStep - 1) / kStep, each = (all + kFewWaves - 1) / kFewWaves, first = min(all, wave * each), steps = min(all - first, each);
@@ -503,9 +506,14 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
             continue;
         }
         if (now.expert >= a.experts) {                        // no expert's rows
+            const float zeros[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                if (first + 16 * j + lane_row < now.end) *reinterpret_cast<vec8<T>*>(static_cast<T*>(a.out) + ((int64_t)(first + 16 * j) * a.ldo + n0) + at_out) = take8<T>(nullptr, true, 8);
+            for (int j = 0; j < 2; j++) {
+                if (first + 16 * j + lane_row >= now.end) continue;
+                const int64_t at = (int64_t)(first + 16 * j) * a.ldo + n0;
+                if constexpr (ACT == kWide) put8_wide(static_cast<float*>(a.out) + at + at_out, zeros);
+                else *reinterpret_cast<vec8<T>*>(static_cast<T*>(a.out) + at + at_out) = take8<T>(nullptr, true, 8);
+            }
             wait_vm0();
             continue;
         }
@@ -1222,7 +1230,7 @@ extern "C" int llsa_experts_fwd(const llsa_experts_args* a, void* stream) {
                  "experts_fwd: rows of x and w must be 16-byte aligned and a multiple of 8 long (zeros beyond the end)");
     LLSA_REQUIRE(a->out != nullptr && offsets32(a->ldo) && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->N))), "experts_fwd: output, padded rows 16-byte aligned and a multiple of 8 long");
     LLSA_REQUIRE(a->slopes == nullptr || (rows16(a->slopes, a->ldz) && a->ldz >= pad8(a->N) && a->act != LLSA_ACT_NONE), "experts_fwd: rows of slopes must be 16-byte aligned and padded to a multiple of 8");
-    LLSA_REQUIRE(!a->wide || (a->padded && a->act == LLSA_ACT_NONE && !a->gaps && !a->gather_x), "experts_fwd: rows of fp32 are padded, without an activation, gaps or gathered rows");
+    LLSA_REQUIRE(!a->wide || (a->padded && a->act == LLSA_ACT_NONE && !a->gather_x), "experts_fwd: rows of fp32 are padded, without an activation or gathered rows");
     LLSA_REQUIRE(!a->gather_x || llsa_experts_gathers(a->rows, a->E, a->N, a->K), "experts_fwd: rows of this many tokens have to be gathered beforehand");
     return BY_TYPE(experts_fwd);
 }
@@ -1232,7 +1240,7 @@ extern "C" int llsa_experts_dx(const llsa_experts_args* a, void* stream) {
     LLSA_REQUIRE(rows16(a->dz, a->lddz) && rows16(a->w, a->ldw) && a->lddz >= pad8(a->N) && a->ldw >= pad8(a->K), "experts_dx: rows of dz and w must be 16-byte aligned and padded to a multiple of 8");
     LLSA_REQUIRE(a->out != nullptr && offsets32(a->ldo) && (!a->padded || (rows16(a->out, a->ldo) && a->ldo >= pad8(a->K))), "experts_dx: output, padded rows 16-byte aligned and a multiple of 8 long");
     LLSA_REQUIRE(a->slopes == nullptr || (rows16(a->slopes, a->ldz) && a->ldz >= pad8(a->K)), "experts_dx: rows of slopes must be 16-byte aligned and padded to a multiple of 8");
-    LLSA_REQUIRE(!a->wide || (a->padded && a->slopes == nullptr && !a->gaps), "experts_dx: rows of fp32 are padded, without slopes or gaps");
+    LLSA_REQUIRE(!a->wide || (a->padded && a->slopes == nullptr), "experts_dx: rows of fp32 are padded, without slopes");
     return BY_TYPE(experts_dx);
 }
 extern "C" int llsa_experts_dw(const llsa_experts_args* a, void* stream) {

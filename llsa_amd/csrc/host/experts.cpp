@@ -333,7 +333,7 @@ struct ExpertFeedForwardBackward : public BlockNode {
                 const Tensor each = wide_rows(call, rows, C);
                 llsa_experts_args a = base;
                 set_weights(a, w1);
-                a.dz = dz.p(); a.lddz = dz.ld; a.out = each.data_ptr(); a.ldo = each.size(1); a.padded = 1; a.wide = 1;
+                a.dz = dz.p(); a.lddz = dz.ld; a.out = each.data_ptr(); a.ldo = each.size(1); a.padded = 1; a.wide = 1; a.gaps = 1;
                 lib->check(lib->experts_dx(&a, call.stream()), "experts_dx");
                 llsa_experts_args s = base;
                 s.x = each.data_ptr(); s.ldx = each.size(1); s.out = dx.data_ptr(); s.ldo = C; s.N = static_cast<int32_t>(C); s.K = 8;
@@ -428,6 +428,7 @@ Tensor expert_feed_forward(const std::shared_ptr<Library>& lib, const Tensor& x_
             set_weights(two, w2);
             two.x = h.data_ptr(); two.ldx = h.size(1); two.bias = bias2.defined() ? bias2.data_ptr() : nullptr;
             two.out = y.data_ptr(); two.ldo = y.size(1); two.wide = 1;
+            two.gaps = 1;                                     // (a caller's places may lie where no expert's rows do)
             lib->check(lib->experts_fwd(&two, call.stream()), "experts_fwd");
             const Rows residual = call.addend(residual_p);
             all.weights = weights.data_ptr<float>();

@@ -52,7 +52,8 @@ def expert_feed_forward(x: torch.Tensor, routing: Routing, w_in: torch.Tensor, b
     """residual + gate * sum over a token's experts e of weight_e * (activation(x @ w_in[e].T + b_in[e]) @ w_out[e].T + b_out[e]).
 
     x is (..., C), routing what route_tokens returned for logits (..., experts) of the same tokens, w_in (experts, F, C), b_in (experts, F), w_out (experts, N, F),
-    b_out (experts, N), gate (B, N) for an x of (B, ..., C), residual (..., N); all but the routing bf16 or all fp16.  A token without an expert gets its residual.
+    b_out (experts, N), gate (B, N) for an x of (B, ..., C), residual (..., N); all but the routing bf16 or all fp16.  A token without an expert gets its residual, and
+    nothing comes from places in front of offsets[0] or behind the last of the offsets.
     Sums in fp32, each expert's result among them; the hidden rows and the gradients of either product's result are rounded to that type, and the backward keeps the activation's slopes in
     16 bits as grouped_linear does.  Differentiable in x, routing.weights, the weights and biases, gate and residual (once)."""
     lib = current_lib()
