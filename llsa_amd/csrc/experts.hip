@@ -570,8 +570,9 @@ __global__ __launch_bounds__(64 * kResWaves) void grouped_resident_kernel(const 
 // ---------------------------------------------------------------------------------------
 // dW: C_e[m][n] = sum over an expert's rows p of X[p][m] Y[p][n].  All rows are taken in chunks of one length, whatever the
 // experts' are, so that the workgroups are alike; one that meets the end of an expert's rows writes its sums and goes on with the next expert's.  An expert
-// within one chunk is written straight away, the sums of the others meet in a second launch, which also writes the zeros of an expert without rows.  Expert
-// e's sums of chunk c are number c + e: with every next one either grows.  us: 262144 rows of eight experts, 384 and 1536 channels, 376 to 390 (0.8 PFLOP/s, the matrix units
+// within one chunk is written straight away, the sums of the others meet in a second launch, which also writes the zeros of an expert without rows.  A border of
+// two chunks cuts one expert at most: its sums in front of border b (between chunks b and b + 1) are number 2 b, those behind it up to the next border number 2 b + 1.  Sums of
+// the rows alone, which are small, have a place for every expert and chunk: c + e, as with every next one either grows.  us: 262144 rows of eight experts, 384 and 1536 channels, 376 to 390 (0.8 PFLOP/s, the matrix units
 // at work 33 % of the time; a library's product of one weight 950 to 990), the sums 20; 16384 rows of 2048 and 2048 channels 180 to 203 and 12, where pieces of every
 // expert's own took 303 and 70.
 // ---------------------------------------------------------------------------------------
@@ -583,13 +584,13 @@ struct GroupedWeights {
     int experts, rows, chunk;             // chunk: rows of one, a multiple of 64
     int M, N, nx, ny, tiles_m, tiles_n;
     T *out, *sums;                        // (experts, M, N), (experts, M) or NULL
-    float *part, *part_sum;               // [number][M][ld_part], [number][tiles_n][M]
+    float *part, *part_sum;               // [cut][M][ld_part], [chunk + expert][tiles_n][M]
     int64_t ld_part;
     int wide_out;
 };
-// Rows first .. end - 1 of an expert; alone: they are all it has
+// Rows first .. end - 1 of an expert; cut: number of their sums, -1 where they are all it has; number: of the rows' sums
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N>
-__device__ __forceinline__ void grouped_dw_piece(const GroupedWeights<T>& a, T* lds, int expert, int first, int end, bool alone, int number, int m0, int n0, int lane, int wave) {
+__device__ __forceinline__ void grouped_dw_piece(const GroupedWeights<T>& a, T* lds, int expert, int first, int end, int cut, int number, int m0, int n0, int lane, int wave) {
     constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
     typedef Operand<T, true, BM, kWaves> OperandX;
     typedef Operand<T, true, BN, kWaves> OperandY;
@@ -666,10 +667,10 @@ __device__ __forceinline__ void grouped_dw_piece(const GroupedWeights<T>& a, T* 
                 v[4 + e] = __uint_as_float(w[1]);
             }
             if (m >= a.M || left <= 0) continue;
-            if (alone) {
+            if (cut < 0) {
                 store8(a.out + ((int64_t)expert * a.M + m) * a.N + n, v, a.wide_out, left);
             } else {
-                float* const o = a.part + ((int64_t)number * a.M + m) * a.ld_part + n;
+                float* const o = a.part + ((int64_t)cut * a.M + m) * a.ld_part + n;
                 *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
                 *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
             }
@@ -697,7 +698,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(c
             p = runs.among(first, chunk1);
         }
         if (p.expert < 0) return;
-        grouped_dw_piece<T, BM, BN, WAVES_M, WAVES_N>(a, lds, p.expert, max(p.begin, chunk0), min(p.end, chunk1), p.begin >= chunk0 && p.end <= chunk1, chunk + p.expert, m0, n0, fresh(lane), wave);
+        const int cut = p.begin < chunk0 ? 2 * chunk - 1 : p.end > chunk1 ? 2 * chunk : -1;
+        grouped_dw_piece<T, BM, BN, WAVES_M, WAVES_N>(a, lds, p.expert, max(p.begin, chunk0), min(p.end, chunk1), cut, chunk + p.expert, m0, n0, fresh(lane), wave);
         first = p.end;
         __syncthreads();                                      // (everyone is done with what the next one's copies overwrite)
     }
@@ -707,7 +709,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void grouped_dw_kernel(c
 template <typename T>
 __global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<T> a, int ways) {
     __shared__ f32x4 rest[3][64];
-    __shared__ int first[LLSA_MAX_EXPERTS], chunks[LLSA_MAX_EXPERTS], cut[LLSA_MAX_EXPERTS], cuts;
+    __shared__ int first[LLSA_MAX_EXPERTS], chunks[LLSA_MAX_EXPERTS], cut[LLSA_MAX_EXPERTS], cuts;      // first: chunk
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     {
         Runs runs;
@@ -720,7 +722,7 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<
                 const bool joins = e < a.experts && c != 1;
                 const uint64_t all = __ballot(joins);
                 if (e < a.experts) {
-                    first[e] = c0 + e;
+                    first[e] = c0;
                     chunks[e] = c;
                 }
                 if (joins) cut[n + __popcll((unsigned long long)(all & (((uint64_t)1 << lane) - 1)))] = e;
@@ -749,7 +751,7 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<
             const int i = block * at_once + mine, m = min(i, of_one - 1) / n4, n = (min(i, of_one - 1) - m * n4) * 4;
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-            for (int s = part; s < count; s += ways) v += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)(from + s) * a.M + m) * a.ld_part + n);
+            for (int s = part; s < count; s += ways) v += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)(2 * (from + s) - (s > 0 ? 1 : 0)) * a.M + m) * a.ld_part + n);
             v = join(v);
             if (part > 0 || i >= of_one) continue;
             T* const out = a.out + ((int64_t)e * a.M + m) * a.N + n;
@@ -765,7 +767,7 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(const GroupedWeights<
         const int i = min(i0 + mine, rows - 1), e = i / a.M, m = i - e * a.M;
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-        for (int s = part; s < chunks[e] * a.tiles_n; s += ways) v[0] += a.part_sum[((int64_t)first[e] * a.tiles_n + s) * a.M + m];
+        for (int s = part; s < chunks[e] * a.tiles_n; s += ways) v[0] += a.part_sum[((int64_t)(first[e] + e) * a.tiles_n + s) * a.M + m];
         v = join(v);
         if (part == 0 && i0 + mine < rows) a.sums[i] = (T)v[0];
     }
@@ -1094,7 +1096,7 @@ int64_t chunk_rows(int64_t rows, int64_t N, int64_t K) {
     }
     return ceil_div(ceil_div(rows, best), kStep) * kStep;
 }
-int64_t part_count(int64_t rows, int64_t experts, int64_t N, int64_t K) { return ceil_div(rows, chunk_rows(rows, N, K)) + experts; }
+int64_t cut_count(int64_t rows, int64_t N, int64_t K) { return 2 * (ceil_div(rows, chunk_rows(rows, N, K)) - 1); }
 template <typename T, int BM, int BN>
 int launch_grouped_dw(GroupedWeights<T>& a, hipStream_t stream) {
     a.tiles_m = (int)ceil_div(a.M, BM);
@@ -1121,7 +1123,7 @@ int experts_dw(const llsa_experts_args& q, hipStream_t stream) {
     a.out = (T*)q.out; a.sums = (T*)q.dbias;
     a.ld_part = pad8(q.K);
     a.part = (float*)q.workspace;
-    a.part_sum = q.dbias != nullptr ? a.part + part_count(q.rows, q.E, q.N, q.K) * a.M * a.ld_part : nullptr;
+    a.part_sum = q.dbias != nullptr ? a.part + cut_count(q.rows, q.N, q.K) * a.M * a.ld_part : nullptr;
     a.wide_out = q.K % 8 == 0 && aligned16(q.out);
     const bool small = small_tiles(q.rows, q.N, q.K);
     const int rc = small ? launch_grouped_dw<T, 64, 64>(a, stream) : grouped_rows(a.M) == 192 ? launch_grouped_dw<T, 192, 128>(a, stream) : launch_grouped_dw<T, 128, 128>(a, stream);
@@ -1213,7 +1215,8 @@ using namespace llsa;
 
 extern "C" int64_t llsa_experts_dw_workspace_bytes(int64_t rows, int E, int N, int K) {
     if (rows <= 0 || E <= 0 || N <= 0 || K <= 0) return 0;
-    return 4 * part_count(rows, E, N, K) * N * (pad8(K) + ceil_div(K, 64));
+    const int64_t cuts = cut_count(rows, N, K);
+    return 4 * N * (cuts * pad8(K) + (cuts / 2 + 1 + E) * ceil_div(K, 64));
 }
 extern "C" int llsa_experts_gathers(int64_t rows, int E, int N, int K) { return rows > 0 && E > 0 && N > 0 && K > 0 && grouped_tiles(rows, E, N, K, false, false) <= k64; }
 extern "C" int llsa_experts_gather(const llsa_experts_args* a, void* stream) {
