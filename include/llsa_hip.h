@@ -44,7 +44,7 @@ extern "C" {
 #define LLSA_DTYPE_F32 1
 #define LLSA_DTYPE_F16 2
 
-#define LLSA_ABI_VERSION 221     /* changes with every change of a signature or argument structure below */
+#define LLSA_ABI_VERSION 222     /* changes with every change of a signature or argument structure below */
 int llsa_version(void);          /* LLSA_ABI_VERSION of the built library                                    */
 const char* llsa_last_error_string(void);
 
@@ -537,6 +537,11 @@ typedef struct llsa_experts_args {
 } llsa_experts_args;
 int llsa_experts_gather(const llsa_experts_args* a, void* stream);
 int llsa_experts_gathers(int64_t rows, int E, int N, int K);
+/* Which kernel a product of this many rows takes, N columns out and K of the contraction (back: dx, whose columns out are the weights' K; slopes: times act'; stores16: rows of out
+ * are padded, or 16-byte aligned and a multiple of 8 long): 0, 1, 2 few rows of each expert, 16, 32 or 64 at a time; 3 to 6 tiles of 64 x 64, 128 x 128, 192 x 128, 256 x 256;
+ * LLSA_EXPERTS_RESIDENT weights in registers; -1: no such sizes. */
+#define LLSA_EXPERTS_RESIDENT 7
+int llsa_experts_form(int64_t rows, int E, int N, int K, int back, int slopes, int stores16);
 int llsa_experts_fwd(const llsa_experts_args* a, void* stream);
 int llsa_experts_dx(const llsa_experts_args* a, void* stream);
 int llsa_experts_dz(const llsa_experts_args* a, void* stream);

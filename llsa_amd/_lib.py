@@ -177,6 +177,7 @@ _SIGNATURES = {
     "llsa_route_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
     "llsa_experts_gather": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
     "llsa_experts_gathers": (c_int, [c_int64, c_int, c_int, c_int]),
+    "llsa_experts_form": (c_int, [c_int64] + [c_int] * 6),
     "llsa_experts_fwd": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
     "llsa_experts_dx": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
     "llsa_experts_dz": (c_int, [C.POINTER(ExpertsArgs), c_void_p]),
@@ -189,7 +190,7 @@ _SIGNATURES = {
 
 EXPORTS = tuple(_SIGNATURES)
 CHUNK_FINE_MAX = 256                                        # LLSA_CHUNK_FINE_MAX of include/llsa_hip.h
-ABI_VERSION = 221                                           # LLSA_ABI_VERSION
+ABI_VERSION = 222                                           # LLSA_ABI_VERSION
 STATIC_PARTIALS_MAX = 262144                                # LLSA_STATIC_PARTIALS_MAX
 
 

@@ -963,20 +963,21 @@ Order order_of(const int32_t* slots, int k, int64_t tokens, int64_t rows) {
 int64_t pieces_of(int64_t rows, int64_t experts, int64_t size) { return rows / size + std::min<int64_t>(experts + 2, rows); }
 
 // Whether the weights stay in registers: a contraction of five or six steps, columns of which a wave has 32 or none and at most a quarter of the waves none (as
-// linear.hip's resident() has it, with both sides' times), and tiles enough for each workgroup that they pay for the weights' way there, also where it meets the next expert.
-bool resident(int64_t rows, int64_t experts, int64_t N, int64_t K) {
+// linear.hip's resident() has it, with both sides' times), rows of out that take 16-byte stores, and tiles enough for each workgroup that they pay for the weights' way
+// there, also where it meets the next expert.
+bool resident(int64_t rows, int64_t experts, int64_t N, int64_t K, bool wide_out) {
     const int64_t blocks = ceil_div(N, kResColumns);
-    if ((K != 5 * kStep && K != 6 * kStep) || N % 32 != 0 || 4 * N < 3 * kResColumns * blocks || blocks > kCus / 8) return false;
+    if (!wide_out || (K != 5 * kStep && K != 6 * kStep) || N % 32 != 0 || 4 * N < 3 * kResColumns * blocks || blocks > kCus / 8) return false;
     const int64_t slots = kCus / 8 / blocks * 8;
     return rows >= 8 * kResRows * experts && rows >= 8 * kResRows * slots;
 }
 // Which tiles: few rows for each expert on the average (64 and less are one workgroup's), small tiles while there are few of them for each CU, large ones beyond.
 // us, 16384 rows of eight experts 2048 > 2048: 256 x 256 181, 192 x 128 161 to 171; 262144 rows 1536 > 384: 128 x 128 425, 192 x 128 389; back 498 and 428 to 447.
-enum GroupedTiles { kFew16, kFew32, kFew64, k64, k128, k192, k256, kResident };
-GroupedTiles grouped_tiles(int64_t rows, int64_t experts, int64_t N, int64_t K, bool dx, bool slope) {
+enum GroupedTiles { kFew16, kFew32, kFew64, k64, k128, k192, k256, kResident = LLSA_EXPERTS_RESIDENT };
+GroupedTiles grouped_tiles(int64_t rows, int64_t experts, int64_t N, int64_t K, bool dx, bool slope, bool wide_out) {
     const int64_t each = ceil_div(rows, experts);
     if (each <= 64 || (rows / 64 + experts) * ceil_div(N, kFewColumns) <= kCus) return each <= 12 ? kFew16 : each <= 28 ? kFew32 : kFew64;
-    if (resident(rows, experts, N, K)) return kResident;
+    if (resident(rows, experts, N, K, wide_out)) return kResident;
     if ((rows / 64 + experts) * ceil_div(N, 64) <= 4 * kCus) return k64;
     // beyond, by linear.hip's lengths of a round, with half a tile more for each expert
     const auto rounds = [&](int bm, int bn, int slots) {
@@ -1030,7 +1031,7 @@ int launch_grouped_resident(Grouped<T>& a, hipStream_t stream) {
 template <typename T, bool YC, int ACT>
 int launch_grouped(Grouped<T>& a, hipStream_t stream) {
     a.group = (int64_t)a.N * a.K <= (1 << 20) ? 1 : 8;        // (rows of tiles that share y while it does not fit the L2 beside them)
-    const GroupedTiles t = grouped_tiles(a.rows, a.experts, a.N, a.K, YC, YC && ACT == kBySlope);
+    const GroupedTiles t = grouped_tiles(a.rows, a.experts, a.N, a.K, YC, YC && ACT == kBySlope, a.wide_out != 0);
     switch (t) {
         case kFew16: return launch_grouped_few<T, YC, 1, ACT>(a, stream);
         case kFew32: return launch_grouped_few<T, YC, 2, ACT>(a, stream);
@@ -1218,7 +1219,11 @@ extern "C" int64_t llsa_experts_dw_workspace_bytes(int64_t rows, int E, int N, i
     const int64_t cuts = cut_count(rows, N, K);
     return 4 * N * (cuts * pad8(K) + (cuts / 2 + 1 + E) * ceil_div(K, 64));
 }
-extern "C" int llsa_experts_gathers(int64_t rows, int E, int N, int K) { return rows > 0 && E > 0 && N > 0 && K > 0 && grouped_tiles(rows, E, N, K, false, false) <= k64; }
+extern "C" int llsa_experts_form(int64_t rows, int E, int N, int K, int back, int slopes, int stores16) {
+    if (rows <= 0 || E <= 0 || N <= 0 || K <= 0) return -1;
+    return grouped_tiles(rows, E, N, K, back != 0, back != 0 && slopes != 0, stores16 != 0);
+}
+extern "C" int llsa_experts_gathers(int64_t rows, int E, int N, int K) { return rows > 0 && E > 0 && N > 0 && K > 0 && grouped_tiles(rows, E, N, K, false, false, true) <= k64; }
 extern "C" int llsa_experts_gather(const llsa_experts_args* a, void* stream) {
     if (int rc = check_experts("experts_gather", a)) return rc;
     if (a->rows == 0) return 0;
