@@ -20,6 +20,7 @@ a workload for timing the operator inside a training step, not a weight-compatib
 from __future__ import annotations
 
 import math
+import weakref
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -54,18 +55,60 @@ def of(layer: nn.Linear, dtype: torch.dtype):
     return layer.weight.to(dtype), None if layer.bias is None else layer.bias.to(dtype)
 
 
-def keep_in_8_bits(layer: nn.Linear) -> None:
-    """The layer's weight as whole numbers with a scale for each channel out, beside the weight itself; project() then takes these."""
-    q, scale = quantize_rows(layer.weight.detach())
-    layer.register_buffer("weight_q", q, persistent=False)
-    layer.register_buffer("weight_scale", scale, persistent=False)
+class MadeOf:
+    """The weight that whole numbers were made of: its memory, and how often that has been written to.  A copy of this, or one out of a file, is of no weight."""
+
+    def __init__(self, weight: Optional[torch.Tensor] = None):
+        self.memory = None if weight is None else weakref.ref(weight.untyped_storage())
+        self.state = None if weight is None else self.state_of(weight)
+
+    @staticmethod
+    def state_of(weight: torch.Tensor):
+        return weight.data_ptr(), None if weight.is_inference() else weight._version
+
+    def still(self, weight: torch.Tensor) -> bool:
+        return self.memory is not None and self.memory() is weight.untyped_storage() and self.state == self.state_of(weight)
+
+    def __reduce__(self):
+        return MadeOf, ()
+
+
+def in_8_bits(layer: nn.Linear) -> bool:
+    return hasattr(layer, "weight_q")
+
+
+def keep_in_8_bits(layer: nn.Linear, keep: bool = True):
+    """The layer's weight as whole numbers with a scale for each channel out, beside the weight itself; project() then takes these.  Made once more they stay
+    where they are, so that captured graphs follow."""
+    if not keep:
+        if in_8_bits(layer):
+            del layer.weight_q, layer.weight_scale, layer.weight_made_of
+        return None
+    with torch.inference_mode(False), torch.no_grad():        # (buffers that may be written to in any mode)
+        q, scale = quantize_rows(layer.weight.detach())
+        if layer.weight.is_cuda and torch.cuda.is_current_stream_capturing():
+            return q, scale                                   # (of that graph, whose replays make them)
+        if in_8_bits(layer) and (layer.weight_q.shape, layer.weight_q.device, layer.weight_scale.dtype) == (q.shape, q.device, scale.dtype):
+            layer.weight_q.copy_(q)
+            layer.weight_scale.copy_(scale)
+        else:
+            layer.register_buffer("weight_q", q, persistent=False)
+            layer.register_buffer("weight_scale", scale, persistent=False)
+    layer.weight_made_of = MadeOf(layer.weight)
+    return layer.weight_q, layer.weight_scale
+
+
+def kept_in_8_bits(layer: nn.Linear):
+    """The whole numbers and scales of the layer's present weight: made again if it is another, or has been written to, cast or moved since."""
+    fresh = layer.weight_made_of.still(layer.weight) and layer.weight_scale.dtype == torch.float32 and layer.weight_q.device == layer.weight.device
+    return (layer.weight_q, layer.weight_scale) if fresh else keep_in_8_bits(layer)
 
 
 def project(layer: nn.Linear, x: torch.Tensor, rows=None, **epilogue) -> torch.Tensor:
     """The layer by this package's operators.  rows: x as quantize_rows gives it, for layers that share it."""
-    if hasattr(layer, "weight_q"):
+    if in_8_bits(layer):
         bias = None if layer.bias is None else layer.bias.to(x.dtype)
-        return linear_int8(x if rows is None else rows, layer.weight_q, layer.weight_scale, bias, dtype=x.dtype, **epilogue)
+        return linear_int8(x if rows is None else rows, *kept_in_8_bits(layer), bias, dtype=x.dtype, **epilogue)
     return linear(x, *of(layer, x.dtype), **epilogue)
 
 
@@ -135,7 +178,7 @@ class LlsaSelfAttention(nn.Module):
                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         B, N, _ = x.shape
         split = lambda y: y.view(B, N, self.heads, self.head_dim).transpose(1, 2)
-        rows = quantize_rows(x) if self.fused_layers and hasattr(self.to_q, "weight_q") else None
+        rows = quantize_rows(x) if self.fused_layers and in_8_bits(self.to_q) else None
         q, k, v = (split(project(layer, x, rows) if self.fused_layers else layer(x)) for layer in (self.to_q, self.to_k, self.to_v))
         norm = None
         if self.norm_q_weight is not None:
@@ -203,7 +246,7 @@ class RopeTransformerBlock(nn.Module):
             h = layer_norm(x, scale=scale_mlp, shift=shift_mlp, eps=self.norm3.eps)
             if self.num_experts:
                 return self.experts(h, gate_mlp, x)
-            if hasattr(self.ff_in, "weight_q"):
+            if in_8_bits(self.ff_in):
                 return project(self.ff_out, project(self.ff_in, h, activation="gelu_tanh"), gate=gate_mlp, residual=x)
             return feed_forward(h, *of(self.ff_in, h.dtype), *of(self.ff_out, h.dtype), activation="gelu_tanh", gate=gate_mlp, residual=x)
         h = self.norm3(x) * (1 + scale_mlp[:, None]) + shift_mlp[:, None]
@@ -242,15 +285,16 @@ class PixelDiT(nn.Module):
         # the table is kept in Z-order and in bf16, as register_rope_emb builds it (:153-173)
         self.register_buffer("freq", rope_table(sample_size, tuple(axes_dims_rope), dtype=torch.bfloat16), persistent=False)
 
-    def quantize_for_sampling(self) -> "PixelDiT":
-        """Keeps the blocks' projections and feed-forward weights (not an experts') as 8-bit integers, which the forward then multiplies with; call it
-        again after the weights have changed.  The model gives no gradients from then on: sample under torch.no_grad()."""
+    def quantize_for_sampling(self, on: bool = True) -> "PixelDiT":
+        """Keeps the blocks' projections and feed-forward weights (not an experts') as 8-bit integers, which the forward then multiplies with: sample under
+        torch.no_grad(), as the model gives no gradients until quantize_for_sampling(False).  A forward makes the integers of a weight again that has been loaded, replaced, written
+        to, cast or moved; call this again after writing through `weight.data`, which leaves no trace, and before replaying graphs captured earlier."""
         if not self.fused_layers:
             raise ValueError("quantize_for_sampling needs fused_layers=True")
         for block in self.transformer_blocks:
             a = block.attn1
             for layer in [a.to_q, a.to_k, a.to_v, a.to_out] + ([] if block.num_experts else [block.ff_in, block.ff_out]):
-                keep_in_8_bits(layer)
+                keep_in_8_bits(layer, on)
         return self
 
     def forward(self, images: torch.Tensor, timestep: torch.Tensor) -> torch.Tensor:
