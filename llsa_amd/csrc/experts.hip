@@ -13,7 +13,8 @@
 // spilled: 1050 us instead of 490).
 //
 // Sums are fp32, and so are what happens on the way out and the rows that each expert gives a token (y, and dx of each), which are added up.  Rounded to 16 bits
-// besides the results is what a product takes in that another made (h, g, dz), as in the linear layers: half a step of each, 2^-8 of it in bf16 (fp16 2^-11).  What a
+// besides the results is what a product takes in that another made (h, g, dz), as in the linear layers: half a step of each, 2^-8 of it in bf16 (fp16 2^-11, and 2^-25 below
+// 2^-14, where g and dz lie as the linear layers' dz does: a scale of the loss moves them).  What a
 // backward wants of z is act'(z), which lies between -0.13 and 1.13: 16 bits hold it in steps of 2^-14, and to seven bits and more where it is small, far below zero; z
 // itself would be half a step of bf16 off.
 #include "experts_device.h"

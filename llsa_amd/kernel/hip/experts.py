@@ -54,7 +54,8 @@ def expert_feed_forward(x: torch.Tensor, routing: Routing, w_in: torch.Tensor, b
     x is (..., C), routing what route_tokens returned for logits (..., experts) of the same tokens, w_in (experts, F, C), b_in (experts, F), w_out (experts, N, F),
     b_out (experts, N), gate (B, N) for an x of (B, ..., C), residual (..., N); all but the routing bf16 or all fp16.  A token without an expert gets its residual, and
     nothing comes from places in front of offsets[0] or behind the last of the offsets.
-    Sums in fp32, each expert's result among them; the hidden rows and the gradients of either product's result are rounded to that type, and the backward keeps the activation's slopes in
+    Sums in fp32, each expert's result among them; the hidden rows and the gradients of either product's result (weight * gate * its own) are rounded to that type,
+    which in fp16 wants a scaled loss, and the backward keeps the activation's slopes in
     16 bits as grouped_linear does.  Differentiable in x, routing.weights, the weights and biases, gate and residual (once)."""
     lib = current_lib()
     weights, experts, order, offsets, places = routing
