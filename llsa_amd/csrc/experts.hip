@@ -58,23 +58,31 @@ __device__ __forceinline__ bool find_tile(const P& a, Here& h, int lane) {
 }
 
 // act'(z) in 16 bits.  What matters for the products is its error beside 1: from -0.13 to 1.13 steps of 2^-14.  What matters to a unit far below zero, where all three
-// activations' slopes are negative and shrink to the least numbers, is its error beside itself: negative ones above -2^-4 are kept with an exponent.  Of the numbers of
-// 16 bits the steps take -2130 (-0.13) to 18500, so that 0x8000 to 0xf200 are left for those: from -0 on the upper half of the float (seven bits behind the leading one),
-// and from 2^-19 to 2^-4 ten bits behind it.  The two meet where they are equal, and above it the second, below it the first is the larger.  (Positive ones below
-// 2^-4 lie where act' crosses zero, and are no better known than z.)
+// activations' slopes are negative and shrink to the least numbers, is its error beside itself: negative ones above -2^-4 are kept with an exponent.  (Positive ones
+// below 2^-4 lie where act' crosses zero, and are no better known than z.)  The steps are numbers from 0 on, 4096 of them below zero.  Numbers with the sign bit are one
+// more than: from -0 on the upper half of the float (seven bits behind the leading one), and from 2^-19 to 2^-4 ten bits behind it.  The two meet where they are equal, and
+// above it the second, below it the first is the larger.  0x8000 is left for a NaN, and reads as one by itself.
 typedef __attribute__((ext_vector_type(8))) int16_t s16x8;
-constexpr int16_t kNoSlope = 32767;       // of a NaN
 constexpr unsigned kSlopeJoin = (108u << 23) - (108u << 20);          // 2^-19: number 108 << 7 of either kind
+// (a value that is made in any case: of a choice between two the compiler makes a branch for each element, and 262144 rows 384 > 1536 back by the slopes took 520 us where
+// they take 450)
+__device__ __forceinline__ unsigned made(unsigned v) {
+#ifndef LLSA_CPU_EMU_BUILD
+    asm("" : "+v"(v));
+#endif
+    return v;
+}
 __device__ __forceinline__ int16_t slope_kept(float z, float slope) {
     const unsigned bits = __float_as_uint(slope);
-    const int seven = (int)((bits + 0x8000u) >> 16), ten = (int)(bits + 0x1000u - 0x80000000u - kSlopeJoin + (0x8000u << 13)) >> 13;
+    const int seven = (int)((bits + 0x18000u) >> 16), ten = (int)(bits + 0x3000u - 0x80000000u - kSlopeJoin + (0x8000u << 13)) >> 13;
     // (added to 1.5 2^23 a number's last bits are its whole part, rounded)
-    const int step = (int)__float_as_uint(fmaf(slope, 16384.f, 12582912.f));
-    return z != z ? kNoSlope : (int16_t)((int)bits < (int)0xbd800000u ? max(seven, ten) : step);      // (0xbd800000: -2^-4; as integers negative floats are the lowest)
+    const unsigned step = __float_as_uint(fmaf(slope, 16384.f, 12582912.f + 4096.f)), small = made((unsigned)max(seven, ten));
+    return z != z ? (int16_t)-32768 : (int16_t)((int)bits < (int)0xbd800000u ? small : step);      // (0xbd800000: -2^-4; as integers negative floats are the lowest)
 }
 __device__ __forceinline__ float slope_of(int16_t kept) {
-    const unsigned k = (uint16_t)kept, seven = k << 16, ten = (k << 13) + (kSlopeJoin + 0x80000000u - (0x8000u << 13));
-    return kept == kNoSlope ? __uint_as_float(0x7fc00000u) : kept < -2304 ? __uint_as_float(min(seven, ten)) : (float)kept * 0x1p-14f;
+    const unsigned k = (uint16_t)kept, seven = (k << 16) - 0x10000u, ten = (k << 13) + (kSlopeJoin + 0x80000000u - (0x8001u << 13));
+    const unsigned step = __float_as_uint(fmaf((float)kept, 0x1p-14f, -0.25f)), small = made(min(seven, ten));
+    return __uint_as_float(kept < 0 ? small : step);
 }
 
 // Eight values of a row on their way out.  kept: the slopes, in the forward; early: those of the layer in front, in dx
@@ -100,7 +108,10 @@ __device__ __forceinline__ void way_out(const Grouped<T>& a, float (&v)[8], cons
         }
     } else if constexpr (ACT == kBySlope) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] *= slope_of(early[e]);
+        for (int e = 0; e < 8; e++) {
+            v[e] *= slope_of(early[e]);
+            if (TIGHT && e % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+        }
     }
 }
 template <typename T>
