@@ -150,7 +150,7 @@ __device__ __forceinline__ void write_zeros(const Grouped<T>& a, const Here& h) 
 }
 
 // The tiles of linear.hip's product_kernel, with an expert's weights; GATHERED: rows of tokens, brought into order on their way into LDS.  Bound as those are by the
-// operands' way from L2, and by the last tile of each expert, half of it empty on the average.  us, rows of eight experts: 16384, 2048 > 2048 171 (0.81 PFLOP/s;
+// operands' way, whose copies every step of 64 waits for, and by the last tile of each expert, half of it empty on the average.  us, rows of eight experts: 16384, 2048 > 2048 171 (0.81 PFLOP/s;
 // 256 x 256 181), its dx 168 to 180; 262144, 1536 > 384 to fp32 385 to 396 (0.78; a library's product of as many rows with one weight, to bf16, 324), dx 1536 > 384 428 to
 // 447; the matrix units work 28 to 32 % of the last two's time.
 template <typename T, bool YC, bool GATHERED, int BM, int BN, int WAVES_M, int WAVES_N, int ACT>
@@ -399,8 +399,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void grouped_few_kernel(const Gr
 
 // Many rows for each expert, a short contraction: the weights stay in registers (linear.hip's resident_kernel).  A workgroup of twelve waves keeps 384 columns of
 // an expert's weights, 32 columns a wave, and takes its share of the rows through LDS, 32 at a time and two such tiles ahead; where the expert changes it takes
-// in the next one's weights.  262144 rows 384 > 1536, us, tiles of 128 x 128 / this: GELU with slopes kept 823 / 535, back by the slopes 950 / 455 (501 and
-// 443 on another card).  Back it moves 1.9 GB at 4.1 to 4.3 TB/s, most of what a copy reaches; the forward writes 1.6 GB and has its vector units at work 52 % of the time.
+// in the next one's weights.  262144 rows 384 > 1536, us by card: GELU with slopes kept 535 to 573, back by the slopes 448 to 477 (in
+// tiles of 128 x 128, with slopes in steps alone, 823 and 950 where this took 501 to 535 and 433 to 455).  Back it moves 1.9 GB at 4.0 to 4.3 TB/s; the forward writes 1.6 GB and issues a vector
+// instruction for 0.58 of every four cycles of a SIMD (a kernel of nothing but fp32 fma: 0.9), most of them GELU, its slope and the slope's 16 bits.
 constexpr int kResWaves = 12, kResColumns = 32 * kResWaves, kResRows = 32, kResStages = 3, kResOwn = 32 * kStep + 64;
 struct Entry { int expert, begin, end, first, upto; };       // upto: number of the first tile behind its own
 template <typename T, bool YC, int ACT, int STEPS>

@@ -84,8 +84,8 @@ __device__ __forceinline__ Steps steps_for(float s) {
 }
 template <typename T>
 __device__ __forceinline__ int8_t whole_number(T x, const Steps& t) { return (int8_t)(t.zero ? 0 : nearest((float)x * t.lift, t.step, t.inverse, t.half)); }
-// Eight of them.  Without the cases that hardly a row has (halves that are exact, steps near the least numbers, no numbers), which are looked at once more: it is
-// these instructions that bound the pass (131072 rows of 1536: 136 us with all of nearest() for each, 112 % of the vector units' time by their counter).
+// Eight of them.  Without the cases that hardly a row has (halves that are exact, steps near the least numbers, no numbers), which are looked at once more:
+// with all of nearest() for each, more instructions and nothing else, 131072 rows of 1536 took 136 us instead of 106.
 template <typename T>
 __device__ __forceinline__ u32x2 whole_numbers(const vec8any<T>& x, const Steps& t) {
     union { int8_t b[8]; u32x2 w; } o;
@@ -103,8 +103,9 @@ __device__ __forceinline__ u32x2 whole_numbers(const vec8any<T>& x, const Steps&
     return o.w;
 }
 
-// LANES lanes hold a row, PIECES pieces of 8 elements each; longer rows (256 lanes only) are read a second time.  Bound by memory and, still, by
-// its vector instructions (107 % by that counter): 131072 rows of 1536 106 to 128 us by card (5.7 to 4.7 TB/s).
+// LANES lanes hold a row, PIECES pieces of 8 elements each; longer rows (256 lanes only) are read a second time.  Bound by memory (131072 rows of
+// 1536 106 to 128 us by card, 5.7 to 4.7 TB/s) and near what the vector units issue: one instruction for every four cycles of a SIMD, where a kernel of nothing but fp32 fma issues 0.9
+// and one of integer operations or conversions 1.6.
 template <typename T, int LANES, int PIECES>
 __global__ __launch_bounds__(256) void quantize_kernel(const Quantize a) {
     typedef typename Bits<T>::type B;
@@ -252,7 +253,7 @@ __device__ __forceinline__ void scales8(float (&v)[8], const float* p, bool wide
 }
 // WAY: the activation, everything in pieces of 16 bytes; -1: any activation and alignment.  8192 x 4096 x 4096 129 to 136 us by card (2.0 to 2.1 POP/s; a library's product without
 // scales 129), 131072 x 1536 x 384 with gate and residual 122 to 138 (a library's plain one 159; 168 here in tiles of 256 x 256 before the residual was read ahead and whole
-// lines stored).  Bound by the operands' way, as the 16-bit products are: the matrix units work 40 % and 25 % of the time.
+// lines stored).  Bound by the operands' way and the wait for it at every step, as the 16-bit products are: the matrix units work 40 % and 25 % of the time.
 template <typename T, int BM, int BN, int WAVES_M, int WAVES_N, int WAY>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void product8_kernel(const Product8<T> a) {
     constexpr int kWaves = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MT = WM / 16, NT = WN / 16, kTileX = BM * kStep, kTileY = BN * kStep;
