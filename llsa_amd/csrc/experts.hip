@@ -795,12 +795,12 @@ struct Gather {
     T* out;
     const float* weights;
     Order order;
-    int64_t ldx, ldo, s_gate, per_sample;
+    int64_t ldx, ldo, s_gate, per_sample, first;              // first: workgroup of this launch
     int rows, N, pieces, wide, wide_gate;
 };
 template <typename T>
 __global__ __launch_bounds__(256) void gather_kernel(const Gather<T> a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, place = i / a.pieces;
+    const int64_t i = (a.first + blockIdx.x) * 256 + threadIdx.x, place = i / a.pieces;
     if (place >= a.rows) return;                              // (places behind the last expert's hold a row as well, whichever: it is not read)
     const int n = (int)(i - place * a.pieces) * 8, left = a.N - n, token = a.order.token((int)place);
     vec8<T> v = take8(a.x + token * a.ldx + n, a.wide, left);
@@ -833,12 +833,12 @@ struct Combine {
     const int32_t* places;
     const float* weights;                 // or NULL: 1
     T* out;
-    int64_t ldy, s_gate, ldr, ldo, tokens, per_sample;
+    int64_t ldy, s_gate, ldr, ldo, tokens, per_sample, first;
     int k, rows, N, pieces, wide, wide_side, wide_out;       // pieces: of eight, of a row
 };
 template <typename T>
 __global__ __launch_bounds__(256) void combine_kernel(const Combine<T> a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / a.pieces;
+    const int64_t i = (a.first + blockIdx.x) * 256 + threadIdx.x, m = i / a.pieces;
     if (m >= a.tokens) return;
     const int n = (int)(i - m * a.pieces) * 8, left = a.N - n;
     float v[8];
@@ -874,13 +874,13 @@ struct DWeights {
     const float *y, *weights;
     const int32_t* places;
     float *dweights, *part;               // either may be NULL; part: [sample][piece][N]
-    int64_t ldd, ldy, s_gate, per_sample;
+    int64_t ldd, ldy, s_gate, per_sample, first;
     int k, rows, N, wide, wide_gate, piece, pieces;
 };
 template <typename T>
 __global__ __launch_bounds__(256) void dweights_kernel(const DWeights<T> a) {
     __shared__ float sums[4][512];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sample = (int)blockIdx.x / a.pieces, piece = (int)blockIdx.x - sample * a.pieces;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, block = (int)(a.first + blockIdx.x), sample = block / a.pieces, piece = block - sample * a.pieces;
     const int64_t t0 = sample * a.per_sample + (int64_t)piece * a.piece, t1 = min((int64_t)(sample + 1) * a.per_sample, t0 + a.piece);
     for (int n0 = 0; n0 < a.N; n0 += 512) {
         const int n = n0 + lane * 8, left = a.N - n;
@@ -933,15 +933,15 @@ __global__ __launch_bounds__(256) void dweights_kernel(const DWeights<T> a) {
         for (int e = 0; e < 8; e++) sums[wave][lane * 8 + e] = acc[e];
         __syncthreads();
         for (int c = threadIdx.x; c < 512; c += 256)
-            if (n0 + c < a.N) a.part[(int64_t)blockIdx.x * a.N + n0 + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+            if (n0 + c < a.N) a.part[(int64_t)block * a.N + n0 + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
         __syncthreads();
     }
 }
 // The pieces of dgate added up: four waves take every fourth of the same 64 columns' (a thread alone would wait for one after another)
 template <typename T>
-__global__ __launch_bounds__(256) void expert_gate_kernel(const float* part, T* dgate, int N, int pieces, int groups) {
+__global__ __launch_bounds__(256) void expert_gate_kernel(const float* part, T* dgate, int N, int pieces, int groups, int64_t first) {
     __shared__ float rest[3][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sample = (int)blockIdx.x / groups, n = ((int)blockIdx.x - sample * groups) * 64 + lane;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, block = (int)(first + blockIdx.x), sample = block / groups, n = (block - sample * groups) * 64 + lane;
     float v = 0.f;
     if (n < N) {
 #pragma unroll 8
@@ -954,8 +954,8 @@ __global__ __launch_bounds__(256) void expert_gate_kernel(const float* part, T* 
 
 // dz = dout * slope, of all rows.  Bound by memory.
 template <typename T>
-__global__ __launch_bounds__(256) void slope_rows_kernel(const T* dout, int64_t ldd, const int16_t* slopes, int64_t lds, T* dz, int64_t ldz, int64_t rows, int N, int pieces, int wide) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / pieces;
+__global__ __launch_bounds__(256) void slope_rows_kernel(const T* dout, int64_t ldd, const int16_t* slopes, int64_t lds, T* dz, int64_t ldz, int64_t rows, int N, int pieces, int wide, int64_t first) {
+    const int64_t i = (first + blockIdx.x) * 256 + threadIdx.x, m = i / pieces;
     if (m >= rows) return;
     const int n = (int)(i - m * pieces) * 8, left = N - n;
     const vec8<T> d = take8(dout + m * ldd + n, wide, left);
@@ -1155,9 +1155,10 @@ int experts_gather(const llsa_experts_args& q, hipStream_t stream) {
     a.rows = (int)q.rows; a.N = q.N; a.pieces = (int)(pad8(q.N) / 8);
     a.wide = q.N % 8 == 0 && wide8(q.x, q.ldx);
     a.wide_gate = q.N % 8 == 0 && wide8(q.gate, q.s_gate);
-    const int64_t grid = ceil_div(q.rows * a.pieces, 256);
-    LLSA_REQUIRE(grid <= kMaxGrid, "experts_gather: too many rows");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(gather_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+    in_launches(ceil_div(q.rows * a.pieces, 256), [&](int64_t first, dim3 grid) {
+        a.first = first;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(gather_kernel<T>), grid, dim3(256), 0, stream, a);
+    });
     return launch_status("experts_gather");
 }
 template <typename T>
@@ -1171,9 +1172,10 @@ int experts_combine(const llsa_experts_args& q, hipStream_t stream) {
     a.wide = q.N % 8 == 0 && wide8(q.gate, q.s_gate);
     a.wide_side = q.N % 8 == 0 && wide8(q.residual, q.ldr);
     a.wide_out = q.N % 8 == 0 && wide8(q.out, q.ldo);
-    const int64_t grid = ceil_div(q.tokens * a.pieces, 256);
-    LLSA_REQUIRE(grid <= kMaxGrid, "experts_combine: too many rows");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(combine_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+    in_launches(ceil_div(q.tokens * a.pieces, 256), [&](int64_t first, dim3 grid) {
+        a.first = first;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(combine_kernel<T>), grid, dim3(256), 0, stream, a);
+    });
     return launch_status("experts_combine");
 }
 // About 1024 workgroups, each of at least 16 tokens
@@ -1195,18 +1197,23 @@ int experts_dweights(const llsa_experts_args& q, hipStream_t stream) {
     a.wide_gate = q.N % 8 == 0 && wide8(q.gate, q.s_gate);
     const int64_t groups = ceil_div(q.N, 64);
     LLSA_REQUIRE(samples * p.count <= kMaxGrid && samples * groups <= kMaxGrid, "experts_dweights: too many samples");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(dweights_kernel<T>), dim3((unsigned)(samples * p.count)), dim3(256), 0, stream, a);
+    in_launches(samples * p.count, [&](int64_t first, dim3 grid) {
+        a.first = first;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(dweights_kernel<T>), grid, dim3(256), 0, stream, a);
+    });
     if (q.dgate != nullptr)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(expert_gate_kernel<T>), dim3((unsigned)(samples * groups)), dim3(256), 0, stream, a.part, (T*)q.dgate, q.N, p.count, (int)groups);
+        in_launches(samples * groups, [&](int64_t first, dim3 grid) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(expert_gate_kernel<T>), grid, dim3(256), 0, stream, a.part, (T*)q.dgate, q.N, p.count, (int)groups, first);
+        });
     return launch_status("experts_dweights");
 }
 template <typename T>
 int experts_dz(const llsa_experts_args& q, hipStream_t stream) {
     const int pieces = (int)(pad8(q.N) / 8);
-    const int64_t grid = ceil_div(q.rows * pieces, 256);
-    LLSA_REQUIRE(grid <= kMaxGrid, "experts_dz: too many rows");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(slope_rows_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, (const T*)q.dz, q.lddz, (const int16_t*)q.slopes, q.ldz, (T*)q.out, q.ldo, q.rows, q.N,
-                       pieces, q.N % 8 == 0 && wide8(q.dz, q.lddz));
+    in_launches(ceil_div(q.rows * pieces, 256), [&](int64_t first, dim3 grid) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(slope_rows_kernel<T>), grid, dim3(256), 0, stream, (const T*)q.dz, q.lddz, (const int16_t*)q.slopes, q.ldz, (T*)q.out, q.ldo, q.rows, q.N,
+                           pieces, q.N % 8 == 0 && wide8(q.dz, q.lddz), first);
+    });
     return launch_status("experts_dz");
 }
 

@@ -21,7 +21,7 @@ struct Quantize {
     float* scale;
     int64_t ldx, ldq, rows;
     int K, wide_x, wide_q;                // wide_q: rows of q are 16-byte aligned and filled with zeros to a multiple of 16; else K numbers are written
-    int64_t row_blocks;
+    int64_t row_blocks, first;            // first: workgroup of this launch
     // rows of integers that are copied beside: to 16-byte aligned rows filled with zeros
     llsa_pad_job pad[kPads];
     int64_t pad_end[kPads];               // pieces of 16, of this and the one before it
@@ -112,8 +112,9 @@ __global__ __launch_bounds__(256) void quantize_kernel(const Quantize a) {
     constexpr int kRows = 256 / LANES;
     __shared__ unsigned most[4];
     const int tid = threadIdx.x;
-    if ((int64_t)blockIdx.x >= a.row_blocks) {                // (uniform) the copies beside
-        int64_t i = ((int64_t)blockIdx.x - a.row_blocks) * 256 + tid;
+    const int64_t block = a.first + blockIdx.x;
+    if (block >= a.row_blocks) {                              // (uniform) the copies beside
+        int64_t i = (block - a.row_blocks) * 256 + tid;
         int k = 0;
         while (k < kPads && i >= a.pad_end[k]) k++;
         if (k == kPads) return;
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const Quantize a) {
         return;
     }
     const int lane = tid % LANES;
-    const int64_t row = (int64_t)blockIdx.x * kRows + tid / LANES;
+    const int64_t row = block * kRows + tid / LANES;
     const bool there = row < a.rows;
     const T* const x = static_cast<const T*>(a.x) + (there ? row : a.rows - 1) * a.ldx;
     const int pieces = (a.K + 7) / 8, runs = LANES < 256 ? 1 : (pieces + LANES * PIECES - 1) / (LANES * PIECES);
@@ -573,7 +574,10 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_rows_direct8_kernel(con
 template <typename T, int LANES, int PIECES>
 void launch_quantize(Quantize& a, int64_t pads, hipStream_t stream) {
     a.row_blocks = ceil_div(a.rows, 256 / LANES);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<T, LANES, PIECES>), dim3((unsigned)(a.row_blocks + ceil_div(pads, 256))), dim3(256), 0, stream, a);
+    in_launches(a.row_blocks + ceil_div(pads, 256), [&](int64_t first, dim3 grid) {
+        a.first = first;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(quantize_kernel<T, LANES, PIECES>), grid, dim3(256), 0, stream, a);
+    });
 }
 template <typename T>
 void quantize(Quantize& a, int64_t pads, hipStream_t stream) {
@@ -679,7 +683,6 @@ extern "C" int llsa_quantize_rows(const llsa_quantize_args* a, void* stream) {
         q.pad_end[i] = pads;
     }
     if (q.rows == 0 && pads == 0) return 0;
-    LLSA_REQUIRE(q.rows + ceil_div(pads, 256) <= kMaxGrid, "quantize_rows: too many rows");
     if (a->dtype == LLSA_DTYPE_BF16) quantize<bf16>(q, pads, (hipStream_t)stream);
     else if (a->dtype == LLSA_DTYPE_F16) quantize<_Float16>(q, pads, (hipStream_t)stream);
     else quantize<float>(q, pads, (hipStream_t)stream);

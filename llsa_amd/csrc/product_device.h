@@ -262,6 +262,13 @@ __device__ __forceinline__ void arrange_lines(vec8<T>& first, vec8<T>& second, i
 constexpr int64_t kMaxGrid = (int64_t(1) << 31) - 1;
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Workgroups of 256 threads in launches that have fewer than 2^32 threads each, all that a launch takes: f(first, count)
+constexpr int64_t kMaxBlocks = ((int64_t(1) << 32) - 1) / 256;
+template <typename F>
+void in_launches(int64_t blocks, F f) {
+    for (int64_t first = 0; first < blocks; first += kMaxBlocks) f(first, dim3((unsigned)std::min(kMaxBlocks, blocks - first)));
+}
+
 constexpr int kCus = 256;
 bool wide8(const void* p, int64_t ld) { return p == nullptr || (aligned16(p) && ld % 8 == 0); }
 

@@ -19,6 +19,7 @@ struct Route {
     int M, E, k, normalize, wide, chunks, per;                // per: tokens of a chunk
     const float* dweights;
     void* dlogits;
+    int64_t first;                                            // back: workgroup of this launch
 };
 constexpr int kRouteThreads = 1024, kRouteSlots = 4096, kRouteChunks = 256;
 
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(kRouteThreads) void place_kernel(const Route a) {
 template <typename T, int LANES, int PER>
 __global__ __launch_bounds__(256) void route_bwd_kernel(const Route a) {
     const int part = (int)threadIdx.x % LANES;
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES, m = min(at, (int64_t)a.M - 1);      // (all lanes: they ask one another)
+    const int64_t at = ((a.first + blockIdx.x) * 256 + threadIdx.x) / LANES, m = min(at, (int64_t)a.M - 1);      // (all lanes: they ask one another)
     const T* const logits = static_cast<const T*>(a.logits) + m * a.ld;
     float v[PER], g[PER];
     bool chosen[PER];
@@ -291,7 +292,10 @@ int route_chunks(int64_t M, int64_t k) { return (int)std::max<int64_t>(1, std::m
 template <typename T, int LANES, int PER>
 void launch_route(Route& a, hipStream_t stream) {
     if (a.dlogits != nullptr) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(route_bwd_kernel<T, LANES, PER>), dim3((unsigned)ceil_div((int64_t)a.M * LANES, 256)), dim3(256), 0, stream, a);
+        in_launches(ceil_div((int64_t)a.M * LANES, 256), [&](int64_t first, dim3 grid) {
+            a.first = first;
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(route_bwd_kernel<T, LANES, PER>), grid, dim3(256), 0, stream, a);
+        });
     } else if (a.chunks == 1) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(route_kernel<T, LANES, PER, true>), dim3(1), dim3(kRouteThreads), 0, stream, a);
     } else {
