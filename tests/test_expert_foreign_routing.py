@@ -70,8 +70,10 @@ CUTS = {"front": lambda o, rows: o.clamp(min=rows // 3), "back": lambda o, rows:
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("cut", list(CUTS))
 def test_places_without_an_expert(dev, no_numbers_in_new_memory, cut, dtype):
-    _check(dev, dtype, 2, 19, 4, 2, 24, 40, 24, CUTS[cut])
-    _check(dev, dtype, 1, 33, 3, 1, 13, 21, 9, CUTS[cut])
+    if dev.type == "cuda" or dtype == BF16:                   # (the emulation takes seconds for either)
+        _check(dev, dtype, 2, 19, 4, 2, 24, 40, 24, CUTS[cut])
+    if dev.type == "cuda" or dtype == FP16:
+        _check(dev, dtype, 1, 33, 3, 1, 13, 21, 9, CUTS[cut])
 
 
 @pytest.mark.gpu
